@@ -18,6 +18,9 @@ Public surface (mirrors the reference's interface for this path):
     fp8 (e4m3 weights, per-channel scales) variant of the same step
   * ``sample`` (and ``argmax_rows``, ``sample_rows``) -- the reference's
     ``sample(logits, temperature)``: argmax, or one softmax draw per row
+  * ``KV4Cache`` with ``kv4_append``, ``kv4_read``, ``kv4_attention``,
+    ``kv4_weights`` and ``kv4_evict`` -- the target's side of a draft block's
+    verification over a key/value cache held in 4 bits
 """
 
 from .checkpoints import detect_local_head_checkpoint_kind
@@ -26,6 +29,7 @@ from .local_head import (DeLSLocalHead, MarkovDeLSLocalHead, PositionMixJointHea
 from .ops import (Fp8Weight, PackedWeight, argmax_rows, fused_argmax, fused_argmax_fp8, gather_argmax, gru_step,
                   lowrank_argmax, lowrank_argmax_fp8, pack_operand, pack_operand_fp8, quantize_e4m3_rows,
                   quantize_pack_fp8, rank_proj, sample_rows, domino_argmax, lm_head, pack_lm_head)
+from .kv4 import KV4Cache, kv4_append, kv4_attention, kv4_evict, kv4_read, kv4_weights
 from .sampling import sample
 from .draft_step import DeLSDraftStep
 from .runner import DeLSGraphRunner
@@ -65,5 +69,11 @@ __all__ = [
     "quantize_pack_fp8",
     "fused_argmax_fp8",
     "lowrank_argmax_fp8",
+    "KV4Cache",
+    "kv4_append",
+    "kv4_read",
+    "kv4_attention",
+    "kv4_weights",
+    "kv4_evict",
     "synth",
 ]

@@ -26,6 +26,9 @@ LAYOUT_ROWMAJOR, LAYOUT_MFMA16 = 0, 1
 LAYOUT_FP8_K128, LAYOUT_FP8_K32 = 2, 3
 # the Domino correction MLP's middle layer (DELS_MIDDLE_*): name -> code
 MIDDLE_CODES = {"silu": 0, "identity": 1, "relu": 2, "gelu": 3, "gelu_tanh": 4, "tanh": 5, "sigmoid": 6}
+# which of a block's own slots its rows see in the 4-bit cache (DELS_KV4_*)
+KV4_BLOCK_CODES = {"causal": 0, "full": 1, "none": 2}
+KV4_BLOCK_MASK = 3
 NOALLOC_SCRATCH_BYTES = 16 << 20      # DELS_NOALLOC_SCRATCH_BYTES
 
 _i64 = ctypes.c_int64
@@ -96,6 +99,17 @@ class MarkovRolloutParams(ctypes.Structure):
     ]
 
 
+class Kv4CacheParams(ctypes.Structure):
+    """Mirror of ``struct dels_kv4_cache`` in include/dels.h."""
+
+    _fields_ = [
+        ("data", _ptr), ("num_pages", _i64), ("kv_heads", _i64), ("head_dim", _i64),
+        ("table", _ptr), ("ld_table", _i64), ("batch", _i64), ("max_pages", _i64),
+    ]
+
+
+_kv4 = ctypes.POINTER(Kv4CacheParams)
+
 # name -> (restype, argtypes); every symbol include/dels.h declares.
 SIGNATURES = {
     "dels_abi_version": (_int, []),
@@ -159,6 +173,16 @@ SIGNATURES = {
     "dels_lowrank_argmax_fp8": (_int, [_ptr, _i64, _ptr, _fptr, _ptr, _int, _ptr, _fptr, _ptr, _i64, _int, _ptr,
                                        _int, _fptr, _i64, _fptr, _i64, _i64, _i64, _i64, _i64, _ptr, _ptr, _i64,
                                        _ptr, _sz, _ptr]),
+    "dels_kv4_page_bytes": (_sz, [_i64]),
+    "dels_kv4_append": (_int, [_kv4, _ptr, _i64, _i64, _i64, _ptr, _i64, _i64, _i64, _int, _ptr, _ptr, _i64, _ptr]),
+    "dels_kv4_read": (_int, [_kv4, _ptr, _ptr, _i64, _ptr, _ptr, _int, _ptr]),
+    "dels_kv4_attention_ws_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64, _i64]),
+    "dels_kv4_attention": (_int, [_kv4, _ptr, _i64, _i64, _i64, _int, _i64, _i64, _ptr, _ptr, _int, _ptr, _i64,
+                                  ctypes.c_float, _ptr, _i64, _i64, _i64, _ptr, _ptr, _sz, _ptr]),
+    "dels_kv4_weights": (_int, [_kv4, _ptr, _i64, _i64, _i64, _int, _i64, _i64, _ptr, _ptr, _ptr, _int, _ptr, _i64,
+                                ctypes.c_float, _ptr, _ptr, _ptr, _ptr]),
+    "dels_kv4_evict_ws_bytes": (_sz, [_i64, _i64, _i64]),
+    "dels_kv4_evict": (_int, [_kv4, _ptr, _ptr, _i64, _i64, _ptr, _ptr, _ptr, _ptr, _sz, _ptr]),
 }
 
 _lock = threading.Lock()

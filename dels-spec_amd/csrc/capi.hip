@@ -25,7 +25,7 @@ constexpr int kRolloutDecodeMinG = 1024;
 
 static thread_local std::string g_last_error;
 
-static int fail(int code, const char* fmt, ...) {
+int fail(int code, const char* fmt, ...) {
     char buf[512];
     va_list ap;
     va_start(ap, fmt);
@@ -35,7 +35,7 @@ static int fail(int code, const char* fmt, ...) {
     return code;
 }
 
-static int hip_fail(hipError_t e, const char* what) {
+int hip_fail(hipError_t e, const char* what) {
     return fail(DELS_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
 }
 
@@ -176,7 +176,7 @@ static int check_argmax_args(const void* rank, int64_t ldrank, const void* B, in
     return DELS_OK;
 }
 
-static int check_ws(const void* ws, size_t ws_bytes, size_t need) {
+int check_ws(const void* ws, size_t ws_bytes, size_t need) {
     if (need == 0) return fail(DELS_ERR_UNSUPPORTED, "shape past the supported extents");
     if (!ws) return fail(DELS_ERR_WORKSPACE, "workspace is NULL (%zu bytes needed)", need);
     if ((reinterpret_cast<uintptr_t>(ws) & 255u) != 0) return fail(DELS_ERR_WORKSPACE, "workspace must be 256-byte aligned");

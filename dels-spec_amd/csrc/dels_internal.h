@@ -303,4 +303,68 @@ hipError_t launch_pack_fp8(const uint8_t* W, int64_t ldw, int64_t rows, int64_t 
 // Device properties of the current device (cached per device id).
 int device_cu_count();
 
+// ---- host checks shared by the files of the C ABI (capi.hip) ---------------------
+
+// Records the calling thread's error text (dels_last_error) and returns `code`.
+int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
+int hip_fail(hipError_t e, const char* what);
+int check_ws(const void* ws, size_t ws_bytes, size_t need);
+
+// ---- 4-bit key/value cache (kv4_*.hip) -----------------------------------------
+
+constexpr int kKv4Page = 64;             // slots of a page
+
+// The pages and each sequence's row of page numbers (struct dels_kv4_cache).
+struct Kv4Cache {
+    uint8_t* data; int num_pages, heads, head_dim;
+    const int32_t* table; int64_t ld_table;
+    int batch, max_pages;
+    __host__ __device__ int slots() const { return max_pages * kKv4Page; }
+};
+
+// A tensor [batch, tokens, heads, D] with unit channel stride.
+struct Kv4Rows { const void* p; int64_t batch, token, head; };
+
+// dtype as DELS_DTYPE_*.
+hipError_t launch_kv4_append(const Kv4Cache& c, const Kv4Rows& k, const Kv4Rows& v, int dtype, const int32_t* lengths,
+                             const int32_t* counts, int T, hipStream_t s);
+hipError_t launch_kv4_read(const Kv4Cache& c, const int32_t* starts, const int32_t* counts, int T, void* k, void* v,
+                           int dtype, hipStream_t s);
+
+// Which slots the rows of a block see beside their sequence's context.
+struct Kv4Block {
+    const int32_t* lengths;              // context: slots [0, lengths[b])
+    const int32_t* counts;               // valid rows of the block (null: T)
+    int T, mode;                         // DELS_KV4_CAUSAL .. DELS_KV4_MASK
+    const int64_t* mask; int64_t ld_mask;
+};
+
+struct Kv4AttentionArgs {
+    Kv4Cache cache; Kv4Block block;
+    Kv4Rows q; int dtype, q_heads;
+    float scale;
+    void* out; int64_t out_batch, out_token, out_head;
+    float* lse;                          // [batch, T, q_heads]
+};
+hipError_t launch_kv4_attention(const Kv4AttentionArgs& a, hipStream_t s);
+
+struct Kv4WeightsArgs {
+    Kv4Cache cache; Kv4Block block;
+    Kv4Rows q; int dtype, q_heads;
+    float scale;
+    const int32_t* accepted;
+    const float* lse; const float* weights; float* out;
+};
+hipError_t launch_kv4_weights(const Kv4WeightsArgs& a, hipStream_t s);
+
+struct Kv4EvictArgs {
+    Kv4Cache cache;
+    const int32_t* lengths; const float* weights;
+    int keep, recent;
+    int32_t* out_lengths; float* out_weights; int32_t* source;
+};
+// Words of the workspace's data region that the selection keeps its holes in.
+size_t kv4_evict_data_bytes(int64_t batch, int64_t heads, int64_t keep);
+hipError_t launch_kv4_evict(const Kv4EvictArgs& a, void* ws, size_t data_off, hipStream_t s);
+
 }  // namespace dels

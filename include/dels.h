@@ -544,6 +544,110 @@ size_t dels_markov_rollout_ws_bytes(int64_t batch, int64_t r, int64_t V);
 int dels_markov_rollout_enqueue(const dels_markov_rollout* p, void* stream);
 int dels_markov_graph_create(const dels_markov_rollout* p, void** graph_out);
 
+/* ---- key/value cache held in 4 bits -------------------------------------------
+ *
+ * What the verification of a draft block (code/dflash.py:637-651) reads and
+ * writes on the target's side, with the cache in 4 bits a value; the reference
+ * keeps its cache in bf16 inside transformers.  Pages of 64 slots of one
+ * key/value head; D = 64 or 128 channels.  A page of 66 D + 128 bytes holds
+ *   key codes    64 rows of D/2 bytes, channel 2c in the low half of byte c;
+ *   key scales   one byte e, 2^(e-127), per slot and 32 channels: slot
+ *                32 s + 8 rh + 4 a + rl of block m at byte 64 m + 16 rh + 4 rl + 2 s + a;
+ *   value codes  8 rows of D little-endian words, slot 8 g + i in bits 4 i .. 4 i + 3
+ *                of its channel's word of row g;
+ *   value scales 64 bf16 numbers, one per slot.
+ * Codes are e2m1 (0, .5, 1, 1.5, 2, 3, 4, 6 and a sign bit), rounded to nearest
+ * with ties to the even code, saturating.  A key block's exponent is the
+ * smallest whose sevenfold 7 * 2^(e-127) holds its largest magnitude, in 1 .. 252;
+ * a value scale is max(bf16(amax * fp32(1/6)), 2^-126).  NaN counts as 0,
+ * magnitudes over 3e38 as 3e38.
+ *
+ * Every sequence has a row of page numbers; slot j of sequence b lies in page
+ * table[b * ld_table + j / 64].  An entry outside [0, num_pages) names no page: writes
+ * to it are dropped, reads give 0, attention does not see it.  Lengths and counts
+ * are device arrays that the kernels clamp (lengths to [0, 64 max_pages], counts
+ * to [0, T]); nothing is read back to the host.  `data` is 128-byte aligned.
+ */
+typedef struct dels_kv4_cache {
+    void* data;                /* [num_pages, kv_heads, 66 * head_dim + 128] bytes */
+    int64_t num_pages;
+    int64_t kv_heads;
+    int64_t head_dim;          /* 64 or 128 */
+    const int32_t* table;      /* [batch, max_pages] page numbers, row stride ld_table */
+    int64_t ld_table;
+    int64_t batch;
+    int64_t max_pages;
+} dels_kv4_cache;
+
+/* What the rows of a block see beside their sequence's context, slots [0, lengths[b]).
+ * Row t < counts[b] of the block lies in slot lengths[b] + t. */
+#define DELS_KV4_CAUSAL 0      /* the block's slots up to their own */
+#define DELS_KV4_FULL 1        /* the block's valid slots */
+#define DELS_KV4_NONE 2        /* the context alone */
+#define DELS_KV4_MASK 3        /* the block's valid slots i with bit i of the row's mask set; T <= 64 */
+
+/* Bytes of a page of one head (0 for a head size that is not supported). */
+size_t dels_kv4_page_bytes(int64_t head_dim);
+
+/*
+ * Quantise rows t < counts[b] (NULL: T) of k and v [batch, T, kv_heads, D] into slots
+ * lengths[b] + t; rows past the table's slots are dropped.  Strides in elements, unit
+ * channel stride, 16-byte aligned rows.  dtype DELS_DTYPE_*.
+ */
+int dels_kv4_append(const dels_kv4_cache* c, const void* k, int64_t k_batch, int64_t k_token, int64_t k_head,
+                    const void* v, int64_t v_batch, int64_t v_token, int64_t v_head, int dtype,
+                    const int32_t* lengths, const int32_t* counts, int64_t T, void* stream);
+
+/*
+ * The values that slots starts[b] + t, t < counts[b] (NULL: T), stand for, into
+ * contiguous k and v [batch, T, kv_heads, D] of `dtype`; 0 from counts[b] on and past the
+ * table's slots.
+ */
+int dels_kv4_read(const dels_kv4_cache* c, const int32_t* starts, const int32_t* counts, int64_t T, void* k, void* v,
+                  int dtype, void* stream);
+
+/*
+ * Attention of a block's rows over the cache: out[b, t, hq] = softmax(scale * q . K^T) V over the
+ * slots that row t sees, head hq reading key/value head hq / (q_heads / kv_heads), and
+ * lse[b, t, hq] (contiguous fp32), the logarithm of the softmax's sum.  A row that sees
+ * nothing, and rows from counts[b] on, give out = 0 and lse = -inf.  q [batch, T, q_heads, D]
+ * bf16 or fp16, out the same type, any strides that keep rows 16-byte aligned.  With fp16 q
+ * the keys that the cache holds must be below 2^20 in magnitude.
+ */
+size_t dels_kv4_attention_ws_bytes(int64_t batch, int64_t T, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                                   int64_t max_pages);
+int dels_kv4_attention(const dels_kv4_cache* c, const void* q, int64_t q_batch, int64_t q_token, int64_t q_head,
+                       int dtype, int64_t q_heads, int64_t T, const int32_t* lengths, const int32_t* counts,
+                       int block, const int64_t* mask, int64_t ld_mask, float scale, void* out, int64_t out_batch,
+                       int64_t out_token, int64_t out_head, float* lse, void* ws, size_t ws_bytes, void* stream);
+
+/*
+ * Attention weights that rows t < accepted[b] (NULL: all valid rows) gave to each slot, added
+ * up over the query heads of each key/value head:
+ *   out[b, h, j] = (j < lengths[b] ? weights[b, h, j] : 0) + sum_t,hq exp(scale * q . k_j - lse[b, t, hq])
+ * lse as dels_kv4_attention wrote it for the same block.  weights and out contiguous
+ * fp32 [batch, kv_heads, 64 * max_pages]; out may be weights.
+ */
+int dels_kv4_weights(const dels_kv4_cache* c, const void* q, int64_t q_batch, int64_t q_token, int64_t q_head,
+                     int dtype, int64_t q_heads, int64_t T, const int32_t* lengths, const int32_t* counts,
+                     const int32_t* accepted, int block, const int64_t* mask, int64_t ld_mask, float scale,
+                     const float* lse, const float* weights, float* out, void* stream);
+
+/*
+ * Shrink every (sequence, head) of more than `keep` slots to `keep`: its last `recent`
+ * slots stay, and of the others those of largest weight (equal weights: lowest slot; NaN
+ * as -inf).  Slots that stay from `keep` on move, in ascending order, into the places
+ * given up below it, in ascending order; the cache changes in place.
+ *   out_lengths[b] = min(lengths[b], keep)
+ *   source[b, h, j], j < keep: the slot whose content place j holds now, -1 from
+ *     out_lengths[b] on
+ *   out_weights: the weights in their new places, 0 from out_lengths[b] on
+ * No output may be one of the inputs.
+ */
+size_t dels_kv4_evict_ws_bytes(int64_t batch, int64_t kv_heads, int64_t keep);
+int dels_kv4_evict(const dels_kv4_cache* c, const int32_t* lengths, const float* weights, int64_t keep, int64_t recent,
+                   int32_t* out_lengths, float* out_weights, int32_t* source, void* ws, size_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -10,3 +10,4 @@ from .dels_oracle import *  # noqa: F401,F403
 from . import sampling  # noqa: F401
 from . import domino  # noqa: F401
 from . import bounds  # noqa: F401
+from . import kv4  # noqa: F401
