@@ -59,6 +59,13 @@ int check_type(int dtype, bool single) {
     return fail(DELS_ERR_INVALID_ARGUMENT, "unknown or unsupported element type %d", dtype);
 }
 
+// Extents that attention and its weights take: the pages of all rows stay below 2^30.
+bool attention_ok(int64_t batch, int64_t T, int64_t q_heads, int64_t kv_heads, int64_t max_pages) {
+    return extent_ok(batch) && extent_ok(T) && extent_ok(q_heads) && extent_ok(kv_heads) && kv_heads > 0 &&
+           q_heads % kv_heads == 0 && max_pages >= 0 && grid_ok({T, q_heads / kv_heads, 64}) &&
+           grid_ok({batch, kv_heads, T * (q_heads / kv_heads) / 16 + 1, max_pages});
+}
+
 // The arguments that attention and its weights share.
 int check_block(const Kv4Cache& c, const void* q, int64_t qb, int64_t qt, int64_t qh, int dtype, int64_t q_heads,
                 int64_t T, const int32_t* lengths, int block, const int64_t* mask, int64_t ld_mask, float scale) {
@@ -78,7 +85,7 @@ int check_block(const Kv4Cache& c, const void* q, int64_t qb, int64_t qt, int64_
     if (!(scale == scale) || scale == __builtin_inff() || scale == -__builtin_inff())
         return fail(DELS_ERR_INVALID_ARGUMENT, "scale must be finite");
     if (!lengths) return fail(DELS_ERR_INVALID_ARGUMENT, "lengths is NULL");
-    if (!grid_ok({c.batch, T, q_heads}) || !grid_ok({c.batch, c.heads, c.max_pages}) || !grid_ok({T, q_heads, 128}))
+    if (!attention_ok(c.batch, T, q_heads, c.heads, c.max_pages))
         return fail(DELS_ERR_UNSUPPORTED, "shape past the supported extents");
     return check_rows(q, qb, qt, qh, dtype, "q");
 }
@@ -129,7 +136,11 @@ int dels_kv4_read(const dels_kv4_cache* p, const int32_t* starts, const int32_t*
     return e == hipSuccess ? DELS_OK : hip_fail(e, "cache read launch");
 }
 
-size_t dels_kv4_attention_ws_bytes(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t) { return kDataOff; }
+size_t dels_kv4_attention_ws_bytes(int64_t batch, int64_t T, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                                   int64_t max_pages) {
+    if (!attention_ok(batch, T, q_heads, kv_heads, max_pages) || (head_dim != 64 && head_dim != 128)) return 0;
+    return kDataOff + kv4_attention_data_bytes(batch, T, q_heads, kv_heads, head_dim, max_pages);
+}
 
 int dels_kv4_attention(const dels_kv4_cache* p, const void* q, int64_t q_batch, int64_t q_token, int64_t q_head,
                        int dtype, int64_t q_heads, int64_t T, const int32_t* lengths, const int32_t* counts,
@@ -150,7 +161,7 @@ int dels_kv4_attention(const dels_kv4_cache* p, const void* q, int64_t q_batch, 
     a.q = {q, q_batch, q_token, q_head};
     a.dtype = dtype, a.q_heads = (int)q_heads, a.scale = scale;
     a.out = out, a.out_batch = out_batch, a.out_token = out_token, a.out_head = out_head, a.lse = lse;
-    const hipError_t e = launch_kv4_attention(a, static_cast<hipStream_t>(stream));
+    const hipError_t e = launch_kv4_attention(a, ws, kDataOff, static_cast<hipStream_t>(stream));
     return e == hipSuccess ? DELS_OK : hip_fail(e, "cache attention launch");
 }
 

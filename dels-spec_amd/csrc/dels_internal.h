@@ -346,7 +346,10 @@ struct Kv4AttentionArgs {
     void* out; int64_t out_batch, out_token, out_head;
     float* lse;                          // [batch, T, q_heads]
 };
-hipError_t launch_kv4_attention(const Kv4AttentionArgs& a, hipStream_t s);
+// Bytes of the workspace's data region for the states of split rows.
+size_t kv4_attention_data_bytes(int64_t batch, int64_t T, int64_t q_heads, int64_t heads, int64_t head_dim,
+                                int64_t max_pages);
+hipError_t launch_kv4_attention(const Kv4AttentionArgs& a, void* ws, size_t data_off, hipStream_t s);
 
 struct Kv4WeightsArgs {
     Kv4Cache cache; Kv4Block block;
