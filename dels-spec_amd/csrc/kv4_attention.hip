@@ -87,10 +87,9 @@ __device__ __forceinline__ float key_scale(uint32_t word, int byte) {
     return __uint_as_float((uint32_t)max(e - kKeyShift<T>, 0) << 23);
 }
 
-// Shapes of a wave's work on RT rows: MT x MT tiles of the matrix instructions.
-template <int D, int RT> struct Shape {
-    static constexpr int MT = RT == 16 ? 16 : 32;
-    static constexpr int NR = RT / MT;              // tiles of rows
+// Shapes of a wave's work on MT rows: MT x MT tiles of the matrix instructions.
+template <int D, int MT_> struct Shape {
+    static constexpr int MT = MT_;
     static constexpr int NG = 64 / MT;              // lane groups: lane = MT * group + row
     static constexpr int DL = D / NG;               // channels of a key that a lane holds
     static constexpr int KS = DL / 8;               // steps of the first product
@@ -101,7 +100,6 @@ template <int D, int RT> struct Shape {
     static constexpr int CT = D / MT;               // channel tiles of the output
     static constexpr int VW = MT == 16 ? 4 : D / 32;    // consecutive channels of a lane: words of a load
     static constexpr int VL = CT / VW;              // loads of value words per operand
-    static constexpr int STEP = RT == 64 ? 1 : 2;   // 32-slot halves per softmax step
     using Acc = typename std::conditional<MT == 16, f32x4, f32x16>::type;
     // slot within 32 that row r of key tile a holds
     __device__ static int slot_of(int a, int r) {
@@ -115,12 +113,15 @@ template <int D, int RT> struct Shape {
     }
 };
 
-// The line of pages: pages of (b, h, row tile) one after the other, b first.
+// The line of pages: those of (b, h, row tile) one after the other, b first.  It is
+// cut every `share` pages; a cut within `snap` pages of a row tile's end moves there,
+// so that no piece holds a few pages of one tile and the rest of another's.
 struct Line {
     int tiles;                 // row tiles per (b, h)
     int pieces;                // workgroups
     int min_pages;             // fewest pages of a piece
 };
+constexpr int kSnap = 8;       // one page for each wave
 
 __device__ __forceinline__ int seq_end(const Kv4Block& k, int b, int slots) {
     const int n = kv4_length(k.lengths, b, slots);
@@ -132,36 +133,68 @@ __device__ __forceinline__ int seq_pages(const Kv4Block& k, int b, int slots) {
     return max(1, (seq_end(k, b, slots) + kKv4Page - 1) / kKv4Page);
 }
 
-// Where unit `u` of the line lies, by all lanes of a wave.
-struct Place { int b, start, pages; };          // `start`: first unit of sequence b
-__device__ __forceinline__ int line_units(const Kv4Block& k, const Kv4Cache& c, int per) {
-    const int lane = threadIdx.x & 63;
-    int sum = 0;
-    for (int b = lane; b < c.batch; b += 64) sum += seq_pages(k, b, c.slots());
+// What all lanes of a wave hold alike, kept in a scalar register.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// Scan of the sequences' units by a wave, 64 at a time; up to 64 it is kept.
+struct Scan {
+    const Kv4Block& k;
+    const Kv4Cache& c;
+    int per;                   // row tiles of a sequence
+    int own, cum;              // units of this lane's sequence, and of all up to it, in the 64 from b0
+    int b0, before, total;
+
+    __device__ Scan(const Kv4Block& k_, const Kv4Cache& c_, int per_) : k(k_), c(c_), per(per_) {
+        seek(0, 0);
+        total = __builtin_amdgcn_readlane(cum, 63);
+        for (int b = 64 + (threadIdx.x & 63), rest = 0; c.batch > 64; b += 64) {
+            rest += b < c.batch ? seq_pages(k, b, c.slots()) * per : 0;
+            if ((b & ~63) + 64 >= c.batch) {
 #pragma unroll
-    for (int off = 1; off < 64; off <<= 1) sum += __shfl_xor(sum, off, 64);
-    return sum * per;
-}
-__device__ __forceinline__ Place line_place(const Kv4Block& k, const Kv4Cache& c, int per, int u) {
-    const int lane = threadIdx.x & 63;
-    int before = 0;
-    for (int b0 = 0;; b0 += 64) {
-        const int own = b0 + lane < c.batch ? seq_pages(k, b0 + lane, c.slots()) * per : 0;
-        int cum = own;
+                for (int off = 1; off < 64; off <<= 1) rest += __shfl_xor(rest, off, 64);
+                total += uniform(rest);
+                break;
+            }
+        }
+    }
+    __device__ void seek(int b0_, int before_) {
+        const int lane = threadIdx.x & 63;
+        b0 = b0_, before = before_;
+        own = b0 + lane < c.batch ? seq_pages(k, b0 + lane, c.slots()) * per : 0;
+        cum = own;
 #pragma unroll
         for (int off = 1; off < 64; off <<= 1) {
             const int o = __shfl_up(cum, off, 64);
             cum += lane >= off ? o : 0;
         }
-        const int all = __shfl(cum, 63, 64);
-        if (u < before + all || b0 + 64 >= c.batch) {
-            const unsigned long long past = __ballot(before + cum > u);
-            const int l = past ? __builtin_ctzll(past) : 63;
-            return {b0 + l, before + __shfl(cum - own, l, 64), __shfl(own, l, 64) / per};
-        }
-        before += all;
     }
-}
+    // Sequence of unit u < total, its first unit and its pages.
+    struct Place { int b, start, pages; };
+    __device__ Place place(int u) {
+        if (u < before) seek(0, 0);
+        for (;;) {
+            const unsigned long long past = __ballot(before + cum > u);
+            if (past) {
+                const int l = __builtin_ctzll(past);
+                return {b0 + l, __builtin_amdgcn_readlane(before + cum - own, l),
+                        __builtin_amdgcn_readlane(own, l) / per};
+            }
+            const int all = __builtin_amdgcn_readlane(cum, 63);
+            seek(b0 + 64, before + all);
+        }
+    }
+    // Where the cut at unit u comes to lie.
+    __device__ int cut(int u, int share) {
+        if (u >= total) return total;
+        const Place at = place(u);
+        const int lo = at.start + (u - at.start) / at.pages * at.pages, hi = lo + at.pages;
+        return snap(u, lo, hi, share);
+    }
+    __device__ static int snap(int u, int lo, int hi, int share) {
+        const int reach = min(share / 2, kSnap);
+        return u - lo <= reach ? lo : hi - u <= reach ? hi : u;
+    }
+};
 
 template <typename T> __device__ __forceinline__ uint16_t round_to(float x);
 template <> __device__ __forceinline__ uint16_t round_to<bf16_t>(float x) { return f32_to_bf16_bits(x); }
@@ -213,395 +246,379 @@ __device__ __forceinline__ float fade(float m, float ref) {
 }
 
 // Floats of a piece's state in the workspace: outputs as the lanes hold them, then references and sums.
-template <int D, int RT> constexpr int kStateFloats = RT * D + 2 * RT;
+template <int D, int MT> constexpr int kStateFloats = MT * D + 2 * MT;
 
-template <typename T, int D, int RT>
-__global__ __launch_bounds__(kAttnThreads, RT == 16 ? 4 : 2) void kv4_attention_kernel(Kv4AttentionArgs a, Line line,
-                                                                                      float* __restrict__ states) {
-    using S = Shape<D, RT>;
+// What a wave loads of a page.
+template <int D, int MT> struct PageWords {
+    using S = Shape<D, MT>;
+    uint32_t key[2][S::KT][S::KS];
+    uint32_t key_scale[S::KB];
+    uint32_t value[2][S::PF][S::CT];
+    u32x4 value_scale[2][S::PF];
+
+    // Byte offsets of a lane within a page; what differs between its loads is constant,
+    // so that a load is a scalar page address, a lane offset and an immediate.
+    struct Lane {
+        uint32_t key, key_scale, half, value, value_scale;
+        __device__ Lane(int col, int g) {
+            const int r = S::slot_of(0, col);
+            key = r * Kv4<D>::kKeyRow + g * (S::DL / 2);
+            key_scale = Kv4<D>::kKeyScale + 64 * (g * S::DL / 32) + 16 * ((r >> 3) & 3) + 4 * (r & 3);
+            half = 8 * ((r >> 2) & 1);         // key tiles of 32 rows: their slot's byte within the scales
+            value = Kv4<D>::kValue + 4 * (g * D + col * S::VW);
+            value_scale = Kv4<D>::kValueScale + 16 * g;
+        }
+    };
+    __device__ __forceinline__ void load(const uint8_t* page, const Lane& at) {
+        auto word = [&](uint32_t lane_off, int imm) { return reinterpret_cast<const uint32_t*>(page + lane_off + imm); };
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int t = 0; t < S::KT; ++t)
+#pragma unroll
+                for (int k = 0; k < S::KS; ++k) key[s][t][k] = word(at.key, (32 * s + 4 * t) * Kv4<D>::kKeyRow)[k];
+#pragma unroll
+        for (int i = 0; i < S::KB; ++i) key_scale[i] = *word(at.key_scale, 64 * i);
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int f = 0; f < S::PF; ++f) {
+                const int kg = 4 * s + 2 * f;  // past the lane group's own
+#pragma unroll
+                for (int l = 0; l < S::VL; ++l)
+#pragma unroll
+                    for (int i = 0; i < S::VW; ++i)
+                        value[s][f][l * S::VW + i] = word(at.value, 4 * (kg * D + l * MT * S::VW))[i];
+                value_scale[s][f] = *reinterpret_cast<const u32x4*>(word(at.value_scale, 16 * kg));
+            }
+    }
+};
+
+// The rows' state of a wave, and one page's part in it.
+template <typename T, int D, int MT> struct Rows {
+    using S = Shape<D, MT>;
     using F = typename Frag<T>::type;
-    constexpr int MT = S::MT, NR = S::NR;
-    constexpr int kRegs = S::CT * S::ACC;                   // output registers of a row tile
+    F q[S::KS];
+    typename S::Acc o[S::CT];
+    float top, total;          // running maximum (in raw products) and this lane's part of the sum
+    int lim;                   // the row sees slots below it,
+    uint64_t bits;             // and those of the block whose bits are set
+
+    // n, filled: context, and the slots that hold anything; unit: binary logarithms per raw product
+    __device__ __forceinline__ void page(PageWords<D, MT>& w, uint32_t half, int first_slot, int n, int filled,
+                                         int slots, int g, float unit) {
+        const bool masked = first_slot + kKv4Page > n;
+        if (masked) {
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int f = 0; f < S::PF; ++f) {
+                    const int j = first_slot + 32 * s + 8 * (MT == 16 ? g : 2 * f + g);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        w.value_scale[s][f][i] &= (j + 2 * i < filled ? 0xffffu : 0u) |
+                                                  (j + 2 * i + 1 < filled ? 0xffff0000u : 0u);
+                }
+        }
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            // without these fences the scheduler decodes whole pages ahead and spills
+            __builtin_amdgcn_sched_barrier(0);
+            typename S::Acc acc[S::KT];
+#pragma unroll
+            for (int t = 0; t < S::KT; ++t) {
+#pragma unroll
+                for (int i = 0; i < S::ACC; ++i) acc[t][i] = 0.f;
+#pragma unroll
+                for (int k = 0; k < S::KS; ++k) {
+                    const uint32_t scales = w.key_scale[k * 8 / 32 % S::KB] >> (MT == 16 ? 8 * t : half);
+                    const float sc = key_scale<T>(scales, 2 * s);
+                    acc[t] = mma(decode8<T>(w.key[s][t][k], sc), q[k], acc[t]);
+                }
+            }
+            float x[S::PF][8];
+#pragma unroll
+            for (int f = 0; f < S::PF; ++f)
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    x[f][i] = MT == 16 ? acc[i >> 2 & (S::KT - 1)][i & 3] : acc[0][(8 * f + i) % S::ACC];
+            if (masked) {
+#pragma unroll
+                for (int f = 0; f < S::PF; ++f)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int j = first_slot + 32 * s + 8 * (MT == 16 ? g : 2 * f + g) + i, d = j - n;
+                        const bool by_bit = d >= 0 && d < 64 && ((bits >> (d & 63)) & 1) && j < slots;
+                        if (!(j < lim || by_bit)) x[f][i] = -__builtin_inff();
+                    }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            float best = x[0][0];
+#pragma unroll
+            for (int f = 0; f < S::PF; ++f)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) best = fmaxf(best, x[f][i]);
+#pragma unroll
+            for (int off = MT; off < 64; off <<= 1) best = fmaxf(best, __shfl_xor(best, off, 64));
+            if (__any((best - top) * unit > kLag)) {
+                const float now = fmaxf(top, best), f = fade(top * unit, now * unit);
+                top = now;
+                total *= f;
+#pragma unroll
+                for (int t = 0; t < S::CT; ++t)
+#pragma unroll
+                    for (int i = 0; i < S::ACC; ++i) o[t][i] *= f;
+            }
+            const float ref = top == -__builtin_inff() ? 0.f : top * unit;
+#pragma unroll
+            for (int f = 0; f < S::PF; ++f) {
+                __builtin_amdgcn_sched_barrier(0);
+                bf16x8 hi, lo;
+                float sum = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[f][i], unit, -ref));
+                    sum += e;
+                    const uint32_t vs = w.value_scale[s][f][i / 2];
+                    const float v = e * __uint_as_float(i & 1 ? vs & 0xffff0000u : vs << 16);
+                    hi[i] = (__bf16)v;
+                    lo[i] = (__bf16)(v - (float)hi[i]);
+                }
+                total += sum;
+#pragma unroll
+                for (int t = 0; t < S::CT; ++t) {
+                    const bf16x8 vf = decode8<bf16_t>(w.value[s][f][t], 1.f);
+                    o[t] = mma(vf, hi, o[t]);
+                    o[t] = mma(vf, lo, o[t]);
+                }
+            }
+        }
+    }
+};
+
+// A page number, the same for all lanes.
+__device__ __forceinline__ int page_id(const int32_t* row, int p) {
+    return uniform(row[p]);
+}
+
+#ifndef KV4_OCC
+#define KV4_OCC 2
+#endif
+template <typename T, int D, int MT>
+__global__ __launch_bounds__(kAttnThreads, MT == 16 ? KV4_OCC : 2) void kv4_attention_kernel(Kv4AttentionArgs a, Line line,
+                                                                                float* __restrict__ states) {
+    using S = Shape<D, MT>;
+    constexpr int kRegs = S::CT * S::ACC;                   // output registers
     constexpr int kRound = 32;                              // registers joined at a time
     __shared__ float s_o[kAttnWaves][kRound][64];
-    __shared__ float s_m[kAttnWaves][RT], s_l[kAttnWaves][RT];
-    __shared__ F s_q[RT == 64 ? NR * S::KS * 64 : 1];       // queries in operand order (64 rows; else registers)
+    __shared__ float s_m[kAttnWaves][MT], s_l[kAttnWaves][MT];
 
     const Kv4Cache& c = a.cache;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane % MT, g = lane / MT;
-    const int slots = c.slots(), group = a.q_heads / c.heads, per = c.heads * line.tiles;
+    const int slots = c.slots(), group = a.q_heads / c.heads;
     // pieces that follow each other on one XCD: they share pages where a head has several row tiles
     const int piece = (int)gridDim.x % 8 ? (int)blockIdx.x
                                          : (int)(blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8);
-    const int units = line_units(a.block, c, per);
-    const int share = max(line.min_pages, (units + line.pieces - 1) / line.pieces);
-    int u = piece * share;
-    const int u_end = min(units, u + share);
+    const typename PageWords<D, MT>::Lane at_lane(col, g);
+    Scan scan(a.block, c, c.heads * line.tiles);
+    const int share = max(line.min_pages, (scan.total + line.pieces - 1) / line.pieces);
+    if ((int64_t)piece * share >= scan.total) return;
+    int u = scan.cut(piece * share, share);
+    const int u_end = scan.cut((int)min((int64_t)(piece + 1) * share, (int64_t)scan.total), share);
     if (u >= u_end) return;
-    Place at = line_place(a.block, c, per, u);
+    Scan::Place at = scan.place(u);
     // scores in units of the maximum: |scale| and the query's sign
     const float mag = fabsf(a.scale);
     const float unit = (mag == 0.f ? 1.f : mag) * kLog2e * (float)(1 << kKeyShift<T>);
     const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u, zero = mag == 0.f ? 0u : ~0u;
 
     while (u < u_end) {
-        if (u >= at.start + at.pages * per) at = line_place(a.block, c, per, u);
-        const int b = __builtin_amdgcn_readfirstlane(at.b);
+        if (u >= at.start + at.pages * scan.per) at = scan.place(u);
+        const int b = at.b;
         const int rel = u - at.start, ht = rel / at.pages, first = rel - ht * at.pages;
         const int h = ht / line.tiles, rt = ht - h * line.tiles;
         const int last = min(at.pages, first + (u_end - u));
-        const int n = kv4_length(a.block.lengths, b, slots), count = kv4_count(a.block.counts, b, a.block.T);
-        const int filled = seq_end(a.block, b, slots);       // slots past it may hold anything
+        const int n = uniform(kv4_length(a.block.lengths, b, slots));
+        const int count = uniform(kv4_count(a.block.counts, b, a.block.T));
+        const int filled = uniform(seq_end(a.block, b, slots));   // slots past it may hold anything
         int end = filled;
         if (a.block.mode == DELS_KV4_CAUSAL)                  // no row of the tile sees past its last token
-            end = (int)min((int64_t)end, (int64_t)n + (rt * RT + RT - 1) / group + 1);
+            end = (int)min((int64_t)end, (int64_t)n + (rt * MT + MT - 1) / group + 1);
         const int stop = min(last, (end + kKv4Page - 1) / kKv4Page);
 
-        // rows of this lane: the slots below `lim`, and by mask
-        int lim[NR];
-        uint64_t bits[NR];
-        F q[RT == 64 ? 1 : NR * S::KS];
-#pragma unroll
-        for (int nr = 0; nr < NR; ++nr) {
-            const Row row = row_of(rt * RT + nr * MT + col, group, h, a.block.T, count);
-            bits[nr] = 0;
-            lim[nr] = 0;
-            if (row.valid) {
-                lim[nr] = a.block.mode == DELS_KV4_CAUSAL ? n + row.t + 1 : a.block.mode == DELS_KV4_FULL ? n + count : n;
-                if (a.block.mode == DELS_KV4_MASK)
-                    bits[nr] = (uint64_t)a.block.mask[(int64_t)b * a.block.ld_mask + row.t] &
-                               (count >= 64 ? ~0ull : (1ull << count) - 1);
-            }
-            lim[nr] = min(lim[nr], slots);
-            const uint16_t* qp = static_cast<const uint16_t*>(a.q.p) + (int64_t)b * a.q.batch +
-                                 (int64_t)row.t * a.q.token + (int64_t)row.hq * a.q.head + g * S::DL;
-#pragma unroll
-            for (int k = 0; k < S::KS; ++k) {
-                if (RT == 64 && k % kAttnWaves != wave) continue;
-                u32x4 w = {0u, 0u, 0u, 0u};
-                if (row.valid) w = *reinterpret_cast<const u32x4*>(qp + 8 * k);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = (w[i] ^ flip) & zero;
-                if constexpr (RT == 64) s_q[(nr * S::KS + k) * 64 + lane] = __builtin_bit_cast(F, w);
-                else q[nr * S::KS + k] = __builtin_bit_cast(F, w);
-            }
+        // the wave's pages, the next one loaded while one is worked on; a page that the
+        // table does not name is passed over
+        const int32_t* ids = c.table + (int64_t)b * c.ld_table;
+        const uint8_t* heads = c.data + (int64_t)h * Kv4<D>::kBytes;
+        const int64_t page_stride = (int64_t)c.heads * Kv4<D>::kBytes;
+        int p = first + wave;
+        int id_a = p < stop ? page_id(ids, p) : -1, id_b = p + kAttnWaves < stop ? page_id(ids, p + kAttnWaves) : -1;
+
+        const Row row = row_of(rt * MT + col, group, h, a.block.T, count);
+        Rows<T, D, MT> rows;
+        rows.bits = 0;
+        rows.lim = 0;
+        if (row.valid) {
+            rows.lim = a.block.mode == DELS_KV4_CAUSAL ? n + row.t + 1 : a.block.mode == DELS_KV4_FULL ? n + count : n;
+            if (a.block.mode == DELS_KV4_MASK)
+                rows.bits = (uint64_t)a.block.mask[(int64_t)b * a.block.ld_mask + row.t] &
+                            (count >= 64 ? ~0ull : (1ull << count) - 1);
         }
-        if constexpr (RT == 64) __syncthreads();
-
-        typename S::Acc o[NR][S::CT];
-        float top[NR], total[NR];
+        rows.lim = min(rows.lim, slots);
+        const uint16_t* qp = static_cast<const uint16_t*>(a.q.p) + (int64_t)b * a.q.batch +
+                             (int64_t)row.t * a.q.token + (int64_t)row.hq * a.q.head + g * S::DL;
 #pragma unroll
-        for (int nr = 0; nr < NR; ++nr) {
-            top[nr] = -__builtin_inff();
-            total[nr] = 0.f;
+        for (int k = 0; k < S::KS; ++k) {
+            u32x4 w = {0u, 0u, 0u, 0u};
+            if (row.valid) w = *reinterpret_cast<const u32x4*>(qp + 8 * k);
 #pragma unroll
-            for (int t = 0; t < S::CT; ++t)
-#pragma unroll
-                for (int i = 0; i < S::ACC; ++i) o[nr][t][i] = 0.f;
+            for (int i = 0; i < 4; ++i) w[i] = (w[i] ^ flip) & zero;
+            rows.q[k] = __builtin_bit_cast(typename Frag<T>::type, w);
         }
+        rows.top = -__builtin_inff();
+        rows.total = 0.f;
+#pragma unroll
+        for (int t = 0; t < S::CT; ++t)
+#pragma unroll
+            for (int i = 0; i < S::ACC; ++i) rows.o[t][i] = 0.f;
 
-        for (int p = first + wave; p < stop; p += kAttnWaves) {
-            const uint8_t* page = kv4_page(c, b, h, p, Kv4<D>::kBytes);
-            const bool bad = page == nullptr;
-            if (bad) continue;
-            // ---- loads of the page
-            uint32_t kw[2][S::KT][S::KS];
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-#pragma unroll
-                for (int t = 0; t < S::KT; ++t) {
-                    const uint32_t* kp = reinterpret_cast<const uint32_t*>(
-                        page + (32 * s + S::slot_of(t, col)) * Kv4<D>::kKeyRow + g * (S::DL / 2));
-#pragma unroll
-                    for (int k = 0; k < S::KS; ++k) kw[s][t][k] = kp[k];
-                }
-            uint32_t ks[S::KB];
-            {
-                const int blk = g * S::DL / 32;
-                const int r = S::slot_of(0, col);             // its byte position holds for all tiles but the half
-#pragma unroll
-                for (int i = 0; i < S::KB; ++i)
-                    ks[i] = *reinterpret_cast<const uint32_t*>(page + Kv4<D>::kKeyScale + 64 * (blk + i) +
-                                                               16 * ((r >> 3) & 3) + 4 * (r & 3)) >>
-                            (8 * ((r >> 2) & 1));
-            }
-            uint32_t vw[2][S::PF][S::CT];
-            u32x4 vs[2][S::PF];
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-#pragma unroll
-                for (int f = 0; f < S::PF; ++f) {
-                    const int kg = 4 * s + (MT == 16 ? g : 2 * f + g);
-                    const uint32_t* vp = reinterpret_cast<const uint32_t*>(page + Kv4<D>::kValue) + kg * D;
-#pragma unroll
-                    for (int l = 0; l < S::VL; ++l)
-#pragma unroll
-                        for (int i = 0; i < S::VW; ++i) vw[s][f][l * S::VW + i] = vp[l * MT * S::VW + col * S::VW + i];
-                    vs[s][f] = *reinterpret_cast<const u32x4*>(page + Kv4<D>::kValueScale + 16 * kg);
-                }
-            const bool masked = (p + 1) * kKv4Page > n;
-            if (masked) {
-#pragma unroll
-                for (int s = 0; s < 2; ++s)
-#pragma unroll
-                    for (int f = 0; f < S::PF; ++f) {
-                        const int j = p * kKv4Page + 32 * s + 8 * (MT == 16 ? g : 2 * f + g);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            vs[s][f][i] &= (j + 2 * i < filled ? 0xffffu : 0u) | (j + 2 * i + 1 < filled ? 0xffff0000u : 0u);
-                    }
-            }
-
-#pragma unroll
-            for (int s0 = 0; s0 < 2; s0 += S::STEP) {
-                float x[NR][S::STEP][S::PF][8];
-#pragma unroll
-                for (int s = 0; s < S::STEP; ++s) {
-                    typename S::Acc acc[NR][S::KT];
-#pragma unroll
-                    for (int t = 0; t < S::KT; ++t) {
-#pragma unroll
-                        for (int nr = 0; nr < NR; ++nr)
-#pragma unroll
-                            for (int i = 0; i < S::ACC; ++i) acc[nr][t][i] = 0.f;
-#pragma unroll
-                        for (int k = 0; k < S::KS; ++k) {
-                            const float sc = key_scale<T>(ks[k * 8 / 32 % S::KB], 2 * (s0 + s) + (MT == 16 ? t : 0));
-                            const F kf = decode8<T>(kw[s0 + s][t][k], sc);
-#pragma unroll
-                            for (int nr = 0; nr < NR; ++nr) {
-                                if constexpr (RT == 64) acc[nr][t] = mma(kf, s_q[(nr * S::KS + k) * 64 + lane], acc[nr][t]);
-                                else acc[nr][t] = mma(kf, q[nr * S::KS + k], acc[nr][t]);
-                            }
-                        }
-                    }
-#pragma unroll
-                    for (int nr = 0; nr < NR; ++nr)
-#pragma unroll
-                        for (int f = 0; f < S::PF; ++f)
-#pragma unroll
-                            for (int i = 0; i < 8; ++i)
-                                x[nr][s][f][i] = MT == 16 ? acc[nr][i >> 2 & (S::KT - 1)][i & 3]
-                                                          : acc[nr][0][(8 * f + i) % S::ACC];
-                }
-                // slot of x[.][s][f][i]: 64 p + 32 (s0 + s) + 8 kg' + i
-                if (masked) {
-#pragma unroll
-                    for (int nr = 0; nr < NR; ++nr)
-#pragma unroll
-                        for (int s = 0; s < S::STEP; ++s)
-#pragma unroll
-                            for (int f = 0; f < S::PF; ++f)
-#pragma unroll
-                                for (int i = 0; i < 8; ++i) {
-                                    const int j = p * kKv4Page + 32 * (s0 + s) + 8 * (MT == 16 ? g : 2 * f + g) + i;
-                                    const int d = j - n;
-                                    const bool by_bit = d >= 0 && d < 64 && ((bits[nr] >> (d & 63)) & 1) && j < slots;
-                                    if (!(j < lim[nr] || by_bit)) x[nr][s][f][i] = -__builtin_inff();
-                                }
-                }
-#pragma unroll
-                for (int nr = 0; nr < NR; ++nr) {
-                    float best = x[nr][0][0][0];
-#pragma unroll
-                    for (int s = 0; s < S::STEP; ++s)
-#pragma unroll
-                        for (int f = 0; f < S::PF; ++f)
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) best = fmaxf(best, x[nr][s][f][i]);
-#pragma unroll
-                    for (int off = MT; off < 64; off <<= 1) best = fmaxf(best, __shfl_xor(best, off, 64));
-                    if (__any((best - top[nr]) * unit > kLag)) {
-                        const float now = fmaxf(top[nr], best), f = fade(top[nr] * unit, now * unit);
-                        top[nr] = now;
-                        total[nr] *= f;
-#pragma unroll
-                        for (int t = 0; t < S::CT; ++t)
-#pragma unroll
-                            for (int i = 0; i < S::ACC; ++i) o[nr][t][i] *= f;
-                    }
-                }
-                float ref[NR];
-#pragma unroll
-                for (int nr = 0; nr < NR; ++nr)
-                    ref[nr] = top[nr] == -__builtin_inff() ? 0.f : top[nr] * unit;
-#pragma unroll
-                for (int s = 0; s < S::STEP; ++s)
-#pragma unroll
-                    for (int f = 0; f < S::PF; ++f) {
-                        bf16x8 hi[NR], lo[NR];
-#pragma unroll
-                        for (int nr = 0; nr < NR; ++nr) {
-                            float sum = 0.f;
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) {
-                                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[nr][s][f][i], unit, -ref[nr]));
-                                sum += e;
-                                const uint32_t w = vs[s0 + s][f][i / 2];
-                                const float v = e * __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16);
-                                hi[nr][i] = (__bf16)v;
-                                lo[nr][i] = (__bf16)(v - (float)hi[nr][i]);
-                            }
-                            total[nr] += sum;
-                        }
-#pragma unroll
-                        for (int t = 0; t < S::CT; ++t) {
-                            const bf16x8 vf = decode8<bf16_t>(vw[s0 + s][f][t], 1.f);
-#pragma unroll
-                            for (int nr = 0; nr < NR; ++nr) {
-                                o[nr][t] = mma(vf, hi[nr], o[nr][t]);
-                                o[nr][t] = mma(vf, lo[nr], o[nr][t]);
-                            }
-                        }
-                    }
-            }
+        auto named = [&](int id) { return id >= 0 && id < c.num_pages; };
+        auto next_id = [&](int at_page) { return at_page < stop ? page_id(ids, at_page) : -1; };
+        PageWords<D, MT> wa, wb;
+        if (named(id_a)) wa.load(heads + id_a * page_stride, at_lane);
+        for (; p < stop; p += 2 * kAttnWaves) {
+            if (named(id_b)) wb.load(heads + id_b * page_stride, at_lane);
+            const bool do_a = named(id_a), do_b = named(id_b);
+            id_a = next_id(p + 2 * kAttnWaves);
+            id_b = next_id(p + 3 * kAttnWaves);
+            if (do_a) rows.page(wa, at_lane.half, p * kKv4Page, n, filled, slots, g, unit);
+            if (named(id_a)) wa.load(heads + id_a * page_stride, at_lane);
+            if (do_b) rows.page(wb, at_lane.half, (p + kAttnWaves) * kKv4Page, n, filled, slots, g, unit);
         }
 
         // ---- join the waves
-        float ref[NR];
+        const float ref = rows.top * unit;
+        float total = rows.total;
 #pragma unroll
-        for (int nr = 0; nr < NR; ++nr) {
-            ref[nr] = top[nr] * unit;
-#pragma unroll
-            for (int off = MT; off < 64; off <<= 1) total[nr] += __shfl_xor(total[nr], off, 64);
-            if (g == 0) {
-                s_m[wave][nr * MT + col] = ref[nr];
-                s_l[wave][nr * MT + col] = total[nr];
-            }
+        for (int off = MT; off < 64; off <<= 1) total += __shfl_xor(total, off, 64);
+        if (g == 0) {
+            s_m[wave][col] = ref;
+            s_l[wave][col] = total;
         }
         __syncthreads();
         const bool whole = first == 0 && last == at.pages;
-        float* state = states + (int64_t)(2 * piece + (first == 0 ? 1 : 0)) * kStateFloats<D, RT>;
+        float* state = states + (int64_t)(2 * piece + (first == 0 ? 1 : 0)) * kStateFloats<D, MT>;
+        float m = -__builtin_inff(), l = 0.f;
 #pragma unroll
-        for (int nr = 0; nr < NR; ++nr) {
-            float m = -__builtin_inff(), l = 0.f;
+        for (int w = 0; w < kAttnWaves; ++w) m = fmaxf(m, s_m[w][col]);
 #pragma unroll
-            for (int w = 0; w < kAttnWaves; ++w) m = fmaxf(m, s_m[w][nr * MT + col]);
+        for (int w = 0; w < kAttnWaves; ++w) l += s_l[w][col] * fade(s_m[w][col], m);
+        const float f = fade(ref, m), inv = l > 0.f ? 1.f / l : 0.f;
 #pragma unroll
-            for (int w = 0; w < kAttnWaves; ++w) l += s_l[w][nr * MT + col] * fade(s_m[w][nr * MT + col], m);
-            const float f = fade(ref[nr], m), inv = l > 0.f ? 1.f / l : 0.f;
-            const Row row = row_of(rt * RT + nr * MT + col, group, h, a.block.T, count);
+        for (int r0 = 0; r0 < kRegs; r0 += kRound) {
+            // register (vl, i, v): channel block, row of the tile, channel of the VW
 #pragma unroll
-            for (int r0 = 0; r0 < kRegs; r0 += kRound) {
-                // register (vl, i, v) of the tile: channel block, row of the tile, channel of the VW
-#pragma unroll
-                for (int j = 0; j < kRound && r0 + j < kRegs; ++j) {
-                    const int r = r0 + j, v = r % S::VW, i = r / S::VW % S::ACC, vl = r / S::VW / S::ACC;
-                    s_o[wave][j][lane] = o[nr][vl * S::VW + v][i] * f;
-                }
-                __syncthreads();
-                for (int jg = wave; jg * S::VW < kRound && r0 + jg * S::VW < kRegs; jg += kAttnWaves) {
-                    float sum[S::VW];
-#pragma unroll
-                    for (int v = 0; v < S::VW; ++v) {
-                        sum[v] = 0.f;
-#pragma unroll
-                        for (int w = 0; w < kAttnWaves; ++w) sum[v] += s_o[w][jg * S::VW + v][lane];
-                    }
-                    const int gi = r0 / S::VW + jg, i = gi % S::ACC, vl = gi / S::ACC;
-                    if (whole) {
-                        store_out<T, S::VW>(a, b, row, S::channel_of(vl, i, g), sum, inv);
-                    } else {
-                        float* to = state + ((nr * (kRegs / S::VW) + gi) * 64 + lane) * S::VW;
-#pragma unroll
-                        for (int v = 0; v < S::VW; ++v) to[v] = sum[v];
-                    }
-                }
-                __syncthreads();
+            for (int j = 0; j < kRound && r0 + j < kRegs; ++j) {
+                const int r = r0 + j, v = r % S::VW, i = r / S::VW % S::ACC, vl = r / S::VW / S::ACC;
+                s_o[wave][j][lane] = rows.o[vl * S::VW + v][i] * f;
             }
-            if (wave == 0 && g == 0) {
-                if (whole) {
-                    store_lse(a, b, row, m, l);
-                } else {
-                    state[RT * D + nr * MT + col] = m;
-                    state[RT * D + RT + nr * MT + col] = l;
+            __syncthreads();
+            for (int jg = wave; jg * S::VW < kRound && r0 + jg * S::VW < kRegs; jg += kAttnWaves) {
+                float sum[S::VW];
+#pragma unroll
+                for (int v = 0; v < S::VW; ++v) {
+                    sum[v] = 0.f;
+#pragma unroll
+                    for (int w = 0; w < kAttnWaves; ++w) sum[v] += s_o[w][jg * S::VW + v][lane];
                 }
+                const int gi = r0 / S::VW + jg;
+                if (whole) {
+                    store_out<T, S::VW>(a, b, row, S::channel_of(gi / S::ACC, gi % S::ACC, g), sum, inv);
+                } else {
+                    float* to = state + (gi * 64 + lane) * S::VW;
+#pragma unroll
+                    for (int v = 0; v < S::VW; ++v) to[v] = sum[v];
+                }
+            }
+            __syncthreads();
+        }
+        if (wave == 0 && g == 0) {
+            if (whole) {
+                store_lse(a, b, row, m, l);
+            } else {
+                state[MT * D + col] = m;
+                state[MT * D + MT + col] = l;
             }
         }
-        __syncthreads();
         u += last - first;
     }
 }
 
-// Joins the states of the rows whose pages lie in several pieces: one workgroup
-// per (sequence, head, row tile), lanes as in the kernel above.
-template <typename T, int D, int RT>
-__global__ __launch_bounds__(kAttnThreads) void kv4_join_kernel(Kv4AttentionArgs a, Line line,
-                                                                const float* __restrict__ states) {
-    using S = Shape<D, RT>;
-    constexpr int MT = S::MT, NR = S::NR, kRegs = S::CT * S::ACC;
+// Joins the states of the rows whose pages lie in several pieces.  Grid (sequence x
+// head x row tile, quarter of the output registers), a wave per VW channels.
+constexpr int kJoinWaves = 4;
+template <typename T, int D, int MT>
+__global__ __launch_bounds__(64 * kJoinWaves) void kv4_join_kernel(Kv4AttentionArgs a, Line line,
+                                                                   const float* __restrict__ states) {
+    using S = Shape<D, MT>;
     const Kv4Cache& c = a.cache;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane % MT, g = lane / MT;
     const int per = c.heads * line.tiles, group = a.q_heads / c.heads;
     const int b = blockIdx.x / per, ht = blockIdx.x % per, h = ht / line.tiles, rt = ht % line.tiles;
-    const int units = line_units(a.block, c, per);
-    const int share = max(line.min_pages, (units + line.pieces - 1) / line.pieces);
-    // units before sequence b
-    int before = 0;
+    Scan scan(a.block, c, per);
+    const int share = max(line.min_pages, (scan.total + line.pieces - 1) / line.pieces);
+    int before = 0;                                         // pages of the sequences before b
     for (int i = lane; i < b; i += 64) before += seq_pages(a.block, i, c.slots());
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) before += __shfl_xor(before, off, 64);
     const int pages = seq_pages(a.block, b, c.slots());
-    const int u0 = before * per + ht * pages, u1 = u0 + pages;
-    const int w0 = u0 / share, w1 = (u1 - 1) / share;
-    if (w0 == w1) return;                                   // one piece covered them and wrote the output
-    const int count = kv4_count(a.block.counts, b, a.block.T);
-    auto state_of = [&](int w) {
-        return states + (int64_t)(2 * w + (w * share <= u0 ? 1 : 0)) * kStateFloats<D, RT>;
-    };
+    const int lo = before * per + ht * pages, hi = lo + pages;
+    // cuts w0 .. w1 - 1 stay inside; the piece before the first has the tile's first pages
+    int w0 = (lo + share - 1) / share, w1 = (hi - 1) / share + 1;
+    while (w0 < w1 && Scan::snap(w0 * share, lo, hi, share) == lo) ++w0;
+    while (w0 < w1 && Scan::snap((w1 - 1) * share, lo, hi, share) == hi) --w1;
+    if (w0 >= w1) return;                                   // one piece covered them and wrote the output
+    auto state_of = [&](int w) { return states + (int64_t)(2 * w + (w < w0 ? 1 : 0)) * kStateFloats<D, MT>; };
+    float m = -__builtin_inff(), l = 0.f;
+#pragma unroll 4
+    for (int w = w0 - 1; w < w1; ++w) m = fmaxf(m, state_of(w)[MT * D + col]);
+    const int gi = blockIdx.y * kJoinWaves + wave;
+    float sum[S::VW];
 #pragma unroll
-    for (int nr = 0; nr < NR; ++nr) {
-        const int r = nr * MT + col;
-        float m = -__builtin_inff(), l = 0.f;
-        for (int w = w0; w <= w1; ++w) m = fmaxf(m, state_of(w)[RT * D + r]);
-        for (int w = w0; w <= w1; ++w) {
-            const float* st = state_of(w);
-            l += st[RT * D + RT + r] * fade(st[RT * D + r], m);
-        }
-        const float inv = l > 0.f ? 1.f / l : 0.f;
-        const Row row = row_of(rt * RT + r, group, h, a.block.T, count);
-        for (int gi = wave; gi < kRegs / S::VW; gi += kAttnWaves) {
-            float sum[S::VW];
+    for (int v = 0; v < S::VW; ++v) sum[v] = 0.f;
+#pragma unroll 4
+    for (int w = w0 - 1; w < w1; ++w) {
+        const float* st = state_of(w);
+        const float f = fade(st[MT * D + col], m);
+        l += st[MT * D + MT + col] * f;
+        const float* from = st + (gi * 64 + lane) * S::VW;
 #pragma unroll
-            for (int v = 0; v < S::VW; ++v) sum[v] = 0.f;
-            for (int w = w0; w <= w1; ++w) {
-                const float* st = state_of(w);
-                const float f = fade(st[RT * D + r], m);
-                const float* from = st + ((nr * (kRegs / S::VW) + gi) * 64 + lane) * S::VW;
-#pragma unroll
-                for (int v = 0; v < S::VW; ++v) sum[v] += from[v] * f;
-            }
-            store_out<T, S::VW>(a, b, row, S::channel_of(gi / S::ACC, gi % S::ACC, g), sum, inv);
-        }
-        if (wave == 0 && g == 0) store_lse(a, b, row, m, l);
+        for (int v = 0; v < S::VW; ++v) sum[v] += from[v] * f;
     }
+    const Row row = row_of(rt * MT + col, group, h, a.block.T, kv4_count(a.block.counts, b, a.block.T));
+    store_out<T, S::VW>(a, b, row, S::channel_of(gi / S::ACC, gi % S::ACC, g), sum, l > 0.f ? 1.f / l : 0.f);
+    if (gi == 0 && g == 0) store_lse(a, b, row, m, l);
 }
 
-int rows_of(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
-
-struct Plan { int rt; Line line; bool split; };
+struct Plan { int rows; Line line; };
 
 Plan plan(int64_t batch, int64_t T, int64_t q_heads, int64_t heads, int64_t max_pages) {
     Plan p{};
     const int64_t rows = T * (q_heads / heads);
-    p.rt = rows_of(rows);
-    p.line.tiles = (int)((rows + p.rt - 1) / p.rt);
+    p.rows = rows <= 16 ? 16 : 32;
+    p.line.tiles = (int)((rows + p.rows - 1) / p.rows);
     p.line.min_pages = kAttnWaves;
     const int64_t units = batch * heads * p.line.tiles * std::max<int64_t>(max_pages, 1);
-    const int64_t slots = (int64_t)device_cu_count() * (p.rt == 16 ? 2 : 1);
-    p.line.pieces = (int)std::min<int64_t>(slots, (units + p.line.min_pages - 1) / p.line.min_pages);
-    p.split = true;
+    const int64_t resident = (int64_t)device_cu_count() * (p.rows == 16 ? KV4_OCC / 2 : 1);
+    p.line.pieces = (int)std::min<int64_t>(resident, (units + p.line.min_pages - 1) / p.line.min_pages);
     return p;
 }
 
-template <int RT> size_t state_bytes(int64_t D) { return sizeof(float) * (RT * D + 2 * RT); }
-
-template <typename F> hipError_t by_type(int dtype, int head_dim, int rt, F&& f) {
+template <typename F> hipError_t by_type(int dtype, int head_dim, int rows, F&& f) {
     auto by_rows = [&](auto tag, auto size) {
-        if (rt == 16) f(tag, size, std::integral_constant<int, 16>{});
-        else if (rt == 32) f(tag, size, std::integral_constant<int, 32>{});
-        else f(tag, size, std::integral_constant<int, 64>{});
+        if (rows == 16) f(tag, size, std::integral_constant<int, 16>{});
+        else f(tag, size, std::integral_constant<int, 32>{});
     };
     auto by_size = [&](auto tag) {
         if (head_dim == 64) by_rows(tag, std::integral_constant<int, 64>{});
@@ -617,20 +634,23 @@ template <typename F> hipError_t by_type(int dtype, int head_dim, int rt, F&& f)
 size_t kv4_attention_data_bytes(int64_t batch, int64_t T, int64_t q_heads, int64_t heads, int64_t head_dim,
                                 int64_t max_pages) {
     const Plan p = plan(batch, T, q_heads, heads, max_pages);
-    return align256((size_t)p.line.pieces * 2 * sizeof(float) * (p.rt * head_dim + 2 * p.rt));
+    return align256((size_t)p.line.pieces * 2 * sizeof(float) * (p.rows * head_dim + 2 * p.rows));
 }
 
 hipError_t launch_kv4_attention(const Kv4AttentionArgs& a, void* ws, size_t data_off, hipStream_t s) {
     const Kv4Cache& c = a.cache;
     const Plan p = plan(c.batch, a.block.T, a.q_heads, c.heads, c.max_pages);
     auto* states = reinterpret_cast<float*>(static_cast<char*>(ws) + data_off);
-    return by_type(a.dtype, c.head_dim, p.rt, [&](auto tag, auto size, auto rows) {
+    return by_type(a.dtype, c.head_dim, p.rows, [&](auto tag, auto size, auto rows) {
         using T = decltype(tag);
-        constexpr int D = decltype(size)::value, RT = decltype(rows)::value;
-        hipLaunchKernelGGL((kv4_attention_kernel<T, D, RT>), dim3(p.line.pieces), dim3(kAttnThreads), 0, s, a, p.line,
+        constexpr int D = decltype(size)::value, MT = decltype(rows)::value;
+        using S = Shape<D, MT>;
+        static_assert(S::CT * S::ACC / S::VW % kJoinWaves == 0, "a wave of the join per VW channels");
+        hipLaunchKernelGGL((kv4_attention_kernel<T, D, MT>), dim3(p.line.pieces), dim3(kAttnThreads), 0, s, a, p.line,
                            states);
-        hipLaunchKernelGGL((kv4_join_kernel<T, D, RT>), dim3((unsigned)c.batch * c.heads * p.line.tiles),
-                           dim3(kAttnThreads), 0, s, a, p.line, states);
+        hipLaunchKernelGGL((kv4_join_kernel<T, D, MT>),
+                           dim3((unsigned)c.batch * c.heads * p.line.tiles, S::CT * S::ACC / S::VW / kJoinWaves),
+                           dim3(64 * kJoinWaves), 0, s, a, p.line, states);
     });
 }
 
