@@ -64,6 +64,12 @@ template <> __device__ __forceinline__ f16x8 decode8<f16_t>(uint32_t w, float sc
     return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
+// Two numbers rounded to bf16, the first in the low half.
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
+}
+
 __device__ __forceinline__ f32x4 mma(bf16x8 a, bf16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
@@ -248,37 +254,46 @@ __device__ __forceinline__ float fade(float m, float ref) {
 // Floats of a piece's state in the workspace: outputs as the lanes hold them, then references and sums.
 template <int D, int MT> constexpr int kStateFloats = MT * D + 2 * MT;
 
-// What a wave loads of a page.
-template <int D, int MT> struct PageWords {
-    using S = Shape<D, MT>;
-    uint32_t key[2][S::KT][S::KS];
-    uint32_t key_scale[S::KB];
-    uint32_t value[2][S::PF][S::CT];
-    u32x4 value_scale[2][S::PF];
+// Byte offsets of a lane within a page; what differs between its loads is constant, so
+// that a load is a page address, a lane offset and an immediate.
+template <int D, int MT> struct LaneOffsets {
+    uint32_t key, key_scale, half, value, value_scale;
+    __device__ LaneOffsets(int col, int g) {
+        using S = Shape<D, MT>;
+        const int r = S::slot_of(0, col);
+        key = r * Kv4<D>::kKeyRow + g * (S::DL / 2);
+        key_scale = Kv4<D>::kKeyScale + 64 * (g * S::DL / 32) + 16 * ((r >> 3) & 3) + 4 * (r & 3);
+        half = 8 * ((r >> 2) & 1);         // key tiles of 32 rows: their slot's byte within the scales
+        value = Kv4<D>::kValue + 4 * (g * D + col * S::VW);
+        value_scale = Kv4<D>::kValueScale + 16 * g;
+    }
+};
+__device__ __forceinline__ const uint32_t* page_word(const uint8_t* page, uint32_t lane_off, int imm) {
+    return reinterpret_cast<const uint32_t*>(page + lane_off + imm);
+}
 
-    // Byte offsets of a lane within a page; what differs between its loads is constant,
-    // so that a load is a scalar page address, a lane offset and an immediate.
-    struct Lane {
-        uint32_t key, key_scale, half, value, value_scale;
-        __device__ Lane(int col, int g) {
-            const int r = S::slot_of(0, col);
-            key = r * Kv4<D>::kKeyRow + g * (S::DL / 2);
-            key_scale = Kv4<D>::kKeyScale + 64 * (g * S::DL / 32) + 16 * ((r >> 3) & 3) + 4 * (r & 3);
-            half = 8 * ((r >> 2) & 1);         // key tiles of 32 rows: their slot's byte within the scales
-            value = Kv4<D>::kValue + 4 * (g * D + col * S::VW);
-            value_scale = Kv4<D>::kValueScale + 16 * g;
-        }
-    };
-    __device__ __forceinline__ void load(const uint8_t* page, const Lane& at) {
-        auto word = [&](uint32_t lane_off, int imm) { return reinterpret_cast<const uint32_t*>(page + lane_off + imm); };
+// What a wave loads of a page: keys, and values.
+template <int D, int MT> struct KeyWords {
+    using S = Shape<D, MT>;
+    uint32_t code[2][S::KT][S::KS];
+    uint32_t scale[S::KB];
+    __device__ __forceinline__ void load(const uint8_t* page, const LaneOffsets<D, MT>& at) {
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
             for (int t = 0; t < S::KT; ++t)
 #pragma unroll
-                for (int k = 0; k < S::KS; ++k) key[s][t][k] = word(at.key, (32 * s + 4 * t) * Kv4<D>::kKeyRow)[k];
+                for (int k = 0; k < S::KS; ++k)
+                    code[s][t][k] = page_word(page, at.key, (32 * s + 4 * t) * Kv4<D>::kKeyRow)[k];
 #pragma unroll
-        for (int i = 0; i < S::KB; ++i) key_scale[i] = *word(at.key_scale, 64 * i);
+        for (int i = 0; i < S::KB; ++i) scale[i] = *page_word(page, at.key_scale, 64 * i);
+    }
+};
+template <int D, int MT> struct ValueWords {
+    using S = Shape<D, MT>;
+    uint32_t code[2][S::PF][S::CT];
+    u32x4 scale[2][S::PF];
+    __device__ __forceinline__ void load(const uint8_t* page, const LaneOffsets<D, MT>& at) {
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
@@ -288,8 +303,8 @@ template <int D, int MT> struct PageWords {
                 for (int l = 0; l < S::VL; ++l)
 #pragma unroll
                     for (int i = 0; i < S::VW; ++i)
-                        value[s][f][l * S::VW + i] = word(at.value, 4 * (kg * D + l * MT * S::VW))[i];
-                value_scale[s][f] = *reinterpret_cast<const u32x4*>(word(at.value_scale, 16 * kg));
+                        code[s][f][l * S::VW + i] = page_word(page, at.value, 4 * (kg * D + l * MT * S::VW))[i];
+                scale[s][f] = *reinterpret_cast<const u32x4*>(page_word(page, at.value_scale, 16 * kg));
             }
     }
 };
@@ -304,11 +319,12 @@ template <typename T, int D, int MT> struct Rows {
     int lim;                   // the row sees slots below it,
     uint64_t bits;             // and those of the block whose bits are set
 
-    // n, filled: context, and the slots that hold anything; unit: binary logarithms per raw product
-    __device__ __forceinline__ void page(PageWords<D, MT>& w, uint32_t half, int first_slot, int n, int filled,
-                                         int slots, int g, float unit) {
-        const bool masked = first_slot + kKv4Page > n;
-        if (masked) {
+    // n, filled: context, and the slots that hold anything; unit: binary logarithms per
+    // raw product.  MASKED: the page reaches past the context.
+    template <bool MASKED>
+    __device__ __forceinline__ void page(const KeyWords<D, MT>& keys, ValueWords<D, MT>& values, uint32_t half,
+                                         int first_slot, int n, int filled, int slots, int g, float unit) {
+        if constexpr (MASKED) {
 #pragma unroll
             for (int s = 0; s < 2; ++s)
 #pragma unroll
@@ -316,7 +332,7 @@ template <typename T, int D, int MT> struct Rows {
                     const int j = first_slot + 32 * s + 8 * (MT == 16 ? g : 2 * f + g);
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        w.value_scale[s][f][i] &= (j + 2 * i < filled ? 0xffffu : 0u) |
+                        values.scale[s][f][i] &= (j + 2 * i < filled ? 0xffffu : 0u) |
                                                   (j + 2 * i + 1 < filled ? 0xffff0000u : 0u);
                 }
         }
@@ -331,9 +347,9 @@ template <typename T, int D, int MT> struct Rows {
                 for (int i = 0; i < S::ACC; ++i) acc[t][i] = 0.f;
 #pragma unroll
                 for (int k = 0; k < S::KS; ++k) {
-                    const uint32_t scales = w.key_scale[k * 8 / 32 % S::KB] >> (MT == 16 ? 8 * t : half);
+                    const uint32_t scales = keys.scale[k * 8 / 32 % S::KB] >> (MT == 16 ? 8 * t : half);
                     const float sc = key_scale<T>(scales, 2 * s);
-                    acc[t] = mma(decode8<T>(w.key[s][t][k], sc), q[k], acc[t]);
+                    acc[t] = mma(decode8<T>(keys.code[s][t][k], sc), q[k], acc[t]);
                 }
             }
             float x[S::PF][8];
@@ -342,7 +358,7 @@ template <typename T, int D, int MT> struct Rows {
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
                     x[f][i] = MT == 16 ? acc[i >> 2 & (S::KT - 1)][i & 3] : acc[0][(8 * f + i) % S::ACC];
-            if (masked) {
+            if constexpr (MASKED) {
 #pragma unroll
                 for (int f = 0; f < S::PF; ++f)
 #pragma unroll
@@ -373,23 +389,25 @@ template <typename T, int D, int MT> struct Rows {
 #pragma unroll
             for (int f = 0; f < S::PF; ++f) {
                 __builtin_amdgcn_sched_barrier(0);
-                bf16x8 hi, lo;
+                u32x4 hi, lo;
                 float sum = 0.f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[f][i], unit, -ref));
-                    sum += e;
-                    const uint32_t vs = w.value_scale[s][f][i / 2];
-                    const float v = e * __uint_as_float(i & 1 ? vs & 0xffff0000u : vs << 16);
-                    hi[i] = (__bf16)v;
-                    lo[i] = (__bf16)(v - (float)hi[i]);
+                for (int i = 0; i < 4; ++i) {
+                    const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[f][2 * i], unit, -ref));
+                    const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[f][2 * i + 1], unit, -ref));
+                    sum += e0;
+                    sum += e1;
+                    const uint32_t vs = values.scale[s][f][i];
+                    const float v0 = e0 * __uint_as_float(vs << 16), v1 = e1 * __uint_as_float(vs & 0xffff0000u);
+                    hi[i] = pack_bf16(v0, v1);
+                    lo[i] = pack_bf16(v0 - __uint_as_float(hi[i] << 16), v1 - __uint_as_float(hi[i] & 0xffff0000u));
                 }
                 total += sum;
 #pragma unroll
                 for (int t = 0; t < S::CT; ++t) {
-                    const bf16x8 vf = decode8<bf16_t>(w.value[s][f][t], 1.f);
-                    o[t] = mma(vf, hi, o[t]);
-                    o[t] = mma(vf, lo, o[t]);
+                    const bf16x8 vf = decode8<bf16_t>(values.code[s][f][t], 1.f);
+                    o[t] = mma(vf, __builtin_bit_cast(bf16x8, hi), o[t]);
+                    o[t] = mma(vf, __builtin_bit_cast(bf16x8, lo), o[t]);
                 }
             }
         }
@@ -420,7 +438,7 @@ __global__ __launch_bounds__(kAttnThreads, MT == 16 ? KV4_OCC : 2) void kv4_atte
     // pieces that follow each other on one XCD: they share pages where a head has several row tiles
     const int piece = (int)gridDim.x % 8 ? (int)blockIdx.x
                                          : (int)(blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8);
-    const typename PageWords<D, MT>::Lane at_lane(col, g);
+    const LaneOffsets<D, MT> at_lane(col, g);
     Scan scan(a.block, c, c.heads * line.tiles);
     const int share = max(line.min_pages, (scan.total + line.pieces - 1) / line.pieces);
     if ((int64_t)piece * share >= scan.total) return;
@@ -447,13 +465,11 @@ __global__ __launch_bounds__(kAttnThreads, MT == 16 ? KV4_OCC : 2) void kv4_atte
             end = (int)min((int64_t)end, (int64_t)n + (rt * MT + MT - 1) / group + 1);
         const int stop = min(last, (end + kKv4Page - 1) / kKv4Page);
 
-        // the wave's pages, the next one loaded while one is worked on; a page that the
-        // table does not name is passed over
+        // the wave's pages, the next one loaded while one is worked on
         const int32_t* ids = c.table + (int64_t)b * c.ld_table;
         const uint8_t* heads = c.data + (int64_t)h * Kv4<D>::kBytes;
         const int64_t page_stride = (int64_t)c.heads * Kv4<D>::kBytes;
         int p = first + wave;
-        int id_a = p < stop ? page_id(ids, p) : -1, id_b = p + kAttnWaves < stop ? page_id(ids, p + kAttnWaves) : -1;
 
         const Row row = row_of(rt * MT + col, group, h, a.block.T, count);
         Rows<T, D, MT> rows;
@@ -484,18 +500,33 @@ __global__ __launch_bounds__(kAttnThreads, MT == 16 ? KV4_OCC : 2) void kv4_atte
             for (int i = 0; i < S::ACC; ++i) rows.o[t][i] = 0.f;
 
         auto named = [&](int id) { return id >= 0 && id < c.num_pages; };
-        auto next_id = [&](int at_page) { return at_page < stop ? page_id(ids, at_page) : -1; };
-        PageWords<D, MT> wa, wb;
-        if (named(id_a)) wa.load(heads + id_a * page_stride, at_lane);
-        for (; p < stop; p += 2 * kAttnWaves) {
-            if (named(id_b)) wb.load(heads + id_b * page_stride, at_lane);
-            const bool do_a = named(id_a), do_b = named(id_b);
-            id_a = next_id(p + 2 * kAttnWaves);
-            id_b = next_id(p + 3 * kAttnWaves);
-            if (do_a) rows.page(wa, at_lane.half, p * kKv4Page, n, filled, slots, g, unit);
-            if (named(id_a)) wa.load(heads + id_a * page_stride, at_lane);
-            if (do_b) rows.page(wb, at_lane.half, (p + kAttnWaves) * kKv4Page, n, filled, slots, g, unit);
-        }
+        KeyWords<D, MT> ka, kb;
+        // pages p, p + 8, ... below `to`; one that the table does not name is passed over.
+        // Keys are loaded a page ahead, values at the start of their page's work.
+        auto walk = [&](auto masked, int to) {
+            auto next_id = [&](int at_page) { return at_page < to ? page_id(ids, at_page) : -1; };
+            int id_a = next_id(p), id_b = next_id(p + kAttnWaves);
+            if (named(id_a)) ka.load(heads + id_a * page_stride, at_lane);
+            auto work = [&](int id, const KeyWords<D, MT>& k, int next, KeyWords<D, MT>& nk, int at_page) {
+                ValueWords<D, MT> values;
+                if (named(id)) values.load(heads + id * page_stride, at_lane);
+                if (named(next)) nk.load(heads + next * page_stride, at_lane);
+                if (named(id))
+                    rows.template page<decltype(masked)::value>(k, values, at_lane.half, at_page * kKv4Page, n, filled,
+                                                                slots, g, unit);
+            };
+            for (; p < to; p += 2 * kAttnWaves) {
+                const int id_c = next_id(p + 2 * kAttnWaves), id_d = next_id(p + 3 * kAttnWaves);
+                work(id_a, ka, id_b, kb, p);
+                work(id_b, kb, id_c, ka, p + kAttnWaves);
+                id_a = id_c;
+                id_b = id_d;
+            }
+        };
+        const int inside = min(stop, n / kKv4Page);            // pages of context alone
+        walk(std::integral_constant<bool, false>{}, inside);
+        p = max(inside, first) + (wave + kAttnWaves - max(inside - first, 0) % kAttnWaves) % kAttnWaves;
+        walk(std::integral_constant<bool, true>{}, stop);
 
         // ---- join the waves
         const float ref = rows.top * unit;
