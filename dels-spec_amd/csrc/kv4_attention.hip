@@ -336,10 +336,10 @@ template <typename T, int D, int MT> struct Rows {
                                                   (j + 2 * i + 1 < filled ? 0xffff0000u : 0u);
                 }
         }
+        // scores of the page's 64 slots; unit u = (half, operand) holds slots 32 s + 8 kg .. + 7
+        float x[2 * S::PF][8];
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            // without these fences the scheduler decodes whole pages ahead and spills
-            __builtin_amdgcn_sched_barrier(0);
             typename S::Acc acc[S::KT];
 #pragma unroll
             for (int t = 0; t < S::KT; ++t) {
@@ -348,75 +348,83 @@ template <typename T, int D, int MT> struct Rows {
 #pragma unroll
                 for (int k = 0; k < S::KS; ++k) {
                     const uint32_t scales = keys.scale[k * 8 / 32 % S::KB] >> (MT == 16 ? 8 * t : half);
-                    const float sc = key_scale<T>(scales, 2 * s);
-                    acc[t] = mma(decode8<T>(keys.code[s][t][k], sc), q[k], acc[t]);
+                    acc[t] = mma(decode8<T>(keys.code[s][t][k], key_scale<T>(scales, 2 * s)), q[k], acc[t]);
                 }
             }
-            float x[S::PF][8];
 #pragma unroll
             for (int f = 0; f < S::PF; ++f)
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    x[f][i] = MT == 16 ? acc[i >> 2 & (S::KT - 1)][i & 3] : acc[0][(8 * f + i) % S::ACC];
-            if constexpr (MASKED) {
+                    x[s * S::PF + f][i] = MT == 16 ? acc[i >> 2 & (S::KT - 1)][i & 3] : acc[0][(8 * f + i) % S::ACC];
+        }
+        // without this fence the scheduler decodes values ahead of the scores and spills
+        __builtin_amdgcn_sched_barrier(0);
+        float best = -__builtin_inff();
 #pragma unroll
-                for (int f = 0; f < S::PF; ++f)
+        for (int u = 0; u < 2 * S::PF; ++u)
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int j = first_slot + 32 * s + 8 * (MT == 16 ? g : 2 * f + g) + i, d = j - n;
-                        const bool by_bit = d >= 0 && d < 64 && ((bits >> (d & 63)) & 1) && j < slots;
-                        if (!(j < lim || by_bit)) x[f][i] = -__builtin_inff();
-                    }
+            for (int i = 0; i < 8; ++i) {
+                if constexpr (MASKED) {
+                    const int j = first_slot + 32 * (u / S::PF) + 8 * (MT == 16 ? g : 2 * (u % S::PF) + g) + i, d = j - n;
+                    const bool by_bit = d >= 0 && d < 64 && ((bits >> (d & 63)) & 1) && j < slots;
+                    if (!(j < lim || by_bit)) x[u][i] = -__builtin_inff();
+                }
+                best = fmaxf(best, x[u][i]);
             }
+#pragma unroll
+        for (int off = MT; off < 64; off <<= 1) best = fmaxf(best, __shfl_xor(best, off, 64));
+        if (__any((best - top) * unit > kLag)) {
+            const float now = fmaxf(top, best), f = fade(top * unit, now * unit);
+            top = now;
+            total *= f;
+#pragma unroll
+            for (int t = 0; t < S::CT; ++t)
+#pragma unroll
+                for (int i = 0; i < S::ACC; ++i) o[t][i] *= f;
+        }
+        const float ref = top == -__builtin_inff() ? 0.f : top * unit;
+        // the weights of a unit are made while the one before multiplies the values: eight
+        // matrix instructions with the vector ones of a unit spread between them
+        u32x4 hi[2], lo[2];
+        auto weigh = [&](int u) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[u][2 * i], unit, -ref));
+                const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[u][2 * i + 1], unit, -ref));
+                total += e0;
+                total += e1;
+                const uint32_t vs = values.scale[u / S::PF][u % S::PF][i];
+                const float v0 = e0 * __uint_as_float(vs << 16), v1 = e1 * __uint_as_float(vs & 0xffff0000u);
+                hi[u & 1][i] = pack_bf16(v0, v1);
+                lo[u & 1][i] = pack_bf16(v0 - __uint_as_float(hi[u & 1][i] << 16),
+                                         v1 - __uint_as_float(hi[u & 1][i] & 0xffff0000u));
+            }
+        };
+        weigh(0);
+#pragma unroll
+        for (int u = 0; u < 2 * S::PF; ++u) {
             __builtin_amdgcn_sched_barrier(0);
-            float best = x[0][0];
+            if (u + 1 < 2 * S::PF) weigh(u + 1);
 #pragma unroll
-            for (int f = 0; f < S::PF; ++f)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) best = fmaxf(best, x[f][i]);
-#pragma unroll
-            for (int off = MT; off < 64; off <<= 1) best = fmaxf(best, __shfl_xor(best, off, 64));
-            if (__any((best - top) * unit > kLag)) {
-                const float now = fmaxf(top, best), f = fade(top * unit, now * unit);
-                top = now;
-                total *= f;
-#pragma unroll
-                for (int t = 0; t < S::CT; ++t)
-#pragma unroll
-                    for (int i = 0; i < S::ACC; ++i) o[t][i] *= f;
+            for (int t = 0; t < S::CT; ++t) {
+                const bf16x8 vf = decode8<bf16_t>(values.code[u / S::PF][u % S::PF][t], 1.f);
+                o[t] = mma(vf, __builtin_bit_cast(bf16x8, hi[u & 1]), o[t]);
+                o[t] = mma(vf, __builtin_bit_cast(bf16x8, lo[u & 1]), o[t]);
             }
-            const float ref = top == -__builtin_inff() ? 0.f : top * unit;
 #pragma unroll
-            for (int f = 0; f < S::PF; ++f) {
-                __builtin_amdgcn_sched_barrier(0);
-                u32x4 hi, lo;
-                float sum = 0.f;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[f][2 * i], unit, -ref));
-                    const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[f][2 * i + 1], unit, -ref));
-                    sum += e0;
-                    sum += e1;
-                    const uint32_t vs = values.scale[s][f][i];
-                    const float v0 = e0 * __uint_as_float(vs << 16), v1 = e1 * __uint_as_float(vs & 0xffff0000u);
-                    hi[i] = pack_bf16(v0, v1);
-                    lo[i] = pack_bf16(v0 - __uint_as_float(hi[i] << 16), v1 - __uint_as_float(hi[i] & 0xffff0000u));
-                }
-                total += sum;
-#pragma unroll
-                for (int t = 0; t < S::CT; ++t) {
-                    const bf16x8 vf = decode8<bf16_t>(values.code[s][f][t], 1.f);
-                    o[t] = mma(vf, __builtin_bit_cast(bf16x8, hi), o[t]);
-                    o[t] = mma(vf, __builtin_bit_cast(bf16x8, lo), o[t]);
-                }
+            for (int i = 0; i < 2 * S::CT; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x002, MT == 16 ? 5 : 11, 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
             }
         }
+        __builtin_amdgcn_sched_barrier(0);
     }
 };
 
-// A page number, the same for all lanes.
+// A page number, the same for all lanes: a scalar load, so that its arrival is not
+// waited for together with the loads of a page.
 __device__ __forceinline__ int page_id(const int32_t* row, int p) {
-    return uniform(row[p]);
+    return *(const __attribute__((address_space(4))) int32_t*)(uintptr_t)(row + p);
 }
 
 #ifndef KV4_OCC
@@ -501,16 +509,22 @@ __global__ __launch_bounds__(kAttnThreads, MT == 16 ? KV4_OCC : 2) void kv4_atte
 
         auto named = [&](int id) { return id >= 0 && id < c.num_pages; };
         KeyWords<D, MT> ka, kb;
-        // pages p, p + 8, ... below `to`; one that the table does not name is passed over.
-        // Keys are loaded a page ahead, values at the start of their page's work.
+        // Pages p, p + 8, ... below `to`; one that the table does not name is passed over.
+        // Keys are loaded a page ahead, values at the start of their page's work.  The
+        // loads are unconditional (of page 0 where there is none to load), so that each
+        // wait covers only what it needs.
         auto walk = [&](auto masked, int to) {
             auto next_id = [&](int at_page) { return at_page < to ? page_id(ids, at_page) : -1; };
+            auto address = [&](int id) { return heads + (named(id) ? id : 0) * page_stride; };
+            if (p >= to) return;
             int id_a = next_id(p), id_b = next_id(p + kAttnWaves);
-            if (named(id_a)) ka.load(heads + id_a * page_stride, at_lane);
+            ka.load(address(id_a), at_lane);
             auto work = [&](int id, const KeyWords<D, MT>& k, int next, KeyWords<D, MT>& nk, int at_page) {
                 ValueWords<D, MT> values;
-                if (named(id)) values.load(heads + id * page_stride, at_lane);
-                if (named(next)) nk.load(heads + next * page_stride, at_lane);
+                values.load(address(id), at_lane);
+                asm volatile("" ::: "memory");                 // in this order: the values' wait leaves the keys in flight
+                nk.load(address(next), at_lane);
+                asm volatile("" ::: "memory");
                 if (named(id))
                     rows.template page<decltype(masked)::value>(k, values, at_lane.half, at_page * kKv4Page, n, filled,
                                                                 slots, g, unit);
