@@ -313,18 +313,20 @@ template <int D, int MT> struct ValueWords {
 template <typename T, int D, int MT> struct Rows {
     using S = Shape<D, MT>;
     using F = typename Frag<T>::type;
-    F q[S::KS];
     typename S::Acc o[S::CT];
     float top, total;          // running maximum (in raw products) and this lane's part of the sum
     int lim;                   // the row sees slots below it,
     uint64_t bits;             // and those of the block whose bits are set
 
-    // n, filled: context, and the slots that hold anything; unit: binary logarithms per
-    // raw product.  MASKED: the page reaches past the context.
-    template <bool MASKED>
-    __device__ __forceinline__ void page(const KeyWords<D, MT>& keys, ValueWords<D, MT>& values, uint32_t half,
+    // n, filled: context, and the slots that hold anything; unit: binary logarithms per raw product
+    // q: this lane's operands of the queries in LDS, 64 apart
+    __device__ __forceinline__ void page(const F* q, const KeyWords<D, MT>& keys, ValueWords<D, MT>& values, uint32_t half,
                                          int first_slot, int n, int filled, int slots, int g, float unit) {
-        if constexpr (MASKED) {
+        // a page that reaches past the context (a branch: the statement keeps the compiler from
+        // computing the masks of every page and selecting)
+        const bool masked = first_slot + kKv4Page > n;
+        if (masked) {
+            asm volatile("");
 #pragma unroll
             for (int s = 0; s < 2; ++s)
 #pragma unroll
@@ -337,40 +339,52 @@ template <typename T, int D, int MT> struct Rows {
                 }
         }
         // scores of the page's 64 slots; unit u = (half, operand) holds slots 32 s + 8 kg .. + 7
-        float x[2 * S::PF][8];
+        typename S::Acc acc[2][S::KT];
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            typename S::Acc acc[S::KT];
+        for (int s = 0; s < 2; ++s)
 #pragma unroll
-            for (int t = 0; t < S::KT; ++t) {
+            for (int t = 0; t < S::KT; ++t)
 #pragma unroll
-                for (int i = 0; i < S::ACC; ++i) acc[t][i] = 0.f;
+                for (int i = 0; i < S::ACC; ++i) acc[s][t][i] = 0.f;
 #pragma unroll
-                for (int k = 0; k < S::KS; ++k) {
+        for (int k = 0; k < S::KS; ++k) {
+            const F qk = q[64 * k];
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int t = 0; t < S::KT; ++t) {
                     const uint32_t scales = keys.scale[k * 8 / 32 % S::KB] >> (MT == 16 ? 8 * t : half);
-                    acc[t] = mma(decode8<T>(keys.code[s][t][k], key_scale<T>(scales, 2 * s)), q[k], acc[t]);
+                    acc[s][t] = mma(decode8<T>(keys.code[s][t][k], key_scale<T>(scales, 2 * s)), qk, acc[s][t]);
                 }
-            }
-#pragma unroll
-            for (int f = 0; f < S::PF; ++f)
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    x[s * S::PF + f][i] = MT == 16 ? acc[i >> 2 & (S::KT - 1)][i & 3] : acc[0][(8 * f + i) % S::ACC];
         }
-        // without this fence the scheduler decodes values ahead of the scores and spills
-        __builtin_amdgcn_sched_barrier(0);
-        float best = -__builtin_inff();
+        float x[2 * S::PF][8];
 #pragma unroll
         for (int u = 0; u < 2 * S::PF; ++u)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if constexpr (MASKED) {
-                    const int j = first_slot + 32 * (u / S::PF) + 8 * (MT == 16 ? g : 2 * (u % S::PF) + g) + i, d = j - n;
-                    const bool by_bit = d >= 0 && d < 64 && ((bits >> (d & 63)) & 1) && j < slots;
-                    if (!(j < lim || by_bit)) x[u][i] = -__builtin_inff();
-                }
-                best = fmaxf(best, x[u][i]);
+            for (int i = 0; i < 8; ++i)
+                x[u][i] = MT == 16 ? acc[u / S::PF][i >> 2 & (S::KT - 1)][i & 3]
+                                   : acc[u / S::PF][0][(8 * (u % S::PF) + i) % S::ACC];
+        // without this fence the scheduler decodes values ahead of the scores and spills
+        __builtin_amdgcn_sched_barrier(0);
+        if (masked) {
+            asm volatile("");
+#pragma unroll
+            for (int u = 0; u < 2 * S::PF; ++u) {
+                const int j0 = first_slot + 32 * (u / S::PF) + 8 * (MT == 16 ? g : 2 * (u % S::PF) + g);
+                // the slots that the row sees by its mask, the first one in bit 0
+                const int d = j0 - n;
+                uint32_t by_bit = d >= 64 || d <= -8 ? 0u : (uint32_t)(d >= 0 ? bits >> d : bits << -d) & 255u;
+                by_bit &= slots - j0 >= 8 ? 255u : (1u << max(slots - j0, 0)) - 1u;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (j0 + i >= lim && !(by_bit >> i & 1u)) x[u][i] = -__builtin_inff();
             }
+        }
+        float best = x[0][0];
+#pragma unroll
+        for (int u = 0; u < 2 * S::PF; ++u)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) best = fmaxf(best, x[u][i]);
 #pragma unroll
         for (int off = MT; off < 64; off <<= 1) best = fmaxf(best, __shfl_xor(best, off, 64));
         if (__any((best - top) * unit > kLag)) {
@@ -383,38 +397,42 @@ template <typename T, int D, int MT> struct Rows {
                 for (int i = 0; i < S::ACC; ++i) o[t][i] *= f;
         }
         const float ref = top == -__builtin_inff() ? 0.f : top * unit;
-        // the weights of a unit are made while the one before multiplies the values: eight
-        // matrix instructions with the vector ones of a unit spread between them
+        // The weights of a unit are made while the one before multiplies the values: between
+        // two matrix instructions stand about as many cycles of vector ones, in this order
+        // (the fences keep it), so that neither waits for the other.
         u32x4 hi[2], lo[2];
-        auto weigh = [&](int u) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[u][2 * i], unit, -ref));
-                const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[u][2 * i + 1], unit, -ref));
-                total += e0;
-                total += e1;
-                const uint32_t vs = values.scale[u / S::PF][u % S::PF][i];
-                const float v0 = e0 * __uint_as_float(vs << 16), v1 = e1 * __uint_as_float(vs & 0xffff0000u);
-                hi[u & 1][i] = pack_bf16(v0, v1);
-                lo[u & 1][i] = pack_bf16(v0 - __uint_as_float(hi[u & 1][i] << 16),
-                                         v1 - __uint_as_float(hi[u & 1][i] & 0xffff0000u));
+        float even = 0.f;
+        auto weigh = [&](int u, int i) {
+            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[u][i], unit, -ref));
+            total += e;
+            const uint32_t vs = values.scale[u / S::PF][u % S::PF][i / 2];
+            const float v = e * __uint_as_float(i & 1 ? vs & 0xffff0000u : vs << 16);
+            if (i % 2 == 0) {
+                even = v;
+            } else {
+                const uint32_t h = pack_bf16(even, v);
+                hi[u & 1][i / 2] = h;
+                lo[u & 1][i / 2] = pack_bf16(even - __uint_as_float(h << 16), v - __uint_as_float(h & 0xffff0000u));
             }
         };
-        weigh(0);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) weigh(0, i);
 #pragma unroll
         for (int u = 0; u < 2 * S::PF; ++u) {
-            __builtin_amdgcn_sched_barrier(0);
-            if (u + 1 < 2 * S::PF) weigh(u + 1);
+            const bool more = u + 1 < 2 * S::PF;
+            constexpr int kFirst = S::CT >= 8 ? 0 : 4 / S::CT;     // weights before a tile's first product,
+            constexpr int kBoth = 8 / S::CT;                       // and before its second
 #pragma unroll
             for (int t = 0; t < S::CT; ++t) {
                 const bf16x8 vf = decode8<bf16_t>(values.code[u / S::PF][u % S::PF][t], 1.f);
-                o[t] = mma(vf, __builtin_bit_cast(bf16x8, hi[u & 1]), o[t]);
-                o[t] = mma(vf, __builtin_bit_cast(bf16x8, lo[u & 1]), o[t]);
-            }
 #pragma unroll
-            for (int i = 0; i < 2 * S::CT; ++i) {
-                __builtin_amdgcn_sched_group_barrier(0x002, MT == 16 ? 5 : 11, 0);
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                for (int i = t * kBoth; more && i < t * kBoth + kFirst; ++i) weigh(u + 1, i);
+                __builtin_amdgcn_sched_barrier(0);
+                o[t] = mma(vf, __builtin_bit_cast(bf16x8, hi[u & 1]), o[t]);
+#pragma unroll
+                for (int i = t * kBoth + kFirst; more && i < (t + 1) * kBoth; ++i) weigh(u + 1, i);
+                __builtin_amdgcn_sched_barrier(0);
+                o[t] = mma(vf, __builtin_bit_cast(bf16x8, lo[u & 1]), o[t]);
             }
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -438,6 +456,8 @@ __global__ __launch_bounds__(kAttnThreads, MT == 16 ? KV4_OCC : 2) void kv4_atte
     constexpr int kRound = 32;                              // registers joined at a time
     __shared__ float s_o[kAttnWaves][kRound][64];
     __shared__ float s_m[kAttnWaves][MT], s_l[kAttnWaves][MT];
+    __shared__ typename Frag<T>::type s_q[S::KS][64];
+    static_assert(S::KS <= kAttnWaves, "a wave per step of the first product loads the queries");
 
     const Kv4Cache& c = a.cache;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -490,15 +510,16 @@ __global__ __launch_bounds__(kAttnThreads, MT == 16 ? KV4_OCC : 2) void kv4_atte
                             (count >= 64 ? ~0ull : (1ull << count) - 1);
         }
         rows.lim = min(rows.lim, slots);
-        const uint16_t* qp = static_cast<const uint16_t*>(a.q.p) + (int64_t)b * a.q.batch +
-                             (int64_t)row.t * a.q.token + (int64_t)row.hq * a.q.head + g * S::DL;
-#pragma unroll
-        for (int k = 0; k < S::KS; ++k) {
+        // the queries, in operand order: a wave loads what all of them read
+        if (wave < S::KS) {
             u32x4 w = {0u, 0u, 0u, 0u};
-            if (row.valid) w = *reinterpret_cast<const u32x4*>(qp + 8 * k);
+            if (row.valid)
+                w = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q.p) + (int64_t)b * a.q.batch +
+                                                    (int64_t)row.t * a.q.token + (int64_t)row.hq * a.q.head +
+                                                    g * S::DL + 8 * wave);
 #pragma unroll
             for (int i = 0; i < 4; ++i) w[i] = (w[i] ^ flip) & zero;
-            rows.q[k] = __builtin_bit_cast(typename Frag<T>::type, w);
+            s_q[wave][lane] = __builtin_bit_cast(typename Frag<T>::type, w);
         }
         rows.top = -__builtin_inff();
         rows.total = 0.f;
@@ -507,40 +528,32 @@ __global__ __launch_bounds__(kAttnThreads, MT == 16 ? KV4_OCC : 2) void kv4_atte
 #pragma unroll
             for (int i = 0; i < S::ACC; ++i) rows.o[t][i] = 0.f;
 
+        __syncthreads();
         auto named = [&](int id) { return id >= 0 && id < c.num_pages; };
-        KeyWords<D, MT> ka, kb;
-        // Pages p, p + 8, ... below `to`; one that the table does not name is passed over.
+        // Pages p, p + 8, ... below `stop`; one that the table does not name is passed over.
         // Keys are loaded a page ahead, values at the start of their page's work.  The
-        // loads are unconditional (of page 0 where there is none to load), so that each
-        // wait covers only what it needs.
-        auto walk = [&](auto masked, int to) {
-            auto next_id = [&](int at_page) { return at_page < to ? page_id(ids, at_page) : -1; };
-            auto address = [&](int id) { return heads + (named(id) ? id : 0) * page_stride; };
-            if (p >= to) return;
-            int id_a = next_id(p), id_b = next_id(p + kAttnWaves);
-            ka.load(address(id_a), at_lane);
-            auto work = [&](int id, const KeyWords<D, MT>& k, int next, KeyWords<D, MT>& nk, int at_page) {
-                ValueWords<D, MT> values;
+        // loads are unconditional (of page 0 where there is none to load) and in this
+        // order, so that each wait covers only what it needs.  One copy of the work: two
+        // that swap the keys' registers take longer to fetch than their moves.
+        auto next_id = [&](int at_page) { return at_page < stop ? page_id(ids, at_page) : -1; };
+        auto address = [&](int id) { return heads + (named(id) ? id : 0) * page_stride; };
+        if (p < stop) {
+            KeyWords<D, MT> keys, next_keys;
+            ValueWords<D, MT> values;
+            int id = next_id(p), next = next_id(p + kAttnWaves);
+            keys.load(address(id), at_lane);
+            for (; p < stop; p += kAttnWaves) {
                 values.load(address(id), at_lane);
-                asm volatile("" ::: "memory");                 // in this order: the values' wait leaves the keys in flight
-                nk.load(address(next), at_lane);
                 asm volatile("" ::: "memory");
-                if (named(id))
-                    rows.template page<decltype(masked)::value>(k, values, at_lane.half, at_page * kKv4Page, n, filled,
-                                                                slots, g, unit);
-            };
-            for (; p < to; p += 2 * kAttnWaves) {
-                const int id_c = next_id(p + 2 * kAttnWaves), id_d = next_id(p + 3 * kAttnWaves);
-                work(id_a, ka, id_b, kb, p);
-                work(id_b, kb, id_c, ka, p + kAttnWaves);
-                id_a = id_c;
-                id_b = id_d;
+                next_keys.load(address(next), at_lane);
+                asm volatile("" ::: "memory");
+                const int after = next_id(p + 2 * kAttnWaves);
+                if (named(id)) rows.page(&s_q[0][lane], keys, values, at_lane.half, p * kKv4Page, n, filled, slots, g, unit);
+                keys = next_keys;
+                id = next;
+                next = after;
             }
-        };
-        const int inside = min(stop, n / kKv4Page);            // pages of context alone
-        walk(std::integral_constant<bool, false>{}, inside);
-        p = max(inside, first) + (wave + kAttnWaves - max(inside - first, 0) % kAttnWaves) % kAttnWaves;
-        walk(std::integral_constant<bool, true>{}, stop);
+        }
 
         // ---- join the waves
         const float ref = rows.top * unit;
