@@ -24,100 +24,22 @@
 // writes their output, others write their state, which kv4_join_kernel joins.
 #include <algorithm>
 
-#include "../../include/dels.h"
-#include "kv4.h"
+#include "kv4_mma.h"
 
 namespace dels {
 
 namespace {
 
-constexpr int kAttnWaves = 8;
-constexpr int kAttnThreads = 64 * kAttnWaves;
-constexpr float kLog2e = 1.44269504088896340736f;
 // A row's running maximum follows only when a score passes it by this many binary
 // orders: until then the weights are at most 2^8, which costs fp32 nothing, and the
 // outputs need no rescaling.
 constexpr float kLag = 8.f;
-
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-
-template <typename T> struct Frag;
-template <> struct Frag<bf16_t> { using type = bf16x8; };
-template <> struct Frag<f16_t> { using type = f16x8; };
-
-// Eight codes times a power of two.
-template <typename T> __device__ __forceinline__ typename Frag<T>::type decode8(uint32_t w, float scale);
-template <> __device__ __forceinline__ bf16x8 decode8<bf16_t>(uint32_t w, float scale) {
-    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0);
-    const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1);
-    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2);
-    const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3);
-    return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-}
-template <> __device__ __forceinline__ f16x8 decode8<f16_t>(uint32_t w, float scale) {
-    const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 0);
-    const f16x2 b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 1);
-    const f16x2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 2);
-    const f16x2 d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 3);
-    return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-}
 
 // Two numbers rounded to bf16, the first in the low half.
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
     typedef float f32x2 __attribute__((ext_vector_type(2)));
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
 }
-
-__device__ __forceinline__ f32x4 mma(bf16x8 a, bf16x8 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-}
-__device__ __forceinline__ f32x4 mma(f16x8 a, f16x8 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-}
-__device__ __forceinline__ f32x16 mma(bf16x8 a, bf16x8 b, f32x16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
-}
-__device__ __forceinline__ f32x16 mma(f16x8 a, f16x8 b, f32x16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
-}
-
-// fp16 holds keys of up to 2^20 at a sixteenth of their size; the scale makes up for it.
-template <typename T> constexpr int kKeyShift = 0;
-template <> constexpr int kKeyShift<f16_t> = 4;
-
-template <typename T>
-__device__ __forceinline__ float key_scale(uint32_t word, int byte) {
-    const int e = (int)((word >> (8 * byte)) & 255u);
-    return __uint_as_float((uint32_t)max(e - kKeyShift<T>, 0) << 23);
-}
-
-// Shapes of a wave's work on MT rows: MT x MT tiles of the matrix instructions.
-template <int D, int MT_> struct Shape {
-    static constexpr int MT = MT_;
-    static constexpr int NG = 64 / MT;              // lane groups: lane = MT * group + row
-    static constexpr int DL = D / NG;               // channels of a key that a lane holds
-    static constexpr int KS = DL / 8;               // steps of the first product
-    static constexpr int KB = DL >= 32 ? DL / 32 : 1;   // key scales per lane
-    static constexpr int KT = 32 / MT;              // key tiles of 32 slots
-    static constexpr int ACC = MT == 16 ? 4 : 16;   // accumulator registers of a tile
-    static constexpr int PF = 32 * MT / 64 / 8;     // weight operands (8 slots) per 32 slots
-    static constexpr int CT = D / MT;               // channel tiles of the output
-    static constexpr int VW = MT == 16 ? 4 : D / 32;    // consecutive channels of a lane: words of a load
-    static constexpr int VL = CT / VW;              // loads of value words per operand
-    using Acc = typename std::conditional<MT == 16, f32x4, f32x16>::type;
-    // slot within 32 that row r of key tile a holds
-    __device__ static int slot_of(int a, int r) {
-        if constexpr (MT == 16) return 8 * (r >> 2) + 4 * a + (r & 3);
-        return 16 * (r >> 4) + 8 * ((r >> 2) & 1) + 4 * ((r >> 3) & 1) + (r & 3);
-    }
-    // first of the VW channels that register i of a tile holds in channel block `vl`
-    __device__ static int channel_of(int vl, int i, int g) {
-        const int row = MT == 16 ? 4 * g + i : 8 * (i >> 2) + 4 * g + (i & 3);
-        return vl * MT * VW + row * VW;
-    }
-};
 
 // The line of pages: those of (b, h, row tile) one after the other, b first.  It is
 // cut every `share` pages; a cut within `snap` pages of a row tile's end moves there,
@@ -129,78 +51,17 @@ struct Line {
 };
 constexpr int kSnap = 8;       // one page for each wave
 
-__device__ __forceinline__ int seq_end(const Kv4Block& k, int b, int slots) {
-    const int n = kv4_length(k.lengths, b, slots);
-    if (k.mode == DELS_KV4_NONE) return n;
-    return (int)min((int64_t)slots, (int64_t)n + kv4_count(k.counts, b, k.T));
+// Where the cut at unit u comes to lie; lo, hi: the ends of the row tile that holds it.
+__device__ __forceinline__ int snap(int u, int lo, int hi, int share) {
+    const int reach = min(share / 2, kSnap);
+    return u - lo <= reach ? lo : hi - u <= reach ? hi : u;
 }
-// Pages of sequence b (one at least: rows that see nothing are written too).
-__device__ __forceinline__ int seq_pages(const Kv4Block& k, int b, int slots) {
-    return max(1, (seq_end(k, b, slots) + kKv4Page - 1) / kKv4Page);
+__device__ __forceinline__ int cut(Scan& scan, int u, int share) {
+    if (u >= scan.total) return scan.total;
+    const Scan::Place at = scan.place(u);
+    const int lo = at.start + (u - at.start) / at.pages * at.pages;
+    return snap(u, lo, lo + at.pages, share);
 }
-
-// What all lanes of a wave hold alike, kept in a scalar register.
-__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
-
-// Scan of the sequences' units by a wave, 64 at a time; up to 64 it is kept.
-struct Scan {
-    const Kv4Block& k;
-    const Kv4Cache& c;
-    int per;                   // row tiles of a sequence
-    int own, cum;              // units of this lane's sequence, and of all up to it, in the 64 from b0
-    int b0, before, total;
-
-    __device__ Scan(const Kv4Block& k_, const Kv4Cache& c_, int per_) : k(k_), c(c_), per(per_) {
-        seek(0, 0);
-        total = __builtin_amdgcn_readlane(cum, 63);
-        for (int b = 64 + (threadIdx.x & 63), rest = 0; c.batch > 64; b += 64) {
-            rest += b < c.batch ? seq_pages(k, b, c.slots()) * per : 0;
-            if ((b & ~63) + 64 >= c.batch) {
-#pragma unroll
-                for (int off = 1; off < 64; off <<= 1) rest += __shfl_xor(rest, off, 64);
-                total += uniform(rest);
-                break;
-            }
-        }
-    }
-    __device__ void seek(int b0_, int before_) {
-        const int lane = threadIdx.x & 63;
-        b0 = b0_, before = before_;
-        own = b0 + lane < c.batch ? seq_pages(k, b0 + lane, c.slots()) * per : 0;
-        cum = own;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const int o = __shfl_up(cum, off, 64);
-            cum += lane >= off ? o : 0;
-        }
-    }
-    // Sequence of unit u < total, its first unit and its pages.
-    struct Place { int b, start, pages; };
-    __device__ Place place(int u) {
-        if (u < before) seek(0, 0);
-        for (;;) {
-            const unsigned long long past = __ballot(before + cum > u);
-            if (past) {
-                const int l = __builtin_ctzll(past);
-                return {b0 + l, __builtin_amdgcn_readlane(before + cum - own, l),
-                        __builtin_amdgcn_readlane(own, l) / per};
-            }
-            const int all = __builtin_amdgcn_readlane(cum, 63);
-            seek(b0 + 64, before + all);
-        }
-    }
-    // Where the cut at unit u comes to lie.
-    __device__ int cut(int u, int share) {
-        if (u >= total) return total;
-        const Place at = place(u);
-        const int lo = at.start + (u - at.start) / at.pages * at.pages, hi = lo + at.pages;
-        return snap(u, lo, hi, share);
-    }
-    __device__ static int snap(int u, int lo, int hi, int share) {
-        const int reach = min(share / 2, kSnap);
-        return u - lo <= reach ? lo : hi - u <= reach ? hi : u;
-    }
-};
 
 template <typename T> __device__ __forceinline__ uint16_t round_to(float x);
 template <> __device__ __forceinline__ uint16_t round_to<bf16_t>(float x) { return f32_to_bf16_bits(x); }
@@ -254,41 +115,6 @@ __device__ __forceinline__ float fade(float m, float ref) {
 // Floats of a piece's state in the workspace: outputs as the lanes hold them, then references and sums.
 template <int D, int MT> constexpr int kStateFloats = MT * D + 2 * MT;
 
-// Byte offsets of a lane within a page; what differs between its loads is constant, so
-// that a load is a page address, a lane offset and an immediate.
-template <int D, int MT> struct LaneOffsets {
-    uint32_t key, key_scale, half, value, value_scale;
-    __device__ LaneOffsets(int col, int g) {
-        using S = Shape<D, MT>;
-        const int r = S::slot_of(0, col);
-        key = r * Kv4<D>::kKeyRow + g * (S::DL / 2);
-        key_scale = Kv4<D>::kKeyScale + 64 * (g * S::DL / 32) + 16 * ((r >> 3) & 3) + 4 * (r & 3);
-        half = 8 * ((r >> 2) & 1);         // key tiles of 32 rows: their slot's byte within the scales
-        value = Kv4<D>::kValue + 4 * (g * D + col * S::VW);
-        value_scale = Kv4<D>::kValueScale + 16 * g;
-    }
-};
-__device__ __forceinline__ const uint32_t* page_word(const uint8_t* page, uint32_t lane_off, int imm) {
-    return reinterpret_cast<const uint32_t*>(page + lane_off + imm);
-}
-
-// What a wave loads of a page: keys, and values.
-template <int D, int MT> struct KeyWords {
-    using S = Shape<D, MT>;
-    uint32_t code[2][S::KT][S::KS];
-    uint32_t scale[S::KB];
-    __device__ __forceinline__ void load(const uint8_t* page, const LaneOffsets<D, MT>& at) {
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int t = 0; t < S::KT; ++t)
-#pragma unroll
-                for (int k = 0; k < S::KS; ++k)
-                    code[s][t][k] = page_word(page, at.key, (32 * s + 4 * t) * Kv4<D>::kKeyRow)[k];
-#pragma unroll
-        for (int i = 0; i < S::KB; ++i) scale[i] = *page_word(page, at.key_scale, 64 * i);
-    }
-};
 template <int D, int MT> struct ValueWords {
     using S = Shape<D, MT>;
     uint32_t code[2][S::PF][S::CT];
@@ -346,9 +172,12 @@ template <typename T, int D, int MT> struct Rows {
             for (int t = 0; t < S::KT; ++t)
 #pragma unroll
                 for (int i = 0; i < S::ACC; ++i) acc[s][t][i] = 0.f;
+        F next_q = q[0];
 #pragma unroll
         for (int k = 0; k < S::KS; ++k) {
-            const F qk = q[64 * k];
+            const F qk = next_q;
+            if (k + 1 < S::KS) next_q = q[64 * (k + 1)];       // read a step ahead
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int s = 0; s < 2; ++s)
 #pragma unroll
@@ -385,8 +214,7 @@ template <typename T, int D, int MT> struct Rows {
         for (int u = 0; u < 2 * S::PF; ++u)
 #pragma unroll
             for (int i = 0; i < 8; ++i) best = fmaxf(best, x[u][i]);
-#pragma unroll
-        for (int off = MT; off < 64; off <<= 1) best = fmaxf(best, __shfl_xor(best, off, 64));
+        best = max_over_groups<MT>(best);
         if (__any((best - top) * unit > kLag)) {
             const float now = fmaxf(top, best), f = fade(top * unit, now * unit);
             top = now;
@@ -439,25 +267,16 @@ template <typename T, int D, int MT> struct Rows {
     }
 };
 
-// A page number, the same for all lanes: a scalar load, so that its arrival is not
-// waited for together with the loads of a page.
-__device__ __forceinline__ int page_id(const int32_t* row, int p) {
-    return *(const __attribute__((address_space(4))) int32_t*)(uintptr_t)(row + p);
-}
-
-#ifndef KV4_OCC
-#define KV4_OCC 2
-#endif
 template <typename T, int D, int MT>
-__global__ __launch_bounds__(kAttnThreads, MT == 16 ? KV4_OCC : 2) void kv4_attention_kernel(Kv4AttentionArgs a, Line line,
+__global__ __launch_bounds__(kKv4Threads, 2) void kv4_attention_kernel(Kv4AttentionArgs a, Line line,
                                                                                 float* __restrict__ states) {
     using S = Shape<D, MT>;
     constexpr int kRegs = S::CT * S::ACC;                   // output registers
     constexpr int kRound = 32;                              // registers joined at a time
-    __shared__ float s_o[kAttnWaves][kRound][64];
-    __shared__ float s_m[kAttnWaves][MT], s_l[kAttnWaves][MT];
+    __shared__ float s_o[kKv4Waves][kRound][64];
+    __shared__ float s_m[kKv4Waves][MT], s_l[kKv4Waves][MT];
     __shared__ typename Frag<T>::type s_q[S::KS][64];
-    static_assert(S::KS <= kAttnWaves, "a wave per step of the first product loads the queries");
+    static_assert(S::KS <= kKv4Waves, "a wave per step of the first product loads the queries");
 
     const Kv4Cache& c = a.cache;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -470,8 +289,8 @@ __global__ __launch_bounds__(kAttnThreads, MT == 16 ? KV4_OCC : 2) void kv4_atte
     Scan scan(a.block, c, c.heads * line.tiles);
     const int share = max(line.min_pages, (scan.total + line.pieces - 1) / line.pieces);
     if ((int64_t)piece * share >= scan.total) return;
-    int u = scan.cut(piece * share, share);
-    const int u_end = scan.cut((int)min((int64_t)(piece + 1) * share, (int64_t)scan.total), share);
+    int u = cut(scan, piece * share, share);
+    const int u_end = cut(scan, (int)min((int64_t)(piece + 1) * share, (int64_t)scan.total), share);
     if (u >= u_end) return;
     Scan::Place at = scan.place(u);
     // scores in units of the maximum: |scale| and the query's sign
@@ -535,31 +354,41 @@ __global__ __launch_bounds__(kAttnThreads, MT == 16 ? KV4_OCC : 2) void kv4_atte
         // loads are unconditional (of page 0 where there is none to load) and in this
         // order, so that each wait covers only what it needs.  One copy of the work: two
         // that swap the keys' registers take longer to fetch than their moves.
-        auto next_id = [&](int at_page) { return at_page < stop ? page_id(ids, at_page) : -1; };
         auto address = [&](int id) { return heads + (named(id) ? id : 0) * page_stride; };
         if (p < stop) {
+            // the numbers of the wave's next 64 pages, one a lane: a load per page would be
+            // waited for with the first read of LDS
+            int ids64 = -1, base = 0;
+            auto fetch_ids = [&](int from) {
+                base = from;
+                const int at_page = from + lane * kKv4Waves;
+                ids64 = at_page < stop ? ids[at_page] : -1;
+            };
+            auto id_at = [&](int at_page) {
+                if (at_page - base >= 64 * kKv4Waves) fetch_ids(at_page);
+                return __builtin_amdgcn_readlane(ids64, (at_page - base) / kKv4Waves);
+            };
+            fetch_ids(p);
             KeyWords<D, MT> keys, next_keys;
             ValueWords<D, MT> values;
-            int id = next_id(p), next = next_id(p + kAttnWaves);
+            int id = id_at(p), next = id_at(p + kKv4Waves);
             keys.load(address(id), at_lane);
-            for (; p < stop; p += kAttnWaves) {
+            for (; p < stop; p += kKv4Waves) {
                 values.load(address(id), at_lane);
                 asm volatile("" ::: "memory");
                 next_keys.load(address(next), at_lane);
                 asm volatile("" ::: "memory");
-                const int after = next_id(p + 2 * kAttnWaves);
-                if (named(id)) rows.page(&s_q[0][lane], keys, values, at_lane.half, p * kKv4Page, n, filled, slots, g, unit);
+                if (named(id))
+                    rows.page(&s_q[0][lane], keys, values, at_lane.half, p * kKv4Page, n, filled, slots, g, unit);
                 keys = next_keys;
                 id = next;
-                next = after;
+                next = id_at(p + 2 * kKv4Waves);
             }
         }
 
         // ---- join the waves
         const float ref = rows.top * unit;
-        float total = rows.total;
-#pragma unroll
-        for (int off = MT; off < 64; off <<= 1) total += __shfl_xor(total, off, 64);
+        const float total = sum_over_groups<MT>(rows.total);
         if (g == 0) {
             s_m[wave][col] = ref;
             s_l[wave][col] = total;
@@ -569,9 +398,9 @@ __global__ __launch_bounds__(kAttnThreads, MT == 16 ? KV4_OCC : 2) void kv4_atte
         float* state = states + (int64_t)(2 * piece + (first == 0 ? 1 : 0)) * kStateFloats<D, MT>;
         float m = -__builtin_inff(), l = 0.f;
 #pragma unroll
-        for (int w = 0; w < kAttnWaves; ++w) m = fmaxf(m, s_m[w][col]);
+        for (int w = 0; w < kKv4Waves; ++w) m = fmaxf(m, s_m[w][col]);
 #pragma unroll
-        for (int w = 0; w < kAttnWaves; ++w) l += s_l[w][col] * fade(s_m[w][col], m);
+        for (int w = 0; w < kKv4Waves; ++w) l += s_l[w][col] * fade(s_m[w][col], m);
         const float f = fade(ref, m), inv = l > 0.f ? 1.f / l : 0.f;
 #pragma unroll
         for (int r0 = 0; r0 < kRegs; r0 += kRound) {
@@ -582,13 +411,13 @@ __global__ __launch_bounds__(kAttnThreads, MT == 16 ? KV4_OCC : 2) void kv4_atte
                 s_o[wave][j][lane] = rows.o[vl * S::VW + v][i] * f;
             }
             __syncthreads();
-            for (int jg = wave; jg * S::VW < kRound && r0 + jg * S::VW < kRegs; jg += kAttnWaves) {
+            for (int jg = wave; jg * S::VW < kRound && r0 + jg * S::VW < kRegs; jg += kKv4Waves) {
                 float sum[S::VW];
 #pragma unroll
                 for (int v = 0; v < S::VW; ++v) {
                     sum[v] = 0.f;
 #pragma unroll
-                    for (int w = 0; w < kAttnWaves; ++w) sum[v] += s_o[w][jg * S::VW + v][lane];
+                    for (int w = 0; w < kKv4Waves; ++w) sum[v] += s_o[w][jg * S::VW + v][lane];
                 }
                 const int gi = r0 / S::VW + jg;
                 if (whole) {
@@ -634,8 +463,8 @@ __global__ __launch_bounds__(64 * kJoinWaves) void kv4_join_kernel(Kv4AttentionA
     const int lo = before * per + ht * pages, hi = lo + pages;
     // cuts w0 .. w1 - 1 stay inside; the piece before the first has the tile's first pages
     int w0 = (lo + share - 1) / share, w1 = (hi - 1) / share + 1;
-    while (w0 < w1 && Scan::snap(w0 * share, lo, hi, share) == lo) ++w0;
-    while (w0 < w1 && Scan::snap((w1 - 1) * share, lo, hi, share) == hi) --w1;
+    while (w0 < w1 && snap(w0 * share, lo, hi, share) == lo) ++w0;
+    while (w0 < w1 && snap((w1 - 1) * share, lo, hi, share) == hi) --w1;
     if (w0 >= w1) return;                                   // one piece covered them and wrote the output
     auto state_of = [&](int w) { return states + (int64_t)(2 * w + (w < w0 ? 1 : 0)) * kStateFloats<D, MT>; };
     float m = -__builtin_inff(), l = 0.f;
@@ -666,25 +495,11 @@ Plan plan(int64_t batch, int64_t T, int64_t q_heads, int64_t heads, int64_t max_
     const int64_t rows = T * (q_heads / heads);
     p.rows = rows <= 16 ? 16 : 32;
     p.line.tiles = (int)((rows + p.rows - 1) / p.rows);
-    p.line.min_pages = kAttnWaves;
+    p.line.min_pages = kKv4Waves;
     const int64_t units = batch * heads * p.line.tiles * std::max<int64_t>(max_pages, 1);
-    const int64_t resident = (int64_t)device_cu_count() * (p.rows == 16 ? KV4_OCC / 2 : 1);
+    const int64_t resident = (int64_t)device_cu_count();
     p.line.pieces = (int)std::min<int64_t>(resident, (units + p.line.min_pages - 1) / p.line.min_pages);
     return p;
-}
-
-template <typename F> hipError_t by_type(int dtype, int head_dim, int rows, F&& f) {
-    auto by_rows = [&](auto tag, auto size) {
-        if (rows == 16) f(tag, size, std::integral_constant<int, 16>{});
-        else f(tag, size, std::integral_constant<int, 32>{});
-    };
-    auto by_size = [&](auto tag) {
-        if (head_dim == 64) by_rows(tag, std::integral_constant<int, 64>{});
-        else by_rows(tag, std::integral_constant<int, 128>{});
-    };
-    if (dtype == DELS_DTYPE_BF16) by_size(bf16_t{});
-    else by_size(f16_t{});
-    return hipGetLastError();
 }
 
 }  // namespace
@@ -699,12 +514,12 @@ hipError_t launch_kv4_attention(const Kv4AttentionArgs& a, void* ws, size_t data
     const Kv4Cache& c = a.cache;
     const Plan p = plan(c.batch, a.block.T, a.q_heads, c.heads, c.max_pages);
     auto* states = reinterpret_cast<float*>(static_cast<char*>(ws) + data_off);
-    return by_type(a.dtype, c.head_dim, p.rows, [&](auto tag, auto size, auto rows) {
+    return kv4_by_type(a.dtype, c.head_dim, p.rows, [&](auto tag, auto size, auto rows) {
         using T = decltype(tag);
         constexpr int D = decltype(size)::value, MT = decltype(rows)::value;
         using S = Shape<D, MT>;
         static_assert(S::CT * S::ACC / S::VW % kJoinWaves == 0, "a wave of the join per VW channels");
-        hipLaunchKernelGGL((kv4_attention_kernel<T, D, MT>), dim3(p.line.pieces), dim3(kAttnThreads), 0, s, a, p.line,
+        hipLaunchKernelGGL((kv4_attention_kernel<T, D, MT>), dim3(p.line.pieces), dim3(kKv4Threads), 0, s, a, p.line,
                            states);
         hipLaunchKernelGGL((kv4_join_kernel<T, D, MT>),
                            dim3((unsigned)c.batch * c.heads * p.line.tiles, S::CT * S::ACC / S::VW / kJoinWaves),

@@ -1,0 +1,218 @@
+// What the matrix-core kernels over the 4-bit key/value cache share: operands made of
+// codes, the shapes of a wave's work, a page's key words, and the line of pages that
+// is cut over the workgroups.
+#pragma once
+
+#include "../../include/dels.h"
+#include "kv4.h"
+
+namespace dels {
+
+constexpr int kKv4Waves = 8;                     // waves of a workgroup
+constexpr int kKv4Threads = 64 * kKv4Waves;
+constexpr float kLog2e = 1.44269504088896340736f;
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+template <typename T> struct Frag;
+template <> struct Frag<bf16_t> { using type = bf16x8; };
+template <> struct Frag<f16_t> { using type = f16x8; };
+
+// Eight codes times a power of two.
+template <typename T> __device__ __forceinline__ typename Frag<T>::type decode8(uint32_t w, float scale);
+template <> __device__ __forceinline__ bf16x8 decode8<bf16_t>(uint32_t w, float scale) {
+    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0);
+    const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1);
+    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2);
+    const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3);
+    return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+template <> __device__ __forceinline__ f16x8 decode8<f16_t>(uint32_t w, float scale) {
+    const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 0);
+    const f16x2 b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 1);
+    const f16x2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 2);
+    const f16x2 d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 3);
+    return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// A row's number over the lane groups of MT lanes: the largest, and the sum.
+template <int MT, typename F> __device__ __forceinline__ float over_groups(float x, F&& join) {
+    const uint32_t b = __float_as_uint(x);
+    const auto far = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    x = join(__uint_as_float(far[0]), __uint_as_float(far[1]));
+    if constexpr (MT == 16) {
+        const uint32_t c = __float_as_uint(x);
+        const auto near = __builtin_amdgcn_permlane16_swap(c, c, false, false);
+        x = join(__uint_as_float(near[0]), __uint_as_float(near[1]));
+    }
+    return x;
+}
+template <int MT> __device__ __forceinline__ float max_over_groups(float x) {
+    return over_groups<MT>(x, [](float a, float b) { return fmaxf(a, b); });
+}
+template <int MT> __device__ __forceinline__ float sum_over_groups(float x) {
+    return over_groups<MT>(x, [](float a, float b) { return a + b; });
+}
+
+__device__ __forceinline__ f32x4 mma(bf16x8 a, bf16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma(f16x8 a, f16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma(bf16x8 a, bf16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma(f16x8 a, f16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+// fp16 holds keys of up to 2^20 at a sixteenth of their size; the scale makes up for it.
+template <typename T> constexpr int kKeyShift = std::is_same<T, f16_t>::value ? 4 : 0;
+
+template <typename T>
+__device__ __forceinline__ float key_scale(uint32_t word, int byte) {
+    const int e = (int)((word >> (8 * byte)) & 255u);
+    return __uint_as_float((uint32_t)max(e - kKeyShift<T>, 0) << 23);
+}
+
+// Shapes of a wave's work on MT rows: MT x MT tiles of the matrix instructions.
+template <int D, int MT_> struct Shape {
+    static constexpr int MT = MT_;
+    static constexpr int NG = 64 / MT;              // lane groups: lane = MT * group + row
+    static constexpr int DL = D / NG;               // channels of a key that a lane holds
+    static constexpr int KS = DL / 8;               // steps of the first product
+    static constexpr int KB = DL >= 32 ? DL / 32 : 1;   // key scales per lane
+    static constexpr int KT = 32 / MT;              // key tiles of 32 slots
+    static constexpr int ACC = MT == 16 ? 4 : 16;   // accumulator registers of a tile
+    static constexpr int PF = 32 * MT / 64 / 8;     // weight operands (8 slots) per 32 slots
+    static constexpr int CT = D / MT;               // channel tiles of the output
+    static constexpr int VW = MT == 16 ? 4 : D / 32;    // consecutive channels of a lane: words of a load
+    static constexpr int VL = CT / VW;              // loads of value words per operand
+    using Acc = typename std::conditional<MT == 16, f32x4, f32x16>::type;
+    // slot within 32 that row r of key tile a holds
+    __device__ static int slot_of(int a, int r) {
+        if constexpr (MT == 16) return 8 * (r >> 2) + 4 * a + (r & 3);
+        return 16 * (r >> 4) + 8 * ((r >> 2) & 1) + 4 * ((r >> 3) & 1) + (r & 3);
+    }
+    // first of the VW channels that register i of a tile holds in channel block `vl`
+    __device__ static int channel_of(int vl, int i, int g) {
+        const int row = MT == 16 ? 4 * g + i : 8 * (i >> 2) + 4 * g + (i & 3);
+        return vl * MT * VW + row * VW;
+    }
+};
+
+__device__ __forceinline__ int seq_end(const Kv4Block& k, int b, int slots) {
+    const int n = kv4_length(k.lengths, b, slots);
+    if (k.mode == DELS_KV4_NONE) return n;
+    return (int)min((int64_t)slots, (int64_t)n + kv4_count(k.counts, b, k.T));
+}
+// Pages of sequence b (one at least: rows that see nothing are written too).
+__device__ __forceinline__ int seq_pages(const Kv4Block& k, int b, int slots) {
+    return max(1, (seq_end(k, b, slots) + kKv4Page - 1) / kKv4Page);
+}
+
+// What all lanes of a wave hold alike, kept in a scalar register.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// Scan of the sequences' units by a wave, 64 at a time; up to 64 it is kept.
+struct Scan {
+    const Kv4Block& k;
+    const Kv4Cache& c;
+    int per;                   // row tiles of a sequence
+    int own, cum;              // units of this lane's sequence, and of all up to it, in the 64 from b0
+    int b0, before, total;
+
+    __device__ Scan(const Kv4Block& k_, const Kv4Cache& c_, int per_) : k(k_), c(c_), per(per_) {
+        seek(0, 0);
+        total = __builtin_amdgcn_readlane(cum, 63);
+        for (int b = 64 + (threadIdx.x & 63), rest = 0; c.batch > 64; b += 64) {
+            rest += b < c.batch ? seq_pages(k, b, c.slots()) * per : 0;
+            if ((b & ~63) + 64 >= c.batch) {
+#pragma unroll
+                for (int off = 1; off < 64; off <<= 1) rest += __shfl_xor(rest, off, 64);
+                total += uniform(rest);
+                break;
+            }
+        }
+    }
+    __device__ void seek(int b0_, int before_) {
+        const int lane = threadIdx.x & 63;
+        b0 = b0_, before = before_;
+        own = b0 + lane < c.batch ? seq_pages(k, b0 + lane, c.slots()) * per : 0;
+        cum = own;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const int o = __shfl_up(cum, off, 64);
+            cum += lane >= off ? o : 0;
+        }
+    }
+    // Sequence of unit u < total, its first unit and its pages.
+    struct Place { int b, start, pages; };
+    __device__ Place place(int u) {
+        if (u < before) seek(0, 0);
+        for (;;) {
+            const unsigned long long past = __ballot(before + cum > u);
+            if (past) {
+                const int l = __builtin_ctzll(past);
+                return {b0 + l, __builtin_amdgcn_readlane(before + cum - own, l),
+                        __builtin_amdgcn_readlane(own, l) / per};
+            }
+            const int all = __builtin_amdgcn_readlane(cum, 63);
+            seek(b0 + 64, before + all);
+        }
+    }
+};
+
+// Byte offsets of a lane within a page; what differs between its loads is constant, so
+// that a load is a page address, a lane offset and an immediate.
+template <int D, int MT> struct LaneOffsets {
+    uint32_t key, key_scale, half, value, value_scale;
+    __device__ LaneOffsets(int col, int g) {
+        using S = Shape<D, MT>;
+        const int r = S::slot_of(0, col);
+        key = r * Kv4<D>::kKeyRow + g * (S::DL / 2);
+        key_scale = Kv4<D>::kKeyScale + 64 * (g * S::DL / 32) + 16 * ((r >> 3) & 3) + 4 * (r & 3);
+        half = 8 * ((r >> 2) & 1);         // key tiles of 32 rows: their slot's byte within the scales
+        value = Kv4<D>::kValue + 4 * (g * D + col * S::VW);
+        value_scale = Kv4<D>::kValueScale + 16 * g;
+    }
+};
+__device__ __forceinline__ const uint32_t* page_word(const uint8_t* page, uint32_t lane_off, int imm) {
+    return reinterpret_cast<const uint32_t*>(page + lane_off + imm);
+}
+
+// What a wave loads of a page: keys, and values.
+template <int D, int MT> struct KeyWords {
+    using S = Shape<D, MT>;
+    uint32_t code[2][S::KT][S::KS];
+    uint32_t scale[S::KB];
+    __device__ __forceinline__ void load(const uint8_t* page, const LaneOffsets<D, MT>& at) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int t = 0; t < S::KT; ++t)
+#pragma unroll
+                for (int k = 0; k < S::KS; ++k)
+                    code[s][t][k] = page_word(page, at.key, (32 * s + 4 * t) * Kv4<D>::kKeyRow)[k];
+#pragma unroll
+        for (int i = 0; i < S::KB; ++i) scale[i] = *page_word(page, at.key_scale, 64 * i);
+    }
+};
+template <typename F> hipError_t kv4_by_type(int dtype, int head_dim, int rows, F&& f) {
+    auto by_rows = [&](auto tag, auto size) {
+        if (rows == 16) f(tag, size, std::integral_constant<int, 16>{});
+        else f(tag, size, std::integral_constant<int, 32>{});
+    };
+    auto by_size = [&](auto tag) {
+        if (head_dim == 64) by_rows(tag, std::integral_constant<int, 64>{});
+        else by_rows(tag, std::integral_constant<int, 128>{});
+    };
+    if (dtype == DELS_DTYPE_BF16) by_size(bf16_t{});
+    else by_size(f16_t{});
+    return hipGetLastError();
+}
+
+}  // namespace dels

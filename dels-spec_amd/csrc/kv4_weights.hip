@@ -2,90 +2,194 @@
 // key/value cache (format: kv4.h).
 //
 //     out[b, h, j] = (j < lengths[b] ? weights[b, h, j] : 0) + sum_t,hq exp(scale * q[t, hq] . k[j] - lse[t, hq])
+//
+// The keys are read once, the values not at all: S [rows x slots] = Q K^T on the
+// matrix cores, a slot per lane and rows along its registers, so that the sum over
+// rows is an addition per score and one exchange between lane groups per slot.  A
+// wave turns 32 slots' codes into operands once and takes all row tiles over them.
+// Rows beyond 128 go in further rounds over the piece's pages.  Every slot belongs to
+// one wave: no atomics, one order of additions.
 #include <algorithm>
 
-#include "../../include/dels.h"
-#include "kv4.h"
+#include "kv4_mma.h"
 
 namespace dels {
 
 namespace {
 
-__device__ __forceinline__ float load_q(const bf16_t* p) { return bf16_bits_to_f32(p->bits); }
-__device__ __forceinline__ float load_q(const f16_t* p) { return lds_f32(p); }
+constexpr int kRows = 128;                       // rows whose queries fit LDS at a time
+constexpr int kMinPages = kKv4Waves;             // fewest pages of a workgroup's piece
 
-// Whether row t of the block sees slot j; n and count as the block's sequence has them.
-__device__ __forceinline__ bool kv4_sees(int j, int n, int count, int t, int mode, int64_t bits) {
-    const int i = j - n;
-    if (i < 0) return true;
-    if (i >= count || mode == DELS_KV4_NONE) return false;
-    if (mode == DELS_KV4_CAUSAL) return i <= t;
-    if (mode == DELS_KV4_FULL) return true;
-    return i < 64 && ((bits >> i) & 1) != 0;
-}
+template <typename T, int D, int MT>
+__global__ __launch_bounds__(kKv4Threads, 2) void kv4_weights_kernel(Kv4WeightsArgs a, int pieces) {
+    using S = Shape<D, MT>;
+    using F = typename Frag<T>::type;
+    __shared__ F s_q[kRows / MT][S::KS][64];
+    __shared__ __align__(16) float s_lse[kRows];             // binary logarithms, +inf for a row that does not count
+    __shared__ __align__(16) int s_lim[kRows];               // of the block's slots a row sees those below,
+    __shared__ uint64_t s_bits[kRows];                       // and those whose bits are set
 
-// Dot product of a key row with q (in LDS, fp32).
-template <int D>
-__device__ __forceinline__ float dot_key(const uint8_t* page, int in_page, const float* q) {
-    const uint32_t* row = reinterpret_cast<const uint32_t*>(page + in_page * Kv4<D>::kKeyRow);
-    float sum = 0.f;
-    for (int blk = 0; blk < D / 32; ++blk) {
-        float part = 0.f;
-        for (int w = 0; w < 4; ++w) {
-            const uint32_t word = row[4 * blk + w];
-            for (int i = 0; i < 8; ++i) part += kv4_level((word >> (4 * i)) & 15u) * q[32 * blk + 8 * w + i];
-        }
-        sum += part * kv4_pow2(page[Kv4<D>::scale_byte(in_page, blk)]);
+    const Kv4Cache& c = a.cache;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane % MT, g = lane / MT;
+    const int slots = c.slots(), group = a.q_heads / c.heads;
+    const LaneOffsets<D, MT> at_lane(col, g);
+    Scan scan(a.block, c, c.heads);
+    const int share = max(kMinPages, (scan.total + pieces - 1) / pieces);
+    const float mag = fabsf(a.scale);
+    const float unit = (mag == 0.f ? 1.f : mag) * kLog2e * (float)(1 << kKeyShift<T>);
+    const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u, zero = mag == 0.f ? 0u : ~0u;
+
+    int u = (int)min((int64_t)blockIdx.x * share, (int64_t)scan.total);
+    const int u_end = (int)min((int64_t)u + share, (int64_t)scan.total);
+    Scan::Place at{};
+    at.pages = 0;
+    while (u < u_end) {
+        if (u >= at.start + at.pages * scan.per) at = scan.place(u);
+        const int b = at.b, rel = u - at.start, h = rel / at.pages, first = rel - h * at.pages;
+        const int last = min(at.pages, first + (u_end - u));
+        const int n = uniform(kv4_length(a.block.lengths, b, slots));
+        const int count = uniform(kv4_count(a.block.counts, b, a.block.T));
+        const int rows = uniform(min(kv4_count(a.accepted, b, a.block.T), count)) * group;
+        const int filled = uniform(seq_end(a.block, b, slots));
+        const int32_t* ids = c.table + (int64_t)b * c.ld_table;
+        const uint8_t* heads = c.data + (int64_t)h * Kv4<D>::kBytes;
+        const int64_t page_stride = (int64_t)c.heads * Kv4<D>::kBytes;
+        const int64_t out_row = ((int64_t)b * c.heads + h) * slots;
+        auto id_of = [&](int p) { return p < last && p * kKv4Page < filled ? uniform(ids[p]) : -1; };
+        auto named = [&](int id) { return id >= 0 && id < c.num_pages; };
+
+        int r0 = 0;
+        do {                                                 // once without rows too: the old weights move
+            const int tiles = (min(rows - r0, kRows) + MT - 1) / MT;
+            __syncthreads();
+            for (int i = wave; i < tiles * S::KS; i += kKv4Waves) {
+                const int tile = i / S::KS, k = i % S::KS, r = r0 + tile * MT + col;
+                u32x4 w = {0u, 0u, 0u, 0u};
+                if (r < rows) {
+                    const int t = r / group, hq = h * group + r % group;
+                    w = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q.p) + (int64_t)b * a.q.batch +
+                                                        (int64_t)t * a.q.token + (int64_t)hq * a.q.head + g * S::DL + 8 * k);
+                }
+#pragma unroll
+                for (int x = 0; x < 4; ++x) w[x] = (w[x] ^ flip) & zero;
+                s_q[tile][k][lane] = __builtin_bit_cast(F, w);
+            }
+            if ((int)threadIdx.x < kRows) {
+                const int r = r0 + threadIdx.x, t = r / group;
+                float lse = __builtin_inff();
+                int lim = 0;
+                uint64_t bits = 0;
+                if (r < rows) {
+                    lim = a.block.mode == DELS_KV4_CAUSAL ? t + 1 : a.block.mode == DELS_KV4_FULL ? count : 0;
+                    if (a.block.mode == DELS_KV4_MASK)
+                        bits = (uint64_t)a.block.mask[(int64_t)b * a.block.ld_mask + t] &
+                               (count >= 64 ? ~0ull : (1ull << count) - 1);
+                    lse = a.lse[((int64_t)b * a.block.T + t) * a.q_heads + h * group + r % group] * kLog2e;
+                    if (lse == -__builtin_inff()) lse = __builtin_inff();   // an empty row gave nothing
+                }
+                s_lse[threadIdx.x] = lse;
+                s_lim[threadIdx.x] = lim;
+                s_bits[threadIdx.x] = bits;
+            }
+            __syncthreads();
+
+            KeyWords<D, MT> keys, next_keys;
+            int p = first + wave;
+            int id = id_of(p);
+            if (p < last) keys.load(heads + (named(id) ? id : 0) * page_stride, at_lane);
+            for (; p < last; p += kKv4Waves) {
+                const int next = id_of(p + kKv4Waves);
+                next_keys.load(heads + (named(next) ? next : 0) * page_stride, at_lane);
+                asm volatile("" ::: "memory");
+                // the slot that this lane writes, of the four (two) it has sums for: by its group
+                const int mine = p * kKv4Page + (MT == 16 ? 32 * (g >> 1) + S::slot_of(g & 1, col) : 32 * g + S::slot_of(0, col));
+                float sum = r0 > 0 ? a.out[out_row + mine] : mine < n ? a.weights[out_row + mine] : 0.f;
+                if (named(id) && tiles > 0) {
+                    const bool masked = (p + 1) * kKv4Page > n;
+#pragma unroll
+                    for (int s = 0; s < 2; ++s) {
+                        F kf[S::KT][S::KS];
+#pragma unroll
+                        for (int t = 0; t < S::KT; ++t)
+#pragma unroll
+                            for (int k = 0; k < S::KS; ++k) {
+                                const uint32_t scales = keys.scale[k * 8 / 32 % S::KB] >> (MT == 16 ? 8 * t : at_lane.half);
+                                kf[t][k] = decode8<T>(keys.code[s][t][k], key_scale<T>(scales, 2 * s));
+                            }
+                        float part[S::KT] = {};
+                        for (int tile = 0; tile < tiles; ++tile) {
+                            typename S::Acc acc[S::KT];
+#pragma unroll
+                            for (int t = 0; t < S::KT; ++t)
+#pragma unroll
+                                for (int i = 0; i < S::ACC; ++i) acc[t][i] = 0.f;
+#pragma unroll
+                            for (int k = 0; k < S::KS; ++k) {
+                                const F qk = s_q[tile][k][lane];
+#pragma unroll
+                                for (int t = 0; t < S::KT; ++t) acc[t] = mma(qk, kf[t][k], acc[t]);
+                            }
+                            // registers 4 q .. 4 q + 3 are rows 8 q + 4 g .. (4 g .. of a tile of 16)
+#pragma unroll
+                            for (int q4 = 0; q4 < S::ACC / 4; ++q4) {
+                                const int row = tile * MT + 8 * q4 + 4 * g;
+                                const f32x4 lse = *reinterpret_cast<const f32x4*>(&s_lse[row]);
+                                if (masked) {
+                                    asm volatile("");        // a branch, not a selection on every page
+#pragma unroll
+                                    for (int x = 0; x < 4; ++x) {
+                                        const int lim = s_lim[row + x];
+                                        const uint64_t bits = s_bits[row + x];
+#pragma unroll
+                                        for (int t = 0; t < S::KT; ++t) {
+                                            const int i = p * kKv4Page + 32 * s + S::slot_of(t, col) - n;
+                                            const uint32_t bit = i < 0 || i > 63 ? 0u : (uint32_t)(bits >> (i & 63)) & 1u;
+                                            acc[t][4 * q4 + x] = i < lim || bit ? acc[t][4 * q4 + x] : -__builtin_inff();
+                                        }
+                                    }
+                                }
+#pragma unroll
+                                for (int t = 0; t < S::KT; ++t)
+#pragma unroll
+                                    for (int x = 0; x < 4; ++x)
+                                        part[t] += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[t][4 * q4 + x], unit, -lse[x]));
+                            }
+                        }
+#pragma unroll
+                        for (int t = 0; t < S::KT; ++t) {
+                            const float all = sum_over_groups<MT>(part[t]);
+                            if (g == (MT == 16 ? 2 * s + t : s)) sum += all;
+                        }
+                    }
+                }
+                a.out[out_row + mine] = sum;
+                keys = next_keys;
+                id = next;
+            }
+            r0 += kRows;
+        } while (r0 < rows);
+        u += last - first;
     }
-    return sum;
-}
 
-// One workgroup per (sequence, head, page), a thread per slot.
-template <typename T, int D>
-__global__ __launch_bounds__(kKv4Page) void kv4_weights_kernel(Kv4WeightsArgs a) {
-    __shared__ float s_q[D];
-    const int tid = threadIdx.x;
-    const int p = blockIdx.x % a.cache.max_pages, bh = blockIdx.x / a.cache.max_pages;
-    const int h = bh % a.cache.heads, b = bh / a.cache.heads;
-    const int slots = a.cache.slots();
-    const int n = kv4_length(a.block.lengths, b, slots), count = kv4_count(a.block.counts, b, a.block.T);
-    const int rows = min(kv4_count(a.accepted, b, a.block.T), count), group = a.q_heads / a.cache.heads;
-    const int j = p * kKv4Page + tid;
-    const int end = (int)min((int64_t)slots, (int64_t)n + count);
-    const uint8_t* page = p * kKv4Page < end ? kv4_page(a.cache, b, h, p, Kv4<D>::kBytes) : nullptr;
-    float sum = 0.f;
-    for (int r = 0; page && r < rows * group; ++r) {
-        const int t = r / group, hq = h * group + r % group;
-        const T* q = static_cast<const T*>(a.q.p) + (int64_t)b * a.q.batch + (int64_t)t * a.q.token +
-                     (int64_t)hq * a.q.head;
-        __syncthreads();
-        for (int i = tid; i < D; i += kKv4Page) s_q[i] = load_q(q + i) * a.scale;
-        __syncthreads();
-        const float lse = a.lse[((int64_t)b * a.block.T + t) * a.q_heads + hq];
-        const int64_t bits = a.block.mode == DELS_KV4_MASK ? a.block.mask[(int64_t)b * a.block.ld_mask + t] : 0;
-        if (lse > -__builtin_inff() && j < end && kv4_sees(j, n, count, t, a.block.mode, bits))
-            sum += expf(dot_key<D>(page, tid, s_q) - lse);
+    // slots past the pages of a sequence are 0
+    const int rest = c.batch * c.heads;
+    for (int bh = blockIdx.x; bh < rest; bh += gridDim.x) {
+        const int pages = uniform(seq_pages(a.block, bh / c.heads, slots));
+        for (int j = pages * kKv4Page + threadIdx.x; j < slots; j += kKv4Threads) a.out[(int64_t)bh * slots + j] = 0.f;
     }
-    const int64_t at = (int64_t)bh * slots + j;
-    a.out[at] = (j < n ? a.weights[at] : 0.f) + sum;
-}
-
-template <typename F> hipError_t by_type(int dtype, int head_dim, F&& f) {
-    auto by_size = [&](auto tag) {
-        if (head_dim == 64) f(tag, std::integral_constant<int, 64>{});
-        else f(tag, std::integral_constant<int, 128>{});
-    };
-    if (dtype == DELS_DTYPE_BF16) by_size(bf16_t{});
-    else by_size(f16_t{});
-    return hipGetLastError();
 }
 
 }  // namespace
 
 hipError_t launch_kv4_weights(const Kv4WeightsArgs& a, hipStream_t s) {
-    return by_type(a.dtype, a.cache.head_dim, [&](auto tag, auto size) {
-        hipLaunchKernelGGL((kv4_weights_kernel<decltype(tag), decltype(size)::value>),
-                           dim3((unsigned)a.cache.batch * a.cache.heads * a.cache.max_pages), dim3(kKv4Page), 0, s, a);
+    const Kv4Cache& c = a.cache;
+    const int64_t units = (int64_t)c.batch * c.heads * c.max_pages;
+    const int pieces = (int)std::min<int64_t>(device_cu_count(), (units + kMinPages - 1) / kMinPages);
+    const int rows = (int64_t)a.block.T * (a.q_heads / c.heads) <= 16 ? 16 : 32;
+    return kv4_by_type(a.dtype, c.head_dim, rows, [&](auto tag, auto size, auto tile) {
+        hipLaunchKernelGGL((kv4_weights_kernel<decltype(tag), decltype(size)::value, decltype(tile)::value>), dim3(pieces),
+                           dim3(kKv4Threads), 0, s, a, pieces);
     });
 }
 
