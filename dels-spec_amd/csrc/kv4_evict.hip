@@ -15,7 +15,8 @@ namespace dels {
 
 namespace {
 
-constexpr int kSelectThreads = 1024;
+constexpr int kPerLane = 16;                               // slots of a lane per tile
+constexpr int kBins = 2048;                                // 11 bits of the key at a time
 constexpr int kMoveThreads = 256;
 
 // A larger key is a larger weight; NaN counts as -inf.
@@ -23,14 +24,42 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
     return f32_order_key(w != w ? -__builtin_inff() : w);
 }
 
-// One workgroup per (sequence, head).  The threshold is found eight bits of the
-// key at a time (a histogram in LDS of the weights that share the bits so far),
-// then slots are walked in order: an equal weight's rank among equals, a hole's
-// and a mover's rank come from ballots.
-__global__ __launch_bounds__(kSelectThreads) void kv4_select_kernel(Kv4EvictArgs a, int32_t* hole_list) {
-    __shared__ uint32_t s_hist[256];
+// Sum over the lanes up to this one.
+__device__ __forceinline__ int scan_wave(int x) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const int o = __shfl_up(x, off, 64);
+        x += lane >= off ? o : 0;
+    }
+    return x;
+}
+// Sum of `x` (one value per wave) over the waves before this one, and over all.
+template <int WAVES> __device__ __forceinline__ int2 over_waves(const int* x) {
+    const int wave = threadIdx.x >> 6;
+    int before = 0, all = 0;
+#pragma unroll
+    for (int v = 0; v < WAVES; ++v) {
+        before += v < wave ? x[v] : 0;
+        all += x[v];
+    }
+    return {before, all};
+}
+
+// One workgroup per (sequence, head).  The threshold is found 11 bits of the key at a
+// time (a histogram in LDS of the weights that share the bits so far, scanned from
+// its top); then the slots are walked in order, 16 THREADS at a time and 1024 of them a
+// wave: ranks among equal weights, holes and movers come from ballots, and from the
+// waves' counts in three exchanges a tile.  Bound by latency: the weights are read
+// four times, all but the first from L2.  COPIES of the histogram: lanes of one digit
+// meet on fewer words.
+template <int THREADS, int COPIES>
+__global__ __launch_bounds__(THREADS) void kv4_select_kernel(Kv4EvictArgs a, int32_t* hole_list) {
+    constexpr int kWaves = THREADS / 64, kTile = THREADS * kPerLane, kOwn = kBins / THREADS;
+    __shared__ uint32_t s_hist[COPIES][kBins];
+    __shared__ int s_wave[kWaves];
     __shared__ uint32_t s_pick, s_left;
-    __shared__ int s_wave[3][kSelectThreads / 64];
+    __shared__ int s_count[3][kWaves];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int bh = blockIdx.x, h = bh % a.cache.heads, b = bh / a.cache.heads;
     const int slots = a.cache.slots(), keep = a.keep;
@@ -39,115 +68,214 @@ __global__ __launch_bounds__(kSelectThreads) void kv4_select_kernel(Kv4EvictArgs
     float* out = a.out_weights + (int64_t)bh * slots;
     int32_t* source = a.source + (int64_t)bh * keep;
     if (h == 0 && tid == 0) a.out_lengths[b] = min(n, keep);
-    for (int j = min(n, keep) + tid; j < slots; j += kSelectThreads) out[j] = 0.f;
-    for (int64_t j = tid; j < keep; j += kSelectThreads) source[j] = j < n ? (int32_t)j : -1;
+    for (int j = min(n, keep) + tid; j < slots; j += THREADS) out[j] = 0.f;
     if (n <= keep) {
-        for (int j = tid; j < n; j += kSelectThreads) out[j] = w[j];
+        for (int j = tid; j < n; j += THREADS) out[j] = w[j];
+        for (int64_t j = tid; j < keep; j += THREADS) source[j] = j < n ? (int32_t)j : -1;
         return;
     }
     const int recent = min(a.recent, keep), cand = n - recent;
     uint32_t left = keep - recent;                 // candidates still to choose among the equal prefixes
     uint32_t prefix = 0u;
-    for (int shift = 24; shift >= 0 && left > 0; shift -= 8) {
-        if (tid < 256) s_hist[tid] = 0u;
+    int bits_left = 32;
+    while (bits_left > 0 && left > 0) {
+        const int digit_bits = min(bits_left, 11), shift = bits_left - digit_bits;
+        for (int i = tid; i < COPIES * kBins; i += THREADS) (&s_hist[0][0])[i] = 0u;
         __syncthreads();
-        for (int j = tid; j < cand; j += kSelectThreads) {
-            const uint32_t key = weight_key(w[j]);
-            if (shift == 24 || (key >> (shift + 8)) == prefix) atomicAdd(&s_hist[(key >> shift) & 255u], 1u);
+        for (int j0 = 0; j0 < cand; j0 += kTile) {
+            float x[kPerLane];
+#pragma unroll
+            for (int i = 0; i < kPerLane; ++i) {
+                const int j = j0 + i * THREADS + tid;
+                x[i] = j < cand ? w[j] : 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < kPerLane; ++i) {
+                const uint32_t key = weight_key(x[i]);
+                const bool mine = bits_left == 32 || (key >> bits_left) == prefix;
+                if (j0 + i * THREADS + tid < cand && mine)
+                    atomicAdd(&s_hist[lane % COPIES][(key >> shift) & ((1u << digit_bits) - 1)], 1u);
+            }
         }
         __syncthreads();
-        if (tid == 0) {
-            uint32_t l = left;
-            int d = 255;
-            while (d > 0 && s_hist[d] < l) l -= s_hist[d--];
-            s_pick = (uint32_t)d;
-            s_left = l;
+        // bins from the top, kOwn a thread: the one in which the count of larger keys reaches `left`
+        uint32_t c[kOwn], own = 0u;
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i) {
+            c[i] = 0u;
+#pragma unroll
+            for (int q = 0; q < COPIES; ++q) c[i] += s_hist[q][kBins - 1 - (kOwn * tid + i)];
+            own += c[i];
+        }
+        const int upto = scan_wave((int)own);
+        if (lane == 63) s_wave[wave] = upto;
+        __syncthreads();
+        uint32_t before = (uint32_t)(over_waves<kWaves>(s_wave).x + upto) - own;
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i) {
+            if (before < left && left <= before + c[i]) s_pick = kBins - 1 - (kOwn * tid + i), s_left = left - before;
+            before += c[i];
         }
         __syncthreads();
-        prefix = (prefix << 8) | s_pick;
+        prefix = (prefix << digit_bits) | s_pick;
         left = s_left;
+        bits_left = shift;
         __syncthreads();
     }
-    // keys above `prefix` are kept, and `left` of those equal to it
+    // keys above `prefix` are kept, and the first `left` of those equal to it
     const bool none = keep == recent;
     int32_t* holes = hole_list + (int64_t)bh * keep;
     int equal_before = 0, hole_before = 0, mover_before = 0;
-    for (int j0 = 0; j0 < n; j0 += kSelectThreads) {
-        const int j = j0 + tid;
-        const uint32_t key = j < cand ? weight_key(w[j]) : 0u;
-        const bool equal = j < cand && !none && key == prefix;
-        const unsigned long long eq = __ballot(equal);
-        if (lane == 0) s_wave[0][wave] = __popcll(eq);
-        __syncthreads();
-        int rank = equal_before + __popcll(eq & ((1ull << lane) - 1));
-        for (int v = 0; v < kSelectThreads / 64; ++v) {
-            rank += v < wave ? s_wave[0][v] : 0;
-            equal_before += s_wave[0][v];
+    for (int j0 = 0; j0 < n; j0 += kTile) {
+        // this wave's 1024 slots of the tile, lane by lane
+        const int first = j0 + wave * 64 * kPerLane + lane;
+        float x[kPerLane];
+#pragma unroll
+        for (int i = 0; i < kPerLane; ++i) x[i] = first + 64 * i < n ? w[first + 64 * i] : 0.f;
+        uint32_t kept = 0u, equal = 0u;            // bit i: slot first + 64 i
+        int equals = 0;
+#pragma unroll
+        for (int i = 0; i < kPerLane; ++i) {
+            const int j = first + 64 * i;
+            const uint32_t key = weight_key(x[i]);
+            const bool eq = j < cand && !none && key == prefix;
+            if (j < n && (j >= cand || (!none && key > prefix))) kept |= 1u << i;
+            if (eq) equal |= 1u << i;
+            equals += __popcll(__ballot(eq));
         }
-        const bool kept = j < n && (j >= cand || (!none && (key > prefix || (equal && rank < (int)left))));
-        const bool hole = j < keep && !kept, mover = j >= keep && kept;
-        const unsigned long long hb = __ballot(hole), mb = __ballot(mover);
-        if (lane == 0) s_wave[1][wave] = __popcll(hb), s_wave[2][wave] = __popcll(mb);
+        if (lane == 0) s_count[0][wave] = equals;
         __syncthreads();
-        int hr = hole_before + __popcll(hb & ((1ull << lane) - 1)), mr = mover_before + __popcll(mb & ((1ull << lane) - 1));
-        for (int v = 0; v < kSelectThreads / 64; ++v) {
-            hr += v < wave ? s_wave[1][v] : 0;
-            mr += v < wave ? s_wave[2][v] : 0;
-            hole_before += s_wave[1][v];
-            mover_before += s_wave[2][v];
+        const int2 e = over_waves<kWaves>(s_count[0]);
+        int rank = equal_before + e.x, hole_count = 0, mover_count = 0;
+        equal_before += e.y;
+        const unsigned long long below = (1ull << lane) - 1;
+#pragma unroll
+        for (int i = 0; i < kPerLane; ++i) {
+            const int j = first + 64 * i;
+            const bool eq = equal >> i & 1u;
+            const unsigned long long m = __ballot(eq);
+            if (eq && rank + __popcll(m & below) < (int)left) kept |= 1u << i;
+            rank += __popcll(m);
+            const bool k = kept >> i & 1u;
+            hole_count += __popcll(__ballot(j < keep && !k));
+            mover_count += __popcll(__ballot(j >= keep && k));
         }
-        if (hole) holes[hr] = j;
-        if (j < keep && kept) out[j] = w[j];
-        __syncthreads();                           // also orders the holes before the movers that read them
-        if (mover) {
-            const int to = holes[mr];
-            source[to] = j;
-            out[to] = w[j];
+        if (lane == 0) s_count[1][wave] = hole_count, s_count[2][wave] = mover_count;
+        __syncthreads();
+        const int2 hc = over_waves<kWaves>(s_count[1]), mc = over_waves<kWaves>(s_count[2]);
+        int hr = hole_before + hc.x, mr = mover_before + mc.x;
+        hole_before += hc.y;
+        mover_before += mc.y;
+#pragma unroll
+        for (int i = 0; i < kPerLane; ++i) {
+            const int j = first + 64 * i;
+            const bool k = kept >> i & 1u, hole = j < keep && !k;
+            const unsigned long long m = __ballot(hole);
+            if (hole) holes[hr + __popcll(m & below)] = j;
+            hr += __popcll(m);
+            if (j < keep && k) {
+                source[j] = j;
+                out[j] = x[i];
+            }
+        }
+        __syncthreads();                           // the holes before the movers that go there
+        if (mc.y) {
+#pragma unroll
+            for (int i = 0; i < kPerLane; ++i) {
+                const int j = first + 64 * i;
+                const bool mover = j >= keep && (kept >> i & 1u);
+                const unsigned long long m = __ballot(mover);
+                if (mover) {
+                    const int to = holes[mr + __popcll(m & below)];
+                    source[to] = j;
+                    out[to] = x[i];
+                }
+                mr += __popcll(m);
+            }
         }
     }
 }
 
-// One wave per (sequence, head, 8 places): the places share the value words of
-// their row.  Lanes as in the append kernel for the keys; D / 64 channels each for
-// the values.
+// One wave per (sequence, head, 8 places): the places share the value words of their
+// row, so that no two waves write one word.  What moves is loaded for all eight
+// places before any of it is written: K words 16 (8) lanes a slot, value words of D / 64
+// channels a lane.  A moved slot's value codes lie in D words of eight slots each, so
+// eight times what moves is read: consecutive movers are often neighbours, whose
+// words the caches still hold.
 template <int D>
 __global__ __launch_bounds__(kMoveThreads) void kv4_move_kernel(Kv4Cache c, const int32_t* lengths,
                                                                 const int32_t* __restrict__ sources, int keep,
                                                                 int groups) {
     constexpr int N = D / 64;
+    constexpr int kRowLanes = Kv4<D>::kKeyRow / 4, kSlotsPerLoad = 64 / kRowLanes, kLoads = 8 / kSlotsPerLoad;
+    using P = Kv4<D>;
     const int lane = threadIdx.x & 63;
     const int64_t unit = (int64_t)blockIdx.x * (kMoveThreads / 64) + (threadIdx.x >> 6);
     if (unit >= (int64_t)c.batch * c.heads * groups) return;
     const int g = (int)(unit % groups), bh = (int)(unit / groups), h = bh % c.heads, b = bh / c.heads;
+    // lane i < 8 (and i + 8, ...): the slot that place i takes, and its page.  All of this is
+    // loaded before any of it is looked at.
+    const int i8 = lane & 7;
+    const int mine = 8 * g + i8 < keep ? sources[(int64_t)bh * keep + 8 * g + i8] : -1;
     const int n = kv4_length(lengths, b, c.slots());
+    uint8_t* page = kv4_page(c, b, h, 8 * g / kKv4Page, P::kBytes);
     if (n <= keep || 8 * g >= n) return;
-    const int mine = 8 * g + (lane & 7) < keep ? sources[(int64_t)bh * keep + 8 * g + (lane & 7)] : -1;
-    const bool moves = mine >= keep && mine < n;
+    const int64_t page_stride = (int64_t)c.heads * P::kBytes;
+    const bool comes = mine >= keep && mine < n;
+    const int from_id = comes ? c.table[(int64_t)b * c.ld_table + mine / kKv4Page] : -1;
+    const bool moves = comes && from_id >= 0 && from_id < c.num_pages;
     const uint32_t todo = (uint32_t)__ballot(moves) & 0xffu;
-    if (!todo) return;
-    uint8_t* page = kv4_page(c, b, h, 8 * g / kKv4Page, Kv4<D>::kBytes);
-    if (!page) return;
-    uint32_t* row = reinterpret_cast<uint32_t*>(page + Kv4<D>::kValue) + (8 * g % kKv4Page / 8) * D + lane * N;
-    uint32_t words[N];
+    if (!todo || !page) return;
+    const int in_page = 8 * g % kKv4Page;
+    // a place that takes nothing reads its own content
+    const uint8_t* own_head = c.data + (int64_t)h * P::kBytes;
+    const int64_t from_page = moves ? (int64_t)from_id * page_stride : page - own_head;
+    const int from_slot = moves ? mine % kKv4Page : in_page + i8;
+
+    uint32_t* row = reinterpret_cast<uint32_t*>(page + P::kValue) + (in_page / 8) * D + lane * N;
+    uint32_t words[N], src[8][N], key[kLoads];
 #pragma unroll
     for (int j = 0; j < N; ++j) words[j] = row[j];
-    for (int i = 0; i < 8; ++i) {
-        if (!(todo >> i & 1u)) continue;
-        const int from = __shfl(mine, i, 64), in_from = from % kKv4Page, in_to = (8 * g + i) % kKv4Page;
-        const uint8_t* old = kv4_page(c, b, h, from / kKv4Page, Kv4<D>::kBytes);
-        if (!old) continue;
-        if (lane < Kv4<D>::kKeyRow / 4)
-            reinterpret_cast<uint32_t*>(page + in_to * Kv4<D>::kKeyRow)[lane] =
-                reinterpret_cast<const uint32_t*>(old + in_from * Kv4<D>::kKeyRow)[lane];
-        if (lane < D / 32) page[Kv4<D>::scale_byte(in_to, lane)] = old[Kv4<D>::scale_byte(in_from, lane)];
-        if (lane == 0)
-            *reinterpret_cast<uint16_t*>(page + Kv4<D>::kValueScale + 2 * in_to) =
-                *reinterpret_cast<const uint16_t*>(old + Kv4<D>::kValueScale + 2 * in_from);
-        const uint32_t* src = reinterpret_cast<const uint32_t*>(old + Kv4<D>::kValue) + (in_from >> 3) * D + lane * N;
+    int slot[8];
 #pragma unroll
-        for (int j = 0; j < N; ++j)
-            words[j] = (words[j] & ~(15u << (4 * i))) | (((src[j] >> (4 * (in_from & 7))) & 15u) << (4 * i));
+    for (int i = 0; i < 8; ++i) {
+        slot[i] = __builtin_amdgcn_readlane(from_slot, i);
+        const uint8_t* from = own_head + (((int64_t)__builtin_amdgcn_readlane((int)(from_page >> 32), i) << 32) |
+                                          (uint32_t)__builtin_amdgcn_readlane((int)from_page, i));
+        const uint32_t* at = reinterpret_cast<const uint32_t*>(from + P::kValue) + (slot[i] >> 3) * D + lane * N;
+#pragma unroll
+        for (int j = 0; j < N; ++j) src[i][j] = at[j];
     }
+    auto far = [&](int i) {                        // place i's source, for lanes that differ in i
+        const int lo = __shfl((int)from_page, i, 64), hi = __shfl((int)(from_page >> 32), i, 64);
+        return own_head + (((int64_t)hi << 32) | (uint32_t)lo);
+    };
+    const int sub = lane / kRowLanes, word = lane % kRowLanes;
+#pragma unroll
+    for (int q = 0; q < kLoads; ++q) {
+        const int i = q * kSlotsPerLoad + sub;
+        key[q] = reinterpret_cast<const uint32_t*>(far(i) + __shfl(from_slot, i, 64) * P::kKeyRow)[word];
+    }
+    // scales: a lane per (place, block) and per place
+    constexpr int kBlocks = D / 32;
+    const int si = lane / kBlocks & 7, blk = lane % kBlocks;
+    const uint8_t ks = far(si)[P::scale_byte(__shfl(from_slot, si, 64), blk)];
+    const uint16_t vs = *reinterpret_cast<const uint16_t*>(far(i8) + P::kValueScale + 2 * __shfl(from_slot, i8, 64));
+
+#pragma unroll
+    for (int q = 0; q < kLoads; ++q) {
+        const int i = q * kSlotsPerLoad + sub;
+        if (todo >> i & 1u) reinterpret_cast<uint32_t*>(page + (in_page + i) * P::kKeyRow)[word] = key[q];
+    }
+    if (lane < 8 * kBlocks && (todo >> si & 1u)) page[P::scale_byte(in_page + si, blk)] = ks;
+    if (lane < 8 && (todo >> i8 & 1u)) *reinterpret_cast<uint16_t*>(page + P::kValueScale + 2 * (in_page + i8)) = vs;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (todo >> i & 1u) {
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                words[j] = (words[j] & ~(15u << (4 * i))) | (((src[i][j] >> (4 * (slot[i] & 7))) & 15u) << (4 * i));
+        }
 #pragma unroll
     for (int j = 0; j < N; ++j) row[j] = words[j];
 }
@@ -161,7 +289,12 @@ size_t kv4_evict_data_bytes(int64_t batch, int64_t heads, int64_t keep) {
 hipError_t launch_kv4_evict(const Kv4EvictArgs& a, void* ws, size_t data_off, hipStream_t s) {
     const Kv4Cache& c = a.cache;
     auto* holes = reinterpret_cast<int32_t*>(static_cast<char*>(ws) + data_off);
-    hipLaunchKernelGGL(kv4_select_kernel, dim3(c.batch * c.heads), dim3(kSelectThreads), 0, s, a, holes);
+    // few slots: a short tile and a small workgroup, whose barriers and histogram take less
+    const dim3 grid_select(c.batch * c.heads);
+    if (c.slots() <= 256 * kPerLane)
+        hipLaunchKernelGGL((kv4_select_kernel<256, 1>), grid_select, dim3(256), 0, s, a, holes);
+    else
+        hipLaunchKernelGGL((kv4_select_kernel<1024, 4>), grid_select, dim3(1024), 0, s, a, holes);
     const int groups = (std::min(a.keep, c.slots()) + 7) / 8, waves = kMoveThreads / 64;
     const dim3 grid((unsigned)(((int64_t)c.batch * c.heads * groups + waves - 1) / waves));
     if (c.head_dim == 64)

@@ -21,7 +21,7 @@ constexpr int kRows = 128;                       // rows whose queries fit LDS a
 constexpr int kMinPages = kKv4Waves;             // fewest pages of a workgroup's piece
 
 template <typename T, int D, int MT>
-__global__ __launch_bounds__(kKv4Threads, 2) void kv4_weights_kernel(Kv4WeightsArgs a, int pieces) {
+__global__ __launch_bounds__(kKv4Threads, 4) void kv4_weights_kernel(Kv4WeightsArgs a, int pieces) {
     using S = Shape<D, MT>;
     using F = typename Frag<T>::type;
     __shared__ F s_q[kRows / MT][S::KS][64];
@@ -185,7 +185,8 @@ __global__ __launch_bounds__(kKv4Threads, 2) void kv4_weights_kernel(Kv4WeightsA
 hipError_t launch_kv4_weights(const Kv4WeightsArgs& a, hipStream_t s) {
     const Kv4Cache& c = a.cache;
     const int64_t units = (int64_t)c.batch * c.heads * c.max_pages;
-    const int pieces = (int)std::min<int64_t>(device_cu_count(), (units + kMinPages - 1) / kMinPages);
+    // two workgroups a CU: 32 x 16k slots 74 us with one, 68 so
+    const int pieces = (int)std::min<int64_t>(2 * device_cu_count(), (units + kMinPages - 1) / kMinPages);
     const int rows = (int64_t)a.block.T * (a.q_heads / c.heads) <= 16 ? 16 : 32;
     return kv4_by_type(a.dtype, c.head_dim, rows, [&](auto tag, auto size, auto tile) {
         hipLaunchKernelGGL((kv4_weights_kernel<decltype(tag), decltype(size)::value, decltype(tile)::value>), dim3(pieces),
