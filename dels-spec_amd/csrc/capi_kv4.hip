@@ -205,7 +205,7 @@ int dels_kv4_evict(const dels_kv4_cache* p, const int32_t* lengths, const float*
         return fail(DELS_ERR_INVALID_ARGUMENT, "lengths, weights or an output is NULL");
     if (lengths == out_lengths || (weights && weights == out_weights))
         return fail(DELS_ERR_INVALID_ARGUMENT, "an output is one of the inputs");
-    if (!grid_ok({a.cache.batch, a.cache.heads, a.cache.max_pages}))
+    if (!grid_ok({a.cache.batch, a.cache.heads, a.cache.max_pages}) || a.cache.batch > 65535 || a.cache.heads > 65535)
         return fail(DELS_ERR_UNSUPPORTED, "shape past the supported extents");
     const size_t need = dels_kv4_evict_ws_bytes(a.cache.batch, a.cache.heads, keep);
     if ((rc = check_ws(ws, ws_bytes, need)) != DELS_OK) return rc;

@@ -210,26 +210,27 @@ __global__ __launch_bounds__(kMoveThreads) void kv4_move_kernel(Kv4Cache c, cons
     constexpr int kRowLanes = Kv4<D>::kKeyRow / 4, kSlotsPerLoad = 64 / kRowLanes, kLoads = 8 / kSlotsPerLoad;
     using P = Kv4<D>;
     const int lane = threadIdx.x & 63;
-    const int64_t unit = (int64_t)blockIdx.x * (kMoveThreads / 64) + (threadIdx.x >> 6);
-    if (unit >= (int64_t)c.batch * c.heads * groups) return;
-    const int g = (int)(unit % groups), bh = (int)(unit / groups), h = bh % c.heads, b = bh / c.heads;
+    const int g = blockIdx.x * (kMoveThreads / 64) + (threadIdx.x >> 6), h = blockIdx.y, b = blockIdx.z;
+    if (g >= groups) return;
+    const int64_t bh = (int64_t)b * c.heads + h;
     // lane i < 8 (and i + 8, ...): the slot that place i takes, and its page.  All of this is
     // loaded before any of it is looked at.
     const int i8 = lane & 7;
-    const int mine = 8 * g + i8 < keep ? sources[(int64_t)bh * keep + 8 * g + i8] : -1;
+    const int mine = 8 * g + i8 < keep ? sources[bh * keep + 8 * g + i8] : -1;
     const int n = kv4_length(lengths, b, c.slots());
     uint8_t* page = kv4_page(c, b, h, 8 * g / kKv4Page, P::kBytes);
     if (n <= keep || 8 * g >= n) return;
     const int64_t page_stride = (int64_t)c.heads * P::kBytes;
     const bool comes = mine >= keep && mine < n;
-    const int from_id = comes ? c.table[(int64_t)b * c.ld_table + mine / kKv4Page] : -1;
+    const int32_t* ids = c.table + (int64_t)b * c.ld_table;
+    int from_id = comes ? ids[mine / kKv4Page] : -1;
     const bool moves = comes && from_id >= 0 && from_id < c.num_pages;
     const uint32_t todo = (uint32_t)__ballot(moves) & 0xffu;
     if (!todo || !page) return;
     const int in_page = 8 * g % kKv4Page;
     // a place that takes nothing reads its own content
     const uint8_t* own_head = c.data + (int64_t)h * P::kBytes;
-    const int64_t from_page = moves ? (int64_t)from_id * page_stride : page - own_head;
+    if (!moves) from_id = ids[8 * g / kKv4Page];
     const int from_slot = moves ? mine % kKv4Page : in_page + i8;
 
     uint32_t* row = reinterpret_cast<uint32_t*>(page + P::kValue) + (in_page / 8) * D + lane * N;
@@ -240,16 +241,13 @@ __global__ __launch_bounds__(kMoveThreads) void kv4_move_kernel(Kv4Cache c, cons
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         slot[i] = __builtin_amdgcn_readlane(from_slot, i);
-        const uint8_t* from = own_head + (((int64_t)__builtin_amdgcn_readlane((int)(from_page >> 32), i) << 32) |
-                                          (uint32_t)__builtin_amdgcn_readlane((int)from_page, i));
+        const uint8_t* from = own_head + __builtin_amdgcn_readlane(from_id, i) * page_stride;
         const uint32_t* at = reinterpret_cast<const uint32_t*>(from + P::kValue) + (slot[i] >> 3) * D + lane * N;
 #pragma unroll
         for (int j = 0; j < N; ++j) src[i][j] = at[j];
     }
-    auto far = [&](int i) {                        // place i's source, for lanes that differ in i
-        const int lo = __shfl((int)from_page, i, 64), hi = __shfl((int)(from_page >> 32), i, 64);
-        return own_head + (((int64_t)hi << 32) | (uint32_t)lo);
-    };
+    // place i's source, for lanes that differ in i
+    auto far = [&](int i) { return own_head + (int64_t)__shfl(from_id, i, 64) * page_stride; };
     const int sub = lane / kRowLanes, word = lane % kRowLanes;
 #pragma unroll
     for (int q = 0; q < kLoads; ++q) {
@@ -260,7 +258,7 @@ __global__ __launch_bounds__(kMoveThreads) void kv4_move_kernel(Kv4Cache c, cons
     constexpr int kBlocks = D / 32;
     const int si = lane / kBlocks & 7, blk = lane % kBlocks;
     const uint8_t ks = far(si)[P::scale_byte(__shfl(from_slot, si, 64), blk)];
-    const uint16_t vs = *reinterpret_cast<const uint16_t*>(far(i8) + P::kValueScale + 2 * __shfl(from_slot, i8, 64));
+    const uint16_t vs = *reinterpret_cast<const uint16_t*>(own_head + from_id * page_stride + P::kValueScale + 2 * from_slot);
 
 #pragma unroll
     for (int q = 0; q < kLoads; ++q) {
@@ -296,7 +294,7 @@ hipError_t launch_kv4_evict(const Kv4EvictArgs& a, void* ws, size_t data_off, hi
     else
         hipLaunchKernelGGL((kv4_select_kernel<1024, 4>), grid_select, dim3(1024), 0, s, a, holes);
     const int groups = (std::min(a.keep, c.slots()) + 7) / 8, waves = kMoveThreads / 64;
-    const dim3 grid((unsigned)(((int64_t)c.batch * c.heads * groups + waves - 1) / waves));
+    const dim3 grid((groups + waves - 1) / waves, c.heads, c.batch);
     if (c.head_dim == 64)
         hipLaunchKernelGGL(kv4_move_kernel<64>, grid, dim3(kMoveThreads), 0, s, c, a.lengths, a.source, a.keep, groups);
     else
