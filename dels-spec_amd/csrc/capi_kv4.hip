@@ -154,6 +154,7 @@ int dels_kv4_attention(const dels_kv4_cache* p, const void* q, int64_t q_batch, 
     if (rc != DELS_OK) return rc;
     if ((rc = check_rows(out, out_batch, out_token, out_head, dtype, "out")) != DELS_OK) return rc;
     if (!lse) return fail(DELS_ERR_INVALID_ARGUMENT, "lse is NULL");
+    if (a.cache.num_pages == 0) a.cache.max_pages = 0;       // nothing to see
     const size_t need = dels_kv4_attention_ws_bytes(a.cache.batch, T, q_heads, a.cache.heads, a.cache.head_dim,
                                                     a.cache.max_pages);
     if ((rc = check_ws(ws, ws_bytes, need)) != DELS_OK) return rc;
@@ -176,6 +177,8 @@ int dels_kv4_weights(const dels_kv4_cache* p, const void* q, int64_t q_batch, in
     if (T <= 0) return fail(DELS_ERR_INVALID_ARGUMENT, "bad block length %lld", (long long)T);
     rc = check_block(a.cache, q, q_batch, q_token, q_head, dtype, q_heads, T, lengths, block, mask, ld_mask, scale);
     if (rc != DELS_OK) return rc;
+    if (a.cache.batch * (int64_t)a.cache.heads > 65535 && a.cache.num_pages == 0)
+        return fail(DELS_ERR_UNSUPPORTED, "a cache of no pages: batch x heads <= 65535");
     if (!lse || !weights || !out) return fail(DELS_ERR_INVALID_ARGUMENT, "lse, weights or out is NULL");
     a.block = {lengths, counts, (int)T, block, mask, ld_mask};
     a.q = {q, q_batch, q_token, q_head};

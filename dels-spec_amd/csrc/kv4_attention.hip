@@ -17,9 +17,10 @@
 // alone would round every weight by 2^-8, as much as a bf16 output itself, and f16
 // would lose the small ones).  Scores, maxima, sums and outputs are fp32.
 //
-// A wave takes a page of 64 slots at a time, 8 waves of a workgroup every eighth
-// page; their states are joined through LDS.  The pages of all (sequence, head,
-// rows) are numbered in one line, which is cut into equal pieces, one for each
+// A wave takes a page of 64 slots at a time.  WAYS of the 8 waves of a workgroup share a
+// row tile and take every WAYS-th page, and their states are joined through LDS; 8 / WAYS
+// row tiles go over the same pages at the same time.  The pages of all (sequence,
+// head, tiles) are numbered in one line, which is cut into equal pieces, one for each
 // workgroup, whatever the lengths are: a piece that covers all pages of its rows
 // writes their output, others write their state, which kv4_join_kernel joins.
 #include <algorithm>
@@ -41,17 +42,17 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
 }
 
-// The line of pages: those of (b, h, row tile) one after the other, b first.  It is
-// cut every `share` pages; a cut within `snap` pages of a row tile's end moves there,
-// so that no piece holds a few pages of one tile and the rest of another's.
+// The line of pages: those of (b, h, tiles of a workgroup) one after the other, b
+// first.  It is cut every `share` pages; a cut within kSnap pages of where the next tiles
+// begin moves there, so that no piece holds a few pages of some and the rest of others.
 struct Line {
-    int tiles;                 // row tiles per (b, h)
+    int tiles;                 // groups of 8 / WAYS row tiles per (b, h)
     int pieces;                // workgroups
     int min_pages;             // fewest pages of a piece
 };
 constexpr int kSnap = 8;       // one page for each wave
 
-// Where the cut at unit u comes to lie; lo, hi: the ends of the row tile that holds it.
+// Where the cut at unit u comes to lie; lo, hi: the ends of the tiles that hold it.
 __device__ __forceinline__ int snap(int u, int lo, int hi, int share) {
     const int reach = min(share / 2, kSnap);
     return u - lo <= reach ? lo : hi - u <= reach ? hi : u;
@@ -267,7 +268,7 @@ template <typename T, int D, int MT> struct Rows {
     }
 };
 
-template <typename T, int D, int MT>
+template <typename T, int D, int MT, int WAYS>
 __global__ __launch_bounds__(kKv4Threads, 2) void kv4_attention_kernel(Kv4AttentionArgs a, Line line,
                                                                                 float* __restrict__ states) {
     using S = Shape<D, MT>;
@@ -275,12 +276,12 @@ __global__ __launch_bounds__(kKv4Threads, 2) void kv4_attention_kernel(Kv4Attent
     constexpr int kRound = 32;                              // registers joined at a time
     __shared__ float s_o[kKv4Waves][kRound][64];
     __shared__ float s_m[kKv4Waves][MT], s_l[kKv4Waves][MT];
-    __shared__ typename Frag<T>::type s_q[S::KS][64];
-    static_assert(S::KS <= kKv4Waves, "a wave per step of the first product loads the queries");
+    constexpr int kTiles = kKv4Waves / WAYS;
+    __shared__ typename Frag<T>::type s_q[kTiles][S::KS][64];
 
     const Kv4Cache& c = a.cache;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int col = lane % MT, g = lane / MT;
+    const int col = lane % MT, g = lane / MT, tile = wave / WAYS, way = wave % WAYS;
     const int slots = c.slots(), group = a.q_heads / c.heads;
     // pieces that follow each other on one XCD: they share pages where a head has several row tiles
     const int piece = (int)gridDim.x % 8 ? (int)blockIdx.x
@@ -289,10 +290,14 @@ __global__ __launch_bounds__(kKv4Threads, 2) void kv4_attention_kernel(Kv4Attent
     Scan scan(a.block, c, c.heads * line.tiles);
     const int share = max(line.min_pages, (scan.total + line.pieces - 1) / line.pieces);
     if ((int64_t)piece * share >= scan.total) return;
-    int u = cut(scan, piece * share, share);
-    const int u_end = cut(scan, (int)min((int64_t)(piece + 1) * share, (int64_t)scan.total), share);
+    int u = 0, u_end = 0;
+#pragma nounroll
+    for (int e = 0; e < 2; ++e) {
+        u = u_end;
+        u_end = cut(scan, (int)min((int64_t)(piece + e) * share, (int64_t)scan.total), share);
+    }
     if (u >= u_end) return;
-    Scan::Place at = scan.place(u);
+    Scan::Place at{};
     // scores in units of the maximum: |scale| and the query's sign
     const float mag = fabsf(a.scale);
     const float unit = (mag == 0.f ? 1.f : mag) * kLog2e * (float)(1 << kKeyShift<T>);
@@ -302,22 +307,48 @@ __global__ __launch_bounds__(kKv4Threads, 2) void kv4_attention_kernel(Kv4Attent
         if (u >= at.start + at.pages * scan.per) at = scan.place(u);
         const int b = at.b;
         const int rel = u - at.start, ht = rel / at.pages, first = rel - ht * at.pages;
-        const int h = ht / line.tiles, rt = ht - h * line.tiles;
+        const int h = ht / line.tiles, rt0 = (ht - h * line.tiles) * kTiles, rt = rt0 + tile;
         const int last = min(at.pages, first + (u_end - u));
-        const int n = uniform(kv4_length(a.block.lengths, b, slots));
-        const int count = uniform(kv4_count(a.block.counts, b, a.block.T));
-        const int filled = uniform(seq_end(a.block, b, slots));   // slots past it may hold anything
+        const int n = at.n, count = at.count;
+        const int filled = seq_end(a.block, n, count, slots);     // slots past it may hold anything
         int end = filled;
         if (a.block.mode == DELS_KV4_CAUSAL)                  // no row of the tile sees past its last token
             end = (int)min((int64_t)end, (int64_t)n + (rt * MT + MT - 1) / group + 1);
+        if (rt * MT >= a.block.T * group) end = 0;            // past the block's rows
         const int stop = min(last, (end + kKv4Page - 1) / kKv4Page);
 
         // the wave's pages, the next one loaded while one is worked on
         const int32_t* ids = c.table + (int64_t)b * c.ld_table;
         const uint8_t* heads = c.data + (int64_t)h * Kv4<D>::kBytes;
         const int64_t page_stride = (int64_t)c.heads * Kv4<D>::kBytes;
-        int p = first + wave;
+        int p = first + way;
+        // the numbers of the wave's next 64 pages, one a lane: a load per page would be
+        // waited for with the first read of LDS
+        int ids64, base;
+        auto fetch_ids = [&](int from) {
+            base = from;
+            const int at_page = from + lane * WAYS;
+            ids64 = at_page < stop ? ids[at_page] : -1;
+        };
+        auto id_at = [&](int at_page) {
+            if (at_page - base >= 64 * WAYS) fetch_ids(at_page);
+            return __builtin_amdgcn_readlane(ids64, (at_page - base) / WAYS);
+        };
+        fetch_ids(p);
 
+        // the queries of all tiles, in operand order
+        constexpr int kPerWave = (kTiles * S::KS + kKv4Waves - 1) / kKv4Waves;
+        u32x4 qw[kPerWave];
+#pragma unroll
+        for (int i = 0; i < kPerWave; ++i) {
+            const int e = wave + i * kKv4Waves, k = e % S::KS;
+            const Row of = row_of((rt0 + e / S::KS) * MT + col, group, h, a.block.T, count);
+            qw[i] = u32x4{0u, 0u, 0u, 0u};
+            if (of.valid && e < kTiles * S::KS)
+                qw[i] = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q.p) + (int64_t)b * a.q.batch +
+                                                        (int64_t)of.t * a.q.token + (int64_t)of.hq * a.q.head +
+                                                        g * S::DL + 8 * k);
+        }
         const Row row = row_of(rt * MT + col, group, h, a.block.T, count);
         Rows<T, D, MT> rows;
         rows.bits = 0;
@@ -329,17 +360,6 @@ __global__ __launch_bounds__(kKv4Threads, 2) void kv4_attention_kernel(Kv4Attent
                             (count >= 64 ? ~0ull : (1ull << count) - 1);
         }
         rows.lim = min(rows.lim, slots);
-        // the queries, in operand order: a wave loads what all of them read
-        if (wave < S::KS) {
-            u32x4 w = {0u, 0u, 0u, 0u};
-            if (row.valid)
-                w = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q.p) + (int64_t)b * a.q.batch +
-                                                    (int64_t)row.t * a.q.token + (int64_t)row.hq * a.q.head +
-                                                    g * S::DL + 8 * wave);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = (w[i] ^ flip) & zero;
-            s_q[wave][lane] = __builtin_bit_cast(typename Frag<T>::type, w);
-        }
         rows.top = -__builtin_inff();
         rows.total = 0.f;
 #pragma unroll
@@ -347,43 +367,35 @@ __global__ __launch_bounds__(kKv4Threads, 2) void kv4_attention_kernel(Kv4Attent
 #pragma unroll
             for (int i = 0; i < S::ACC; ++i) rows.o[t][i] = 0.f;
 
-        __syncthreads();
-        auto named = [&](int id) { return id >= 0 && id < c.num_pages; };
-        // Pages p, p + 8, ... below `stop`; one that the table does not name is passed over.
+        // Pages p, p + WAYS, ... below `stop`; one that the table does not name is passed over.
         // Keys are loaded a page ahead, values at the start of their page's work.  The
         // loads are unconditional (of page 0 where there is none to load) and in this
         // order, so that each wait covers only what it needs.  One copy of the work: two
         // that swap the keys' registers take longer to fetch than their moves.
+        auto named = [&](int id) { return id >= 0 && id < c.num_pages; };
         auto address = [&](int id) { return heads + (named(id) ? id : 0) * page_stride; };
-        if (p < stop) {
-            // the numbers of the wave's next 64 pages, one a lane: a load per page would be
-            // waited for with the first read of LDS
-            int ids64 = -1, base = 0;
-            auto fetch_ids = [&](int from) {
-                base = from;
-                const int at_page = from + lane * kKv4Waves;
-                ids64 = at_page < stop ? ids[at_page] : -1;
-            };
-            auto id_at = [&](int at_page) {
-                if (at_page - base >= 64 * kKv4Waves) fetch_ids(at_page);
-                return __builtin_amdgcn_readlane(ids64, (at_page - base) / kKv4Waves);
-            };
-            fetch_ids(p);
-            KeyWords<D, MT> keys, next_keys;
-            ValueWords<D, MT> values;
-            int id = id_at(p), next = id_at(p + kKv4Waves);
-            keys.load(address(id), at_lane);
-            for (; p < stop; p += kKv4Waves) {
-                values.load(address(id), at_lane);
-                asm volatile("" ::: "memory");
-                next_keys.load(address(next), at_lane);
-                asm volatile("" ::: "memory");
-                if (named(id))
-                    rows.page(&s_q[0][lane], keys, values, at_lane.half, p * kKv4Page, n, filled, slots, g, unit);
-                keys = next_keys;
-                id = next;
-                next = id_at(p + 2 * kKv4Waves);
-            }
+        KeyWords<D, MT> keys, next_keys;
+        ValueWords<D, MT> values;
+        int id = id_at(p), next = id_at(p + WAYS);
+        if (p < stop) keys.load(address(id), at_lane);
+#pragma unroll
+        for (int i = 0; i < kPerWave; ++i) {
+            const int e = wave + i * kKv4Waves;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) qw[i][x] = (qw[i][x] ^ flip) & zero;
+            if (e < kTiles * S::KS) s_q[e / S::KS][e % S::KS][lane] = __builtin_bit_cast(typename Frag<T>::type, qw[i]);
+        }
+        lds_barrier();                                        // the keys stay in flight
+        for (; p < stop; p += WAYS) {
+            values.load(address(id), at_lane);
+            asm volatile("" ::: "memory");
+            next_keys.load(address(next), at_lane);
+            asm volatile("" ::: "memory");
+            if (named(id))
+                rows.page(&s_q[tile][0][lane], keys, values, at_lane.half, p * kKv4Page, n, filled, slots, g, unit);
+            keys = next_keys;
+            id = next;
+            next = id_at(p + 2 * WAYS);
         }
 
         // ---- join the waves
@@ -395,12 +407,12 @@ __global__ __launch_bounds__(kKv4Threads, 2) void kv4_attention_kernel(Kv4Attent
         }
         __syncthreads();
         const bool whole = first == 0 && last == at.pages;
-        float* state = states + (int64_t)(2 * piece + (first == 0 ? 1 : 0)) * kStateFloats<D, MT>;
+        float* state = states + ((int64_t)(2 * piece + (first == 0 ? 1 : 0)) * kTiles + tile) * kStateFloats<D, MT>;
         float m = -__builtin_inff(), l = 0.f;
 #pragma unroll
-        for (int w = 0; w < kKv4Waves; ++w) m = fmaxf(m, s_m[w][col]);
+        for (int w = tile * WAYS; w < (tile + 1) * WAYS; ++w) m = fmaxf(m, s_m[w][col]);
 #pragma unroll
-        for (int w = 0; w < kKv4Waves; ++w) l += s_l[w][col] * fade(s_m[w][col], m);
+        for (int w = tile * WAYS; w < (tile + 1) * WAYS; ++w) l += s_l[w][col] * fade(s_m[w][col], m);
         const float f = fade(ref, m), inv = l > 0.f ? 1.f / l : 0.f;
 #pragma unroll
         for (int r0 = 0; r0 < kRegs; r0 += kRound) {
@@ -411,13 +423,13 @@ __global__ __launch_bounds__(kKv4Threads, 2) void kv4_attention_kernel(Kv4Attent
                 s_o[wave][j][lane] = rows.o[vl * S::VW + v][i] * f;
             }
             __syncthreads();
-            for (int jg = wave; jg * S::VW < kRound && r0 + jg * S::VW < kRegs; jg += kKv4Waves) {
+            for (int jg = way; jg * S::VW < kRound && r0 + jg * S::VW < kRegs; jg += WAYS) {
                 float sum[S::VW];
 #pragma unroll
                 for (int v = 0; v < S::VW; ++v) {
                     sum[v] = 0.f;
 #pragma unroll
-                    for (int w = 0; w < kKv4Waves; ++w) sum[v] += s_o[w][jg * S::VW + v][lane];
+                    for (int w = 0; w < WAYS; ++w) sum[v] += s_o[tile * WAYS + w][jg * S::VW + v][lane];
                 }
                 const int gi = r0 / S::VW + jg;
                 if (whole) {
@@ -430,7 +442,7 @@ __global__ __launch_bounds__(kKv4Threads, 2) void kv4_attention_kernel(Kv4Attent
             }
             __syncthreads();
         }
-        if (wave == 0 && g == 0) {
+        if (way == 0 && g == 0) {
             if (whole) {
                 store_lse(a, b, row, m, l);
             } else {
@@ -445,14 +457,17 @@ __global__ __launch_bounds__(kKv4Threads, 2) void kv4_attention_kernel(Kv4Attent
 // Joins the states of the rows whose pages lie in several pieces.  Grid (sequence x
 // head x row tile, quarter of the output registers), a wave per VW channels.
 constexpr int kJoinWaves = 4;
-template <typename T, int D, int MT>
+template <typename T, int D, int MT, int WAYS>
 __global__ __launch_bounds__(64 * kJoinWaves) void kv4_join_kernel(Kv4AttentionArgs a, Line line,
                                                                    const float* __restrict__ states) {
     using S = Shape<D, MT>;
     const Kv4Cache& c = a.cache;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane % MT, g = lane / MT;
+    constexpr int kTiles = kKv4Waves / WAYS;
     const int per = c.heads * line.tiles, group = a.q_heads / c.heads;
-    const int b = blockIdx.x / per, ht = blockIdx.x % per, h = ht / line.tiles, rt = ht % line.tiles;
+    const int b = blockIdx.x / (per * kTiles), ht = blockIdx.x / kTiles % per, h = ht / line.tiles;
+    const int tile = blockIdx.x % kTiles, rt = ht % line.tiles * kTiles + tile;
+    if (rt * MT >= a.block.T * group) return;
     Scan scan(a.block, c, per);
     const int share = max(line.min_pages, (scan.total + line.pieces - 1) / line.pieces);
     int before = 0;                                         // pages of the sequences before b
@@ -466,7 +481,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void kv4_join_kernel(Kv4AttentionA
     while (w0 < w1 && snap(w0 * share, lo, hi, share) == lo) ++w0;
     while (w0 < w1 && snap((w1 - 1) * share, lo, hi, share) == hi) --w1;
     if (w0 >= w1) return;                                   // one piece covered them and wrote the output
-    auto state_of = [&](int w) { return states + (int64_t)(2 * w + (w < w0 ? 1 : 0)) * kStateFloats<D, MT>; };
+    auto state_of = [&](int w) { return states + ((int64_t)(2 * w + (w < w0 ? 1 : 0)) * kTiles + tile) * kStateFloats<D, MT>; };
     float m = -__builtin_inff(), l = 0.f;
 #pragma unroll 4
     for (int w = w0 - 1; w < w1; ++w) m = fmaxf(m, state_of(w)[MT * D + col]);
@@ -488,17 +503,24 @@ __global__ __launch_bounds__(64 * kJoinWaves) void kv4_join_kernel(Kv4AttentionA
     if (gi == 0 && g == 0) store_lse(a, b, row, m, l);
 }
 
-struct Plan { int rows; Line line; };
+struct Plan { int rows, ways; Line line; };
 
 Plan plan(int64_t batch, int64_t T, int64_t q_heads, int64_t heads, int64_t max_pages) {
     Plan p{};
     const int64_t rows = T * (q_heads / heads);
     p.rows = rows <= 16 ? 16 : 32;
-    p.line.tiles = (int)((rows + p.rows - 1) / p.rows);
+    const int64_t tiles = (rows + p.rows - 1) / p.rows, cus = device_cu_count();
+    // Many row tiles: four of them a workgroup, two waves each, once that fills the GPU
+    // (and hardly a wave is without a tile): a wave has more pages to itself and one state
+    // to be joined with.  2 x 512 rows of 4 heads a group over 4000 slots: 138 us with
+    // eight waves on a tile, 131 so.
+    const int64_t fours = (tiles + 3) / 4;
+    p.ways = p.rows == 32 && batch * heads * fours >= cus && 8 * tiles >= 7 * 4 * fours ? 2 : 8;
+    const int per = kKv4Waves / p.ways;
+    p.line.tiles = (int)((tiles + per - 1) / per);
     p.line.min_pages = kKv4Waves;
     const int64_t units = batch * heads * p.line.tiles * std::max<int64_t>(max_pages, 1);
-    const int64_t resident = (int64_t)device_cu_count();
-    p.line.pieces = (int)std::min<int64_t>(resident, (units + p.line.min_pages - 1) / p.line.min_pages);
+    p.line.pieces = (int)std::min<int64_t>(cus, (units + p.line.min_pages - 1) / p.line.min_pages);
     return p;
 }
 
@@ -507,7 +529,7 @@ Plan plan(int64_t batch, int64_t T, int64_t q_heads, int64_t heads, int64_t max_
 size_t kv4_attention_data_bytes(int64_t batch, int64_t T, int64_t q_heads, int64_t heads, int64_t head_dim,
                                 int64_t max_pages) {
     const Plan p = plan(batch, T, q_heads, heads, max_pages);
-    return align256((size_t)p.line.pieces * 2 * sizeof(float) * (p.rows * head_dim + 2 * p.rows));
+    return align256((size_t)p.line.pieces * 2 * (kKv4Waves / p.ways) * sizeof(float) * (p.rows * head_dim + 2 * p.rows));
 }
 
 hipError_t launch_kv4_attention(const Kv4AttentionArgs& a, void* ws, size_t data_off, hipStream_t s) {
@@ -519,11 +541,19 @@ hipError_t launch_kv4_attention(const Kv4AttentionArgs& a, void* ws, size_t data
         constexpr int D = decltype(size)::value, MT = decltype(rows)::value;
         using S = Shape<D, MT>;
         static_assert(S::CT * S::ACC / S::VW % kJoinWaves == 0, "a wave of the join per VW channels");
-        hipLaunchKernelGGL((kv4_attention_kernel<T, D, MT>), dim3(p.line.pieces), dim3(kKv4Threads), 0, s, a, p.line,
-                           states);
-        hipLaunchKernelGGL((kv4_join_kernel<T, D, MT>),
-                           dim3((unsigned)c.batch * c.heads * p.line.tiles, S::CT * S::ACC / S::VW / kJoinWaves),
-                           dim3(64 * kJoinWaves), 0, s, a, p.line, states);
+        auto go = [&](auto ways) {
+            constexpr int WAYS = decltype(ways)::value;
+            hipLaunchKernelGGL((kv4_attention_kernel<T, D, MT, WAYS>), dim3(p.line.pieces), dim3(kKv4Threads), 0, s, a,
+                               p.line, states);
+            hipLaunchKernelGGL((kv4_join_kernel<T, D, MT, WAYS>),
+                               dim3((unsigned)c.batch * c.heads * p.line.tiles * (kKv4Waves / WAYS),
+                                    S::CT * S::ACC / S::VW / kJoinWaves),
+                               dim3(64 * kJoinWaves), 0, s, a, p.line, states);
+        };
+        if constexpr (MT == 32) {
+            if (p.ways == 2) return go(std::integral_constant<int, 2>{});
+        }
+        go(std::integral_constant<int, 8>{});
     });
 }
 

@@ -104,25 +104,27 @@ template <int D, int MT_> struct Shape {
     }
 };
 
-__device__ __forceinline__ int seq_end(const Kv4Block& k, int b, int slots) {
-    const int n = kv4_length(k.lengths, b, slots);
-    if (k.mode == DELS_KV4_NONE) return n;
-    return (int)min((int64_t)slots, (int64_t)n + kv4_count(k.counts, b, k.T));
+// Where a sequence's slots that hold anything end, and its pages (one at least: rows that
+// see nothing are written too).
+__device__ __forceinline__ int seq_end(const Kv4Block& k, int n, int count, int slots) {
+    return k.mode == DELS_KV4_NONE ? n : (int)min((int64_t)slots, (int64_t)n + count);
 }
-// Pages of sequence b (one at least: rows that see nothing are written too).
+__device__ __forceinline__ int seq_pages(int end) { return max(1, (end + kKv4Page - 1) / kKv4Page); }
 __device__ __forceinline__ int seq_pages(const Kv4Block& k, int b, int slots) {
-    return max(1, (seq_end(k, b, slots) + kKv4Page - 1) / kKv4Page);
+    return seq_pages(seq_end(k, kv4_length(k.lengths, b, slots), kv4_count(k.counts, b, k.T), slots));
 }
 
 // What all lanes of a wave hold alike, kept in a scalar register.
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
-// Scan of the sequences' units by a wave, 64 at a time; up to 64 it is kept.
+// Scan of the sequences' units by a wave, 64 at a time; up to 64 it is kept, with what
+// was loaded for it.
 struct Scan {
     const Kv4Block& k;
     const Kv4Cache& c;
     int per;                   // row tiles of a sequence
-    int own, cum;              // units of this lane's sequence, and of all up to it, in the 64 from b0
+    int n, count, pages;       // context, valid rows and pages of this lane's sequence
+    int cum;                   // units of all up to it, in the 64 from b0
     int b0, before, total;
 
     __device__ Scan(const Kv4Block& k_, const Kv4Cache& c_, int per_) : k(k_), c(c_), per(per_) {
@@ -139,26 +141,31 @@ struct Scan {
         }
     }
     __device__ void seek(int b0_, int before_) {
-        const int lane = threadIdx.x & 63;
+        const int lane = threadIdx.x & 63, slots = c.slots();
         b0 = b0_, before = before_;
-        own = b0 + lane < c.batch ? seq_pages(k, b0 + lane, c.slots()) * per : 0;
-        cum = own;
+        n = count = pages = 0;
+        if (b0 + lane < c.batch) {
+            n = kv4_length(k.lengths, b0 + lane, slots);
+            count = kv4_count(k.counts, b0 + lane, k.T);
+            pages = seq_pages(seq_end(k, n, count, slots));
+        }
+        cum = pages * per;
 #pragma unroll
         for (int off = 1; off < 64; off <<= 1) {
             const int o = __shfl_up(cum, off, 64);
             cum += lane >= off ? o : 0;
         }
     }
-    // Sequence of unit u < total, its first unit and its pages.
-    struct Place { int b, start, pages; };
+    // Sequence of unit u < total, its first unit, its pages, context and valid rows.
+    struct Place { int b, start, pages, n, count; };
     __device__ Place place(int u) {
         if (u < before) seek(0, 0);
         for (;;) {
             const unsigned long long past = __ballot(before + cum > u);
             if (past) {
-                const int l = __builtin_ctzll(past);
-                return {b0 + l, __builtin_amdgcn_readlane(before + cum - own, l),
-                        __builtin_amdgcn_readlane(own, l) / per};
+                const int l = __builtin_ctzll(past), p = __builtin_amdgcn_readlane(pages, l);
+                return {b0 + l, before + __builtin_amdgcn_readlane(cum, l) - p * per, p,
+                        __builtin_amdgcn_readlane(n, l), __builtin_amdgcn_readlane(count, l)};
             }
             const int all = __builtin_amdgcn_readlane(cum, 63);
             seek(b0 + 64, before + all);

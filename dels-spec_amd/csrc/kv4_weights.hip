@@ -48,10 +48,9 @@ __global__ __launch_bounds__(kKv4Threads, 4) void kv4_weights_kernel(Kv4WeightsA
         if (u >= at.start + at.pages * scan.per) at = scan.place(u);
         const int b = at.b, rel = u - at.start, h = rel / at.pages, first = rel - h * at.pages;
         const int last = min(at.pages, first + (u_end - u));
-        const int n = uniform(kv4_length(a.block.lengths, b, slots));
-        const int count = uniform(kv4_count(a.block.counts, b, a.block.T));
+        const int n = at.n, count = at.count;
         const int rows = uniform(min(kv4_count(a.accepted, b, a.block.T), count)) * group;
-        const int filled = uniform(seq_end(a.block, b, slots));
+        const int filled = seq_end(a.block, n, count, slots);
         const int32_t* ids = c.table + (int64_t)b * c.ld_table;
         const uint8_t* heads = c.data + (int64_t)h * Kv4<D>::kBytes;
         const int64_t page_stride = (int64_t)c.heads * Kv4<D>::kBytes;
@@ -180,10 +179,23 @@ __global__ __launch_bounds__(kKv4Threads, 4) void kv4_weights_kernel(Kv4WeightsA
     }
 }
 
+// A cache of no pages: the old weights, cut off at the lengths.
+__global__ void kv4_no_weights_kernel(Kv4WeightsArgs a) {
+    const int slots = a.cache.slots(), b = blockIdx.y / a.cache.heads;
+    const int n = kv4_length(a.block.lengths, b, slots);
+    const int64_t row = (int64_t)blockIdx.y * slots;
+    for (int j = blockIdx.x * blockDim.x + threadIdx.x; j < slots; j += gridDim.x * blockDim.x)
+        a.out[row + j] = j < n ? a.weights[row + j] : 0.f;
+}
+
 }  // namespace
 
 hipError_t launch_kv4_weights(const Kv4WeightsArgs& a, hipStream_t s) {
     const Kv4Cache& c = a.cache;
+    if (c.num_pages == 0) {
+        hipLaunchKernelGGL(kv4_no_weights_kernel, dim3((c.slots() + 1023) / 1024, c.batch * c.heads), dim3(256), 0, s, a);
+        return hipGetLastError();
+    }
     const int64_t units = (int64_t)c.batch * c.heads * c.max_pages;
     // two workgroups a CU: 32 x 16k slots 74 us with one, 68 so
     const int pieces = (int)std::min<int64_t>(2 * device_cu_count(), (units + kMinPages - 1) / kMinPages);

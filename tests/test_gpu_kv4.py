@@ -228,6 +228,68 @@ def test_attention_rising_scores(pkg, dev):
     check_attention(cache, q, "bf16", "none", [n], None, None, 1.0, out, lse)
 
 
+@pytest.mark.parametrize("B,H,T,G,D,dtype,block,ragged", [
+    (32, 8, 32, 4, 64, "bf16", "causal", True),             # 4 row tiles
+    (20, 4, 75, 3, 64, "f16", "full", False),               # 8, the last one of one row
+    (16, 8, 64, 8, 128, "bf16", "mask", True),              # 16
+])
+def test_attention_of_many_row_tiles(pkg, dev, B, H, T, G, D, dtype, block, ragged):
+    """Sizes at which a workgroup takes several row tiles: every row against 64-bit products."""
+    say("attention many tiles", B, H, T, G, D, dtype, block)
+    pages = 3
+    counts = [1 + (7 * b) % T for b in range(B)] if ragged else None
+    lengths = [(13 * b + 5) % (192 - T) for b in range(B)]
+    cache, q, masks = attention_inputs(pkg, dev, B, T, H * G, H, D, pages, dtype, block, lengths, counts, B)
+    out, lse = pkg.kv4_attention(q.to(dev), cache, ints(lengths, dev), counts=ints(counts, dev),
+                                 block=block if masks is None else masks.to(dev))
+    torch.cuda.synchronize()
+    K, V = (torch.tensor(x).to(dev) for x in contents(cache))
+    q64 = q.double().to(dev).view(B, T, H, G, D)
+    n, c = ints(lengths, dev)[:, None, None], ints([T] * B if counts is None else counts, dev)[:, None, None]
+    j, t = torch.arange(192, device=dev)[None, None], torch.arange(T, device=dev)[None, :, None]
+    inside = (j >= n) & (j - n < c)
+    if masks is not None:
+        inside = inside & ((masks.to(dev)[:, :, None] >> (j - n).clamp(0, 63)) & 1).bool()
+    elif block == "causal":
+        inside = inside & (j - n <= t)
+    seen = ((j < n) | inside) & (t < c)
+    for b in range(B):
+        x = torch.einsum("thgd,hjd->thgj", q64[b], K[b]) * D ** -0.5
+        mass = torch.einsum("thgd,hjd->thgj", q64[b].abs(), K[b].abs()) * D ** -0.5
+        mass = mass.masked_fill(~seen[b][:, None, None], 0).amax(-1)
+        x = x.masked_fill(~seen[b][:, None, None], float("-inf"))
+        rl = torch.logsumexp(x, -1)
+        p = torch.exp(x - torch.where(rl > float("-inf"), rl, torch.zeros_like(rl))[..., None])
+        ro = torch.einsum("thgj,hjd->thgd", p, V[b])
+        weight = torch.einsum("thgj,hjd->thgd", p, V[b].abs())
+        err = mass * 2.0 ** -16 + (q64[b].abs().sum(-1) * D ** -0.5 * 2.0 ** -20 if dtype == "f16" else 0)
+        assert torch.all((out[b].double().view(T, H, G, D) - ro).abs()
+                         <= weight * (2.0 ** -8 * 1.01 + 2 * err[..., None]) + 1e-30), b
+        got = lse[b].double().view(T, H, G)
+        f = rl > float("-inf")
+        assert torch.equal(f, got > float("-inf"))
+        assert torch.all((got[f] - rl[f]).abs() <= err[f] + 2.0 ** -20 * (1 + rl[f].abs()))
+
+
+def test_cache_of_no_pages(pkg, dev):
+    say("no pages")
+    cache = pkg.KV4Cache(torch.empty(0, 2, 4352, dtype=torch.uint8, device=dev),
+                         torch.zeros(2, 3, dtype=torch.int32, device=dev), 64)
+    n = ints([100, 0], dev)
+    q, kv = (torch.randn(2, 3, h, 64, device=dev).to(torch.bfloat16) for h in (4, 2))
+    pkg.kv4_append(cache, kv, kv, n)
+    k, v = pkg.kv4_read(cache, n, 3)
+    out, lse = pkg.kv4_attention(q, cache, n)
+    w = torch.rand(2, 2, 192, device=dev)
+    nw = pkg.kv4_weights(q, cache, n, lse, w)
+    nl, ew, source = pkg.kv4_evict(cache, n, w, 10, 2)
+    torch.cuda.synchronize()
+    assert not k.any() and not v.any() and not out.any() and torch.all(lse == float("-inf"))
+    assert torch.equal(nw[0, :, :100], w[0, :, :100]) and not nw[0, :, 100:].any() and not nw[1].any()
+    assert nl.tolist() == [10, 0] and torch.all(source[1] == -1)
+    assert torch.equal(ew[0, 0, :10], w[0, 0][source[0, 0].long()])
+
+
 def test_attention_takes_strides_given_outputs_and_other_streams(pkg, dev):
     say("attention strides")
     B, T, HQ, H, D = 2, 5, 4, 2, 64
@@ -355,6 +417,29 @@ def test_evict_keeps_the_oracles_slots(pkg, dev, B, H, D, pages, lengths, keep, 
             for x, y in zip(after, before):
                 assert np.array_equal(x[b, h, :m], y[b, h][ref[:m]])
                 assert np.array_equal(x[b, h, keep:], y[b, h, keep:])
+
+
+@pytest.mark.parametrize("n,keep,recent,kind", [(5100, 900, 40, "rand"), (4480, 4000, 0, "ties"),
+                                                (17000, 5000, 300, "rand"), (33001, 16500, 16000, "ties")])
+def test_evict_from_long_sequences(pkg, dev, n, keep, recent, kind):
+    """More slots than one walk of the selection holds, with the budget inside and past the first."""
+    say("evict long", n, keep, recent, kind)
+    pages = -(-n // 64)
+    data = torch.randint(0, 256, (pages, 1, 4352), generator=torch.Generator().manual_seed(n), dtype=torch.uint8)
+    cache = pkg.KV4Cache(data.to(dev), torch.arange(pages - 1, -1, -1, dtype=torch.int32, device=dev)[None], 64)
+    g = torch.Generator().manual_seed(keep)
+    w = torch.exp(3 * torch.randn(1, 1, cache.slots, generator=g))
+    if kind == "ties":
+        w = torch.randint(0, 5, w.shape, generator=g).float()
+    k0, v0 = pkg.kv4_read(cache, ints([0], dev), n, dtype=torch.float32)
+    _, nw, source = pkg.kv4_evict(cache, ints([n], dev), w.to(dev), keep, recent)
+    k1, v1 = pkg.kv4_read(cache, ints([0], dev), keep, dtype=torch.float32)
+    torch.cuda.synchronize()
+    ref = torch.tensor(O.evict(w[0, 0, :n].double().numpy(), n, keep, recent))
+    assert torch.equal(source[0, 0].cpu().long(), ref)
+    assert torch.equal(nw[0, 0, :keep].cpu(), w[0, 0][ref]) and not nw[0, 0, keep:].any()
+    for a, b in ((k0, k1), (v0, v1)):
+        assert torch.equal(a[0, ref.to(dev)].view(torch.int32), b[0].view(torch.int32))
 
 
 # ---- together -------------------------------------------------------------------------
