@@ -455,7 +455,7 @@ __global__ __launch_bounds__(kKv4Threads, 2) void kv4_attention_kernel(Kv4Attent
 }
 
 // Joins the states of the rows whose pages lie in several pieces.  Grid (sequence x
-// head x row tile, quarter of the output registers), a wave per VW channels.
+// head x row tile, parts of the output registers), a wave per VW channels in turn.
 constexpr int kJoinWaves = 4;
 template <typename T, int D, int MT, int WAYS>
 __global__ __launch_bounds__(64 * kJoinWaves) void kv4_join_kernel(Kv4AttentionArgs a, Line line,
@@ -484,23 +484,29 @@ __global__ __launch_bounds__(64 * kJoinWaves) void kv4_join_kernel(Kv4AttentionA
     auto state_of = [&](int w) { return states + ((int64_t)(2 * w + (w < w0 ? 1 : 0)) * kTiles + tile) * kStateFloats<D, MT>; };
     float m = -__builtin_inff(), l = 0.f;
 #pragma unroll 4
-    for (int w = w0 - 1; w < w1; ++w) m = fmaxf(m, state_of(w)[MT * D + col]);
-    const int gi = blockIdx.y * kJoinWaves + wave;
-    float sum[S::VW];
-#pragma unroll
-    for (int v = 0; v < S::VW; ++v) sum[v] = 0.f;
-#pragma unroll 4
     for (int w = w0 - 1; w < w1; ++w) {
-        const float* st = state_of(w);
-        const float f = fade(st[MT * D + col], m);
-        l += st[MT * D + MT + col] * f;
-        const float* from = st + (gi * 64 + lane) * S::VW;
-#pragma unroll
-        for (int v = 0; v < S::VW; ++v) sum[v] += from[v] * f;
+        const float part = state_of(w)[MT * D + col], sum = state_of(w)[MT * D + MT + col];
+        const float now = fmaxf(m, part);
+        l = l * fade(m, now) + sum * fade(part, now);
+        m = now;
     }
+    const float inv = l > 0.f ? 1.f / l : 0.f;
     const Row row = row_of(rt * MT + col, group, h, a.block.T, kv4_count(a.block.counts, b, a.block.T));
-    store_out<T, S::VW>(a, b, row, S::channel_of(gi / S::ACC, gi % S::ACC, g), sum, l > 0.f ? 1.f / l : 0.f);
-    if (gi == 0 && g == 0) store_lse(a, b, row, m, l);
+    for (int gi = blockIdx.y * kJoinWaves + wave; gi < S::CT * S::ACC / S::VW; gi += gridDim.y * kJoinWaves) {
+        float sum[S::VW];
+#pragma unroll
+        for (int v = 0; v < S::VW; ++v) sum[v] = 0.f;
+#pragma unroll 4
+        for (int w = w0 - 1; w < w1; ++w) {
+            const float* st = state_of(w);
+            const float f = fade(st[MT * D + col], m);
+            const float* from = st + (gi * 64 + lane) * S::VW;
+#pragma unroll
+            for (int v = 0; v < S::VW; ++v) sum[v] += from[v] * f;
+        }
+        store_out<T, S::VW>(a, b, row, S::channel_of(gi / S::ACC, gi % S::ACC, g), sum, inv);
+    }
+    if (blockIdx.y == 0 && wave == 0 && g == 0) store_lse(a, b, row, m, l);
 }
 
 struct Plan { int rows, ways; Line line; };
@@ -545,10 +551,11 @@ hipError_t launch_kv4_attention(const Kv4AttentionArgs& a, void* ws, size_t data
             constexpr int WAYS = decltype(ways)::value;
             hipLaunchKernelGGL((kv4_attention_kernel<T, D, MT, WAYS>), dim3(p.line.pieces), dim3(kKv4Threads), 0, s, a,
                                p.line, states);
-            hipLaunchKernelGGL((kv4_join_kernel<T, D, MT, WAYS>),
-                               dim3((unsigned)c.batch * c.heads * p.line.tiles * (kKv4Waves / WAYS),
-                                    S::CT * S::ACC / S::VW / kJoinWaves),
-                               dim3(64 * kJoinWaves), 0, s, a, p.line, states);
+            // few row tiles: their channels over several workgroups
+            const unsigned tiles = (unsigned)c.batch * c.heads * p.line.tiles * (kKv4Waves / WAYS);
+            const unsigned parts = (int)tiles <= device_cu_count() ? S::CT * S::ACC / S::VW / kJoinWaves : 1;
+            hipLaunchKernelGGL((kv4_join_kernel<T, D, MT, WAYS>), dim3(tiles, parts), dim3(64 * kJoinWaves), 0, s, a,
+                               p.line, states);
         };
         if constexpr (MT == 32) {
             if (p.ways == 2) return go(std::integral_constant<int, 2>{});
