@@ -110,7 +110,8 @@ int dels_kv4_append(const dels_kv4_cache* p, const void* k, int64_t k_batch, int
     if (rc != DELS_OK) return rc;
     if ((rc = check_type(dtype, true)) != DELS_OK) return rc;
     if (!extent_ok(T)) return fail(DELS_ERR_INVALID_ARGUMENT, "bad block length %lld", (long long)T);
-    if (!grid_ok({c.batch, c.heads, T / 8 + 2})) return fail(DELS_ERR_UNSUPPORTED, "shape past the supported extents");
+    if (!grid_ok({c.batch, c.heads, T / 8 + 2}) || c.batch > 65535 || c.heads > 65535)
+        return fail(DELS_ERR_UNSUPPORTED, "shape past the supported extents");
     if (c.batch == 0 || T == 0) return DELS_OK;
     if ((rc = check_rows(k, k_batch, k_token, k_head, dtype, "k")) != DELS_OK) return rc;
     if ((rc = check_rows(v, v_batch, v_token, v_head, dtype, "v")) != DELS_OK) return rc;
@@ -128,7 +129,8 @@ int dels_kv4_read(const dels_kv4_cache* p, const int32_t* starts, const int32_t*
     if (rc != DELS_OK) return rc;
     if ((rc = check_type(dtype, true)) != DELS_OK) return rc;
     if (!extent_ok(T)) return fail(DELS_ERR_INVALID_ARGUMENT, "bad block length %lld", (long long)T);
-    if (!grid_ok({c.batch, c.heads, T / 8 + 2})) return fail(DELS_ERR_UNSUPPORTED, "shape past the supported extents");
+    if (!grid_ok({c.batch, c.heads, T / 8 + 2}) || c.batch > 65535 || c.heads > 65535)
+        return fail(DELS_ERR_UNSUPPORTED, "shape past the supported extents");
     if (c.batch == 0 || T == 0) return DELS_OK;
     if (!starts || !k || !v) return fail(DELS_ERR_INVALID_ARGUMENT, "starts, k or v is NULL");
     if (!aligned(k, 16) || !aligned(v, 16)) return fail(DELS_ERR_ALIGNMENT, "k and v must be 16-byte aligned");

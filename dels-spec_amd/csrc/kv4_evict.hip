@@ -58,7 +58,7 @@ __global__ __launch_bounds__(THREADS) void kv4_select_kernel(Kv4EvictArgs a, int
     constexpr int kWaves = THREADS / 64, kTile = THREADS * kPerLane, kOwn = kBins / THREADS;
     __shared__ uint32_t s_hist[COPIES][kBins];
     __shared__ int s_wave[kWaves];
-    __shared__ uint32_t s_pick, s_left;
+    __shared__ uint32_t s_pick, s_left, s_held;
     __shared__ int s_count[3][kWaves];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int bh = blockIdx.x, h = bh % a.cache.heads, b = bh / a.cache.heads;
@@ -113,16 +113,19 @@ __global__ __launch_bounds__(THREADS) void kv4_select_kernel(Kv4EvictArgs a, int
         uint32_t before = (uint32_t)(over_waves<kWaves>(s_wave).x + upto) - own;
 #pragma unroll
         for (int i = 0; i < kOwn; ++i) {
-            if (before < left && left <= before + c[i]) s_pick = kBins - 1 - (kOwn * tid + i), s_left = left - before;
+            if (before < left && left <= before + c[i])
+                s_pick = kBins - 1 - (kOwn * tid + i), s_left = left - before, s_held = c[i];
             before += c[i];
         }
         __syncthreads();
         prefix = (prefix << digit_bits) | s_pick;
         left = s_left;
         bits_left = shift;
+        const bool all = s_held == left;           // every key of the prefix is kept: its other bits do not matter
         __syncthreads();
+        if (all) break;
     }
-    // keys above `prefix` are kept, and the first `left` of those equal to it
+    // keys whose bits so far are above `prefix` are kept, and the first `left` of those equal to it
     const bool none = keep == recent;
     int32_t* holes = hole_list + (int64_t)bh * keep;
     int equal_before = 0, hole_before = 0, mover_before = 0;
@@ -137,7 +140,7 @@ __global__ __launch_bounds__(THREADS) void kv4_select_kernel(Kv4EvictArgs a, int
 #pragma unroll
         for (int i = 0; i < kPerLane; ++i) {
             const int j = first + 64 * i;
-            const uint32_t key = weight_key(x[i]);
+            const uint32_t key = weight_key(x[i]) >> bits_left;
             const bool eq = j < cand && !none && key == prefix;
             if (j < n && (j >= cand || (!none && key > prefix))) kept |= 1u << i;
             if (eq) equal |= 1u << i;

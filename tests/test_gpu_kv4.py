@@ -129,6 +129,30 @@ def test_read_gives_the_values_of_slots(pkg, dev, B, T, H, D, dtype, lengths, co
         assert torch.equal(got.cpu(), torch.tensor(x).float().to(DT[dtype]))
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_append_rounds_ties_and_their_neighbours(pkg, dev, dtype):
+    """Values at every threshold times their row's scale, and one unit of their type to either side."""
+    say("append ties", dtype)
+    D, T = 128, 600
+    g = torch.Generator().manual_seed(5)
+    amax = torch.exp(torch.randn(T, generator=g) * 3).clamp(1e-3, 6e4).to(DT[dtype])
+    step = torch.tensor(O.encode_values(amax.float().numpy()[:, None])[1])
+    mids = torch.tensor(np.concatenate([O.MIDPOINTS, -O.MIDPOINTS]))
+    x = (step[:, None] * mids).to(DT[dtype])                 # a tie, where the type holds it
+    bits = x.view(torch.int32 if dtype == "f32" else torch.int16)
+    near = [x] + [(bits + d).view(DT[dtype]) for d in (-1, 1, -3, 3, 40, -40)]
+    v = torch.cat(near + [torch.randn(T, D - 7 * 14 - 1, generator=g).to(DT[dtype]) * step[:, None].to(DT[dtype])], 1)
+    v = torch.where(v.abs() > amax[:, None], torch.zeros_like(v), v)
+    v = torch.cat([amax[:, None], v], 1)[None, :, None]
+    cache = pkg.KV4Cache.allocate(1, T, 1, D, dev)
+    pkg.kv4_append(cache, v.to(dev), v.to(dev), ints([0], dev))
+    torch.cuda.synchronize()
+    kc, ke, vc, vs = O.unpack(cache.data.cpu().numpy(), cache.block_table.cpu().numpy(), D)
+    f = v[0, :, 0].float().numpy()
+    for got, want in zip((kc, ke, vc, vs), (*O.encode_keys(f), *O.encode_values(f))):
+        assert np.array_equal(got[0, 0, :T], want)
+
+
 # ---- attention ---------------------------------------------------------------------
 
 ATTENTION = [
