@@ -149,12 +149,17 @@ struct Scan {
             count = kv4_count(k.counts, b0 + lane, k.T);
             pages = seq_pages(seq_end(k, n, count, slots));
         }
-        cum = pages * per;
+        cum = sum_upto(pages * per);
+    }
+    // Sum over the lanes up to this one.
+    __device__ static int sum_upto(int x) {
+        const int lane = threadIdx.x & 63;
 #pragma unroll
         for (int off = 1; off < 64; off <<= 1) {
-            const int o = __shfl_up(cum, off, 64);
-            cum += lane >= off ? o : 0;
+            const int o = __shfl_up(x, off, 64);
+            x += lane >= off ? o : 0;
         }
+        return x;
     }
     // Sequence of unit u < total, its first unit, its pages, context and valid rows.
     struct Place { int b, start, pages, n, count; };
