@@ -22,7 +22,8 @@
 // row tiles go over the same pages at the same time.  The pages of all (sequence,
 // head, tiles) are numbered in one line, which is cut into equal pieces, one for each
 // workgroup, whatever the lengths are: a piece that covers all pages of its rows
-// writes their output, others write their state, which kv4_join_kernel joins.
+// writes their output, others write their state, and the last of them to arrive joins
+// the states in their order, so that results do not depend on who that is.
 #include <algorithm>
 
 #include "kv4_mma.h"
@@ -48,6 +49,7 @@ struct Line {
     int pieces;                // workgroups
 };
 constexpr int kMinPages = kKv4Waves;   // fewest pages of a piece
+constexpr int kCounterWords = 16;      // words from one arrival counter to the next
 
 // How the line is cut into at most `pieces` pieces.
 //  * Where it is not much less even, every tile group into parts of its own, as many as
@@ -327,8 +329,8 @@ template <typename T, int D, int MT> struct Rows {
 };
 
 template <typename T, int D, int MT, int WAYS>
-__global__ __launch_bounds__(kKv4Threads, 2) void kv4_attention_kernel(Kv4AttentionArgs a, Line line,
-                                                                                float* __restrict__ states) {
+__global__ __launch_bounds__(kKv4Threads, 2) void kv4_attention_kernel(Kv4AttentionArgs a, Line line, float* states,
+                                                                       unsigned int* counters) {
     using S = Shape<D, MT>;
     constexpr int kRegs = S::CT * S::ACC;                   // output registers
     constexpr int kRound = 32;                              // registers joined at a time
@@ -336,6 +338,7 @@ __global__ __launch_bounds__(kKv4Threads, 2) void kv4_attention_kernel(Kv4Attent
     __shared__ float s_m[kKv4Waves][MT], s_l[kKv4Waves][MT];
     constexpr int kTiles = kKv4Waves / WAYS;
     __shared__ typename Frag<T>::type s_q[kTiles][S::KS][64];
+    __shared__ bool s_last;
 
     const Kv4Cache& c = a.cache;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -461,7 +464,11 @@ __global__ __launch_bounds__(kKv4Threads, 2) void kv4_attention_kernel(Kv4Attent
         }
         __syncthreads();
         const bool whole = first == 0 && last == at.pages;
-        float* state = states + ((int64_t)(2 * piece + (first == 0 ? 1 : 0)) * kTiles + tile) * kStateFloats<D, MT>;
+        // a piece has at most one state of rows that it begins and one of rows that it goes on with
+        auto state_of = [&](int w, bool begins) {
+            return states + ((int64_t)(2 * w + (begins ? 1 : 0)) * kTiles + tile) * kStateFloats<D, MT>;
+        };
+        float* state = state_of(piece, first == 0);
         float m = -__builtin_inff(), l = 0.f;
 #pragma unroll
         for (int w = tile * WAYS; w < (tile + 1) * WAYS; ++w) m = fmaxf(m, s_m[w][col]);
@@ -489,9 +496,11 @@ __global__ __launch_bounds__(kKv4Threads, 2) void kv4_attention_kernel(Kv4Attent
                 if (whole) {
                     store_out<T, S::VW>(a, b, row, S::channel_of(gi / S::ACC, gi % S::ACC, g), sum, inv);
                 } else {
-                    float* to = state + (gi * 64 + lane) * S::VW;
+                    auto* to = reinterpret_cast<unsigned long long*>(state + (gi * 64 + lane) * S::VW);
 #pragma unroll
-                    for (int v = 0; v < S::VW; ++v) to[v] = sum[v];
+                    for (int v = 0; v < S::VW; v += 2)
+                        atomic_store_u64(to + v / 2, (unsigned long long)__float_as_uint(sum[v + 1]) << 32 |
+                                                         __float_as_uint(sum[v]));
                 }
             }
             __syncthreads();
@@ -500,65 +509,85 @@ __global__ __launch_bounds__(kKv4Threads, 2) void kv4_attention_kernel(Kv4Attent
             if (whole) {
                 store_lse(a, b, row, m, l);
             } else {
-                state[MT * D + col] = m;
-                state[MT * D + MT + col] = l;
+                auto* to = reinterpret_cast<unsigned int*>(state + MT * D + col);
+                atomic_store_u32(to, __float_as_uint(m));
+                atomic_store_u32(to + MT, __float_as_uint(l));
+            }
+        }
+        if (!whole) {
+            // The states are written and read with device-coherent stores and loads, and every
+            // store is waited for before the arrival is counted: no cache fences.
+            const int lo = at.start + ht * at.pages;
+            const int2 held = cuts.holders(scan, b, ht, lo, lo + at.pages);
+            __builtin_amdgcn_s_waitcnt(0);
+            asm volatile("" ::: "memory");
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                unsigned int* counter = counters + held.x * kCounterWords;
+                const unsigned prev = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                s_last = prev == (unsigned)(held.y - held.x) - 1u;
+                if (s_last) __hip_atomic_exchange(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+            __syncthreads();
+            if (s_last) {
+                auto load = [&](const float* p) {
+                    return __uint_as_float(__hip_atomic_load(reinterpret_cast<const unsigned int*>(p), __ATOMIC_RELAXED,
+                                                             __HIP_MEMORY_SCOPE_AGENT));
+                };
+                constexpr int kMine = (kRegs / S::VW + WAYS - 1) / WAYS;
+                float sum[kMine][S::VW];
+#pragma unroll
+                for (int i = 0; i < kMine; ++i)
+#pragma unroll
+                    for (int v = 0; v < S::VW; ++v) sum[i][v] = 0.f;
+                m = -__builtin_inff(), l = 0.f;
+                // several states in flight: their loads go to memory (131k slots, 16 states: 91 us one
+                // at a time, 76 eight)
+                constexpr int kFlight = WAYS;
+                for (int w0 = held.x; w0 < held.y; w0 += kFlight) {
+                    float tops[kFlight], sums[kFlight];
+                    unsigned long long two[kFlight][kMine][S::VW / 2];
+#pragma unroll
+                    for (int e = 0; e < kFlight; ++e) {
+                        const int w = min(w0 + e, held.y - 1);
+                        const float* st = state_of(w, w == held.x);
+                        tops[e] = load(st + MT * D + col);
+                        sums[e] = load(st + MT * D + MT + col);
+#pragma unroll
+                        for (int i = 0; i < kMine; ++i) {
+                            const int gi = min(way + i * WAYS, kRegs / S::VW - 1);
+                            auto* from = reinterpret_cast<unsigned long long*>(
+                                const_cast<float*>(st + (gi * 64 + lane) * S::VW));
+#pragma unroll
+                            for (int v = 0; v < S::VW / 2; ++v) two[e][i][v] = atomic_load_u64(from + v);
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < kFlight; ++e) {
+                        if (w0 + e >= held.y) break;
+                        const float now = fmaxf(m, tops[e]), old = fade(m, now), f = fade(tops[e], now);
+                        m = now;
+                        l = l * old + sums[e] * f;
+#pragma unroll
+                        for (int i = 0; i < kMine; ++i)
+#pragma unroll
+                            for (int v = 0; v < S::VW; ++v)
+                                sum[i][v] = sum[i][v] * old +
+                                            __uint_as_float((uint32_t)(two[e][i][v / 2] >> (32 * (v & 1)))) * f;
+                    }
+                }
+                const float inv = l > 0.f ? 1.f / l : 0.f;
+#pragma unroll
+                for (int i = 0; i < kMine; ++i) {
+                    const int gi = way + i * WAYS;
+                    if (gi < kRegs / S::VW)
+                        store_out<T, S::VW>(a, b, row, S::channel_of(gi / S::ACC, gi % S::ACC, g), sum[i], inv);
+                }
+                if (way == 0 && g == 0) store_lse(a, b, row, m, l);
             }
         }
         u += last - first;
     }
-}
-
-// Joins the states of the rows whose pages lie in several pieces.  Grid (sequence x
-// head x row tile, parts of the output registers), a wave per VW channels in turn.
-constexpr int kJoinWaves = 4;
-template <typename T, int D, int MT, int WAYS>
-__global__ __launch_bounds__(64 * kJoinWaves) void kv4_join_kernel(Kv4AttentionArgs a, Line line,
-                                                                   const float* __restrict__ states) {
-    using S = Shape<D, MT>;
-    const Kv4Cache& c = a.cache;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane % MT, g = lane / MT;
-    constexpr int kTiles = kKv4Waves / WAYS;
-    const int per = c.heads * line.tiles, group = a.q_heads / c.heads;
-    const int b = blockIdx.x / (per * kTiles), ht = blockIdx.x / kTiles % per, h = ht / line.tiles;
-    const int tile = blockIdx.x % kTiles, rt = ht % line.tiles * kTiles + tile;
-    if (rt * MT >= a.block.T * group) return;
-    Scan scan(a.block, c, per);
-    const Cuts cuts(scan, line);
-    int before = 0;                                         // pages of the sequences before b
-    for (int i = lane; i < b; i += 64) before += seq_pages(a.block, i, c.slots());
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) before += __shfl_xor(before, off, 64);
-    const int pages = seq_pages(a.block, b, c.slots());
-    const int lo = uniform(before) * per + ht * pages;
-    const int2 held = cuts.holders(scan, b, ht, lo, lo + pages);
-    if (held.y - held.x <= 1) return;                       // one piece covered them and wrote the output
-    const int w0 = held.x + 1, w1 = held.y;
-    auto state_of = [&](int w) { return states + ((int64_t)(2 * w + (w < w0 ? 1 : 0)) * kTiles + tile) * kStateFloats<D, MT>; };
-    float m = -__builtin_inff(), l = 0.f;
-#pragma unroll 4
-    for (int w = w0 - 1; w < w1; ++w) {
-        const float part = state_of(w)[MT * D + col], sum = state_of(w)[MT * D + MT + col];
-        const float now = fmaxf(m, part);
-        l = l * fade(m, now) + sum * fade(part, now);
-        m = now;
-    }
-    const float inv = l > 0.f ? 1.f / l : 0.f;
-    const Row row = row_of(rt * MT + col, group, h, a.block.T, kv4_count(a.block.counts, b, a.block.T));
-    for (int gi = blockIdx.y * kJoinWaves + wave; gi < S::CT * S::ACC / S::VW; gi += gridDim.y * kJoinWaves) {
-        float sum[S::VW];
-#pragma unroll
-        for (int v = 0; v < S::VW; ++v) sum[v] = 0.f;
-#pragma unroll 4
-        for (int w = w0 - 1; w < w1; ++w) {
-            const float* st = state_of(w);
-            const float f = fade(st[MT * D + col], m);
-            const float* from = st + (gi * 64 + lane) * S::VW;
-#pragma unroll
-            for (int v = 0; v < S::VW; ++v) sum[v] += from[v] * f;
-        }
-        store_out<T, S::VW>(a, b, row, S::channel_of(gi / S::ACC, gi % S::ACC, g), sum, inv);
-    }
-    if (blockIdx.y == 0 && wave == 0 && g == 0) store_lse(a, b, row, m, l);
 }
 
 struct Plan { int rows, ways; Line line; };
@@ -577,7 +606,7 @@ Plan plan(int64_t batch, int64_t T, int64_t q_heads, int64_t heads, int64_t max_
     const int per = kKv4Waves / p.ways;
     p.line.tiles = (int)((tiles + per - 1) / per);
     const int64_t units = batch * heads * p.line.tiles * std::max<int64_t>(max_pages, 1);
-    p.line.pieces = (int)std::min<int64_t>(cus, (units + kMinPages - 1) / kMinPages);
+    p.line.pieces = (int)std::min<int64_t>({cus, kMaxCounters / kCounterWords, (units + kMinPages - 1) / kMinPages});
     return p;
 }
 
@@ -593,20 +622,14 @@ hipError_t launch_kv4_attention(const Kv4AttentionArgs& a, void* ws, size_t data
     const Kv4Cache& c = a.cache;
     const Plan p = plan(c.batch, a.block.T, a.q_heads, c.heads, c.max_pages);
     auto* states = reinterpret_cast<float*>(static_cast<char*>(ws) + data_off);
+    auto* counters = reinterpret_cast<unsigned int*>(static_cast<char*>(ws) + kCountersOff);
     return kv4_by_type(a.dtype, c.head_dim, p.rows, [&](auto tag, auto size, auto rows) {
         using T = decltype(tag);
         constexpr int D = decltype(size)::value, MT = decltype(rows)::value;
-        using S = Shape<D, MT>;
-        static_assert(S::CT * S::ACC / S::VW % kJoinWaves == 0, "a wave of the join per VW channels");
         auto go = [&](auto ways) {
             constexpr int WAYS = decltype(ways)::value;
             hipLaunchKernelGGL((kv4_attention_kernel<T, D, MT, WAYS>), dim3(p.line.pieces), dim3(kKv4Threads), 0, s, a,
-                               p.line, states);
-            // few row tiles: their channels over several workgroups
-            const unsigned tiles = (unsigned)c.batch * c.heads * p.line.tiles * (kKv4Waves / WAYS);
-            const unsigned parts = (int)tiles <= device_cu_count() ? S::CT * S::ACC / S::VW / kJoinWaves : 1;
-            hipLaunchKernelGGL((kv4_join_kernel<T, D, MT, WAYS>), dim3(tiles, parts), dim3(64 * kJoinWaves), 0, s, a,
-                               p.line, states);
+                               p.line, states, counters);
         };
         if constexpr (MT == 32) {
             if (p.ways == 2) return go(std::integral_constant<int, 2>{});
