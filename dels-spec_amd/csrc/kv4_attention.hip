@@ -43,86 +43,10 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
 }
 
-// The line of pages: those of (b, h, tiles of a workgroup) one after the other, b first.
-struct Line {
-    int tiles;                 // groups of 8 / WAYS row tiles per (b, h)
-    int pieces;                // workgroups
-};
-constexpr int kMinPages = kKv4Waves;   // fewest pages of a piece
 constexpr int kCounterWords = 16;      // words from one arrival counter to the next
-
-// How the line is cut into at most `pieces` pieces.
-//  * Where it is not much less even, every tile group into parts of its own, as many as
-//    its pages call for, a workgroup each: the smallest part for which there are
-//    workgroups enough, up to a quarter (and a page a wave) over an even share.
-//  * Else every `share` pages; a cut within kSnap pages of where the next tiles begin moves
-//    there, so that no piece holds a few pages of some and the rest of others.  A piece
-//    over several tile groups begins and joins its waves for each (about 8 us).
-// 8 x 16 rows over up to 4000 slots: 35 us with even cuts alone, 27 with parts.
-struct Cuts {
-    static constexpr int kSnap = 8;
-    int share;
-    int parts, upto;           // of this lane's sequence: parts per tile group; pieces of all up to it
-    bool own_parts;
-
-    __device__ Cuts(const Scan& s, const Line& line) {
-        share = max(kMinPages, (s.total + line.pieces - 1) / line.pieces);
-        own_parts = false;
-        parts = upto = 0;
-        if (s.c.batch > 64) return;
-        const int step = kKv4Waves * max(1, share / 64);
-        for (int part = (share + 7) / 8 * 8; part <= share + share / 4 + kKv4Waves; part += step) {
-            parts = (s.pages + part - 1) / part;
-            upto = Scan::sum_upto(parts * s.per);
-            own_parts = __builtin_amdgcn_readlane(upto, 63) <= line.pieces;
-            if (own_parts) return;
-        }
-    }
-    // Units of a piece: first, past the last.
-    __device__ int2 piece(Scan& s, int w) const {
-        if (own_parts) {
-            const unsigned long long past = __ballot(upto > w);
-            if (!past) return {0, 0};
-            const int l = __builtin_ctzll(past), n = __builtin_amdgcn_readlane(parts, l);
-            const int pages = __builtin_amdgcn_readlane(s.pages, l);
-            const int i = w - (__builtin_amdgcn_readlane(upto, l) - n * s.per), ht = i / n, k = i - ht * n;
-            const int at = __builtin_amdgcn_readlane(s.cum, l) - pages * s.per + ht * pages;
-            return {at + k * pages / n, at + (k + 1) * pages / n};
-        }
-        if ((int64_t)w * share >= s.total) return {0, 0};
-        int2 r = {0, 0};
-#pragma nounroll
-        for (int e = 0; e < 2; ++e) {
-            r.x = r.y;
-            const int u = (int)min((int64_t)(w + e) * share, (int64_t)s.total);
-            r.y = u;
-            if (u < s.total) {
-                const Scan::Place at = s.place(u);
-                const int lo = at.start + (u - at.start) / at.pages * at.pages;
-                r.y = snap(u, lo, lo + at.pages);
-            }
-        }
-        return r;
-    }
-    // Pieces that hold the pages lo .. hi - 1 of tile group ht of sequence b: first, past the last.
-    __device__ int2 holders(const Scan& s, int b, int ht, int lo, int hi) const {
-        if (own_parts) {
-            const int n = __builtin_amdgcn_readlane(parts, b);
-            const int w = __builtin_amdgcn_readlane(upto, b) - n * s.per + ht * n;
-            return {w, w + n};
-        }
-        // cuts w0 .. w1 - 1 stay inside; the piece before the first has the first pages
-        int w0 = (lo + share - 1) / share, w1 = (hi - 1) / share + 1;
-        while (w0 < w1 && snap(w0 * share, lo, hi) == lo) ++w0;
-        while (w0 < w1 && snap((w1 - 1) * share, lo, hi) == hi) --w1;
-        return {w0 - 1, w1};
-    }
-    // Where the cut at unit u comes to lie; lo, hi: the ends of the tiles that hold it.
-    __device__ int snap(int u, int lo, int hi) const {
-        const int reach = min(share / 2, kSnap);
-        return u - lo <= reach ? lo : hi - u <= reach ? hi : u;
-    }
-};
+// Most pieces of one tile group: their states are joined by one workgroup, about 0.25 us
+// each (one row over 94k slots: 45 us in 184 pieces, 29 in 32).
+constexpr int kMostParts = 32;
 
 template <typename T> __device__ __forceinline__ uint16_t round_to(float x);
 template <> __device__ __forceinline__ uint16_t round_to<bf16_t>(float x) { return f32_to_bf16_bits(x); }
@@ -349,7 +273,7 @@ __global__ __launch_bounds__(kKv4Threads, 2) void kv4_attention_kernel(Kv4Attent
                                          : (int)(blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8);
     const LaneOffsets<D, MT> at_lane(col, g);
     Scan scan(a.block, c, c.heads * line.tiles);
-    const Cuts cuts(scan, line);
+    const Cuts cuts(scan, line, kMostParts);
     const int2 mine = cuts.piece(scan, piece);
     int u = mine.x;
     const int u_end = mine.y;
@@ -606,7 +530,8 @@ Plan plan(int64_t batch, int64_t T, int64_t q_heads, int64_t heads, int64_t max_
     const int per = kKv4Waves / p.ways;
     p.line.tiles = (int)((tiles + per - 1) / per);
     const int64_t units = batch * heads * p.line.tiles * std::max<int64_t>(max_pages, 1);
-    p.line.pieces = (int)std::min<int64_t>({cus, kMaxCounters / kCounterWords, (units + kMinPages - 1) / kMinPages});
+    p.line.pieces = (int)std::min<int64_t>({cus, kMaxCounters / kCounterWords,
+                                            std::max(batch * heads * p.line.tiles, (units + kMinPages - 1) / kMinPages)});
     return p;
 }
 

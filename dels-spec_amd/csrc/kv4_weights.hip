@@ -18,7 +18,6 @@ namespace dels {
 namespace {
 
 constexpr int kRows = 128;                       // rows whose queries fit LDS at a time
-constexpr int kMinPages = kKv4Waves;             // fewest pages of a workgroup's piece
 
 template <typename T, int D, int MT>
 __global__ __launch_bounds__(kKv4Threads, 4) void kv4_weights_kernel(Kv4WeightsArgs a, int pieces) {
@@ -35,13 +34,14 @@ __global__ __launch_bounds__(kKv4Threads, 4) void kv4_weights_kernel(Kv4WeightsA
     const int slots = c.slots(), group = a.q_heads / c.heads;
     const LaneOffsets<D, MT> at_lane(col, g);
     Scan scan(a.block, c, c.heads);
-    const int share = max(kMinPages, (scan.total + pieces - 1) / pieces);
+    const Cuts cuts(scan, Line{1, pieces}, INT32_MAX);
     const float mag = fabsf(a.scale);
     const float unit = (mag == 0.f ? 1.f : mag) * kLog2e * (float)(1 << kKeyShift<T>);
     const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u, zero = mag == 0.f ? 0u : ~0u;
 
-    int u = (int)min((int64_t)blockIdx.x * share, (int64_t)scan.total);
-    const int u_end = (int)min((int64_t)u + share, (int64_t)scan.total);
+    const int2 piece = cuts.piece(scan, blockIdx.x);
+    int u = piece.x;
+    const int u_end = piece.y;
     Scan::Place at{};
     at.pages = 0;
     while (u < u_end) {
@@ -198,7 +198,8 @@ hipError_t launch_kv4_weights(const Kv4WeightsArgs& a, hipStream_t s) {
     }
     const int64_t units = (int64_t)c.batch * c.heads * c.max_pages;
     // two workgroups a CU: 32 x 16k slots 74 us with one, 68 so
-    const int pieces = (int)std::min<int64_t>(2 * device_cu_count(), (units + kMinPages - 1) / kMinPages);
+    const int pieces = (int)std::min<int64_t>(2 * device_cu_count(), std::max<int64_t>((int64_t)c.batch * c.heads,
+                                                                                       (units + kMinPages - 1) / kMinPages));
     const int rows = (int64_t)a.block.T * (a.q_heads / c.heads) <= 16 ? 16 : 32;
     return kv4_by_type(a.dtype, c.head_dim, rows, [&](auto tag, auto size, auto tile) {
         hipLaunchKernelGGL((kv4_weights_kernel<decltype(tag), decltype(size)::value, decltype(tile)::value>), dim3(pieces),

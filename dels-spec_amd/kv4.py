@@ -21,13 +21,12 @@ alike: row ``t`` of a block lies in slot ``lengths[b] + t``.
 from __future__ import annotations
 
 import ctypes
-import math
 from typing import Optional, Union
 
 import torch
 
 from . import _lib
-from .ops import _DTYPES, _require_cuda, _stream_ptr, workspace
+from .ops import _DTYPES, _WORKSPACES, _require_cuda, _stream_ptr, workspace
 
 PAGE = 64              # slots of a page
 HEAD_DIMS = (64, 128)
@@ -71,6 +70,9 @@ class KV4Cache:
         self.batch, self.max_pages = (int(x) for x in block_table.shape)
         self.slots = self.max_pages * PAGE
         self.device = data.device
+        self._index = data.get_device()
+        self._scale = self.head_dim ** -0.5
+        self._ws_bytes = {}                    # attention's workspace size by (T, q_heads)
         self._params = _lib.Kv4CacheParams(data.data_ptr(), data.shape[0], self.kv_heads, self.head_dim,
                                            block_table.data_ptr(), max(block_table.stride(0), self.max_pages),
                                            self.batch, self.max_pages)
@@ -85,23 +87,29 @@ class KV4Cache:
         return cls(data, table, head_dim)
 
 
+def _elsewhere(t, cache: KV4Cache, name: str) -> None:
+    """Raise for a tensor that is not on the cache's GPU."""
+    _require_cuda(t, name)
+    raise ValueError(f"{name} is on {t.device}, the cache on {cache.device}")
+
+
 def _require_ints(t: Optional[torch.Tensor], cache: KV4Cache, name: str) -> Optional[int]:
     """Pointer of an int32 [batch] device array (None where there is none)."""
     if t is None:
         return None
-    _require_cuda(t, name)
-    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != cache.batch:
+    if not isinstance(t, torch.Tensor) or t.get_device() != cache._index:
+        _elsewhere(t, cache, name)
+    if t.dtype != torch.int32 or t.shape != (cache.batch,):
         raise ValueError(f"{name} must be int32 [{cache.batch}], got {t.dtype} {tuple(t.shape)}")
-    if t.device != cache.device:
-        raise ValueError(f"{name} is on {t.device}, the cache on {cache.device}")
-    if t.shape[0] > 1 and t.stride(0) != 1:
+    if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
     return t.data_ptr()
 
 
 def _require_rows(t: torch.Tensor, cache: KV4Cache, heads: Optional[int], name: str, dtypes) -> tuple[int, int, int, int]:
     """(pointer, strides) of a [batch, T, heads, head_dim] tensor with unit channel stride."""
-    _require_cuda(t, name)
+    if not isinstance(t, torch.Tensor) or t.get_device() != cache._index:
+        _elsewhere(t, cache, name)
     if t.dtype not in dtypes:
         raise TypeError(f"{name} dtype {t.dtype} not supported")
     shape = t.shape
@@ -109,13 +117,11 @@ def _require_rows(t: torch.Tensor, cache: KV4Cache, heads: Optional[int], name: 
             heads is not None and shape[2] != heads):
         raise ValueError(f"{name} must be [{cache.batch}, T, {'heads' if heads is None else heads}, "
                          f"{cache.head_dim}], got {tuple(shape)}")
-    if t.device != cache.device:
-        raise ValueError(f"{name} is on {t.device}, the cache on {cache.device}")
-    s = t.stride()
-    if s[3] != 1:
+    sb, st, sh, sc = t.stride()
+    if sc != 1:
         raise ValueError(f"{name} must have unit channel stride")
     # a dimension of one has no stride that matters
-    return (t.data_ptr(), s[0] if shape[0] > 1 else 0, s[1] if shape[1] > 1 else 0, s[2] if shape[2] > 1 else 0)
+    return (t.data_ptr(), sb if shape[0] > 1 else 0, st if shape[1] > 1 else 0, sh if shape[2] > 1 else 0)
 
 
 _Q_DTYPES = (torch.bfloat16, torch.float16)
@@ -149,8 +155,8 @@ def kv4_read(cache: KV4Cache, starts: torch.Tensor, T: int, *, counts: Optional[
     if dtype not in _DTYPES:
         raise TypeError(f"dtype {dtype} not supported")
     sp, cp = _require_ints(starts, cache, "starts"), _require_ints(counts, cache, "counts")
-    kv = torch.empty(2, cache.batch, T, cache.kv_heads, cache.head_dim, dtype=dtype, device=cache.device)
-    k, v = kv.unbind(0)
+    k = torch.empty(cache.batch, T, cache.kv_heads, cache.head_dim, dtype=dtype, device=cache.device)
+    v = torch.empty_like(k)
     lib = _lib.load()
     _lib.check(lib.dels_kv4_read(cache._ref, sp, cp, T, k.data_ptr(), v.data_ptr(), _DTYPES[dtype],
                                  _stream_ptr(cache.device)), "dels_kv4_read")
@@ -163,7 +169,8 @@ Block = Union[str, torch.Tensor]
 def _block_args(block: Block, cache: KV4Cache, T: int) -> tuple[int, Optional[int], int]:
     """(mode, mask pointer, mask row stride)."""
     if isinstance(block, torch.Tensor):
-        _require_cuda(block, "block")
+        if block.get_device() != cache._index:
+            _elsewhere(block, cache, "block")
         if block.dtype != torch.int64 or block.shape != (cache.batch, T):
             raise ValueError(f"a block mask must be int64 [{cache.batch}, {T}], got {block.dtype} "
                              f"{tuple(block.shape)}")
@@ -209,23 +216,29 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, lengths: torch.Tensor, *, bl
     else:
         _require_lse(lse, cache, T, q_heads)
     lib = _lib.load()
-    ws = workspace(cache.device, lib.dels_kv4_attention_ws_bytes(batch, T, q_heads, cache.kv_heads, D,
-                                                                 cache.max_pages))
+    need = cache._ws_bytes.get((T, q_heads))
+    if need is None:
+        need = lib.dels_kv4_attention_ws_bytes(batch, T, q_heads, cache.kv_heads, D, cache.max_pages)
+        cache._ws_bytes[T, q_heads] = need
+    stream = _stream_ptr(cache.device)
+    ws = _WORKSPACES.get(cache.device, need, stream)
     _lib.check(lib.dels_kv4_attention(cache._ref, *qp, _DTYPES[q.dtype], q_heads, T, lp, cp, mode, mask, ld_mask,
-                                      1.0 / math.sqrt(D) if scale is None else scale, *op, lse.data_ptr(),
-                                      ws.data_ptr(), ws.numel(), _stream_ptr(cache.device)), "dels_kv4_attention")
+                                      cache._scale if scale is None else scale, *op, lse.data_ptr(),
+                                      ws.data_ptr(), ws.numel(), stream), "dels_kv4_attention")
     return out, lse
 
 
 def _require_lse(lse: torch.Tensor, cache: KV4Cache, T: int, q_heads: int) -> None:
-    _require_cuda(lse, "lse")
+    if not isinstance(lse, torch.Tensor) or lse.get_device() != cache._index:
+        _elsewhere(lse, cache, "lse")
     if lse.dtype != torch.float32 or lse.shape != (cache.batch, T, q_heads) or not lse.is_contiguous():
         raise ValueError(f"lse must be contiguous float32 [{cache.batch}, {T}, {q_heads}], got {lse.dtype} "
                          f"{tuple(lse.shape)}")
 
 
 def _require_weights(w: torch.Tensor, cache: KV4Cache, name: str) -> None:
-    _require_cuda(w, name)
+    if not isinstance(w, torch.Tensor) or w.get_device() != cache._index:
+        _elsewhere(w, cache, name)
     if w.dtype != torch.float32 or w.shape != (cache.batch, cache.kv_heads, cache.slots) or not w.is_contiguous():
         raise ValueError(f"{name} must be contiguous float32 [{cache.batch}, {cache.kv_heads}, {cache.slots}], got "
                          f"{w.dtype} {tuple(w.shape)}")
@@ -250,7 +263,8 @@ def kv4_weights(q: torch.Tensor, cache: KV4Cache, lengths: torch.Tensor, lse: to
     lp, cp = _require_ints(lengths, cache, "lengths"), _require_ints(counts, cache, "counts")
     ap = _require_ints(accepted, cache, "accepted")
     mode, mask, ld_mask = _block_args(block, cache, T)
-    _require_cuda(lse, "lse")
+    if not isinstance(lse, torch.Tensor) or lse.get_device() != cache._index:
+        _elsewhere(lse, cache, "lse")
     if lse.dtype == torch.float32 and not lse.is_contiguous():
         lse = lse.contiguous()
     _require_lse(lse, cache, T, q_heads)
@@ -261,7 +275,7 @@ def kv4_weights(q: torch.Tensor, cache: KV4Cache, lengths: torch.Tensor, lse: to
         _require_weights(out, cache, "out")
     lib = _lib.load()
     _lib.check(lib.dels_kv4_weights(cache._ref, *qp, _DTYPES[q.dtype], q_heads, T, lp, cp, ap, mode, mask, ld_mask,
-                                    1.0 / math.sqrt(D) if scale is None else scale, lse.data_ptr(),
+                                    cache._scale if scale is None else scale, lse.data_ptr(),
                                     weights.data_ptr(), out.data_ptr(), _stream_ptr(cache.device)),
                "dels_kv4_weights")
     return out
