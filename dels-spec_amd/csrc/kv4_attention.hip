@@ -43,6 +43,7 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
 }
 
+constexpr int kMinPages = 2 * kKv4Waves;      // fewest pages of a piece (one row over 700 slots: 10.6 us in two of eight, 9.2 in one)
 constexpr int kCounterWords = 16;      // words from one arrival counter to the next
 // Most pieces of one tile group: their states are joined by one workgroup, about 0.25 us
 // each (one row over 94k slots: 45 us in 184 pieces, 29 in 32).
@@ -61,7 +62,7 @@ template <> __device__ __forceinline__ uint16_t round_to<f16_t>(float x) {
 struct Row { int t, hq; bool in_block, valid; };
 __device__ __forceinline__ Row row_of(int r, int group, int h, int T, int count) {
     Row x;
-    x.t = r / group;
+    x.t = divide(r, group);
     x.hq = h * group + (r - x.t * group);
     x.in_block = x.t < T;
     x.valid = x.t < count;
@@ -274,11 +275,11 @@ __global__ __launch_bounds__(kKv4Threads, 2) void kv4_attention_kernel(Kv4Attent
     const LaneOffsets<D, MT> at_lane(col, g);
     Scan scan(a.block, c, c.heads * line.tiles);
     const Cuts cuts(scan, line, kMostParts);
-    const int2 mine = cuts.piece(scan, piece);
+    Scan::Place at{};
+    const int2 mine = cuts.piece(scan, piece, at);
     int u = mine.x;
     const int u_end = mine.y;
     if (u >= u_end) return;
-    Scan::Place at{};
     // scores in units of the maximum: |scale| and the query's sign
     const float mag = fabsf(a.scale);
     const float unit = (mag == 0.f ? 1.f : mag) * kLog2e * (float)(1 << kKeyShift<T>);
@@ -287,14 +288,14 @@ __global__ __launch_bounds__(kKv4Threads, 2) void kv4_attention_kernel(Kv4Attent
     while (u < u_end) {
         if (u >= at.start + at.pages * scan.per) at = scan.place(u);
         const int b = at.b;
-        const int rel = u - at.start, ht = rel / at.pages, first = rel - ht * at.pages;
-        const int h = ht / line.tiles, rt0 = (ht - h * line.tiles) * kTiles, rt = rt0 + tile;
+        const int rel = u - at.start, ht = divide(rel, at.pages), first = rel - ht * at.pages;
+        const int h = divide(ht, line.tiles), rt0 = (ht - h * line.tiles) * kTiles, rt = rt0 + tile;
         const int last = min(at.pages, first + (u_end - u));
         const int n = at.n, count = at.count;
         const int filled = seq_end(a.block, n, count, slots);     // slots past it may hold anything
         int end = filled;
         if (a.block.mode == DELS_KV4_CAUSAL)                  // no row of the tile sees past its last token
-            end = (int)min((int64_t)end, (int64_t)n + (rt * MT + MT - 1) / group + 1);
+            end = (int)min((int64_t)end, (int64_t)n + divide(rt * MT + MT - 1, group) + 1);
         if (rt * MT >= a.block.T * group) end = 0;            // past the block's rows
         const int stop = min(last, (end + kKv4Page - 1) / kKv4Page);
 
@@ -529,6 +530,7 @@ Plan plan(int64_t batch, int64_t T, int64_t q_heads, int64_t heads, int64_t max_
     p.ways = p.rows == 32 && batch * heads * fours >= cus && 8 * tiles >= 7 * 4 * fours ? 2 : 8;
     const int per = kKv4Waves / p.ways;
     p.line.tiles = (int)((tiles + per - 1) / per);
+    p.line.least = kMinPages;
     const int64_t units = batch * heads * p.line.tiles * std::max<int64_t>(max_pages, 1);
     p.line.pieces = (int)std::min<int64_t>({cus, kMaxCounters / kCounterWords,
                                             std::max(batch * heads * p.line.tiles, (units + kMinPages - 1) / kMinPages)});

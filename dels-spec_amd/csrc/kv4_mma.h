@@ -117,6 +117,9 @@ __device__ __forceinline__ int seq_pages(const Kv4Block& k, int b, int slots) {
 // What all lanes of a wave hold alike, kept in a scalar register.
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
+// Quotient of numbers that are not negative, two thirds of the signed one's instructions.
+__device__ __forceinline__ int divide(int x, int y) { return (int)((unsigned)x / (unsigned)y); }
+
 // Scan of the sequences' units by a wave, 64 at a time; up to 64 it is kept, with what
 // was loaded for it.
 struct Scan {
@@ -151,26 +154,29 @@ struct Scan {
         }
         cum = sum_upto(pages * per);
     }
-    // Sum over the lanes up to this one.
+    // Sum over the lanes up to this one: within rows of 16 lanes, then from row to row.
     __device__ static int sum_upto(int x) {
-        const int lane = threadIdx.x & 63;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const int o = __shfl_up(x, off, 64);
-            x += lane >= off ? o : 0;
-        }
+        x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);     // row_shr:1, 2, 4, 8
+        x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+        x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+        x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+        x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);     // row_bcast:15 into rows 1 and 3
+        x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);     // row_bcast:31 into rows 2 and 3
         return x;
     }
     // Sequence of unit u < total, its first unit, its pages, context and valid rows.
     struct Place { int b, start, pages, n, count; };
+    __device__ Place of_lane(int l) const {
+        const int p = __builtin_amdgcn_readlane(pages, l);
+        return {b0 + l, before + __builtin_amdgcn_readlane(cum, l) - p * per, p, __builtin_amdgcn_readlane(n, l),
+                __builtin_amdgcn_readlane(count, l)};
+    }
     __device__ Place place(int u) {
         if (u < before) seek(0, 0);
         for (;;) {
             const unsigned long long past = __ballot(before + cum > u);
             if (past) {
-                const int l = __builtin_ctzll(past), p = __builtin_amdgcn_readlane(pages, l);
-                return {b0 + l, before + __builtin_amdgcn_readlane(cum, l) - p * per, p,
-                        __builtin_amdgcn_readlane(n, l), __builtin_amdgcn_readlane(count, l)};
+                return of_lane(__builtin_ctzll(past));
             }
             const int all = __builtin_amdgcn_readlane(cum, 63);
             seek(b0 + 64, before + all);
@@ -182,8 +188,8 @@ struct Scan {
 struct Line {
     int tiles;                 // groups of 8 / WAYS row tiles per (b, h)
     int pieces;                // workgroups
+    int least;                 // fewest pages of a piece
 };
-constexpr int kMinPages = kKv4Waves;   // fewest pages of a piece
 
 // How the line is cut into at most `pieces` pieces.
 //  * Where it is not much less even, every tile group into parts of its own, as many as
@@ -200,29 +206,30 @@ struct Cuts {
     bool own_parts;
 
     __device__ Cuts(const Scan& s, const Line& line, int most) {
-        share = max(kMinPages, (s.total + line.pieces - 1) / line.pieces);
+        share = max(line.least, divide(s.total + line.pieces - 1, line.pieces));
         own_parts = false;
         parts = upto = 0;
         if (s.c.batch > 64) return;
         const int step = kKv4Waves * max(1, share / 64);
         for (int part = (share + 7) / 8 * 8; part <= share + share / 4 + kKv4Waves; part += step) {
-            parts = min((s.pages + part - 1) / part, most);
+            parts = min(divide(s.pages + part - 1, part), most);
             upto = Scan::sum_upto(parts * s.per);
             own_parts = __builtin_amdgcn_readlane(upto, 63) <= line.pieces;
             if (own_parts) return;
         }
     }
-    // Units of a piece: first, past the last.
-    __device__ int2 piece(Scan& s, int w) const {
+    // Units of a piece: first, past the last; and the place of the first, where it is known.
+    __device__ int2 piece(Scan& s, int w, Scan::Place& first) const {
         if (own_parts) {
             const unsigned long long past = __ballot(upto > w);
             if (!past) return {0, 0};
             const int l = __builtin_ctzll(past), n = __builtin_amdgcn_readlane(parts, l);
             const int pages = __builtin_amdgcn_readlane(s.pages, l);
-            const int i = w - (__builtin_amdgcn_readlane(upto, l) - n * s.per), ht = i / n, k = i - ht * n;
-            const int at = __builtin_amdgcn_readlane(s.cum, l) - pages * s.per + ht * pages;
-            const int q = pages / n, r = pages - q * n;        // k * pages / n, without its overflow
-            return {at + k * q + k * r / n, at + (k + 1) * q + (k + 1) * r / n};
+            const int i = w - (__builtin_amdgcn_readlane(upto, l) - n * s.per), ht = divide(i, n), k = i - ht * n;
+            first = s.of_lane(l);
+            const int at = first.start + ht * pages;
+            const int q = divide(pages, n), r = pages - q * n;   // k * pages / n, without its overflow
+            return {at + k * q + divide(k * r, n), at + (k + 1) * q + divide((k + 1) * r, n)};
         }
         if ((int64_t)w * share >= s.total) return {0, 0};
         int2 r = {0, 0};
@@ -233,7 +240,7 @@ struct Cuts {
             r.y = u;
             if (u < s.total) {
                 const Scan::Place at = s.place(u);
-                const int lo = at.start + (u - at.start) / at.pages * at.pages;
+                const int lo = at.start + divide(u - at.start, at.pages) * at.pages;
                 r.y = snap(u, lo, lo + at.pages);
             }
         }

@@ -17,6 +17,7 @@ namespace dels {
 
 namespace {
 
+constexpr int kMinPages = kKv4Waves;             // fewest pages of a workgroup's piece
 constexpr int kRows = 128;                       // rows whose queries fit LDS at a time
 
 template <typename T, int D, int MT>
@@ -34,39 +35,43 @@ __global__ __launch_bounds__(kKv4Threads, 4) void kv4_weights_kernel(Kv4WeightsA
     const int slots = c.slots(), group = a.q_heads / c.heads;
     const LaneOffsets<D, MT> at_lane(col, g);
     Scan scan(a.block, c, c.heads);
-    const Cuts cuts(scan, Line{1, pieces}, INT32_MAX);
+    const Cuts cuts(scan, Line{1, pieces, kMinPages}, INT32_MAX);
     const float mag = fabsf(a.scale);
     const float unit = (mag == 0.f ? 1.f : mag) * kLog2e * (float)(1 << kKeyShift<T>);
     const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u, zero = mag == 0.f ? 0u : ~0u;
 
-    const int2 piece = cuts.piece(scan, blockIdx.x);
+    Scan::Place at{};
+    const int2 piece = cuts.piece(scan, blockIdx.x, at);
     int u = piece.x;
     const int u_end = piece.y;
-    Scan::Place at{};
-    at.pages = 0;
     while (u < u_end) {
         if (u >= at.start + at.pages * scan.per) at = scan.place(u);
-        const int b = at.b, rel = u - at.start, h = rel / at.pages, first = rel - h * at.pages;
+        const int b = at.b, rel = u - at.start, h = divide(rel, at.pages), first = rel - h * at.pages;
         const int last = min(at.pages, first + (u_end - u));
         const int n = at.n, count = at.count;
-        const int rows = uniform(min(kv4_count(a.accepted, b, a.block.T), count)) * group;
+        const int first_page = first + wave;
         const int filled = seq_end(a.block, n, count, slots);
         const int32_t* ids = c.table + (int64_t)b * c.ld_table;
+        auto id_at = [&](int p) { return p < last && p * kKv4Page < filled ? ids[p] : -1; };
+        const int first_id = id_at(first_page);
+        const int rows = uniform(min(kv4_count(a.accepted, b, a.block.T), count)) * group;
         const uint8_t* heads = c.data + (int64_t)h * Kv4<D>::kBytes;
         const int64_t page_stride = (int64_t)c.heads * Kv4<D>::kBytes;
         const int64_t out_row = ((int64_t)b * c.heads + h) * slots;
-        auto id_of = [&](int p) { return p < last && p * kKv4Page < filled ? uniform(ids[p]) : -1; };
         auto named = [&](int id) { return id >= 0 && id < c.num_pages; };
 
         int r0 = 0;
         do {                                                 // once without rows too: the old weights move
             const int tiles = (min(rows - r0, kRows) + MT - 1) / MT;
+            KeyWords<D, MT> keys, next_keys;                 // the first are on their way with the queries
+            int p = first_page, id = uniform(first_id);
+            if (p < last) keys.load(heads + (named(id) ? id : 0) * page_stride, at_lane);
             __syncthreads();
             for (int i = wave; i < tiles * S::KS; i += kKv4Waves) {
                 const int tile = i / S::KS, k = i % S::KS, r = r0 + tile * MT + col;
                 u32x4 w = {0u, 0u, 0u, 0u};
                 if (r < rows) {
-                    const int t = r / group, hq = h * group + r % group;
+                    const int t = divide(r, group), hq = h * group + r - t * group;
                     w = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q.p) + (int64_t)b * a.q.batch +
                                                         (int64_t)t * a.q.token + (int64_t)hq * a.q.head + g * S::DL + 8 * k);
                 }
@@ -75,7 +80,7 @@ __global__ __launch_bounds__(kKv4Threads, 4) void kv4_weights_kernel(Kv4WeightsA
                 s_q[tile][k][lane] = __builtin_bit_cast(F, w);
             }
             if ((int)threadIdx.x < kRows) {
-                const int r = r0 + threadIdx.x, t = r / group;
+                const int r = r0 + threadIdx.x, t = divide(r, group);
                 float lse = __builtin_inff();
                 int lim = 0;
                 uint64_t bits = 0;
@@ -84,7 +89,7 @@ __global__ __launch_bounds__(kKv4Threads, 4) void kv4_weights_kernel(Kv4WeightsA
                     if (a.block.mode == DELS_KV4_MASK)
                         bits = (uint64_t)a.block.mask[(int64_t)b * a.block.ld_mask + t] &
                                (count >= 64 ? ~0ull : (1ull << count) - 1);
-                    lse = a.lse[((int64_t)b * a.block.T + t) * a.q_heads + h * group + r % group] * kLog2e;
+                    lse = a.lse[((int64_t)b * a.block.T + t) * a.q_heads + h * group + r - t * group] * kLog2e;
                     if (lse == -__builtin_inff()) lse = __builtin_inff();   // an empty row gave nothing
                 }
                 s_lse[threadIdx.x] = lse;
@@ -93,12 +98,8 @@ __global__ __launch_bounds__(kKv4Threads, 4) void kv4_weights_kernel(Kv4WeightsA
             }
             __syncthreads();
 
-            KeyWords<D, MT> keys, next_keys;
-            int p = first + wave;
-            int id = id_of(p);
-            if (p < last) keys.load(heads + (named(id) ? id : 0) * page_stride, at_lane);
             for (; p < last; p += kKv4Waves) {
-                const int next = id_of(p + kKv4Waves);
+                const int next = uniform(id_at(p + kKv4Waves));
                 next_keys.load(heads + (named(next) ? next : 0) * page_stride, at_lane);
                 asm volatile("" ::: "memory");
                 // the slot that this lane writes, of the four (two) it has sums for: by its group
@@ -197,7 +198,7 @@ hipError_t launch_kv4_weights(const Kv4WeightsArgs& a, hipStream_t s) {
         return hipGetLastError();
     }
     const int64_t units = (int64_t)c.batch * c.heads * c.max_pages;
-    // two workgroups a CU: 32 x 16k slots 74 us with one, 68 so
+    // two workgroups a CU: 32 x 16k slots 74 us with one, 68 with two (66 with the first keys ahead of the queries)
     const int pieces = (int)std::min<int64_t>(2 * device_cu_count(), std::max<int64_t>((int64_t)c.batch * c.heads,
                                                                                        (units + kMinPages - 1) / kMinPages));
     const int rows = (int64_t)a.block.T * (a.q_heads / c.heads) <= 16 ? 16 : 32;
