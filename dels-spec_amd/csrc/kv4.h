@@ -45,6 +45,17 @@ __device__ __forceinline__ uint8_t* kv4_page(const Kv4Cache& c, int b, int h, in
 }
 
 // Context length and valid block rows of sequence b, within the table's slots.
+// Sum over the lanes up to this one: within rows of 16 lanes, then from row to row.
+__device__ __forceinline__ int sum_upto(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);     // row_shr:1, 2, 4, 8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);     // row_bcast:15 into rows 1 and 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);     // row_bcast:31 into rows 2 and 3
+    return x;
+}
+
 __device__ __forceinline__ int kv4_length(const int32_t* lengths, int b, int slots) {
     return min(max(lengths[b], 0), slots);
 }

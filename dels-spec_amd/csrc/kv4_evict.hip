@@ -15,7 +15,7 @@ namespace dels {
 
 namespace {
 
-constexpr int kPerLane = 16;                               // slots of a lane per tile
+constexpr int kPerLane = 16;                               // consecutive slots of a lane per tile
 constexpr int kBins = 2048;                                // 11 bits of the key at a time
 constexpr int kMoveThreads = 256;
 
@@ -24,15 +24,11 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
     return f32_order_key(w != w ? -__builtin_inff() : w);
 }
 
-// Sum over the lanes up to this one.
-__device__ __forceinline__ int scan_wave(int x) {
-    const int lane = threadIdx.x & 63;
+// A lane's slots of a row's weights, those past n whatever follows (a row is whole pages).
+__device__ __forceinline__ void load_slots(const float* w, int first, int n, float (&x)[kPerLane]) {
 #pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const int o = __shfl_up(x, off, 64);
-        x += lane >= off ? o : 0;
-    }
-    return x;
+    for (int i = 0; i < kPerLane; ++i) x[i] = 0.f;
+    if (first < n) __builtin_memcpy(x, w + first, sizeof(x));
 }
 // Sum of `x` (one value per wave) over the waves before this one, and over all.
 template <int WAVES> __device__ __forceinline__ int2 over_waves(const int* x) {
@@ -48,18 +44,19 @@ template <int WAVES> __device__ __forceinline__ int2 over_waves(const int* x) {
 
 // One workgroup per (sequence, head).  The threshold is found 11 bits of the key at a
 // time (a histogram in LDS of the weights that share the bits so far, scanned from
-// its top); then the slots are walked in order, 16 THREADS at a time and 1024 of them a
-// wave: ranks among equal weights, holes and movers come from ballots, and from the
-// waves' counts in three exchanges a tile.  Bound by latency: the weights are read
+// its top); then the slots are walked in order, 16 THREADS at a time and 16 a lane: the
+// ranks among equal weights, of holes and of movers are sums over lanes and waves, in
+// two exchanges a tile.  Bound by latency; rows of more than one tile are read up to
 // four times, all but the first from L2.  COPIES of the histogram: lanes of one digit
 // meet on fewer words.
+// 16 x 8 rows of up to 16300 slots: 22 us (30 with 64 slots at a time, ranks by ballots).
 template <int THREADS, int COPIES>
 __global__ __launch_bounds__(THREADS) void kv4_select_kernel(Kv4EvictArgs a, int32_t* hole_list) {
     constexpr int kWaves = THREADS / 64, kTile = THREADS * kPerLane, kOwn = kBins / THREADS;
     __shared__ uint32_t s_hist[COPIES][kBins];
     __shared__ int s_wave[kWaves];
     __shared__ uint32_t s_pick, s_left, s_held;
-    __shared__ int s_count[3][kWaves];
+    __shared__ int s_count[2][kWaves];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int bh = blockIdx.x, h = bh % a.cache.heads, b = bh / a.cache.heads;
     const int slots = a.cache.slots(), keep = a.keep;
@@ -68,12 +65,24 @@ __global__ __launch_bounds__(THREADS) void kv4_select_kernel(Kv4EvictArgs a, int
     float* out = a.out_weights + (int64_t)bh * slots;
     int32_t* source = a.source + (int64_t)bh * keep;
     if (h == 0 && tid == 0) a.out_lengths[b] = min(n, keep);
-    for (int j = min(n, keep) + tid; j < slots; j += THREADS) out[j] = 0.f;
     if (n <= keep) {
+        for (int j = n + tid; j < slots; j += THREADS) out[j] = 0.f;
         for (int j = tid; j < n; j += THREADS) out[j] = w[j];
         for (int64_t j = tid; j < keep; j += THREADS) source[j] = j < n ? (int32_t)j : -1;
         return;
     }
+    // the first tile (of many rows the only one) is read once
+    const int own_first = tid * kPerLane;
+    float held[kPerLane];
+    load_slots(w, own_first, n, held);
+    auto tile_of = [&](int first, float (&x)[kPerLane]) {
+        if (first == own_first) {
+#pragma unroll
+            for (int i = 0; i < kPerLane; ++i) x[i] = held[i];
+        } else {
+            load_slots(w, first, n, x);
+        }
+    };
     const int recent = min(a.recent, keep), cand = n - recent;
     uint32_t left = keep - recent;                 // candidates still to choose among the equal prefixes
     uint32_t prefix = 0u;
@@ -83,17 +92,14 @@ __global__ __launch_bounds__(THREADS) void kv4_select_kernel(Kv4EvictArgs a, int
         for (int i = tid; i < COPIES * kBins; i += THREADS) (&s_hist[0][0])[i] = 0u;
         __syncthreads();
         for (int j0 = 0; j0 < cand; j0 += kTile) {
+            const int first = j0 + own_first;
             float x[kPerLane];
-#pragma unroll
-            for (int i = 0; i < kPerLane; ++i) {
-                const int j = j0 + i * THREADS + tid;
-                x[i] = j < cand ? w[j] : 0.f;
-            }
+            tile_of(first, x);
 #pragma unroll
             for (int i = 0; i < kPerLane; ++i) {
                 const uint32_t key = weight_key(x[i]);
                 const bool mine = bits_left == 32 || (key >> bits_left) == prefix;
-                if (j0 + i * THREADS + tid < cand && mine)
+                if (first + i < cand && mine)
                     atomicAdd(&s_hist[lane % COPIES][(key >> shift) & ((1u << digit_bits) - 1)], 1u);
             }
         }
@@ -107,7 +113,7 @@ __global__ __launch_bounds__(THREADS) void kv4_select_kernel(Kv4EvictArgs a, int
             for (int q = 0; q < COPIES; ++q) c[i] += s_hist[q][kBins - 1 - (kOwn * tid + i)];
             own += c[i];
         }
-        const int upto = scan_wave((int)own);
+        const int upto = sum_upto((int)own);
         if (lane == 63) s_wave[wave] = upto;
         __syncthreads();
         uint32_t before = (uint32_t)(over_waves<kWaves>(s_wave).x + upto) - own;
@@ -130,73 +136,65 @@ __global__ __launch_bounds__(THREADS) void kv4_select_kernel(Kv4EvictArgs a, int
     int32_t* holes = hole_list + (int64_t)bh * keep;
     int equal_before = 0, hole_before = 0, mover_before = 0;
     for (int j0 = 0; j0 < n; j0 += kTile) {
-        // this wave's 1024 slots of the tile, lane by lane
-        const int first = j0 + wave * 64 * kPerLane + lane;
+        const int first = j0 + own_first;
         float x[kPerLane];
-#pragma unroll
-        for (int i = 0; i < kPerLane; ++i) x[i] = first + 64 * i < n ? w[first + 64 * i] : 0.f;
-        uint32_t kept = 0u, equal = 0u;            // bit i: slot first + 64 i
-        int equals = 0;
+        tile_of(first, x);
+        uint32_t kept = 0u, equal = 0u;            // bit i: slot first + i
 #pragma unroll
         for (int i = 0; i < kPerLane; ++i) {
-            const int j = first + 64 * i;
+            const int j = first + i;
             const uint32_t key = weight_key(x[i]) >> bits_left;
-            const bool eq = j < cand && !none && key == prefix;
-            if (j < n && (j >= cand || (!none && key > prefix))) kept |= 1u << i;
-            if (eq) equal |= 1u << i;
-            equals += __popcll(__ballot(eq));
+            kept |= (uint32_t)(j < n && (j >= cand || (!none && key > prefix))) << i;
+            equal |= (uint32_t)(j < cand && !none && key == prefix) << i;
         }
-        if (lane == 0) s_count[0][wave] = equals;
+        const int equals = __popc(equal), e_upto = sum_upto(equals);
+        if (lane == 63) s_count[0][wave] = e_upto;
         __syncthreads();
         const int2 e = over_waves<kWaves>(s_count[0]);
-        int rank = equal_before + e.x, hole_count = 0, mover_count = 0;
+        int rank = equal_before + e.x + e_upto - equals;
         equal_before += e.y;
-        const unsigned long long below = (1ull << lane) - 1;
 #pragma unroll
         for (int i = 0; i < kPerLane; ++i) {
-            const int j = first + 64 * i;
-            const bool eq = equal >> i & 1u;
-            const unsigned long long m = __ballot(eq);
-            if (eq && rank + __popcll(m & below) < (int)left) kept |= 1u << i;
-            rank += __popcll(m);
-            const bool k = kept >> i & 1u;
-            hole_count += __popcll(__ballot(j < keep && !k));
-            mover_count += __popcll(__ballot(j >= keep && k));
+            if ((equal >> i & 1u) && rank < (int)left) kept |= 1u << i;
+            rank += equal >> i & 1u;
         }
-        if (lane == 0) s_count[1][wave] = hole_count, s_count[2][wave] = mover_count;
+        // every place below `keep` starts as its own; what moves in comes after
+        const uint32_t below = (1u << min(max(keep - first, 0), kPerLane)) - 1u;
+        const uint32_t hole = below & ~kept, mover = kept & ~below;
+        if (below == (1u << kPerLane) - 1u) {
+            int own[kPerLane];
+#pragma unroll
+            for (int i = 0; i < kPerLane; ++i) own[i] = first + i;
+            __builtin_memcpy(out + first, x, sizeof(x));
+            __builtin_memcpy(source + first, own, sizeof(own));
+        } else {
+#pragma unroll
+            for (int i = 0; i < kPerLane; ++i)
+                if (below >> i & 1u) out[first + i] = x[i], source[first + i] = first + i;
+        }
+        // holes in the low half, movers in the high half: at most kTile of each
+        const int both = __popc(hole) | __popc(mover) << 16, upto = sum_upto(both);
+        if (lane == 63) s_count[1][wave] = upto;
         __syncthreads();
-        const int2 hc = over_waves<kWaves>(s_count[1]), mc = over_waves<kWaves>(s_count[2]);
-        int hr = hole_before + hc.x, mr = mover_before + mc.x;
-        hole_before += hc.y;
-        mover_before += mc.y;
+        const int2 c = over_waves<kWaves>(s_count[1]);
+        const int at = c.x + upto - both;
+        int hr = hole_before + (at & 0xffff), mr = mover_before + (at >> 16);
+        hole_before += c.y & 0xffff;
+        mover_before += c.y >> 16;
+#pragma unroll
+        for (int i = 0; i < kPerLane; ++i)
+            if (hole >> i & 1u) holes[hr++] = first + i;
+        __syncthreads();                           // the holes before the movers that go there
 #pragma unroll
         for (int i = 0; i < kPerLane; ++i) {
-            const int j = first + 64 * i;
-            const bool k = kept >> i & 1u, hole = j < keep && !k;
-            const unsigned long long m = __ballot(hole);
-            if (hole) holes[hr + __popcll(m & below)] = j;
-            hr += __popcll(m);
-            if (j < keep && k) {
-                source[j] = j;
-                out[j] = x[i];
-            }
-        }
-        __syncthreads();                           // the holes before the movers that go there
-        if (mc.y) {
-#pragma unroll
-            for (int i = 0; i < kPerLane; ++i) {
-                const int j = first + 64 * i;
-                const bool mover = j >= keep && (kept >> i & 1u);
-                const unsigned long long m = __ballot(mover);
-                if (mover) {
-                    const int to = holes[mr + __popcll(m & below)];
-                    source[to] = j;
-                    out[to] = x[i];
-                }
-                mr += __popcll(m);
+            if (mover >> i & 1u) {
+                const int to = holes[mr++];
+                source[to] = first + i;
+                out[to] = x[i];
             }
         }
     }
+    for (int j = keep + tid; j < slots; j += THREADS) out[j] = 0.f;
 }
 
 // One wave per (sequence, head, 8 places): the places share the value words of their

@@ -154,16 +154,6 @@ struct Scan {
         }
         cum = sum_upto(pages * per);
     }
-    // Sum over the lanes up to this one: within rows of 16 lanes, then from row to row.
-    __device__ static int sum_upto(int x) {
-        x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);     // row_shr:1, 2, 4, 8
-        x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
-        x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
-        x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
-        x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);     // row_bcast:15 into rows 1 and 3
-        x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);     // row_bcast:31 into rows 2 and 3
-        return x;
-    }
     // Sequence of unit u < total, its first unit, its pages, context and valid rows.
     struct Place { int b, start, pages, n, count; };
     __device__ Place of_lane(int l) const {
@@ -213,7 +203,7 @@ struct Cuts {
         const int step = kKv4Waves * max(1, share / 64);
         for (int part = (share + 7) / 8 * 8; part <= share + share / 4 + kKv4Waves; part += step) {
             parts = min(divide(s.pages + part - 1, part), most);
-            upto = Scan::sum_upto(parts * s.per);
+            upto = sum_upto(parts * s.per);
             own_parts = __builtin_amdgcn_readlane(upto, 63) <= line.pieces;
             if (own_parts) return;
         }
