@@ -520,6 +520,9 @@ struct Plan { int rows, ways; Line line; };
 Plan plan(int64_t batch, int64_t T, int64_t q_heads, int64_t heads, int64_t max_pages) {
     Plan p{};
     const int64_t rows = T * (q_heads / heads);
+    // Up to 16 rows in a tile of 16 (4 rows, 32 x 16k slots: 96 us, 122 in a tile of 32), more in
+    // tiles of 32, each of which turns the codes into operands for itself (64 rows, 8 x 4000
+    // slots: 25 us, 28.5 in tiles of 16).
     p.rows = rows <= 16 ? 16 : 32;
     const int64_t tiles = (rows + p.rows - 1) / p.rows, cus = device_cu_count();
     // Many row tiles: four of them a workgroup, two waves each, once that fills the GPU
@@ -550,18 +553,17 @@ hipError_t launch_kv4_attention(const Kv4AttentionArgs& a, void* ws, size_t data
     const Plan p = plan(c.batch, a.block.T, a.q_heads, c.heads, c.max_pages);
     auto* states = reinterpret_cast<float*>(static_cast<char*>(ws) + data_off);
     auto* counters = reinterpret_cast<unsigned int*>(static_cast<char*>(ws) + kCountersOff);
-    return kv4_by_type(a.dtype, c.head_dim, p.rows, [&](auto tag, auto size, auto rows) {
+    return kv4_by_type(a.dtype, c.head_dim, [&](auto tag, auto size) {
         using T = decltype(tag);
-        constexpr int D = decltype(size)::value, MT = decltype(rows)::value;
-        auto go = [&](auto ways) {
-            constexpr int WAYS = decltype(ways)::value;
-            hipLaunchKernelGGL((kv4_attention_kernel<T, D, MT, WAYS>), dim3(p.line.pieces), dim3(kKv4Threads), 0, s, a,
-                               p.line, states, counters);
+        constexpr int D = decltype(size)::value;
+        auto go = [&](auto rows, auto ways) {
+            hipLaunchKernelGGL((kv4_attention_kernel<T, D, decltype(rows)::value, decltype(ways)::value>),
+                               dim3(p.line.pieces), dim3(kKv4Threads), 0, s, a, p.line, states, counters);
         };
-        if constexpr (MT == 32) {
-            if (p.ways == 2) return go(std::integral_constant<int, 2>{});
-        }
-        go(std::integral_constant<int, 8>{});
+        using std::integral_constant;
+        if (p.rows == 16) go(integral_constant<int, 16>{}, integral_constant<int, 8>{});
+        else if (p.ways == 8) go(integral_constant<int, 32>{}, integral_constant<int, 8>{});
+        else go(integral_constant<int, 32>{}, integral_constant<int, 2>{});
     });
 }
 

@@ -288,7 +288,8 @@ size_t kv4_evict_data_bytes(int64_t batch, int64_t heads, int64_t keep) {
 hipError_t launch_kv4_evict(const Kv4EvictArgs& a, void* ws, size_t data_off, hipStream_t s) {
     const Kv4Cache& c = a.cache;
     auto* holes = reinterpret_cast<int32_t*>(static_cast<char*>(ws) + data_off);
-    // few slots: a short tile and a small workgroup, whose barriers and histogram take less
+    // one tile of a small workgroup where that holds a row: its barriers and histogram take less
+    // (600 slots: 10.6 us, 14.2 by the large one)
     const dim3 grid_select(c.batch * c.heads);
     if (c.slots() <= 256 * kPerLane)
         hipLaunchKernelGGL((kv4_select_kernel<256, 1>), grid_select, dim3(256), 0, s, a, holes);

@@ -291,14 +291,12 @@ template <int D, int MT> struct KeyWords {
         for (int i = 0; i < S::KB; ++i) scale[i] = *page_word(page, at.key_scale, 64 * i);
     }
 };
-template <typename F> hipError_t kv4_by_type(int dtype, int head_dim, int rows, F&& f) {
-    auto by_rows = [&](auto tag, auto size) {
-        if (rows == 16) f(tag, size, std::integral_constant<int, 16>{});
-        else f(tag, size, std::integral_constant<int, 32>{});
-    };
+
+// f(query type, head size) as types.
+template <typename F> hipError_t kv4_by_type(int dtype, int head_dim, F&& f) {
     auto by_size = [&](auto tag) {
-        if (head_dim == 64) by_rows(tag, std::integral_constant<int, 64>{});
-        else by_rows(tag, std::integral_constant<int, 128>{});
+        if (head_dim == 64) f(tag, std::integral_constant<int, 64>{});
+        else f(tag, std::integral_constant<int, 128>{});
     };
     if (dtype == DELS_DTYPE_BF16) by_size(bf16_t{});
     else by_size(f16_t{});

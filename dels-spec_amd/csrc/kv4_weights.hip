@@ -9,6 +9,12 @@
 // wave turns 32 slots' codes into operands once and takes all row tiles over them.
 // Rows beyond 128 go in further rounds over the piece's pages.  Every slot belongs to
 // one wave: no atomics, one order of additions.
+//
+// Tiles of 16 rows whatever their number: the products are few enough that the shorter
+// chains of the 16-row instruction count for more than its rate (64 rows: 8 x 4000
+// slots 17.8 us with tiles of 32, 14.1 with 16; 64 x 8000 slots 110 and 101; 4 x 2000 slots
+// of 2048 rows 196 and 175).  Long caches are bound by the read of their keys (32 x 16k
+// slots, one token: 66 us, 4.3 TB/s), short ones by latency.
 #include <algorithm>
 
 #include "kv4_mma.h"
@@ -18,9 +24,10 @@ namespace dels {
 namespace {
 
 constexpr int kMinPages = kKv4Waves;             // fewest pages of a workgroup's piece
+constexpr int MT = 16;                           // rows of a tile
 constexpr int kRows = 128;                       // rows whose queries fit LDS at a time
 
-template <typename T, int D, int MT>
+template <typename T, int D>
 __global__ __launch_bounds__(kKv4Threads, 4) void kv4_weights_kernel(Kv4WeightsArgs a, int pieces) {
     using S = Shape<D, MT>;
     using F = typename Frag<T>::type;
@@ -102,8 +109,8 @@ __global__ __launch_bounds__(kKv4Threads, 4) void kv4_weights_kernel(Kv4WeightsA
                 const int next = uniform(id_at(p + kKv4Waves));
                 next_keys.load(heads + (named(next) ? next : 0) * page_stride, at_lane);
                 asm volatile("" ::: "memory");
-                // the slot that this lane writes, of the four (two) it has sums for: by its group
-                const int mine = p * kKv4Page + (MT == 16 ? 32 * (g >> 1) + S::slot_of(g & 1, col) : 32 * g + S::slot_of(0, col));
+                // the slot that this lane writes, of the four it has sums for: by its group
+                const int mine = p * kKv4Page + 32 * (g >> 1) + S::slot_of(g & 1, col);
                 float sum = r0 > 0 ? a.out[out_row + mine] : mine < n ? a.weights[out_row + mine] : 0.f;
                 if (named(id) && tiles > 0) {
                     const bool masked = (p + 1) * kKv4Page > n;
@@ -114,7 +121,7 @@ __global__ __launch_bounds__(kKv4Threads, 4) void kv4_weights_kernel(Kv4WeightsA
                         for (int t = 0; t < S::KT; ++t)
 #pragma unroll
                             for (int k = 0; k < S::KS; ++k) {
-                                const uint32_t scales = keys.scale[k * 8 / 32 % S::KB] >> (MT == 16 ? 8 * t : at_lane.half);
+                                const uint32_t scales = keys.scale[k * 8 / 32 % S::KB] >> (8 * t);
                                 kf[t][k] = decode8<T>(keys.code[s][t][k], key_scale<T>(scales, 2 * s));
                             }
                         float part[S::KT] = {};
@@ -130,36 +137,33 @@ __global__ __launch_bounds__(kKv4Threads, 4) void kv4_weights_kernel(Kv4WeightsA
 #pragma unroll
                                 for (int t = 0; t < S::KT; ++t) acc[t] = mma(qk, kf[t][k], acc[t]);
                             }
-                            // registers 4 q .. 4 q + 3 are rows 8 q + 4 g .. (4 g .. of a tile of 16)
+                            // a lane's registers are rows 4 g .. 4 g + 3 of the tile
+                            const int row = tile * MT + 4 * g;
+                            const f32x4 lse = *reinterpret_cast<const f32x4*>(&s_lse[row]);
+                            if (masked) {
+                                asm volatile("");            // a branch, not a selection on every page
 #pragma unroll
-                            for (int q4 = 0; q4 < S::ACC / 4; ++q4) {
-                                const int row = tile * MT + 8 * q4 + 4 * g;
-                                const f32x4 lse = *reinterpret_cast<const f32x4*>(&s_lse[row]);
-                                if (masked) {
-                                    asm volatile("");        // a branch, not a selection on every page
+                                for (int x = 0; x < 4; ++x) {
+                                    const int lim = s_lim[row + x];
+                                    const uint64_t bits = s_bits[row + x];
 #pragma unroll
-                                    for (int x = 0; x < 4; ++x) {
-                                        const int lim = s_lim[row + x];
-                                        const uint64_t bits = s_bits[row + x];
-#pragma unroll
-                                        for (int t = 0; t < S::KT; ++t) {
-                                            const int i = p * kKv4Page + 32 * s + S::slot_of(t, col) - n;
-                                            const uint32_t bit = i < 0 || i > 63 ? 0u : (uint32_t)(bits >> (i & 63)) & 1u;
-                                            acc[t][4 * q4 + x] = i < lim || bit ? acc[t][4 * q4 + x] : -__builtin_inff();
-                                        }
+                                    for (int t = 0; t < S::KT; ++t) {
+                                        const int i = p * kKv4Page + 32 * s + S::slot_of(t, col) - n;
+                                        const uint32_t bit = i < 0 || i > 63 ? 0u : (uint32_t)(bits >> (i & 63)) & 1u;
+                                        acc[t][x] = i < lim || bit ? acc[t][x] : -__builtin_inff();
                                     }
                                 }
-#pragma unroll
-                                for (int t = 0; t < S::KT; ++t)
-#pragma unroll
-                                    for (int x = 0; x < 4; ++x)
-                                        part[t] += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[t][4 * q4 + x], unit, -lse[x]));
                             }
+#pragma unroll
+                            for (int t = 0; t < S::KT; ++t)
+#pragma unroll
+                                for (int x = 0; x < 4; ++x)
+                                    part[t] += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[t][x], unit, -lse[x]));
                         }
 #pragma unroll
                         for (int t = 0; t < S::KT; ++t) {
                             const float all = sum_over_groups<MT>(part[t]);
-                            if (g == (MT == 16 ? 2 * s + t : s)) sum += all;
+                            if (g == 2 * s + t) sum += all;
                         }
                     }
                 }
@@ -201,10 +205,9 @@ hipError_t launch_kv4_weights(const Kv4WeightsArgs& a, hipStream_t s) {
     // two workgroups a CU: 32 x 16k slots 74 us with one, 68 with two (66 with the first keys ahead of the queries)
     const int pieces = (int)std::min<int64_t>(2 * device_cu_count(), std::max<int64_t>((int64_t)c.batch * c.heads,
                                                                                        (units + kMinPages - 1) / kMinPages));
-    const int rows = (int64_t)a.block.T * (a.q_heads / c.heads) <= 16 ? 16 : 32;
-    return kv4_by_type(a.dtype, c.head_dim, rows, [&](auto tag, auto size, auto tile) {
-        hipLaunchKernelGGL((kv4_weights_kernel<decltype(tag), decltype(size)::value, decltype(tile)::value>), dim3(pieces),
-                           dim3(kKv4Threads), 0, s, a, pieces);
+    return kv4_by_type(a.dtype, c.head_dim, [&](auto tag, auto size) {
+        hipLaunchKernelGGL((kv4_weights_kernel<decltype(tag), decltype(size)::value>), dim3(pieces), dim3(kKv4Threads), 0, s,
+                           a, pieces);
     });
 }
 
