@@ -43,7 +43,7 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
 }
 
-constexpr int kMinPages = 2 * kKv4Waves;      // fewest pages of a piece (one row over 700 slots: 10.6 us in two of eight, 9.2 in one)
+constexpr int kMinPages = 2 * kKv4Waves;      // fewest pages of a part (one row over 700 slots: 10.6 us in two of eight, 9.2 in one)
 constexpr int kCounterWords = 16;      // words from one arrival counter to the next
 // Most pieces of one tile group: their states are joined by one workgroup, about 0.25 us
 // each (one row over 94k slots: 45 us in 184 pieces, 29 in 32).

@@ -178,7 +178,7 @@ struct Scan {
 struct Line {
     int tiles;                 // groups of 8 / WAYS row tiles per (b, h)
     int pieces;                // workgroups
-    int least;                 // fewest pages of a piece
+    int least;                 // fewest pages of a part of a tile group's pages
 };
 
 // How the line is cut into at most `pieces` pieces.
@@ -196,7 +196,9 @@ struct Cuts {
     bool own_parts;
 
     __device__ Cuts(const Scan& s, const Line& line, int most) {
-        share = max(line.least, divide(s.total + line.pieces - 1, line.pieces));
+        // `least` keeps tiles of few pages whole; it gathers no more of them than an even share
+        const int groups = s.c.batch * s.per;
+        share = max(min(line.least, divide(s.total + groups - 1, groups)), divide(s.total + line.pieces - 1, line.pieces));
         own_parts = false;
         parts = upto = 0;
         if (s.c.batch > 64) return;

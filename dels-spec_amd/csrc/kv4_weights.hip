@@ -23,7 +23,7 @@ namespace dels {
 
 namespace {
 
-constexpr int kMinPages = kKv4Waves;             // fewest pages of a workgroup's piece
+constexpr int kMinPages = kKv4Waves;             // fewest pages of a part
 constexpr int MT = 16;                           // rows of a tile
 constexpr int kRows = 128;                       // rows whose queries fit LDS at a time
 
