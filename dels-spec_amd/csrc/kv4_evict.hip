@@ -202,7 +202,9 @@ __global__ __launch_bounds__(THREADS) void kv4_select_kernel(Kv4EvictArgs a, int
 // places before any of it is written: K words 16 (8) lanes a slot, value words of D / 64
 // channels a lane.  A moved slot's value codes lie in D words of eight slots each, so
 // eight times what moves is read: consecutive movers are often neighbours, whose
-// words the caches still hold.
+// words the caches still hold.  Bound by those requests: 16 x 8 rows of up to 16300 slots to
+// 4096, head size 128: 62 us, 62 MB written (38 us without
+// the values, 52 without the keys, 55 without the scales).
 template <int D>
 __global__ __launch_bounds__(kMoveThreads) void kv4_move_kernel(Kv4Cache c, const int32_t* lengths,
                                                                 const int32_t* __restrict__ sources, int keep,

@@ -85,3 +85,11 @@ def test_refusals_before_the_gpu(pkg):
     assert evict(cache(pkg), ow=0x5000) == -1
     assert evict(cache(pkg), ws_bytes=4) == -4
     assert evict(cache(pkg), w=None) == -1
+
+
+def test_workspace_of_the_longest_block_serves_shorter_ones(pkg):
+    lib = pkg._lib.load()
+    for batch, q_heads, heads in ((1, 8, 8), (3, 32, 8), (40, 32, 8), (7, 64, 8)):
+        for max_pages in (1, 40, 2000):
+            sizes = [lib.dels_kv4_attention_ws_bytes(batch, T, q_heads, heads, 128, max_pages) for T in range(1, 700)]
+            assert all(x <= y for x, y in zip(sizes, sizes[1:]))
