@@ -31,7 +31,7 @@ int cache_of(const dels_kv4_cache* p, Kv4Cache& c) {
         !extent_ok(p->batch) || p->max_pages < 0 || p->max_pages > (int64_t(1) << 24))
         return fail(DELS_ERR_INVALID_ARGUMENT, "bad cache extents pages=%lld heads=%lld batch=%lld max_pages=%lld",
                     (long long)p->num_pages, (long long)p->kv_heads, (long long)p->batch, (long long)p->max_pages);
-    if (p->ld_table < p->max_pages || p->ld_table >= (int64_t(1) << 40))
+    if ((p->ld_table < p->max_pages && p->ld_table != 0) || p->ld_table >= (int64_t(1) << 40))
         return fail(DELS_ERR_INVALID_ARGUMENT, "table row stride %lld out of range", (long long)p->ld_table);
     if (p->batch && p->max_pages && !p->table) return fail(DELS_ERR_INVALID_ARGUMENT, "page table is NULL");
     if (p->num_pages && !p->data) return fail(DELS_ERR_INVALID_ARGUMENT, "cache data is NULL");
@@ -79,7 +79,7 @@ int check_block(const Kv4Cache& c, const void* q, int64_t qb, int64_t qt, int64_
     if (block == DELS_KV4_MASK) {
         if (!mask) return fail(DELS_ERR_INVALID_ARGUMENT, "block mask is NULL");
         if (T > 64) return fail(DELS_ERR_UNSUPPORTED, "a block mask holds 64 slots (T = %lld)", (long long)T);
-        if (ld_mask < T || ld_mask >= (int64_t(1) << 40))
+        if ((ld_mask < T && ld_mask != 0) || ld_mask >= (int64_t(1) << 40))
             return fail(DELS_ERR_INVALID_ARGUMENT, "mask row stride %lld out of range", (long long)ld_mask);
     }
     if (!(scale == scale) || scale == __builtin_inff() || scale == -__builtin_inff())

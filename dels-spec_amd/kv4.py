@@ -39,6 +39,16 @@ def page_bytes(head_dim: int) -> int:
     return 66 * head_dim + 128
 
 
+def _row_stride(t: torch.Tensor, columns: int, name: str) -> int:
+    """Row stride of a 2-d tensor: 0 where all rows are one (an expanded tensor), else at least ``columns``."""
+    stride = t.stride(0)
+    if t.shape[0] <= 1:
+        return columns                     # one row: no stride that matters
+    if 0 < stride < columns:
+        raise ValueError(f"{name} must not have overlapping rows (row stride {stride}, {columns} columns)")
+    return stride
+
+
 class KV4Cache:
     """Pages of a 4-bit key/value cache and the table that hands them out.
 
@@ -46,7 +56,8 @@ class KV4Cache:
     ``block_table`` int32 ``[batch, max_pages]``, unit column stride: slot ``j`` of
     sequence ``b`` is slot ``j % 64`` of page ``block_table[b, j // 64]``.  Entries
     outside ``[0, num_pages)`` name no page.  Pages may be shared by sequences that
-    only read them.  The cache keeps both tensors; a table can be rewritten in place.
+    only read them, and a whole row by an expanded table.  The cache keeps both
+    tensors; a table can be rewritten in place.
     """
 
     def __init__(self, data: torch.Tensor, block_table: torch.Tensor, head_dim: int):
@@ -74,7 +85,8 @@ class KV4Cache:
         self._scale = self.head_dim ** -0.5
         self._ws_bytes = {}                    # attention's workspace size by (T, q_heads)
         self._params = _lib.Kv4CacheParams(data.data_ptr(), data.shape[0], self.kv_heads, self.head_dim,
-                                           block_table.data_ptr(), max(block_table.stride(0), self.max_pages),
+                                           block_table.data_ptr(),
+                                           _row_stride(block_table, self.max_pages, "block_table"),
                                            self.batch, self.max_pages)
         self._ref = ctypes.byref(self._params)
 
@@ -175,7 +187,7 @@ def _block_args(block: Block, cache: KV4Cache, T: int) -> tuple[int, Optional[in
                              f"{tuple(block.shape)}")
         if T > 1 and block.stride(1) != 1:
             raise ValueError("a block mask must have unit column stride")
-        return _lib.KV4_BLOCK_MASK, block.data_ptr(), max(block.stride(0), T)
+        return _lib.KV4_BLOCK_MASK, block.data_ptr(), _row_stride(block, T, "a block mask")
     if block not in _lib.KV4_BLOCK_CODES:
         raise ValueError(f"block must be one of {sorted(_lib.KV4_BLOCK_CODES)} or an int64 mask, got {block!r}")
     return _lib.KV4_BLOCK_CODES[block], None, 0
@@ -191,8 +203,8 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, lengths: torch.Tensor, *, bl
     cache's heads.  Every row sees slots ``[0, lengths[b])``; of the block's own slots
     (which ``kv4_append`` wrote) ``block`` says which: ``"causal"``, ``"full"``, ``"none"``, or
     an int64 ``[batch, T]`` of bits, bit ``i`` of row ``t`` for slot ``lengths[b] + i`` (a tree of
-    drafts; T at most 64).  ``counts`` int32 ``[batch]`` are the valid rows (None: T).
-    ``scale`` defaults to ``head_dim ** -0.5``.  Returns ``(out, lse)``: ``out`` like ``q``, ``lse``
+    drafts; T at most 64; expanded where all sequences have one tree).  ``counts`` int32
+    ``[batch]`` are the valid rows (None: T).  ``scale`` defaults to ``head_dim ** -0.5``.  Returns ``(out, lse)``: ``out`` like ``q``, ``lse``
     fp32 ``[batch, T, q_heads]``, the logarithm of each softmax's sum; rows that see
     nothing give 0 and -inf.
     """

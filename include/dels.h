@@ -563,17 +563,18 @@ int dels_markov_graph_create(const dels_markov_rollout* p, void** graph_out);
  * magnitudes over 3e38 as 3e38.
  *
  * Every sequence has a row of page numbers; slot j of sequence b lies in page
- * table[b * ld_table + j / 64].  An entry outside [0, num_pages) names no page: writes
- * to it are dropped, reads give 0, attention does not see it.  Lengths and counts
- * are device arrays that the kernels clamp (lengths to [0, 64 max_pages], counts
- * to [0, T]); nothing is read back to the host.  `data` is 128-byte aligned.
+ * table[b * ld_table + j / 64] (ld_table 0: one row that all sequences read).  An entry
+ * outside [0, num_pages) names no page: writes to it are dropped, reads give 0,
+ * attention does not see it.  Lengths and counts are device arrays that the kernels
+ * clamp (lengths to [0, 64 max_pages], counts to [0, T]); nothing is read back to the
+ * host.  `data` is 128-byte aligned.
  */
 typedef struct dels_kv4_cache {
     void* data;                /* [num_pages, kv_heads, 66 * head_dim + 128] bytes */
     int64_t num_pages;
     int64_t kv_heads;
     int64_t head_dim;          /* 64 or 128 */
-    const int32_t* table;      /* [batch, max_pages] page numbers, row stride ld_table */
+    const int32_t* table;      /* [batch, max_pages] page numbers, row stride ld_table (>= max_pages, or 0) */
     int64_t ld_table;
     int64_t batch;
     int64_t max_pages;
@@ -584,7 +585,8 @@ typedef struct dels_kv4_cache {
 #define DELS_KV4_CAUSAL 0      /* the block's slots up to their own */
 #define DELS_KV4_FULL 1        /* the block's valid slots */
 #define DELS_KV4_NONE 2        /* the context alone */
-#define DELS_KV4_MASK 3        /* the block's valid slots i with bit i of the row's mask set; T <= 64 */
+#define DELS_KV4_MASK 3        /* the block's valid slots i with bit i of mask[b * ld_mask + t] set; T <= 64,
+                                * ld_mask >= T, or 0 for one [T] mask that all sequences share */
 
 /* Bytes of a page of one head (0 for a head size that is not supported). */
 size_t dels_kv4_page_bytes(int64_t head_dim);

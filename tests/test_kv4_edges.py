@@ -1,0 +1,55 @@
+"""CPU tests of what the 4-bit cache's Python calls hand to the C ABI: no kernel is launched."""
+
+import types
+
+import pytest
+import torch
+
+import test_kv4_host as host
+
+
+@pytest.fixture
+def on_cpu(pkg, monkeypatch):
+    """The wrappers' checks with CPU tensors in the GPU's place."""
+    monkeypatch.setattr(pkg.kv4, "_require_cuda", lambda *a: None)
+    return pkg
+
+
+def last_row_ends(stride, rows, columns):
+    return (rows - 1) * stride + columns
+
+
+@pytest.mark.parametrize("T", [1, 5, 64])
+def test_a_block_mask_is_read_inside_its_storage(pkg, T):
+    cache = types.SimpleNamespace(_index=-1, batch=4, device="cpu")
+    for mask in (torch.zeros(1, T, dtype=torch.int64).expand(4, T), torch.zeros(4, T, dtype=torch.int64),
+                 torch.zeros(4, T + 3, dtype=torch.int64)[:, :T]):
+        mode, p, ld = pkg.kv4._block_args(mask, cache, T)
+        assert mode == 3 and p == mask.data_ptr()
+        assert last_row_ends(ld, 4, T) <= mask.untyped_storage().nbytes() // 8
+        assert ld == mask.stride(0)
+    if T > 1:
+        with pytest.raises(ValueError, match="overlapping rows"):
+            pkg.kv4._block_args(torch.zeros(T + 3, dtype=torch.int64).as_strided((4, T), (1, 1)), cache, T)
+
+
+def test_a_page_table_is_read_inside_its_storage(on_cpu):
+    data = torch.zeros(5, 2, 4352, dtype=torch.uint8)
+    for table in (torch.zeros(1, 3, dtype=torch.int32).expand(4, 3), torch.zeros(4, 3, dtype=torch.int32),
+                  torch.zeros(4, 7, dtype=torch.int32)[:, 2:5], torch.zeros(4, 1, dtype=torch.int32),
+                  torch.zeros(1, 1, dtype=torch.int32).expand(4, 1), torch.zeros(1, 3, dtype=torch.int32)):
+        params = on_cpu.KV4Cache(data, table, 64)._params
+        room = table.untyped_storage().nbytes() // 4 - table.storage_offset()
+        assert last_row_ends(params.ld_table, table.shape[0], table.shape[1]) <= room
+    with pytest.raises(ValueError, match="overlapping rows"):
+        on_cpu.KV4Cache(data, torch.zeros(9, dtype=torch.int32).as_strided((4, 3), (2, 1)), 64)
+
+
+def test_one_row_for_all_sequences_is_a_stride_of_zero(pkg):
+    lib = pkg._lib.load()
+    assert lib.dels_kv4_append(host.cache(pkg, ld_table=0), 0x1000, 512, 128, 128, 0x2000, 512, 128, 128, 1, 0x3000,
+                               None, 0, None) == 0
+    # past the stride checks: the workspace is refused next
+    for ld in (0, 4):
+        assert lib.dels_kv4_attention(host.cache(pkg), 0x1000, 4096, 1024, 128, 1, 8, 4, 0x3000, None, 3, 0x9000, ld,
+                                      1.0, 0x4000, 4096, 1024, 128, 0x5000, None, 0, None) == -4
