@@ -6,7 +6,10 @@ block, rejected rows are cropped by going on from a shorter length.  The
 reference keeps the cache in bf16 inside transformers; here it is pages of 64
 slots in 4 bits a value (include/dels.h describes a page), which a sequence's row
 of page numbers names.  Lengths live on the GPU and no call reads them back, so
-every call can be captured into a graph.
+every call can be captured into a graph.  A captured call has a workspace of its
+own, from the graph's memory, whose counters a node of the graph clears; one that is
+given (``workspace``, from ``ops.new_workspace``) saves that node and is the caller's to
+keep: calls that share it must not overlap, in whatever graphs and streams they are.
 
   * ``kv4_append``    -- a block's rows into the cache
   * ``kv4_read``      -- the values that slots of the cache stand for
@@ -26,10 +29,11 @@ from typing import Optional, Union
 import torch
 
 from . import _lib
-from .ops import _DTYPES, _WORKSPACES, _require_cuda, _stream_ptr, workspace
+from .ops import _DTYPES, _WORKSPACES, _require_cuda, _stream_ptr
 
 PAGE = 64              # slots of a page
 HEAD_DIMS = (64, 128)
+_CONTROL_BYTES = 1 << 16    # a workspace's control area (include/dels.h): the arrival counters lie there
 
 
 def page_bytes(head_dim: int) -> int:
@@ -136,6 +140,28 @@ def _require_rows(t: torch.Tensor, cache: KV4Cache, heads: Optional[int], name: 
     return (t.data_ptr(), sb if shape[0] > 1 else 0, st if shape[1] > 1 else 0, sh if shape[2] > 1 else 0)
 
 
+def _call_workspace(given: Optional[torch.Tensor], cache: KV4Cache, need: int, stream: int, *,
+                    counters: bool) -> torch.Tensor:
+    """The caller's workspace, a captured call's own, or else the stream's shared one.
+
+    The shared one may be replaced by a larger one between a graph's replays, its zero
+    fill would belong to the one graph that captured it, and graphs that are replayed on
+    several streams would meet in it.
+    """
+    if given is not None:
+        if not isinstance(given, torch.Tensor) or given.get_device() != cache._index:
+            _elsewhere(given, cache, "workspace")
+        if given.dtype != torch.uint8 or not given.is_contiguous():
+            raise ValueError("workspace must be contiguous uint8")
+        return given
+    if not torch.cuda.is_current_stream_capturing():
+        return _WORKSPACES.get(cache.device, need, stream)
+    ws = torch.empty(need, dtype=torch.uint8, device=cache.device)
+    if counters:
+        ws[:_CONTROL_BYTES].zero_()
+    return ws
+
+
 _Q_DTYPES = (torch.bfloat16, torch.float16)
 
 
@@ -195,8 +221,8 @@ def _block_args(block: Block, cache: KV4Cache, T: int) -> tuple[int, Optional[in
 
 def kv4_attention(q: torch.Tensor, cache: KV4Cache, lengths: torch.Tensor, *, block: Block = "causal",
                   counts: Optional[torch.Tensor] = None, scale: Optional[float] = None,
-                  out: Optional[torch.Tensor] = None,
-                  lse: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
+                  out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
+                  workspace: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
     """Attention of a block's rows over their sequences' context and the block itself.
 
     ``q`` ``[batch, T, q_heads, head_dim]`` bf16 or fp16, ``q_heads`` a multiple of the
@@ -232,7 +258,7 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, lengths: torch.Tensor, *, bl
         need = lib.dels_kv4_attention_ws_bytes(batch, T, q_heads, cache.kv_heads, D, cache.max_pages)
         cache._ws_bytes[T, q_heads] = need
     stream = _stream_ptr(cache.device)
-    ws = _WORKSPACES.get(cache.device, need, stream)
+    ws = _call_workspace(workspace, cache, need, stream, counters=True)
     _lib.check(lib.dels_kv4_attention(cache._ref, *qp, _DTYPES[q.dtype], q_heads, T, lp, cp, mode, mask, ld_mask,
                                       cache._scale if scale is None else scale, *op, lse.data_ptr(),
                                       ws.data_ptr(), ws.numel(), stream), "dels_kv4_attention")
@@ -292,8 +318,8 @@ def kv4_weights(q: torch.Tensor, cache: KV4Cache, lengths: torch.Tensor, lse: to
     return out
 
 
-def kv4_evict(cache: KV4Cache, lengths: torch.Tensor, weights: torch.Tensor, keep: int,
-              recent: int = 0) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+def kv4_evict(cache: KV4Cache, lengths: torch.Tensor, weights: torch.Tensor, keep: int, recent: int = 0, *,
+              workspace: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Shrink every sequence of more than ``keep`` slots to ``keep``, each cache head by its own weights.
 
     The last ``recent`` slots (at most ``keep``) stay, and of the others those of
@@ -312,8 +338,10 @@ def kv4_evict(cache: KV4Cache, lengths: torch.Tensor, weights: torch.Tensor, kee
     new_weights = torch.empty_like(weights)
     source = torch.empty(cache.batch, cache.kv_heads, keep, dtype=torch.int32, device=cache.device)
     lib = _lib.load()
-    ws = workspace(cache.device, lib.dels_kv4_evict_ws_bytes(cache.batch, cache.kv_heads, keep))
+    need = lib.dels_kv4_evict_ws_bytes(cache.batch, cache.kv_heads, keep)
+    stream = _stream_ptr(cache.device)
+    ws = _call_workspace(workspace, cache, need, stream, counters=False)
     _lib.check(lib.dels_kv4_evict(cache._ref, lp, weights.data_ptr(), keep, recent, new_lengths.data_ptr(),
-                                  new_weights.data_ptr(), source.data_ptr(), ws.data_ptr(), ws.numel(),
-                                  _stream_ptr(cache.device)), "dels_kv4_evict")
+                                  new_weights.data_ptr(), source.data_ptr(), ws.data_ptr(), ws.numel(), stream),
+               "dels_kv4_evict")
     return new_lengths, new_weights, source

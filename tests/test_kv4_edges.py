@@ -53,3 +53,50 @@ def test_one_row_for_all_sequences_is_a_stride_of_zero(pkg):
     for ld in (0, 4):
         assert lib.dels_kv4_attention(host.cache(pkg), 0x1000, 4096, 1024, 128, 1, 8, 4, 0x3000, None, 3, 0x9000, ld,
                                       1.0, 0x4000, 4096, 1024, 128, 0x5000, None, 0, None) == -4
+
+
+class Answers:
+    """A library whose calls succeed; what they got for a workspace is written down."""
+
+    def __init__(self):
+        self.got = []
+
+    def dels_kv4_attention_ws_bytes(self, *a):
+        return 1 << 18
+
+    dels_kv4_evict_ws_bytes = dels_kv4_attention_ws_bytes
+
+    def dels_kv4_attention(self, *a):
+        self.got.append(a[-3:-1])
+        return 0
+
+    dels_kv4_evict = dels_kv4_attention
+
+
+def test_captured_calls_do_not_use_the_streams_shared_workspace(on_cpu, monkeypatch):
+    lib, taken = Answers(), []
+    kv4, cpu = on_cpu.kv4, torch.device("cpu")
+    monkeypatch.setattr(kv4._lib, "load", lambda: lib)
+    monkeypatch.setattr(kv4, "_stream_ptr", lambda device: 0)
+    monkeypatch.setattr(on_cpu.ops, "_stream_ptr", lambda device: 0)
+
+    def shared(device, need, stream):
+        taken.append(need)
+        return torch.zeros(need, dtype=torch.uint8)
+
+    monkeypatch.setattr(kv4._WORKSPACES, "get", shared)
+    cache = on_cpu.KV4Cache(torch.zeros(4, 2, 4352, dtype=torch.uint8), torch.zeros(2, 2, dtype=torch.int32), 64)
+    q, n = torch.zeros(2, 3, 4, 64, dtype=torch.bfloat16, device=cpu), torch.zeros(2, dtype=torch.int32)
+    w = torch.zeros(2, 2, 128)
+    for capturing in (False, True):
+        monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing)
+        on_cpu.kv4_attention(q, cache, n)
+        on_cpu.kv4_evict(cache, n, w, 10)
+        assert len(taken) == 2                       # of the calls that no graph captured
+        assert all(p and size >= 1 << 18 for p, size in lib.got)
+    mine = torch.zeros(1 << 18, dtype=torch.uint8)
+    on_cpu.kv4_attention(q, cache, n, workspace=mine)
+    on_cpu.kv4_evict(cache, n, w, 10, workspace=mine)
+    assert lib.got[-2:] == [(mine.data_ptr(), mine.numel())] * 2 and len(taken) == 2
+    with pytest.raises(ValueError, match="workspace must be"):
+        on_cpu.kv4_attention(q, cache, n, workspace=torch.zeros(1 << 18))
