@@ -91,10 +91,11 @@ __device__ __forceinline__ void store_out(const Kv4AttentionArgs& a, int b, cons
     else *reinterpret_cast<uint32_t*>(p) = w[0];
 }
 
-// `ref`: binary logarithm of the unit that `total` counts in.
+// `ref`: binary logarithm of the unit that `total` counts in.  A sum of 0 is a row that saw
+// nothing (the largest score's weight is at least 1); NaN is a row of scores that are none.
 __device__ __forceinline__ void store_lse(const Kv4AttentionArgs& a, int b, const Row& row, float ref, float total) {
     if (!row.in_block) return;
-    const float x = row.valid && total > 0.f ? (ref + __builtin_amdgcn_logf(total)) * 0.693147180559945309f
+    const float x = row.valid && total != 0.f ? (ref + __builtin_amdgcn_logf(total)) * 0.693147180559945309f
                                              : -__builtin_inff();
     a.lse[((int64_t)b * a.block.T + row.t) * a.q_heads + row.hq] = x;
 }
@@ -405,7 +406,7 @@ __global__ __launch_bounds__(kKv4Threads, 2) void kv4_attention_kernel(Kv4Attent
         for (int w = tile * WAYS; w < (tile + 1) * WAYS; ++w) m = fmaxf(m, s_m[w][col]);
 #pragma unroll
         for (int w = tile * WAYS; w < (tile + 1) * WAYS; ++w) l += s_l[w][col] * fade(s_m[w][col], m);
-        const float f = fade(ref, m), inv = l > 0.f ? 1.f / l : 0.f;
+        const float f = fade(ref, m), inv = l != 0.f ? 1.f / l : 0.f;
 #pragma unroll
         for (int r0 = 0; r0 < kRegs; r0 += kRound) {
             // register (vl, i, v): channel block, row of the tile, channel of the VW
@@ -507,7 +508,7 @@ __global__ __launch_bounds__(kKv4Threads, 2) void kv4_attention_kernel(Kv4Attent
                                             __uint_as_float((uint32_t)(two[e][i][v / 2] >> (32 * (v & 1)))) * f;
                     }
                 }
-                const float inv = l > 0.f ? 1.f / l : 0.f;
+                const float inv = l != 0.f ? 1.f / l : 0.f;
 #pragma unroll
                 for (int i = 0; i < kMine; ++i) {
                     const int gi = way + i * WAYS;

@@ -140,7 +140,11 @@ __global__ __launch_bounds__(kKv4Threads, 4) void kv4_weights_kernel(Kv4WeightsA
                             // a lane's registers are rows 4 g .. 4 g + 3 of the tile
                             const int row = tile * MT + 4 * g;
                             const f32x4 lse = *reinterpret_cast<const f32x4*>(&s_lse[row]);
-                            if (masked) {
+#pragma unroll
+                            for (int t = 0; t < S::KT; ++t)
+#pragma unroll
+                                for (int x = 0; x < 4; ++x) acc[t][x] = __builtin_fmaf(acc[t][x], unit, -lse[x]);
+                            if (masked) {                    // after the sum: a slot unseen gets 0 of a NaN row too
                                 asm volatile("");            // a branch, not a selection on every page
 #pragma unroll
                                 for (int x = 0; x < 4; ++x) {
@@ -158,7 +162,7 @@ __global__ __launch_bounds__(kKv4Threads, 4) void kv4_weights_kernel(Kv4WeightsA
                             for (int t = 0; t < S::KT; ++t)
 #pragma unroll
                                 for (int x = 0; x < 4; ++x)
-                                    part[t] += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[t][x], unit, -lse[x]));
+                                    part[t] += __builtin_amdgcn_exp2f(acc[t][x]);
                         }
 #pragma unroll
                         for (int t = 0; t < S::KT; ++t) {

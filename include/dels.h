@@ -612,7 +612,8 @@ int dels_kv4_read(const dels_kv4_cache* c, const int32_t* starts, const int32_t*
  * Attention of a block's rows over the cache: out[b, t, hq] = softmax(scale * q . K^T) V over the
  * slots that row t sees, head hq reading key/value head hq / (q_heads / kv_heads), and
  * lse[b, t, hq] (contiguous fp32), the logarithm of the softmax's sum.  A row that sees
- * nothing, and rows from counts[b] on, give out = 0 and lse = -inf.  q [batch, T, q_heads, D]
+ * nothing, and rows from counts[b] on, give out = 0 and lse = -inf; a row that sees a
+ * score of NaN or +inf gives NaN in both.  q [batch, T, q_heads, D]
  * bf16 or fp16, out the same type, any strides that keep rows 16-byte aligned.  With fp16 q
  * the keys that the cache holds must be below 2^20 in magnitude.
  */
@@ -627,7 +628,8 @@ int dels_kv4_attention(const dels_kv4_cache* c, const void* q, int64_t q_batch, 
  * Attention weights that rows t < accepted[b] (NULL: all valid rows) gave to each slot, added
  * up over the query heads of each key/value head:
  *   out[b, h, j] = (j < lengths[b] ? weights[b, h, j] : 0) + sum_t,hq exp(scale * q . k_j - lse[b, t, hq])
- * lse as dels_kv4_attention wrote it for the same block.  weights and out contiguous
+ * lse as dels_kv4_attention wrote it for the same block; a row of lse = -inf adds nothing,
+ * one of NaN makes the slots that it sees NaN.  weights and out contiguous
  * fp32 [batch, kv_heads, 64 * max_pages]; out may be weights.
  */
 int dels_kv4_weights(const dels_kv4_cache* c, const void* q, int64_t q_batch, int64_t q_token, int64_t q_head,

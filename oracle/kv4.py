@@ -116,11 +116,11 @@ def sees(j, n, count, t, block, bits):
 
 
 def _scores(q, K, h, t, n, count, block, bits, scale):
-    """Scores of one (row, head) over all slots, -inf where unseen, and the largest sum of |q k| * |scale|."""
+    """Scores of one (row, head) over all slots, -inf where unseen; the largest sum of |q k| * |scale|; which are seen."""
     vis = np.array([sees(j, n, count, t, block, bits) for j in range(K.shape[0])], dtype=bool)
     x = np.where(vis, scale * (K @ q), -np.inf)
     mass = (np.abs(K) @ np.abs(q))[vis].max() * abs(scale) if vis.any() else 0.0
-    return x, mass
+    return x, mass, vis
 
 
 def attention(q, K, V, lengths, counts, block, scale, masks=None):
@@ -133,9 +133,9 @@ def attention(q, K, V, lengths, counts, block, scale, masks=None):
         for t in range(int(counts[b])):
             for hq in range(HQ):
                 h = hq // (HQ // H)
-                x, mass[b, t, hq] = _scores(q[b, t, hq], K[b, h], h, t, lengths[b], counts[b], block,
-                                            masks[b, t] if masks is not None else 0, scale)
-                if not np.isfinite(x).any():
+                x, mass[b, t, hq], _ = _scores(q[b, t, hq], K[b, h], h, t, lengths[b], counts[b], block,
+                                               masks[b, t] if masks is not None else 0, scale)
+                if np.all(x == -np.inf):
                     continue
                 p = np.exp(x - x.max())
                 out[b, t, hq] = p @ V[b, h] / p.sum()
@@ -157,9 +157,9 @@ def weights(q, K, lengths, counts, accepted, block, scale, lse, w, masks=None):
                 if lse[b, t, hq] == -np.inf:
                     continue
                 h = hq // (HQ // H)
-                x, m = _scores(q[b, t, hq], K[b, h], h, t, lengths[b], counts[b], block,
-                               masks[b, t] if masks is not None else 0, scale)
-                added[b, h] += np.exp(x - lse[b, t, hq])
+                x, m, vis = _scores(q[b, t, hq], K[b, h], h, t, lengths[b], counts[b], block,
+                                    masks[b, t] if masks is not None else 0, scale)
+                added[b, h] += np.where(vis, np.exp(x - lse[b, t, hq]), 0.0)
                 mass[b, h] = max(mass[b, h], m)
     return old + added, added, mass
 

@@ -1,9 +1,11 @@
 """GPU tests of the 4-bit cache's calls at the edges of what they take."""
 
+import numpy as np
 import pytest
 import torch
 
-from test_gpu_kv4 import attention_inputs, ints, say
+from oracle import kv4 as O
+from test_gpu_kv4 import attention_inputs, check_attention, contents, ints, say
 
 pytestmark = pytest.mark.gpu
 
@@ -93,3 +95,59 @@ def test_graphs_of_one_cache_are_replayed_on_two_streams(pkg, dev):
         for q, (_, got) in zip(qs, graphs):
             for x, y in zip(got, pkg.kv4_attention(q, cache, lengths, block="none")):
                 assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dtype,T,block", [("bf16", 3, "causal"), ("f16", 9, "full"), ("bf16", 40, "causal")])
+def test_rows_of_nan_and_infinite_queries(pkg, dev, dtype, T, block):
+    """Their out and lse are NaN, and the weights of the slots that they see; other rows are as ever."""
+    say("nan rows", dtype, T, block)
+    B, HQ, H, D, lengths, counts = 3, 4, 2, 64, [130, 700, 0], [T, T, T - 1]
+    cache, q, _ = attention_inputs(pkg, dev, B, T, HQ, H, D, 12, dtype, block, lengths, counts, 17)
+    bad = torch.zeros(B, T, HQ, dtype=torch.bool)
+    for (b, t, hq), x in {(0, 0, 1): "nan", (0, T - 2, 0): "inf", (1, 1, 3): "-inf", (1, T - 1, 3): "nan",
+                          (2, 1, 0): "nan"}.items():
+        q[b, t, hq, 7 * hq + 2] = float(x)
+        bad[b, t, hq] = True
+    q[2, T - 1] = float("nan")                             # no valid row
+    n, c = ints(lengths, dev), ints(counts, dev)
+    out, lse = pkg.kv4_attention(q.to(dev), cache, n, block=block, counts=c)
+    torch.cuda.synchronize()
+    assert torch.equal(lse.cpu().isnan(), bad)
+    assert torch.equal(out.cpu().isnan(), bad[..., None].expand_as(out))
+    # the other rows, as without the bad ones
+    clean = torch.where(bad[..., None] | q.isnan(), torch.zeros_like(q), q)
+    o, l = out.cpu(), lse.cpu()
+    co, cl = (x.cpu() for x in pkg.kv4_attention(clean.to(dev), cache, n, block=block, counts=c))
+    o[bad], l[bad] = co[bad], cl[bad]
+    check_attention(cache, clean, dtype, block, lengths, counts, None, D ** -0.5, o, l)
+
+    w = torch.rand(B, H, cache.slots, generator=torch.Generator().manual_seed(2))
+    K, _ = contents(cache)
+    for accepted in (counts, [1, 1, 1]):
+        got = pkg.kv4_weights(q.to(dev), cache, n, lse, w.to(dev), ints(accepted, dev), block=block, counts=c)
+        with np.errstate(invalid="ignore"):
+            ref, added, mass = O.weights(q.double().numpy(), K, lengths, counts, accepted, block, D ** -0.5,
+                                         lse.double().cpu().numpy(), w.double().numpy())
+        got = got.double().cpu().numpy()
+        assert np.array_equal(np.isnan(got), np.isnan(ref))
+        assert np.isnan(ref).any() and not np.isnan(ref).all()
+        f = ~np.isnan(ref)
+        err = np.abs(clean.double().numpy()).sum(-1).max() * 6 * 2.0 ** -16      # keys are 6 at most
+        assert np.all(np.abs(got - ref)[f] <= (added * (err + 2.0 ** -18) + ref * 2.0 ** -20)[f])
+
+
+def test_rows_of_minus_infinite_scores_are_empty(pkg, dev):
+    """Every score -inf: nothing is seen, though slots are; a score of -inf beside others weighs nothing."""
+    say("-inf scores")
+    D = 64
+    cache = pkg.KV4Cache.allocate(1, 128, 1, D, dev)
+    k = torch.ones(1, 100, 1, D, device=dev)
+    k[0, :50, 0, 3] = 0.0                                  # with a query of -inf there: NaN
+    pkg.kv4_append(cache, k, k, ints([0], dev))
+    q = torch.zeros(1, 2, 1, D, dtype=torch.bfloat16, device=dev)
+    q[0, 0, 0, 5] = float("-inf")
+    q[0, 1, 0, 3] = float("-inf")
+    out, lse = pkg.kv4_attention(q, cache, ints([100], dev), block="none")
+    torch.cuda.synchronize()
+    assert lse[0, 0, 0] == float("-inf") and not out[0, 0].any()
+    assert lse[0, 1, 0].isnan() and out[0, 1].isnan().all()
