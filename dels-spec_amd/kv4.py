@@ -140,13 +140,16 @@ def _require_rows(t: torch.Tensor, cache: KV4Cache, heads: Optional[int], name: 
     return (t.data_ptr(), sb if shape[0] > 1 else 0, st if shape[1] > 1 else 0, sh if shape[2] > 1 else 0)
 
 
-def _call_workspace(given: Optional[torch.Tensor], cache: KV4Cache, need: int, stream: int, *,
-                    counters: bool) -> torch.Tensor:
-    """The caller's workspace, a captured call's own, or else the stream's shared one.
+# whether the current stream is being captured, without the wrapper's call
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
 
-    The shared one may be replaced by a larger one between a graph's replays, its zero
-    fill would belong to the one graph that captured it, and graphs that are replayed on
-    several streams would meet in it.
+
+def _own_workspace(given: Optional[torch.Tensor], cache: KV4Cache, need: int, *, counters: bool) -> torch.Tensor:
+    """The caller's workspace, or else a captured call's own.
+
+    The stream's shared one may be replaced by a larger one between a graph's replays, its
+    zero fill would belong to the one graph that captured it, and graphs that are replayed
+    on several streams would meet in it.
     """
     if given is not None:
         if not isinstance(given, torch.Tensor) or given.get_device() != cache._index:
@@ -154,8 +157,6 @@ def _call_workspace(given: Optional[torch.Tensor], cache: KV4Cache, need: int, s
         if given.dtype != torch.uint8 or not given.is_contiguous():
             raise ValueError("workspace must be contiguous uint8")
         return given
-    if not torch.cuda.is_current_stream_capturing():
-        return _WORKSPACES.get(cache.device, need, stream)
     ws = torch.empty(need, dtype=torch.uint8, device=cache.device)
     if counters:
         ws[:_CONTROL_BYTES].zero_()
@@ -258,7 +259,10 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, lengths: torch.Tensor, *, bl
         need = lib.dels_kv4_attention_ws_bytes(batch, T, q_heads, cache.kv_heads, D, cache.max_pages)
         cache._ws_bytes[T, q_heads] = need
     stream = _stream_ptr(cache.device)
-    ws = _call_workspace(workspace, cache, need, stream, counters=True)
+    if workspace is None and not _capturing():
+        ws = _WORKSPACES.get(cache.device, need, stream)
+    else:
+        ws = _own_workspace(workspace, cache, need, counters=True)
     _lib.check(lib.dels_kv4_attention(cache._ref, *qp, _DTYPES[q.dtype], q_heads, T, lp, cp, mode, mask, ld_mask,
                                       cache._scale if scale is None else scale, *op, lse.data_ptr(),
                                       ws.data_ptr(), ws.numel(), stream), "dels_kv4_attention")
@@ -340,7 +344,10 @@ def kv4_evict(cache: KV4Cache, lengths: torch.Tensor, weights: torch.Tensor, kee
     lib = _lib.load()
     need = lib.dels_kv4_evict_ws_bytes(cache.batch, cache.kv_heads, keep)
     stream = _stream_ptr(cache.device)
-    ws = _call_workspace(workspace, cache, need, stream, counters=False)
+    if workspace is None and not _capturing():
+        ws = _WORKSPACES.get(cache.device, need, stream)
+    else:
+        ws = _own_workspace(workspace, cache, need, counters=False)
     _lib.check(lib.dels_kv4_evict(cache._ref, lp, weights.data_ptr(), keep, recent, new_lengths.data_ptr(),
                                   new_weights.data_ptr(), source.data_ptr(), ws.data_ptr(), ws.numel(), stream),
                "dels_kv4_evict")

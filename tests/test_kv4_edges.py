@@ -89,7 +89,7 @@ def test_captured_calls_do_not_use_the_streams_shared_workspace(on_cpu, monkeypa
     q, n = torch.zeros(2, 3, 4, 64, dtype=torch.bfloat16, device=cpu), torch.zeros(2, dtype=torch.int32)
     w = torch.zeros(2, 2, 128)
     for capturing in (False, True):
-        monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing)
+        monkeypatch.setattr(kv4, "_capturing", lambda: capturing)
         on_cpu.kv4_attention(q, cache, n)
         on_cpu.kv4_evict(cache, n, w, 10)
         assert len(taken) == 2                       # of the calls that no graph captured
