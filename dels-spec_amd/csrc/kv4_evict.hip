@@ -7,6 +7,10 @@
 // from one side of `keep` and written on the other, so the move needs no order,
 // works in place and touches no slot that stays where it is.  (Attention does not
 // depend on the order of the slots.)
+//
+// Slots of an entry that names no page hold nothing: none of them is moved, and as
+// places below `keep` they take nothing, so that a (sequence, head) keeps fewer slots,
+// `room` of them: as many as there are places.
 #include <algorithm>
 
 #include "kv4.h"
@@ -56,6 +60,7 @@ __global__ __launch_bounds__(THREADS) void kv4_select_kernel(Kv4EvictArgs a, int
     __shared__ uint32_t s_hist[COPIES][kBins];
     __shared__ int s_wave[kWaves];
     __shared__ uint32_t s_pick, s_left, s_held;
+    __shared__ int s_named[2];
     __shared__ int s_count[2][kWaves];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int bh = blockIdx.x, h = bh % a.cache.heads, b = bh / a.cache.heads;
@@ -83,23 +88,55 @@ __global__ __launch_bounds__(THREADS) void kv4_select_kernel(Kv4EvictArgs a, int
             load_slots(w, first, n, x);
         }
     };
-    const int recent = min(a.recent, keep), cand = n - recent;
-    uint32_t left = keep - recent;                 // candidates still to choose among the equal prefixes
+    auto clear = [&]() {
+        for (int i = tid; i < COPIES * kBins; i += THREADS) (&s_hist[0][0])[i] = 0u;
+    };
+    // whether any slot lies in no page (a lane's slots lie in one page)
+    const int32_t* ids = a.cache.table + (int64_t)b * a.cache.ld_table;
+    auto in_page = [&](int page) { return ids[page] >= 0 && ids[page] < a.cache.num_pages; };
+    bool gap = false;
+    for (int p = tid; p * kKv4Page < n; p += THREADS) gap |= !in_page(p);
+    clear();
+    if (__any(gap)) gap = true;
+    if (lane == 0) s_wave[wave] = gap;
+    if (tid < 2) s_named[tid] = 0;
+    __syncthreads();
+    const bool gaps = over_waves<kWaves>(s_wave).y != 0;
+    int recent = min(a.recent, keep), chosen = keep - recent;      // chosen by weight
+    if (gaps) {
+        auto slots_in_pages = [&](int from, int to, int* sum) {
+            int mine = 0;
+            for (int p = from / kKv4Page + tid; p * kKv4Page < to; p += THREADS)
+                mine += in_page(p) ? min(to, (p + 1) * kKv4Page) - max(from, p * kKv4Page) : 0;
+            atomicAdd(sum, mine);
+            __syncthreads();
+            return *sum;
+        };
+        const int room = slots_in_pages(0, keep, &s_named[0]);
+        recent = min(recent, room);
+        chosen = room - slots_in_pages(n - recent, n, &s_named[1]);
+    }
+    auto held_at = [&](int first) { return !gaps || (first < n && in_page(first / kKv4Page)); };
+    const int cand = n - recent;
+    uint32_t left = chosen;                        // candidates still to choose among the equal prefixes
     uint32_t prefix = 0u;
     int bits_left = 32;
     while (bits_left > 0 && left > 0) {
         const int digit_bits = min(bits_left, 11), shift = bits_left - digit_bits;
-        for (int i = tid; i < COPIES * kBins; i += THREADS) (&s_hist[0][0])[i] = 0u;
-        __syncthreads();
+        if (bits_left < 32) {
+            clear();
+            __syncthreads();
+        }
         for (int j0 = 0; j0 < cand; j0 += kTile) {
             const int first = j0 + own_first;
             float x[kPerLane];
             tile_of(first, x);
+            const int end = held_at(first) ? cand : 0;
 #pragma unroll
             for (int i = 0; i < kPerLane; ++i) {
                 const uint32_t key = weight_key(x[i]);
                 const bool mine = bits_left == 32 || (key >> bits_left) == prefix;
-                if (first + i < cand && mine)
+                if (first + i < end && mine)
                     atomicAdd(&s_hist[lane % COPIES][(key >> shift) & ((1u << digit_bits) - 1)], 1u);
             }
         }
@@ -132,7 +169,7 @@ __global__ __launch_bounds__(THREADS) void kv4_select_kernel(Kv4EvictArgs a, int
         if (all) break;
     }
     // keys whose bits so far are above `prefix` are kept, and the first `left` of those equal to it
-    const bool none = keep == recent;
+    const bool none = chosen == 0;
     int32_t* holes = hole_list + (int64_t)bh * keep;
     int equal_before = 0, hole_before = 0, mover_before = 0;
     for (int j0 = 0; j0 < n; j0 += kTile) {
@@ -147,6 +184,8 @@ __global__ __launch_bounds__(THREADS) void kv4_select_kernel(Kv4EvictArgs a, int
             kept |= (uint32_t)(j < n && (j >= cand || (!none && key > prefix))) << i;
             equal |= (uint32_t)(j < cand && !none && key == prefix) << i;
         }
+        const bool held_here = held_at(first);
+        if (!held_here) kept = equal = 0u;
         const int equals = __popc(equal), e_upto = sum_upto(equals);
         if (lane == 63) s_count[0][wave] = e_upto;
         __syncthreads();
@@ -160,7 +199,7 @@ __global__ __launch_bounds__(THREADS) void kv4_select_kernel(Kv4EvictArgs a, int
         }
         // every place below `keep` starts as its own; what moves in comes after
         const uint32_t below = (1u << min(max(keep - first, 0), kPerLane)) - 1u;
-        const uint32_t hole = below & ~kept, mover = kept & ~below;
+        const uint32_t hole = held_here ? below & ~kept : 0u, mover = kept & ~below;
         if (below == (1u << kPerLane) - 1u) {
             int own[kPerLane];
 #pragma unroll

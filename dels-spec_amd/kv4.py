@@ -332,7 +332,8 @@ def kv4_evict(cache: KV4Cache, lengths: torch.Tensor, weights: torch.Tensor, kee
     cache changes in place.  Returns ``(lengths, weights, source)``: the new lengths, the
     weights in their new places (0 past them), and int32 ``source`` ``[batch, kv_heads,
     keep]``, the slot whose content each place holds now (-1 past the new length), by
-    which whatever else is kept per slot follows.
+    which whatever else is kept per slot follows.  Slots of a table entry that names no
+    page hold nothing, so none of them stays or moves, and as places they take nothing.
     """
     lp = _require_ints(lengths, cache, "lengths")
     _require_weights(weights, cache, "weights")

@@ -646,6 +646,9 @@ int dels_kv4_weights(const dels_kv4_cache* c, const void* q, int64_t q_batch, in
  *   source[b, h, j], j < keep: the slot whose content place j holds now, -1 from
  *     out_lengths[b] on
  *   out_weights: the weights in their new places, 0 from out_lengths[b] on
+ * Slots of an entry that names no page hold nothing: they are not among those that stay or
+ * move, and a place below `keep` there takes nothing (source j and its own weight), so that
+ * no more slots stay than there are places.
  * No output may be one of the inputs.
  */
 size_t dels_kv4_evict_ws_bytes(int64_t batch, int64_t kv_heads, int64_t keep);

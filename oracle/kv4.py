@@ -164,15 +164,18 @@ def weights(q, K, lengths, counts, accepted, block, scale, lse, w, masks=None):
     return old + added, added, mass
 
 
-def evict(w, n, keep, recent):
-    """Sources [keep] of one (sequence, head) of n slots with weights w."""
+def evict(w, n, keep, recent, named=None):
+    """Sources [keep] of one (sequence, head) of n slots with weights w; named: whether each lies in a page."""
     if n <= keep:
         return np.array(list(range(n)) + [-1] * (keep - n))
-    recent = min(recent, keep)
+    named = np.ones(n, dtype=bool) if named is None else named
+    room = int(named[:keep].sum())
+    recent = min(recent, room)
     clean = np.where(np.isnan(w), -np.inf, w)
-    order = sorted(range(n - recent), key=lambda j: (-clean[j], j))
-    stay = set(order[:keep - recent]) | set(range(n - recent, n))
-    holes = [j for j in range(keep) if j not in stay]
+    stay = {j for j in range(n - recent, n) if named[j]}
+    order = sorted((j for j in range(n - recent) if named[j]), key=lambda j: (-clean[j], j))
+    stay |= set(order[:room - len(stay)])
+    holes = [j for j in range(keep) if named[j] and j not in stay]
     movers = sorted(j for j in stay if j >= keep)
     source = np.arange(keep)
     source[holes] = movers

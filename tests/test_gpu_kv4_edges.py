@@ -151,3 +151,44 @@ def test_rows_of_minus_infinite_scores_are_empty(pkg, dev):
     torch.cuda.synchronize()
     assert lse[0, 0, 0] == float("-inf") and not out[0, 0].any()
     assert lse[0, 1, 0].isnan() and out[0, 1].isnan().all()
+
+
+@pytest.mark.parametrize("n,pages,keep,recent,gone", [
+    (500, 8, 200, 30, [1, 6]),                             # below and above the budget
+    (500, 8, 200, 30, [3]),                                # the budget ends inside a page that is none
+    (500, 8, 200, 200, [0, 2]),                            # fewer places than recent slots
+    (500, 8, 128, 100, [0, 1, 5]),                         # no place at all
+    (500, 8, 200, 150, [7, 6]),                            # the recent slots are in no page
+    (500, 8, 200, 0, list(range(8))),                      # nothing anywhere
+    (20000, 320, 9000, 500, [0, 17, 140, 141, 200, 311]),  # several walks of the selection
+    (500, 8, 600, 10, [1, 2]),                             # a budget that is kept
+])
+def test_evict_beside_entries_that_name_no_page(pkg, dev, n, pages, keep, recent, gone):
+    """No slot there stays, moves or is moved into, and what is said of every place is what it holds."""
+    say("evict no page", n, pages, keep, recent, gone)
+    B, H, D = 2, 2, 64
+    g = torch.Generator().manual_seed(n + keep + len(gone))
+    data = torch.randint(0, 256, (B * pages, H, O.page_bytes(D)), generator=g, dtype=torch.uint8)
+    data[..., 32 * D:34 * D] = torch.randint(100, 140, (B * pages, H, 2 * D), generator=g, dtype=torch.uint8)
+    data[..., 66 * D:] = (torch.rand(B * pages, H, 64, generator=g) + 0.1).to(torch.bfloat16).view(torch.uint8)
+    table = torch.randperm(B * pages, generator=g).view(B, pages).int()
+    for i, p in enumerate(gone):
+        table[0, p] = -1 if i % 2 else 10 ** 6
+    cache = pkg.KV4Cache(data.to(dev), table.to(dev), D)
+    w = torch.randint(0, 50, (B, H, cache.slots), generator=g).float()
+    lengths = ints([n, n], dev)
+    k0, v0 = pkg.kv4_read(cache, ints([0, 0], dev), n, dtype=torch.float32)
+    nl, nw, source = pkg.kv4_evict(cache, lengths, w.to(dev), keep, recent)
+    k1, v1 = pkg.kv4_read(cache, ints([0, 0], dev), min(n, keep), dtype=torch.float32)
+    torch.cuda.synchronize()
+    m = min(n, keep)
+    assert nl.tolist() == [m, m]
+    for b in range(B):
+        named = np.array([0 <= int(table[b, j // 64]) < B * pages for j in range(n)])
+        for h in range(H):
+            ref = O.evict(w[b, h, :n].double().numpy(), n, keep, recent, named)
+            assert np.array_equal(source[b, h].cpu().numpy(), ref), (b, h)
+            src = torch.tensor(ref[:m])
+            assert torch.equal(nw[b, h, :m].cpu(), w[b, h][src]) and not nw[b, h, m:].any()
+            for x, y in ((k0, k1), (v0, v1)):
+                assert torch.equal(x[b, src.to(dev), h], y[b, :, h])
