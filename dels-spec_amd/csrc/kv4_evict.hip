@@ -170,6 +170,7 @@ __global__ __launch_bounds__(THREADS) void kv4_select_kernel(Kv4EvictArgs a, int
     }
     // keys whose bits so far are above `prefix` are kept, and the first `left` of those equal to it
     const bool none = chosen == 0;
+    const int unread = none ? 0 : bits_left;       // low bits of the key that did not matter: below 32
     int32_t* holes = hole_list + (int64_t)bh * keep;
     int equal_before = 0, hole_before = 0, mover_before = 0;
     for (int j0 = 0; j0 < n; j0 += kTile) {
@@ -180,7 +181,7 @@ __global__ __launch_bounds__(THREADS) void kv4_select_kernel(Kv4EvictArgs a, int
 #pragma unroll
         for (int i = 0; i < kPerLane; ++i) {
             const int j = first + i;
-            const uint32_t key = weight_key(x[i]) >> bits_left;
+            const uint32_t key = weight_key(x[i]) >> unread;
             kept |= (uint32_t)(j < n && (j >= cand || (!none && key > prefix))) << i;
             equal |= (uint32_t)(j < cand && !none && key == prefix) << i;
         }
