@@ -337,6 +337,7 @@ hipError_t launch_kv4_evict(const Kv4EvictArgs& a, void* ws, size_t data_off, hi
         hipLaunchKernelGGL((kv4_select_kernel<256, 1>), grid_select, dim3(256), 0, s, a, holes);
     else
         hipLaunchKernelGGL((kv4_select_kernel<1024, 4>), grid_select, dim3(1024), 0, s, a, holes);
+    if (c.slots() == 0) return hipGetLastError();  // nothing to move, and no grid to do it
     const int groups = (std::min(a.keep, c.slots()) + 7) / 8, waves = kMoveThreads / 64;
     const dim3 grid((groups + waves - 1) / waves, c.heads, c.batch);
     if (c.head_dim == 64)

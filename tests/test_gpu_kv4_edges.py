@@ -192,3 +192,21 @@ def test_evict_beside_entries_that_name_no_page(pkg, dev, n, pages, keep, recent
             assert torch.equal(nw[b, h, :m].cpu(), w[b, h][src]) and not nw[b, h, m:].any()
             for x, y in ((k0, k1), (v0, v1)):
                 assert torch.equal(x[b, src.to(dev), h], y[b, :, h])
+
+
+def test_cache_whose_table_has_no_column(pkg, dev):
+    say("no column")
+    cache = pkg.KV4Cache(torch.zeros(3, 2, 4352, dtype=torch.uint8, device=dev),
+                         torch.zeros(2, 0, dtype=torch.int32, device=dev), 64)
+    n = ints([5, 0], dev)
+    q, kv = (torch.randn(2, 3, h, 64, device=dev).to(torch.bfloat16) for h in (4, 2))
+    w = torch.zeros(2, 2, 0, device=dev)
+    pkg.kv4_append(cache, kv, kv, n)
+    k, v = pkg.kv4_read(cache, n, 3)
+    out, lse = pkg.kv4_attention(q, cache, n)
+    nw = pkg.kv4_weights(q, cache, n, lse, w)
+    nl, ew, source = pkg.kv4_evict(cache, n, w, 4, 2)
+    torch.cuda.synchronize()
+    assert not k.any() and not v.any() and not out.any() and torch.all(lse == float("-inf"))
+    assert nw.shape == ew.shape == (2, 2, 0)
+    assert nl.tolist() == [0, 0] and torch.all(source == -1) and not cache.data.any()
