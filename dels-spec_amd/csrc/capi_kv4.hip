@@ -176,12 +176,16 @@ int dels_kv4_weights(const dels_kv4_cache* p, const void* q, int64_t q_batch, in
     int rc = cache_of(p, a.cache);
     if (rc != DELS_OK) return rc;
     if (a.cache.batch == 0 || a.cache.max_pages == 0) return DELS_OK;
-    if (T <= 0) return fail(DELS_ERR_INVALID_ARGUMENT, "bad block length %lld", (long long)T);
-    rc = check_block(a.cache, q, q_batch, q_token, q_head, dtype, q_heads, T, lengths, block, mask, ld_mask, scale);
-    if (rc != DELS_OK) return rc;
-    if (a.cache.batch * (int64_t)a.cache.heads > 65535 && a.cache.num_pages == 0)
-        return fail(DELS_ERR_UNSUPPORTED, "a cache of no pages: batch x heads <= 65535");
-    if (!lse || !weights || !out) return fail(DELS_ERR_INVALID_ARGUMENT, "lse, weights or out is NULL");
+    if (T == 0) {                                             // no rows: neither queries nor lse are there
+        if (!lengths) return fail(DELS_ERR_INVALID_ARGUMENT, "lengths is NULL");
+        if (!grid_ok({a.cache.batch, a.cache.heads, a.cache.max_pages}))
+            return fail(DELS_ERR_UNSUPPORTED, "shape past the supported extents");
+    } else {
+        rc = check_block(a.cache, q, q_batch, q_token, q_head, dtype, q_heads, T, lengths, block, mask, ld_mask, scale);
+        if (rc != DELS_OK) return rc;
+        if (!lse) return fail(DELS_ERR_INVALID_ARGUMENT, "lse is NULL");
+    }
+    if (!weights || !out) return fail(DELS_ERR_INVALID_ARGUMENT, "weights or out is NULL");
     a.block = {lengths, counts, (int)T, block, mask, ld_mask};
     a.q = {q, q_batch, q_token, q_head};
     a.dtype = dtype, a.q_heads = (int)q_heads, a.scale = scale;

@@ -188,21 +188,24 @@ __global__ __launch_bounds__(kKv4Threads, 4) void kv4_weights_kernel(Kv4WeightsA
     }
 }
 
-// A cache of no pages: the old weights, cut off at the lengths.
+// A cache of no pages, or a block of no rows: the old weights, cut off at the lengths.
 __global__ void kv4_no_weights_kernel(Kv4WeightsArgs a) {
-    const int slots = a.cache.slots(), b = blockIdx.y / a.cache.heads;
-    const int n = kv4_length(a.block.lengths, b, slots);
-    const int64_t row = (int64_t)blockIdx.y * slots;
-    for (int j = blockIdx.x * blockDim.x + threadIdx.x; j < slots; j += gridDim.x * blockDim.x)
-        a.out[row + j] = j < n ? a.weights[row + j] : 0.f;
+    const int slots = a.cache.slots(), rows = a.cache.batch * a.cache.heads;
+    for (int bh = blockIdx.y; bh < rows; bh += gridDim.y) {
+        const int n = kv4_length(a.block.lengths, bh / a.cache.heads, slots);
+        const int64_t row = (int64_t)bh * slots;
+        for (int j = blockIdx.x * blockDim.x + threadIdx.x; j < slots; j += gridDim.x * blockDim.x)
+            a.out[row + j] = j < n ? a.weights[row + j] : 0.f;
+    }
 }
 
 }  // namespace
 
 hipError_t launch_kv4_weights(const Kv4WeightsArgs& a, hipStream_t s) {
     const Kv4Cache& c = a.cache;
-    if (c.num_pages == 0) {
-        hipLaunchKernelGGL(kv4_no_weights_kernel, dim3((c.slots() + 1023) / 1024, c.batch * c.heads), dim3(256), 0, s, a);
+    if (c.num_pages == 0 || a.block.T == 0) {
+        const int rows = (int)std::min<int64_t>((int64_t)c.batch * c.heads, 65535);
+        hipLaunchKernelGGL(kv4_no_weights_kernel, dim3((c.slots() + 1023) / 1024, rows), dim3(256), 0, s, a);
         return hipGetLastError();
     }
     const int64_t units = (int64_t)c.batch * c.heads * c.max_pages;

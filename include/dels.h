@@ -630,7 +630,8 @@ int dels_kv4_attention(const dels_kv4_cache* c, const void* q, int64_t q_batch, 
  *   out[b, h, j] = (j < lengths[b] ? weights[b, h, j] : 0) + sum_t,hq exp(scale * q . k_j - lse[b, t, hq])
  * lse as dels_kv4_attention wrote it for the same block; a row of lse = -inf adds nothing,
  * one of NaN makes the slots that it sees NaN.  weights and out contiguous
- * fp32 [batch, kv_heads, 64 * max_pages]; out may be weights.
+ * fp32 [batch, kv_heads, 64 * max_pages]; out may be weights.  A block of no rows (T = 0, q and
+ * lse may be NULL) cuts the weights off at the lengths.
  */
 int dels_kv4_weights(const dels_kv4_cache* c, const void* q, int64_t q_batch, int64_t q_token, int64_t q_head,
                      int dtype, int64_t q_heads, int64_t T, const int32_t* lengths, const int32_t* counts,

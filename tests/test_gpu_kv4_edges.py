@@ -210,3 +210,26 @@ def test_cache_whose_table_has_no_column(pkg, dev):
     assert not k.any() and not v.any() and not out.any() and torch.all(lse == float("-inf"))
     assert nw.shape == ew.shape == (2, 2, 0)
     assert nl.tolist() == [0, 0] and torch.all(source == -1) and not cache.data.any()
+
+
+@pytest.mark.parametrize("pages", [5, 0])
+def test_a_block_of_no_rows_through_every_call(pkg, dev, pages):
+    """Nothing is written or attended to; the weights of the context stay, those past it go."""
+    say("empty block", pages)
+    B, HQ, H, D = 3, 4, 2, 64
+    data = torch.randint(0, 256, (B * pages, H, O.page_bytes(D)), dtype=torch.uint8, device=dev)
+    cache = pkg.KV4Cache(data, torch.arange(B * 5, dtype=torch.int32, device=dev).view(B, 5), D)
+    before, n = data.clone(), ints([0, 300, 77], dev)
+    q, kv = (torch.zeros(B, 0, h, D, dtype=torch.bfloat16, device=dev) for h in (HQ, H))
+    w = torch.rand(B, H, cache.slots, device=dev)
+    pkg.kv4_append(cache, kv, kv, n)
+    k, v = pkg.kv4_read(cache, n, 0)
+    out, lse = pkg.kv4_attention(q, cache, n)
+    nw = pkg.kv4_weights(q, cache, n, lse, w)
+    same = w.clone()
+    assert pkg.kv4_weights(q, cache, n, lse, same, ints([0, 0, 0], dev), block="none", out=same) is same
+    torch.cuda.synchronize()
+    assert k.shape == v.shape == (B, 0, H, D) and out.shape == q.shape and lse.shape == (B, 0, HQ)
+    j = torch.arange(cache.slots, device=dev)
+    want = torch.where(j < n[:, None, None], w, torch.zeros_like(w))
+    assert torch.equal(nw, want) and torch.equal(same, want) and torch.equal(data, before)
