@@ -194,7 +194,8 @@ def kv4_read(cache: KV4Cache, starts: torch.Tensor, T: int, *, counts: Optional[
     if dtype not in _DTYPES:
         raise TypeError(f"dtype {dtype} not supported")
     sp, cp = _require_ints(starts, cache, "starts"), _require_ints(counts, cache, "counts")
-    k, v = torch.empty(2, cache.batch, T, cache.kv_heads, cache.head_dim, dtype=dtype, device=cache.device).unbind(0)
+    k = torch.empty(cache.batch, T, cache.kv_heads, cache.head_dim, dtype=dtype, device=cache.device)
+    v = torch.empty_like(k)
     lib = _lib.load()
     _lib.check(lib.dels_kv4_read(cache._ref, sp, cp, T, k.data_ptr(), v.data_ptr(), _DTYPES[dtype],
                                  _stream_ptr(cache.device)), "dels_kv4_read")

@@ -100,3 +100,18 @@ def test_captured_calls_do_not_use_the_streams_shared_workspace(on_cpu, monkeypa
     assert lib.got[-2:] == [(mine.data_ptr(), mine.numel())] * 2 and len(taken) == 2
     with pytest.raises(ValueError, match="workspace must be"):
         on_cpu.kv4_attention(q, cache, n, workspace=torch.zeros(1 << 18))
+
+
+def test_keys_and_values_that_are_read_are_tensors_of_their_own(on_cpu, monkeypatch):
+    """Either outlives the other alone, and takes in-place operations that autograd records."""
+    kv4 = on_cpu.kv4
+    lib = types.SimpleNamespace(dels_kv4_read=lambda *a: 0)
+    monkeypatch.setattr(kv4._lib, "load", lambda: lib)
+    monkeypatch.setattr(kv4, "_stream_ptr", lambda device: 0)
+    cache = on_cpu.KV4Cache(torch.zeros(4, 2, 4352, dtype=torch.uint8), torch.zeros(2, 2, dtype=torch.int32), 64)
+    k, v = on_cpu.kv4_read(cache, torch.zeros(2, dtype=torch.int32), 5, dtype=torch.float32)
+    for x in (k, v):
+        assert x.shape == (2, 5, 2, 64) and x.is_contiguous()
+        assert x.untyped_storage().nbytes() == x.numel() * 4
+        x.add_(torch.ones(64, requires_grad=True))
+    assert k.untyped_storage().data_ptr() != v.untyped_storage().data_ptr()
