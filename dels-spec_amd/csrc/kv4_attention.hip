@@ -12,7 +12,7 @@
 // so a lane holds scores of eight consecutive slots of one row, which is the
 // operand of the second product: P stays in its lane.  Key codes become bf16 (or
 // f16) by the conversion instruction with their block's scale, value codes bf16 with
-// scale 1; the value scale of a slot multiplies its weight.  That product enters the
+// scale 2^-20 for all; the value scale of a slot multiplies its weight.  That product enters the
 // matrix cores as two bf16 parts (2^-17 of each weight, whatever its size: one part
 // alone would round every weight by 2^-8, as much as a bf16 output itself, and f16
 // would lose the small ones).  Scores, maxima, sums and outputs are fp32.
@@ -38,10 +38,14 @@ namespace dels {
 
 namespace {
 
-// A row's running maximum follows only when a score passes it by this many binary
-// orders: until then the weights are at most 2^8, which costs fp32 nothing, and the
-// outputs need no rescaling.
+// What a row's weights are relative to lies this many binary orders above its largest score
+// when it moves, and moves when a score passes it: until then the outputs need no rescaling,
+// no weight is above 1, and its product with a value scale stays finite.
 constexpr float kLag = 8.f;
+// Values enter their product at 2^-20 of their size (the conversion scales for nothing), so
+// that sums over 2^20 slots of the largest values that the cache holds, 3e38, stay finite;
+// the reciprocal of the weights' sum makes up for it.
+constexpr float kShrink = 0x1p-20f, kGrow = 0x1p20f;
 
 // Two numbers rounded to bf16, the first in the low half.
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
@@ -92,7 +96,7 @@ __device__ __forceinline__ void store_out(const Kv4AttentionArgs& a, int b, cons
 }
 
 // `ref`: binary logarithm of the unit that `total` counts in.  A sum of 0 is a row that saw
-// nothing (the largest score's weight is at least 1); NaN is a row of scores that are none.
+// nothing (the largest score's weight is at least 2^-kLag, or nearly); NaN is a row of scores that are none.
 __device__ __forceinline__ void store_lse(const Kv4AttentionArgs& a, int b, const Row& row, float ref, float total) {
     if (!row.in_block) return;
     const float x = row.valid && total != 0.f ? (ref + __builtin_amdgcn_logf(total)) * 0.693147180559945309f
@@ -133,14 +137,15 @@ template <typename T, int D, int MT> struct Rows {
     using S = Shape<D, MT>;
     using F = typename Frag<T>::type;
     typename S::Acc o[S::CT];
-    float top, total;          // running maximum (in raw products) and this lane's part of the sum
+    float top, total;          // what weights are relative to (in raw products) and this lane's part of their sum
     int lim;                   // the row sees slots below it,
     uint64_t bits;             // and those of the block whose bits are set
 
-    // n, filled: context, and the slots that hold anything; unit: binary logarithms per raw product
+    // n, filled: context, and the slots that hold anything; unit: binary logarithms per raw
+    // product; lag: kLag in raw products
     // q: this lane's operands of the queries in LDS, 64 apart
     __device__ __forceinline__ void page(const F* q, const KeyWords<D, MT>& keys, ValueWords<D, MT>& values, uint32_t half,
-                                         int first_slot, int n, int filled, int slots, int g, float unit) {
+                                         int first_slot, int n, int filled, int slots, int g, float unit, float lag) {
         // a page that reaches past the context (a branch: the statement keeps the compiler from
         // computing the masks of every page and selecting)
         const bool masked = first_slot + kKv4Page > n;
@@ -208,8 +213,8 @@ template <typename T, int D, int MT> struct Rows {
 #pragma unroll
             for (int i = 0; i < 8; ++i) best = fmaxf(best, x[u][i]);
         best = max_over_groups<MT>(best);
-        if (__any((best - top) * unit > kLag)) {
-            const float now = fmaxf(top, best), f = fade(top * unit, now * unit);
+        if (__any(best > top)) {
+            const float now = fmaxf(top, best + lag), f = fade(top * unit, now * unit);
             top = now;
             total *= f;
 #pragma unroll
@@ -245,7 +250,7 @@ template <typename T, int D, int MT> struct Rows {
             constexpr int kBoth = 8 / S::CT;                       // and before its second
 #pragma unroll
             for (int t = 0; t < S::CT; ++t) {
-                const bf16x8 vf = decode8<bf16_t>(values.code[u / S::PF][u % S::PF][t], 1.f);
+                const bf16x8 vf = decode8<bf16_t>(values.code[u / S::PF][u % S::PF][t], kShrink);
 #pragma unroll
                 for (int i = t * kBoth; more && i < t * kBoth + kFirst; ++i) weigh(u + 1, i);
                 __builtin_amdgcn_sched_barrier(0);
@@ -290,6 +295,7 @@ __global__ __launch_bounds__(kKv4Threads, 2) void kv4_attention_kernel(Kv4Attent
     // scores in units of the maximum: |scale| and the query's sign
     const float mag = fabsf(a.scale);
     const float unit = (mag == 0.f ? 1.f : mag) * kLog2e * (float)(1 << kKeyShift<T>);
+    const float lag = fminf(kLag / unit, 1e37f);           // finite where the scale is next to nothing
     const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u, zero = mag == 0.f ? 0u : ~0u;
 
     while (u < u_end) {
@@ -381,7 +387,7 @@ __global__ __launch_bounds__(kKv4Threads, 2) void kv4_attention_kernel(Kv4Attent
             next_keys.load(address(next), at_lane);
             asm volatile("" ::: "memory");
             if (named(id))
-                rows.page(&s_q[tile][0][lane], keys, values, at_lane.half, p * kKv4Page, n, filled, slots, g, unit);
+                rows.page(&s_q[tile][0][lane], keys, values, at_lane.half, p * kKv4Page, n, filled, slots, g, unit, lag);
             keys = next_keys;
             id = next;
             next = id_at(p + 2 * WAYS);
@@ -406,7 +412,7 @@ __global__ __launch_bounds__(kKv4Threads, 2) void kv4_attention_kernel(Kv4Attent
         for (int w = tile * WAYS; w < (tile + 1) * WAYS; ++w) m = fmaxf(m, s_m[w][col]);
 #pragma unroll
         for (int w = tile * WAYS; w < (tile + 1) * WAYS; ++w) l += s_l[w][col] * fade(s_m[w][col], m);
-        const float f = fade(ref, m), inv = l != 0.f ? 1.f / l : 0.f;
+        const float f = fade(ref, m), inv = l != 0.f ? kGrow / l : 0.f;
 #pragma unroll
         for (int r0 = 0; r0 < kRegs; r0 += kRound) {
             // register (vl, i, v): channel block, row of the tile, channel of the VW
@@ -508,7 +514,7 @@ __global__ __launch_bounds__(kKv4Threads, 2) void kv4_attention_kernel(Kv4Attent
                                             __uint_as_float((uint32_t)(two[e][i][v / 2] >> (32 * (v & 1)))) * f;
                     }
                 }
-                const float inv = l != 0.f ? 1.f / l : 0.f;
+                const float inv = l != 0.f ? kGrow / l : 0.f;
 #pragma unroll
                 for (int i = 0; i < kMine; ++i) {
                     const int gi = way + i * WAYS;

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from oracle import kv4 as O
-from test_gpu_kv4 import attention_inputs, check_attention, contents, ints, say
+from test_gpu_kv4 import DT, attention_inputs, check_attention, contents, ints, say
 
 pytestmark = pytest.mark.gpu
 
@@ -233,3 +233,30 @@ def test_a_block_of_no_rows_through_every_call(pkg, dev, pages):
     j = torch.arange(cache.slots, device=dev)
     want = torch.where(j < n[:, None, None], w, torch.zeros_like(w))
     assert torch.equal(nw, want) and torch.equal(same, want) and torch.equal(data, before)
+
+
+@pytest.mark.parametrize("T,n,dtype,step", [(1, 700, "bf16", 0.0), (3, 700, "bf16", 0.01), (40, 300, "bf16", 0.02),
+                                            (2, 5000, "f16", 0.001)])
+def test_values_up_to_what_the_cache_holds(pkg, dev, T, n, dtype, step):
+    """Values of 3e38 (and infinity, held as that), under even weights and rising ones: no sum overflows."""
+    say("large values", T, n, dtype, step)
+    HQ, H, D = 4, 2, 64
+    g = torch.Generator().manual_seed(n)
+    cache = pkg.KV4Cache.allocate(1, n + T, H, D, dev)
+    k = torch.zeros(1, n + T, H, D)
+    k[0, :, :, 0] = (torch.arange(n + T) * 1.0)[:, None]
+    v = torch.where(torch.rand(D, generator=g) < 0.5, -1.0, 1.0).expand(1, n + T, H, D) * 3e38
+    v = v * (0.8 + 0.2 * torch.rand(1, n + T, H, D, generator=g))
+    v[0, 5, 0, 3] = v[0, n - 1, 1, 4] = float("inf")
+    pkg.kv4_append(cache, k.to(dev), v.to(dev), ints([0], dev))
+    q = torch.zeros(1, T, HQ, D, dtype=DT[dtype])
+    q[..., 0] = 1.0
+    scale = step if step else 1e-6
+    out, lse = pkg.kv4_attention(q.to(dev), cache, ints([n], dev), scale=scale)
+    torch.cuda.synchronize()
+    if dtype == "f16":                                     # past the type's range, as the values are
+        K, V = contents(cache)
+        ref = O.attention(q.double().numpy(), K, V, [n], [T], "causal", scale)[0]
+        assert np.array_equal(out.cpu().numpy(), np.sign(ref) * np.inf)
+    else:
+        check_attention(cache, q, dtype, "causal", [n], None, None, scale, out, lse)
