@@ -180,3 +180,24 @@ def evict(w, n, keep, recent, named=None):
     source = np.arange(keep)
     source[holes] = movers
     return source
+
+
+def round_to(x, dtype):
+    """Nearest number of a type ("bf16", "f16"), as float64."""
+    if dtype == "bf16":
+        return _bf16(x)
+    with np.errstate(over="ignore"):
+        return np.asarray(x, dtype=np.float64).astype(np.float16).astype(np.float64)
+
+
+def output_range(out, weight, err, dtype):
+    """The numbers of a type that attention's outputs may be: (lowest, highest).
+
+    err [B, T, HQ]: how far a row's scores may be off.  The weights then are off by that, by
+    the 2^-20 of an argument of the exponential around the row's largest score, and by the
+    two bf16 parts that meet the values (2^-17); sums in fp32 over a few hundred slots add
+    as much.  What comes of it is rounded once, to its type: whatever lies between the
+    roundings of both ends is right.
+    """
+    off = weight * (2.0 ** -16 + 2.0 * (err[..., None] + 2.0 ** -20)) + 1e-30
+    return round_to(out - off, dtype), round_to(out + off, dtype)
