@@ -70,6 +70,8 @@ class KV4Cache:
         if data.dtype != torch.uint8 or data.dim() != 3 or data.shape[2] != page_bytes(head_dim):
             raise ValueError(f"data must be uint8 [num_pages, kv_heads, {page_bytes(head_dim)}], got {data.dtype} "
                              f"{tuple(data.shape)}")
+        if data.shape[1] < 1:
+            raise ValueError("data must have one key/value head at least")
         if not data.is_contiguous():
             raise ValueError("data must be contiguous")
         if block_table.dtype != torch.int32 or block_table.dim() != 2:

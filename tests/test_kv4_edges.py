@@ -115,3 +115,8 @@ def test_keys_and_values_that_are_read_are_tensors_of_their_own(on_cpu, monkeypa
         assert x.untyped_storage().nbytes() == x.numel() * 4
         x.add_(torch.ones(64, requires_grad=True))
     assert k.untyped_storage().data_ptr() != v.untyped_storage().data_ptr()
+
+
+def test_a_cache_of_no_heads_is_refused(on_cpu):
+    with pytest.raises(ValueError, match="one key/value head"):
+        on_cpu.KV4Cache(torch.zeros(4, 0, 4352, dtype=torch.uint8), torch.zeros(2, 2, dtype=torch.int32), 64)
