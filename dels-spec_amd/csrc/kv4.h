@@ -44,7 +44,6 @@ __device__ __forceinline__ uint8_t* kv4_page(const Kv4Cache& c, int b, int h, in
     return c.data + ((int64_t)id * c.heads + h) * page_bytes;
 }
 
-// Context length and valid block rows of sequence b, within the table's slots.
 // Sum over the lanes up to this one: within rows of 16 lanes, then from row to row.
 __device__ __forceinline__ int sum_upto(int x) {
     x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);     // row_shr:1, 2, 4, 8
@@ -56,6 +55,7 @@ __device__ __forceinline__ int sum_upto(int x) {
     return x;
 }
 
+// Context length and valid block rows of sequence b, within the table's slots.
 __device__ __forceinline__ int kv4_length(const int32_t* lengths, int b, int slots) {
     return min(max(lengths[b], 0), slots);
 }
@@ -63,12 +63,6 @@ __device__ __forceinline__ int kv4_count(const int32_t* counts, int b, int T) {
     return counts ? min(max(counts[b], 0), T) : T;
 }
 
-__device__ __forceinline__ float kv4_level(uint32_t code) {
-    // e2m1 to fp32: exponent field 1..3 -> 2^(e-1) (1 + m/2), 0 -> m/2
-    const uint32_t m = code & 7u;
-    const float v = m < 2u ? 0.5f * (float)m : __uint_as_float(((126u + (m >> 1)) << 23) | ((m & 1u) << 22));
-    return code & 8u ? -v : v;
-}
 __device__ __forceinline__ float kv4_pow2(uint32_t e) { return __uint_as_float(e << 23); }
 
 }  // namespace dels
