@@ -260,3 +260,31 @@ def test_values_up_to_what_the_cache_holds(pkg, dev, T, n, dtype, step):
         assert np.array_equal(out.cpu().numpy(), np.sign(ref) * np.inf)
     else:
         check_attention(cache, q, dtype, "causal", [n], None, None, scale, out, lse)
+
+
+def test_pages_past_four_gibibytes(pkg, dev):
+    """The cache's last pages, more than 2^32 bytes in: every call as on a small cache of the same pages."""
+    say("far pages")
+    B, T, HQ, H, D, pages = 2, 5, 8, 4, 128, 6
+    small, q, _ = attention_inputs(pkg, dev, B, T, HQ, H, D, pages, "bf16", "none", [300, 333], None, 50)
+    size = H * O.page_bytes(D)
+    total = (1 << 32) // size + 200
+    data = torch.empty(total, H, O.page_bytes(D), dtype=torch.uint8, device=dev)
+    first = total - small.data.shape[0]
+    assert first * size > 1 << 32
+    data[first:] = small.data
+    far = pkg.KV4Cache(data, small.block_table + first, D)
+    g = torch.Generator().manual_seed(1)
+    k, v = (torch.randn(B, T, H, D, generator=g).to(torch.bfloat16).to(dev) for _ in "kv")
+    w = torch.rand(B, H, small.slots, generator=g).to(dev)
+    n, made = ints([300, 333], dev), []
+    for cache in (small, far):
+        pkg.kv4_append(cache, k, v, n)
+        out, lse = pkg.kv4_attention(q.to(dev), cache, n)
+        nw = pkg.kv4_weights(q.to(dev), cache, n, lse, w)
+        evicted = pkg.kv4_evict(cache, n + T, nw, 130, 20)
+        made.append((out, lse, nw, *evicted, *pkg.kv4_read(cache, ints([0, 0], dev), 130)))
+    torch.cuda.synchronize()
+    for x, y in zip(*made):
+        assert torch.equal(x, y)
+    assert torch.equal(far.data[first:], small.data)
