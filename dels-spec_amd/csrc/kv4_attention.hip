@@ -27,7 +27,7 @@
 //
 // Head size 128, 32 query heads on 8.  One token, 32 sequences of up to 16300 slots: 95 us,
 // bound by memory (5.1 TB/s over the whole, 6 in the loop).  16 tokens over 131k slots:
-// 76 us = 0.45 PFLOP/s, 2 x 512 tokens over up to 3500 slots: 112 us; bound by vector
+// 75 us = 0.46 PFLOP/s, 2 x 512 tokens over up to 3500 slots: 103 us; bound by vector
 // instructions, 650 a page and wave against 48 matrix ones of 32 cycles.  One token over
 // 700 slots: 9 us, bound by latency: 4 until the first page is there.
 #include <algorithm>
@@ -55,8 +55,9 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
 
 constexpr int kMinPages = 2 * kKv4Waves;      // fewest pages of a part (one row over 700 slots: 10.6 us in two of eight, 9.2 in one)
 constexpr int kCounterWords = 16;      // words from one arrival counter to the next
-// Most pieces of one tile group: their states are joined by one workgroup, about 0.25 us
-// each (one row over 94k slots: 45 us in 184 pieces, 29 in 32).
+// Most parts of one tile group (Cuts, kv4_mma.h; even cuts know no limit but the number of
+// workgroups): their states are joined by one workgroup, about 0.25 us each (one row over
+// 94k slots: 45 us in 184 parts, 29 in 32).
 constexpr int kMostParts = 32;
 
 template <typename T> __device__ __forceinline__ uint16_t round_to(float x);

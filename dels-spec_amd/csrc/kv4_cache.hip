@@ -4,9 +4,10 @@
 // of a page row, so no two waves write one word, whatever the block's start.
 // A lane has one slot's D / 8 channels, as eight-nibble words; the value words, eight
 // slots of a channel, are those transposed over the eight lanes of a channel group
-// (three exchanges of halves, bytes and nibbles).  Both kernels are bound by memory
-// where they are long (4 x 2039 rows of 8 heads of 128, fp16: written in 10.8 us, 3.9 TB/s, read
-// in 11.8, 3.6 TB/s) and by latency where short (8 x 16 rows: 4.5 and 4.4 us).
+// (three exchanges of halves, bytes and nibbles).  Long calls run at two thirds of a copy's
+// rate (4 x 2039 rows of 8 heads of 128, fp16, 6629 of 8156 valid: 34 MB written in 11.0 us,
+// 3.1 TB/s, a wave's values being loaded after its keys are done; 40 MB read in 11.9 us,
+// 3.4 TB/s); short ones are bound by latency (8 x 16 rows: 4.6 and 4.5 us).
 #include <algorithm>
 
 #include "kv4.h"

@@ -53,7 +53,9 @@ template <int WAVES> __device__ __forceinline__ int2 over_waves(const int* x) {
 // two exchanges a tile.  Bound by latency; rows of more than one tile are read up to
 // four times, all but the first from L2.  COPIES of the histogram: lanes of one digit
 // meet on fewer words.
-// 16 x 8 rows of up to 16300 slots: 22 us (30 with 64 slots at a time, ranks by ballots).
+// 16 x 8 rows of up to 16300 slots: 22 us (30 with 64 slots at a time, ranks by ballots), of
+// which the first histogram takes 4.6, the two others 4.6 more and the walk the rest; the 128
+// workgroups leave half of the CUs idle.
 template <int THREADS, int COPIES>
 __global__ __launch_bounds__(THREADS) void kv4_select_kernel(Kv4EvictArgs a, int32_t* hole_list) {
     constexpr int kWaves = THREADS / 64, kTile = THREADS * kPerLane, kOwn = kBins / THREADS;
@@ -242,9 +244,9 @@ __global__ __launch_bounds__(THREADS) void kv4_select_kernel(Kv4EvictArgs a, int
 // places before any of it is written: K words 16 (8) lanes a slot, value words of D / 64
 // channels a lane.  A moved slot's value codes lie in D words of eight slots each, so
 // eight times what moves is read: consecutive movers are often neighbours, whose
-// words the caches still hold.  Bound by those requests: 16 x 8 rows of up to 16300 slots to
-// 4096, head size 128: 62 us, 62 MB written (38 us without
-// the values, 52 without the keys, 55 without the scales).
+// words the caches still hold.  16 x 8 rows of up to 16300 slots to 4096, head size 128: 62 us,
+// 62 MB written; 30 us without the values, 45 without the keys, 55 without the scales, 23
+// without any of them (sources, page numbers and addresses, one after the other).
 template <int D>
 __global__ __launch_bounds__(kMoveThreads) void kv4_move_kernel(Kv4Cache c, const int32_t* lengths,
                                                                 const int32_t* __restrict__ sources, int keep,

@@ -187,7 +187,10 @@ struct Line {
 //    there are workgroups enough, up to a quarter (and a page a wave) over an even share.
 //  * Else every `share` pages; a cut within kSnap pages of where the next tiles begin moves
 //    there, so that no piece holds a few pages of some and the rest of others.  A piece
-//    over several tile groups begins and joins its waves for each (about 8 us).
+//    over several tile groups begins and joins its waves for each (about 8 us).  So are
+//    batches of more than 64 sequences cut, whatever their lengths, and `most` does not
+//    hold there: a long sequence among many short ones may lie in as many pieces as its
+//    share of the line.
 // Attention of 8 x 16 rows over up to 4000 slots: 35 us with even cuts alone, 27 with parts.
 struct Cuts {
     static constexpr int kSnap = 8;

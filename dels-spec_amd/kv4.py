@@ -230,7 +230,8 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, lengths: torch.Tensor, *, bl
     """Attention of a block's rows over their sequences' context and the block itself.
 
     ``q`` ``[batch, T, q_heads, head_dim]`` bf16 or fp16, ``q_heads`` a multiple of the
-    cache's heads.  Every row sees slots ``[0, lengths[b])``; of the block's own slots
+    cache's heads (fp16 needs keys below 2^20 in magnitude, and takes them as multiples of
+    2^-20).  Every row sees slots ``[0, lengths[b])``; of the block's own slots
     (which ``kv4_append`` wrote) ``block`` says which: ``"causal"``, ``"full"``, ``"none"``, or
     an int64 ``[batch, T]`` of bits, bit ``i`` of row ``t`` for slot ``lengths[b] + i`` (a tree of
     drafts; T at most 64; expanded where all sequences have one tree).  ``counts`` int32

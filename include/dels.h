@@ -614,8 +614,9 @@ int dels_kv4_read(const dels_kv4_cache* c, const int32_t* starts, const int32_t*
  * lse[b, t, hq] (contiguous fp32), the logarithm of the softmax's sum.  A row that sees
  * nothing, and rows from counts[b] on, give out = 0 and lse = -inf; a row that sees a
  * score of NaN or +inf gives NaN in both.  q [batch, T, q_heads, D]
- * bf16 or fp16, out the same type, any strides that keep rows 16-byte aligned.  With fp16 q
- * the keys that the cache holds must be below 2^20 in magnitude.
+ * bf16 or fp16, out the same type, any strides that keep rows 16-byte aligned.  fp16 q meets
+ * the keys as fp16 numbers of a sixteenth of their size: the keys that the cache holds must be
+ * below 2^20 in magnitude, and those that are no multiple of 2^-20 are rounded to one.
  */
 size_t dels_kv4_attention_ws_bytes(int64_t batch, int64_t T, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
                                    int64_t max_pages);
