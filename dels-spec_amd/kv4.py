@@ -235,9 +235,10 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, lengths: torch.Tensor, *, bl
     (which ``kv4_append`` wrote) ``block`` says which: ``"causal"``, ``"full"``, ``"none"``, or
     an int64 ``[batch, T]`` of bits, bit ``i`` of row ``t`` for slot ``lengths[b] + i`` (a tree of
     drafts; T at most 64; expanded where all sequences have one tree).  ``counts`` int32
-    ``[batch]`` are the valid rows (None: T).  ``scale`` defaults to ``head_dim ** -0.5``.  Returns ``(out, lse)``: ``out`` like ``q``, ``lse``
-    fp32 ``[batch, T, q_heads]``, the logarithm of each softmax's sum; rows that see
-    nothing give 0 and -inf, rows that see a score of NaN or +inf NaN in both.
+    ``[batch]`` are the valid rows (None: T).  ``scale`` defaults to ``head_dim ** -0.5``.
+    Returns ``(out, lse)``: ``out`` like ``q``, ``lse`` fp32 ``[batch, T, q_heads]``, the
+    logarithm of each softmax's sum; rows that see nothing give 0 and -inf, rows that see
+    a score of NaN or +inf NaN in both.
     """
     qp = _require_rows(q, cache, None, "q", _Q_DTYPES)
     batch, T, q_heads, D = q.shape
