@@ -20,6 +20,7 @@
 
 #include "dels_device.h"
 #include "dels_internal.h"
+#include "paged_attention.h"
 
 namespace dels {
 
@@ -38,29 +39,10 @@ template <int D> struct Kv4 {
 
 // Page of (b, h) that holds slots 64 p .. 64 p + 63, or null where the table
 // names no page.
-__device__ __forceinline__ uint8_t* kv4_page(const Kv4Cache& c, int b, int h, int p, int page_bytes) {
+__device__ __forceinline__ uint8_t* kv4_page(const PagedCache& c, int b, int h, int p, int page_bytes) {
     const int id = c.table[(int64_t)b * c.ld_table + p];
     if (id < 0 || id >= c.num_pages) return nullptr;
     return c.data + ((int64_t)id * c.heads + h) * page_bytes;
-}
-
-// Sum over the lanes up to this one: within rows of 16 lanes, then from row to row.
-__device__ __forceinline__ int sum_upto(int x) {
-    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);     // row_shr:1, 2, 4, 8
-    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);     // row_bcast:15 into rows 1 and 3
-    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);     // row_bcast:31 into rows 2 and 3
-    return x;
-}
-
-// Context length and valid block rows of sequence b, within the table's slots.
-__device__ __forceinline__ int kv4_length(const int32_t* lengths, int b, int slots) {
-    return min(max(lengths[b], 0), slots);
-}
-__device__ __forceinline__ int kv4_count(const int32_t* counts, int b, int T) {
-    return counts ? min(max(counts[b], 0), T) : T;
 }
 
 __device__ __forceinline__ float kv4_pow2(uint32_t e) { return __uint_as_float(e << 23); }

@@ -21,7 +21,7 @@
 // row tile and take every WAYS-th page, and their states are joined through LDS; 8 / WAYS
 // row tiles go over the same pages at the same time.  The pages of all (sequence,
 // head, tiles) are numbered in one line and cut into pieces, one for each workgroup
-// (Cuts, kv4_mma.h): a piece that covers all pages of its rows writes their output, others
+// (Cuts, paged_attention.h): a piece that covers all pages of its rows writes their output, others
 // write their state, and the last of them to arrive joins the states in their order, so
 // that results do not depend on who that is.
 //
@@ -47,38 +47,11 @@ constexpr float kLag = 8.f;
 // the reciprocal of the weights' sum makes up for it.
 constexpr float kShrink = 0x1p-20f, kGrow = 0x1p20f;
 
-// Two numbers rounded to bf16, the first in the low half.
-__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
-    typedef float f32x2 __attribute__((ext_vector_type(2)));
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
-}
-
 constexpr int kMinPages = 2 * kKv4Waves;      // fewest pages of a part (one row over 700 slots: 10.6 us in two of eight, 9.2 in one)
-constexpr int kCounterWords = 16;      // words from one arrival counter to the next
-// Most parts of one tile group (Cuts, kv4_mma.h; even cuts know no limit but the number of
+// Most parts of one tile group (Cuts, paged_attention.h; even cuts know no limit but the number of
 // workgroups): their states are joined by one workgroup, about 0.25 us each (one row over
 // 94k slots: 45 us in 184 parts, 29 in 32).
 constexpr int kMostParts = 32;
-
-template <typename T> __device__ __forceinline__ uint16_t round_to(float x);
-template <> __device__ __forceinline__ uint16_t round_to<bf16_t>(float x) { return f32_to_bf16_bits(x); }
-template <> __device__ __forceinline__ uint16_t round_to<f16_t>(float x) {
-    const _Float16 h = (_Float16)x;
-    uint16_t b;
-    __builtin_memcpy(&b, &h, 2);
-    return b;
-}
-
-// A row tile's row of this lane: token, query head, whether it is a valid row.
-struct Row { int t, hq; bool in_block, valid; };
-__device__ __forceinline__ Row row_of(int r, int group, int h, int T, int count) {
-    Row x;
-    x.t = divide(r, group);
-    x.hq = h * group + (r - x.t * group);
-    x.in_block = x.t < T;
-    x.valid = x.t < count;
-    return x;
-}
 
 template <typename T, int VW>
 __device__ __forceinline__ void store_out(const Kv4AttentionArgs& a, int b, const Row& row, int ch, const float* o,
@@ -103,11 +76,6 @@ __device__ __forceinline__ void store_lse(const Kv4AttentionArgs& a, int b, cons
     const float x = row.valid && total != 0.f ? (ref + __builtin_amdgcn_logf(total)) * 0.693147180559945309f
                                              : -__builtin_inff();
     a.lse[((int64_t)b * a.block.T + row.t) * a.q_heads + row.hq] = x;
-}
-
-// exp2(m - ref), 0 for m = -inf, whatever ref is.
-__device__ __forceinline__ float fade(float m, float ref) {
-    return m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - ref);
 }
 
 // Floats of a piece's state in the workspace: outputs as the lanes hold them, then references and sums.
@@ -149,7 +117,7 @@ template <typename T, int D, int MT> struct Rows {
                                          int first_slot, int n, int filled, int slots, int g, float unit, float lag) {
         // a page that reaches past the context (a branch: the statement keeps the compiler from
         // computing the masks of every page and selecting)
-        const bool masked = first_slot + kKv4Page > n;
+        const bool masked = first_slot + kCachePage > n;
         if (masked) {
             asm volatile("");
 #pragma unroll
@@ -278,7 +246,7 @@ __global__ __launch_bounds__(kKv4Threads, 2) void kv4_attention_kernel(Kv4Attent
     __shared__ typename Frag<T>::type s_q[kTiles][S::KS][64];
     __shared__ bool s_last;
 
-    const Kv4Cache& c = a.cache;
+    const PagedCache& c = a.cache;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane % MT, g = lane / MT, tile = wave / WAYS, way = wave % WAYS;
     const int slots = c.slots(), group = a.q_heads / c.heads;
@@ -286,9 +254,10 @@ __global__ __launch_bounds__(kKv4Threads, 2) void kv4_attention_kernel(Kv4Attent
     const int piece = (int)gridDim.x % 8 ? (int)blockIdx.x
                                          : (int)(blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8);
     const LaneOffsets<D, MT> at_lane(col, g);
-    Scan scan(a.block, c, c.heads * line.tiles);
+    const PagedSeqs seqs(a.block, c);
+    Scan<PagedSeqs> scan(seqs, c.heads * line.tiles);
     const Cuts cuts(scan, line, kMostParts);
-    Scan::Place at{};
+    Scan<PagedSeqs>::Place at{};
     const int2 mine = cuts.piece(scan, piece, at);
     int u = mine.x;
     const int u_end = mine.y;
@@ -311,7 +280,7 @@ __global__ __launch_bounds__(kKv4Threads, 2) void kv4_attention_kernel(Kv4Attent
         if (a.block.mode == DELS_KV4_CAUSAL)                  // no row of the tile sees past its last token
             end = (int)min((int64_t)end, (int64_t)n + divide(rt * MT + MT - 1, group) + 1);
         if (rt * MT >= a.block.T * group) end = 0;            // past the block's rows
-        const int stop = min(last, (end + kKv4Page - 1) / kKv4Page);
+        const int stop = min(last, (end + kCachePage - 1) / kCachePage);
 
         // the wave's pages, the next one loaded while one is worked on
         const int32_t* ids = c.table + (int64_t)b * c.ld_table;
@@ -388,7 +357,7 @@ __global__ __launch_bounds__(kKv4Threads, 2) void kv4_attention_kernel(Kv4Attent
             next_keys.load(address(next), at_lane);
             asm volatile("" ::: "memory");
             if (named(id))
-                rows.page(&s_q[tile][0][lane], keys, values, at_lane.half, p * kKv4Page, n, filled, slots, g, unit, lag);
+                rows.page(&s_q[tile][0][lane], keys, values, at_lane.half, p * kCachePage, n, filled, slots, g, unit, lag);
             keys = next_keys;
             id = next;
             next = id_at(p + 2 * WAYS);
@@ -567,7 +536,7 @@ size_t kv4_attention_data_bytes(int64_t batch, int64_t T, int64_t q_heads, int64
 }
 
 hipError_t launch_kv4_attention(const Kv4AttentionArgs& a, void* ws, size_t data_off, hipStream_t s) {
-    const Kv4Cache& c = a.cache;
+    const PagedCache& c = a.cache;
     const Plan p = plan(c.batch, a.block.T, a.q_heads, c.heads, c.max_pages);
     auto* states = reinterpret_cast<float*>(static_cast<char*>(ws) + data_off);
     auto* counters = reinterpret_cast<unsigned int*>(static_cast<char*>(ws) + kCountersOff);

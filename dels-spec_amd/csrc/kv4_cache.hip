@@ -96,21 +96,21 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t w) {
 // Lanes: slot i = lane / 8 of the group, channels N * (lane % 8) .. + N - 1 (N = D / 8).
 template <typename T, int D>
 __global__ __launch_bounds__(kCacheThreads) void kv4_append_kernel(
-    Kv4Cache c, const T* __restrict__ k, int64_t kb, int64_t kt, int64_t kh, const T* __restrict__ v, int64_t vb,
+    PagedCache c, const T* __restrict__ k, int64_t kb, int64_t kt, int64_t kh, const T* __restrict__ v, int64_t vb,
     int64_t vt, int64_t vh, const int32_t* lengths, const int32_t* counts, int T_rows, int groups) {
     constexpr int N = D / 8;
     const int lane = threadIdx.x & 63;
     const int grp = blockIdx.x * (kCacheThreads / 64) + (threadIdx.x >> 6), h = blockIdx.y, b = blockIdx.z;
     if (grp >= groups) return;
     const int slots = c.slots();
-    const int n = kv4_length(lengths, b, slots);
-    const int end = (int)min((int64_t)slots, (int64_t)n + kv4_count(counts, b, T_rows));
+    const int n = paged_length(lengths, b, slots);
+    const int end = (int)min((int64_t)slots, (int64_t)n + paged_count(counts, b, T_rows));
     const int s0 = (n & ~7) + 8 * grp;             // the group's first slot
     if (max(s0, n) >= end) return;
-    uint8_t* page = kv4_page(c, b, h, s0 / kKv4Page, Kv4<D>::kBytes);
+    uint8_t* page = kv4_page(c, b, h, s0 / kCachePage, Kv4<D>::kBytes);
     if (!page) return;
     const int i = lane >> 3, ch = (lane & 7) * N;
-    const int slot = s0 + i, in_page = slot % kKv4Page;
+    const int slot = s0 + i, in_page = slot % kCachePage;
     const bool mine = slot >= n && slot < end;
     const int64_t t = mine ? slot - n : max(n, s0) - n;   // a row that exists, for lanes without one
     float x[N];
@@ -146,7 +146,7 @@ __global__ __launch_bounds__(kCacheThreads) void kv4_append_kernel(
 #pragma unroll
     for (int q = 0; q < 8; ++q) valid |= s0 + q >= n && s0 + q < end ? 15u << (4 * q) : 0u;
     // lane group i then holds channel 8 q + i of its sixteen (eight)
-    uint32_t* row = reinterpret_cast<uint32_t*>(page + Kv4<D>::kValue) + (s0 % kKv4Page / 8) * D + ch + i;
+    uint32_t* row = reinterpret_cast<uint32_t*>(page + Kv4<D>::kValue) + (s0 % kCachePage / 8) * D + ch + i;
 #pragma unroll
     for (int q = 0; q < N / 8; ++q) {
         const uint32_t words = transpose8(encode8<T>(x + 8 * q, step));
@@ -186,7 +186,7 @@ template <typename T> __device__ __forceinline__ void store8(T* p, uint32_t code
 
 // Lanes as in the append kernel: slot i = lane / 8, channels N * (lane % 8) .. + N - 1.
 template <typename T, int D>
-__global__ __launch_bounds__(kCacheThreads) void kv4_read_kernel(Kv4Cache c, const int32_t* starts,
+__global__ __launch_bounds__(kCacheThreads) void kv4_read_kernel(PagedCache c, const int32_t* starts,
                                                                  const int32_t* counts, int T_rows, int groups,
                                                                  T* __restrict__ k, T* __restrict__ v) {
     constexpr int N = D / 8;
@@ -194,21 +194,21 @@ __global__ __launch_bounds__(kCacheThreads) void kv4_read_kernel(Kv4Cache c, con
     const int grp = blockIdx.x * (kCacheThreads / 64) + (threadIdx.x >> 6), h = blockIdx.y, b = blockIdx.z;
     if (grp >= groups) return;
     const int slots = c.slots();
-    const int n = kv4_length(starts, b, slots);
-    const int64_t end = min((int64_t)slots, (int64_t)n + kv4_count(counts, b, T_rows));
+    const int n = paged_length(starts, b, slots);
+    const int64_t end = min((int64_t)slots, (int64_t)n + paged_count(counts, b, T_rows));
     const int64_t s0 = (n & ~7) + 8 * (int64_t)grp;
     if (s0 >= (int64_t)n + T_rows) return;
-    const uint8_t* page = s0 < end ? kv4_page(c, b, h, (int)(s0 / kKv4Page), Kv4<D>::kBytes) : nullptr;
+    const uint8_t* page = s0 < end ? kv4_page(c, b, h, (int)(s0 / kCachePage), Kv4<D>::kBytes) : nullptr;
     const int i = lane >> 3, ch = (lane & 7) * N;
     const int64_t slot = s0 + i;
     const bool wanted = slot >= n && slot < (int64_t)n + T_rows, have = page && slot >= n && slot < end;
-    const int in_page = (int)(slot % kKv4Page);
+    const int in_page = (int)(slot % kCachePage);
     uint32_t kw[N / 8], vw[N / 8];
     float ks = 0.f, vs = 0.f;
 #pragma unroll
     for (int q = 0; q < N / 8; ++q) kw[q] = vw[q] = 0u;
     if (page) {
-        const uint32_t* row = reinterpret_cast<const uint32_t*>(page + Kv4<D>::kValue) + (s0 % kKv4Page / 8) * D + ch + i;
+        const uint32_t* row = reinterpret_cast<const uint32_t*>(page + Kv4<D>::kValue) + (s0 % kCachePage / 8) * D + ch + i;
 #pragma unroll
         for (int q = 0; q < N / 8; ++q) vw[q] = row[8 * q];
     }
@@ -246,7 +246,7 @@ int groups_of(int T) { return (T + 7 + 7) / 8; }
 
 }  // namespace
 
-hipError_t launch_kv4_append(const Kv4Cache& c, const Kv4Rows& k, const Kv4Rows& v, int dtype, const int32_t* lengths,
+hipError_t launch_kv4_append(const PagedCache& c, const PagedRows& k, const PagedRows& v, int dtype, const int32_t* lengths,
                              const int32_t* counts, int T, hipStream_t s) {
     const int groups = groups_of(T), waves = kCacheThreads / 64;
     const dim3 grid((groups + waves - 1) / waves, c.heads, c.batch);
@@ -258,7 +258,7 @@ hipError_t launch_kv4_append(const Kv4Cache& c, const Kv4Rows& k, const Kv4Rows&
     });
 }
 
-hipError_t launch_kv4_read(const Kv4Cache& c, const int32_t* starts, const int32_t* counts, int T, void* k, void* v,
+hipError_t launch_kv4_read(const PagedCache& c, const int32_t* starts, const int32_t* counts, int T, void* k, void* v,
                            int dtype, hipStream_t s) {
     const int groups = groups_of(T), waves = kCacheThreads / 64;
     const dim3 grid((groups + waves - 1) / waves, c.heads, c.batch);

@@ -67,7 +67,7 @@ __global__ __launch_bounds__(THREADS) void kv4_select_kernel(Kv4EvictArgs a, int
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int bh = blockIdx.x, h = bh % a.cache.heads, b = bh / a.cache.heads;
     const int slots = a.cache.slots(), keep = a.keep;
-    const int n = kv4_length(a.lengths, b, slots);
+    const int n = paged_length(a.lengths, b, slots);
     const float* w = a.weights + (int64_t)bh * slots;
     float* out = a.out_weights + (int64_t)bh * slots;
     int32_t* source = a.source + (int64_t)bh * keep;
@@ -97,7 +97,7 @@ __global__ __launch_bounds__(THREADS) void kv4_select_kernel(Kv4EvictArgs a, int
     const int32_t* ids = a.cache.table + (int64_t)b * a.cache.ld_table;
     auto in_page = [&](int page) { return ids[page] >= 0 && ids[page] < a.cache.num_pages; };
     bool gap = false;
-    for (int p = tid; p * kKv4Page < n; p += THREADS) gap |= !in_page(p);
+    for (int p = tid; p * kCachePage < n; p += THREADS) gap |= !in_page(p);
     clear();
     if (__any(gap)) gap = true;
     if (lane == 0) s_wave[wave] = gap;
@@ -108,8 +108,8 @@ __global__ __launch_bounds__(THREADS) void kv4_select_kernel(Kv4EvictArgs a, int
     if (gaps) {
         auto slots_in_pages = [&](int from, int to, int* sum) {
             int mine = 0;
-            for (int p = from / kKv4Page + tid; p * kKv4Page < to; p += THREADS)
-                mine += in_page(p) ? min(to, (p + 1) * kKv4Page) - max(from, p * kKv4Page) : 0;
+            for (int p = from / kCachePage + tid; p * kCachePage < to; p += THREADS)
+                mine += in_page(p) ? min(to, (p + 1) * kCachePage) - max(from, p * kCachePage) : 0;
             atomicAdd(sum, mine);
             __syncthreads();
             return *sum;
@@ -118,7 +118,7 @@ __global__ __launch_bounds__(THREADS) void kv4_select_kernel(Kv4EvictArgs a, int
         recent = min(recent, room);
         chosen = room - slots_in_pages(n - recent, n, &s_named[1]);
     }
-    auto held_at = [&](int first) { return !gaps || (first < n && in_page(first / kKv4Page)); };
+    auto held_at = [&](int first) { return !gaps || (first < n && in_page(first / kCachePage)); };
     const int cand = n - recent;
     uint32_t left = chosen;                        // candidates still to choose among the equal prefixes
     uint32_t prefix = 0u;
@@ -248,7 +248,7 @@ __global__ __launch_bounds__(THREADS) void kv4_select_kernel(Kv4EvictArgs a, int
 // 62 MB written; 30 us without the values, 45 without the keys, 55 without the scales, 23
 // without any of them (sources, page numbers and addresses, one after the other).
 template <int D>
-__global__ __launch_bounds__(kMoveThreads) void kv4_move_kernel(Kv4Cache c, const int32_t* lengths,
+__global__ __launch_bounds__(kMoveThreads) void kv4_move_kernel(PagedCache c, const int32_t* lengths,
                                                                 const int32_t* __restrict__ sources, int keep,
                                                                 int groups) {
     constexpr int N = D / 64;
@@ -262,21 +262,21 @@ __global__ __launch_bounds__(kMoveThreads) void kv4_move_kernel(Kv4Cache c, cons
     // loaded before any of it is looked at.
     const int i8 = lane & 7;
     const int mine = 8 * g + i8 < keep ? sources[bh * keep + 8 * g + i8] : -1;
-    const int n = kv4_length(lengths, b, c.slots());
-    uint8_t* page = kv4_page(c, b, h, 8 * g / kKv4Page, P::kBytes);
+    const int n = paged_length(lengths, b, c.slots());
+    uint8_t* page = kv4_page(c, b, h, 8 * g / kCachePage, P::kBytes);
     if (n <= keep || 8 * g >= n) return;
     const int64_t page_stride = (int64_t)c.heads * P::kBytes;
     const bool comes = mine >= keep && mine < n;
     const int32_t* ids = c.table + (int64_t)b * c.ld_table;
-    int from_id = comes ? ids[mine / kKv4Page] : -1;
+    int from_id = comes ? ids[mine / kCachePage] : -1;
     const bool moves = comes && from_id >= 0 && from_id < c.num_pages;
     const uint32_t todo = (uint32_t)__ballot(moves) & 0xffu;
     if (!todo || !page) return;
-    const int in_page = 8 * g % kKv4Page;
+    const int in_page = 8 * g % kCachePage;
     // a place that takes nothing reads its own content
     const uint8_t* own_head = c.data + (int64_t)h * P::kBytes;
-    if (!moves) from_id = ids[8 * g / kKv4Page];
-    const int from_slot = moves ? mine % kKv4Page : in_page + i8;
+    if (!moves) from_id = ids[8 * g / kCachePage];
+    const int from_slot = moves ? mine % kCachePage : in_page + i8;
 
     uint32_t* row = reinterpret_cast<uint32_t*>(page + P::kValue) + (in_page / 8) * D + lane * N;
     uint32_t words[N], src[8][N], key[kLoads];
@@ -330,7 +330,7 @@ size_t kv4_evict_data_bytes(int64_t batch, int64_t heads, int64_t keep) {
 }
 
 hipError_t launch_kv4_evict(const Kv4EvictArgs& a, void* ws, size_t data_off, hipStream_t s) {
-    const Kv4Cache& c = a.cache;
+    const PagedCache& c = a.cache;
     auto* holes = reinterpret_cast<int32_t*>(static_cast<char*>(ws) + data_off);
     // one tile of a small workgroup where that holds a row: its barriers and histogram take less
     // (600 slots: 10.6 us, 14.2 by the large one)

@@ -36,18 +36,19 @@ __global__ __launch_bounds__(kKv4Threads, 4) void kv4_weights_kernel(Kv4WeightsA
     __shared__ __align__(16) int s_lim[kRows];               // of the block's slots a row sees those below,
     __shared__ uint64_t s_bits[kRows];                       // and those whose bits are set
 
-    const Kv4Cache& c = a.cache;
+    const PagedCache& c = a.cache;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane % MT, g = lane / MT;
     const int slots = c.slots(), group = a.q_heads / c.heads;
     const LaneOffsets<D, MT> at_lane(col, g);
-    Scan scan(a.block, c, c.heads);
+    const PagedSeqs seqs(a.block, c);
+    Scan<PagedSeqs> scan(seqs, c.heads);
     const Cuts cuts(scan, Line{1, pieces, kMinPages}, INT32_MAX);
     const float mag = fabsf(a.scale);
     const float unit = (mag == 0.f ? 1.f : mag) * kLog2e * (float)(1 << kKeyShift<T>);
     const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u, zero = mag == 0.f ? 0u : ~0u;
 
-    Scan::Place at{};
+    Scan<PagedSeqs>::Place at{};
     const int2 piece = cuts.piece(scan, blockIdx.x, at);
     int u = piece.x;
     const int u_end = piece.y;
@@ -59,9 +60,9 @@ __global__ __launch_bounds__(kKv4Threads, 4) void kv4_weights_kernel(Kv4WeightsA
         const int first_page = first + wave;
         const int filled = seq_end(a.block, n, count, slots);
         const int32_t* ids = c.table + (int64_t)b * c.ld_table;
-        auto id_at = [&](int p) { return p < last && p * kKv4Page < filled ? ids[p] : -1; };
+        auto id_at = [&](int p) { return p < last && p * kCachePage < filled ? ids[p] : -1; };
         const int first_id = id_at(first_page);
-        const int rows = uniform(min(kv4_count(a.accepted, b, a.block.T), count)) * group;
+        const int rows = uniform(min(paged_count(a.accepted, b, a.block.T), count)) * group;
         const uint8_t* heads = c.data + (int64_t)h * Kv4<D>::kBytes;
         const int64_t page_stride = (int64_t)c.heads * Kv4<D>::kBytes;
         const int64_t out_row = ((int64_t)b * c.heads + h) * slots;
@@ -110,10 +111,10 @@ __global__ __launch_bounds__(kKv4Threads, 4) void kv4_weights_kernel(Kv4WeightsA
                 next_keys.load(heads + (named(next) ? next : 0) * page_stride, at_lane);
                 asm volatile("" ::: "memory");
                 // the slot that this lane writes, of the four it has sums for: by its group
-                const int mine = p * kKv4Page + 32 * (g >> 1) + S::slot_of(g & 1, col);
+                const int mine = p * kCachePage + 32 * (g >> 1) + S::slot_of(g & 1, col);
                 float sum = r0 > 0 ? a.out[out_row + mine] : mine < n ? a.weights[out_row + mine] : 0.f;
                 if (named(id) && tiles > 0) {
-                    const bool masked = (p + 1) * kKv4Page > n;
+                    const bool masked = (p + 1) * kCachePage > n;
 #pragma unroll
                     for (int s = 0; s < 2; ++s) {
                         F kf[S::KT][S::KS];
@@ -152,7 +153,7 @@ __global__ __launch_bounds__(kKv4Threads, 4) void kv4_weights_kernel(Kv4WeightsA
                                     const uint64_t bits = s_bits[row + x];
 #pragma unroll
                                     for (int t = 0; t < S::KT; ++t) {
-                                        const int i = p * kKv4Page + 32 * s + S::slot_of(t, col) - n;
+                                        const int i = p * kCachePage + 32 * s + S::slot_of(t, col) - n;
                                         const uint32_t bit = i < 0 || i > 63 ? 0u : (uint32_t)(bits >> (i & 63)) & 1u;
                                         acc[t][x] = i < lim || bit ? acc[t][x] : -__builtin_inff();
                                     }
@@ -184,7 +185,7 @@ __global__ __launch_bounds__(kKv4Threads, 4) void kv4_weights_kernel(Kv4WeightsA
     const int rest = c.batch * c.heads;
     for (int bh = blockIdx.x; bh < rest; bh += gridDim.x) {
         const int pages = uniform(seq_pages(a.block, bh / c.heads, slots));
-        for (int j = pages * kKv4Page + threadIdx.x; j < slots; j += kKv4Threads) a.out[(int64_t)bh * slots + j] = 0.f;
+        for (int j = pages * kCachePage + threadIdx.x; j < slots; j += kKv4Threads) a.out[(int64_t)bh * slots + j] = 0.f;
     }
 }
 
@@ -192,7 +193,7 @@ __global__ __launch_bounds__(kKv4Threads, 4) void kv4_weights_kernel(Kv4WeightsA
 __global__ void kv4_no_weights_kernel(Kv4WeightsArgs a) {
     const int slots = a.cache.slots(), rows = a.cache.batch * a.cache.heads;
     for (int bh = blockIdx.y; bh < rows; bh += gridDim.y) {
-        const int n = kv4_length(a.block.lengths, bh / a.cache.heads, slots);
+        const int n = paged_length(a.block.lengths, bh / a.cache.heads, slots);
         const int64_t row = (int64_t)bh * slots;
         for (int j = blockIdx.x * blockDim.x + threadIdx.x; j < slots; j += gridDim.x * blockDim.x)
             a.out[row + j] = j < n ? a.weights[row + j] : 0.f;
@@ -202,7 +203,7 @@ __global__ void kv4_no_weights_kernel(Kv4WeightsArgs a) {
 }  // namespace
 
 hipError_t launch_kv4_weights(const Kv4WeightsArgs& a, hipStream_t s) {
-    const Kv4Cache& c = a.cache;
+    const PagedCache& c = a.cache;
     if (c.num_pages == 0 || a.block.T == 0) {
         const int rows = (int)std::min<int64_t>((int64_t)c.batch * c.heads, 65535);
         hipLaunchKernelGGL(kv4_no_weights_kernel, dim3((c.slots() + 1023) / 1024, rows), dim3(256), 0, s, a);
