@@ -21,6 +21,9 @@ Public surface (mirrors the reference's interface for this path):
   * ``KV4Cache`` with ``kv4_append``, ``kv4_read``, ``kv4_attention``,
     ``kv4_weights`` and ``kv4_evict`` -- the target's side of a draft block's
     verification over a key/value cache held in 4 bits
+  * ``KV8Cache`` with ``RotaryTable``, ``kv8_append``, ``kv8_read`` and
+    ``kv8_attention`` -- the same in 8 bits, with the position rotation on the
+    way into the cache and sliding windows
 """
 
 from .checkpoints import detect_local_head_checkpoint_kind
@@ -30,6 +33,7 @@ from .ops import (Fp8Weight, PackedWeight, argmax_rows, fused_argmax, fused_argm
                   lowrank_argmax, lowrank_argmax_fp8, pack_operand, pack_operand_fp8, quantize_e4m3_rows,
                   quantize_pack_fp8, rank_proj, sample_rows, domino_argmax, lm_head, pack_lm_head)
 from .kv4 import KV4Cache, kv4_append, kv4_attention, kv4_evict, kv4_read, kv4_weights
+from .kv8 import KV8Cache, RotaryTable, kv8_append, kv8_attention, kv8_read
 from .sampling import sample
 from .draft_step import DeLSDraftStep
 from .runner import DeLSGraphRunner
@@ -75,5 +79,10 @@ __all__ = [
     "kv4_attention",
     "kv4_weights",
     "kv4_evict",
+    "KV8Cache",
+    "RotaryTable",
+    "kv8_append",
+    "kv8_read",
+    "kv8_attention",
     "synth",
 ]

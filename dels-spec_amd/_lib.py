@@ -108,7 +108,15 @@ class Kv4CacheParams(ctypes.Structure):
     ]
 
 
+class RotaryParams(ctypes.Structure):
+    """Mirror of ``struct dels_rotary`` in include/dels.h."""
+
+    _fields_ = [("cos", _ptr), ("sin", _ptr), ("ld", _i64), ("positions", _i64), ("channels", _i64),
+                ("interleaved", _int)]
+
+
 _kv4 = ctypes.POINTER(Kv4CacheParams)
+_rotary = ctypes.POINTER(RotaryParams)
 
 # name -> (restype, argtypes); every symbol include/dels.h declares.
 SIGNATURES = {
@@ -183,6 +191,13 @@ SIGNATURES = {
                                 ctypes.c_float, _ptr, _ptr, _ptr, _ptr]),
     "dels_kv4_evict_ws_bytes": (_sz, [_i64, _i64, _i64]),
     "dels_kv4_evict": (_int, [_kv4, _ptr, _ptr, _i64, _i64, _ptr, _ptr, _ptr, _ptr, _sz, _ptr]),
+    "dels_kv8_page_bytes": (_sz, [_i64]),
+    "dels_kv8_append": (_int, [_kv4, _ptr, _i64, _i64, _i64, _ptr, _i64, _i64, _i64, _int, _ptr, _ptr, _i64, _rotary,
+                               _ptr, _i64, _ptr, _i64, _i64, _i64, _i64, _ptr, _i64, _i64, _i64, _ptr]),
+    "dels_kv8_read": (_int, [_kv4, _ptr, _ptr, _i64, _ptr, _ptr, _int, _ptr]),
+    "dels_kv8_attention_ws_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64, _i64]),
+    "dels_kv8_attention": (_int, [_kv4, _ptr, _i64, _i64, _i64, _int, _i64, _i64, _ptr, _ptr, _int, _ptr, _i64,
+                                  ctypes.c_float, _i64, _i64, _ptr, _i64, _i64, _i64, _ptr, _ptr, _sz, _ptr]),
 }
 
 _lock = threading.Lock()

@@ -310,7 +310,7 @@ int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
 int hip_fail(hipError_t e, const char* what);
 int check_ws(const void* ws, size_t ws_bytes, size_t need);
 
-// ---- 4-bit key/value cache (kv4_*.hip) -----------------------------------------
+// ---- paged key/value caches ------------------------------------------------------
 
 constexpr int kCachePage = 64;             // slots of a page
 
@@ -325,12 +325,6 @@ struct PagedCache {
 // A tensor [batch, tokens, heads, D] with unit channel stride.
 struct PagedRows { const void* p; int64_t batch, token, head; };
 
-// dtype as DELS_DTYPE_*.
-hipError_t launch_kv4_append(const PagedCache& c, const PagedRows& k, const PagedRows& v, int dtype, const int32_t* lengths,
-                             const int32_t* counts, int T, hipStream_t s);
-hipError_t launch_kv4_read(const PagedCache& c, const int32_t* starts, const int32_t* counts, int T, void* k, void* v,
-                           int dtype, hipStream_t s);
-
 // Which slots the rows of a block see beside their sequence's context.
 struct PagedBlock {
     const int32_t* lengths;              // context: slots [0, lengths[b])
@@ -338,6 +332,14 @@ struct PagedBlock {
     int T, mode;                         // DELS_KV4_CAUSAL .. DELS_KV4_MASK
     const int64_t* mask; int64_t ld_mask;
 };
+
+// ---- 4-bit key/value cache (kv4_*.hip) -----------------------------------------
+
+// dtype as DELS_DTYPE_*.
+hipError_t launch_kv4_append(const PagedCache& c, const PagedRows& k, const PagedRows& v, int dtype, const int32_t* lengths,
+                             const int32_t* counts, int T, hipStream_t s);
+hipError_t launch_kv4_read(const PagedCache& c, const int32_t* starts, const int32_t* counts, int T, void* k, void* v,
+                           int dtype, hipStream_t s);
 
 struct Kv4AttentionArgs {
     PagedCache cache; PagedBlock block;
@@ -369,5 +371,34 @@ struct Kv4EvictArgs {
 // Words of the workspace's data region that the selection keeps its holes in.
 size_t kv4_evict_data_bytes(int64_t batch, int64_t heads, int64_t keep);
 hipError_t launch_kv4_evict(const Kv4EvictArgs& a, void* ws, size_t data_off, hipStream_t s);
+
+// ---- 8-bit key/value cache (kv8_*.hip) -----------------------------------------
+
+// Angles of positions (struct dels_rotary), and which position each row of a block has.
+struct KvRotary {
+    const float *cos, *sin; int64_t ld, positions;
+    int rot;                             // channels that are rotated, 0: none
+    bool interleaved;
+    const int32_t* at; int64_t ld_at;    // [batch, T] positions (null: lengths[b] + t)
+};
+
+// q_heads 0: no queries.
+hipError_t launch_kv8_append(const PagedCache& c, const PagedRows& k, const PagedRows& v, int dtype,
+                             const int32_t* lengths, const int32_t* counts, int T, const KvRotary& rotary,
+                             const PagedRows& q, int q_heads, const PagedRows& q_out, hipStream_t s);
+hipError_t launch_kv8_read(const PagedCache& c, const int32_t* starts, const int32_t* counts, int T, void* k, void* v,
+                           int dtype, hipStream_t s);
+
+struct Kv8AttentionArgs {
+    PagedCache cache; PagedBlock block;
+    PagedRows q; int dtype, q_heads;
+    float scale;
+    int64_t window, sinks;               // window 0: rows see their whole context
+    void* out; int64_t out_batch, out_token, out_head;
+    float* lse;                          // [batch, T, q_heads]
+};
+size_t kv8_attention_data_bytes(int64_t batch, int64_t T, int64_t q_heads, int64_t heads, int64_t head_dim,
+                                int64_t max_pages);
+hipError_t launch_kv8_attention(const Kv8AttentionArgs& a, void* ws, size_t data_off, hipStream_t s);
 
 }  // namespace dels

@@ -1,0 +1,656 @@
+// Attention over the 8-bit key/value cache (format: kv8.h), whole or through a window.
+//
+//     x[t, j] = scale * q[t] . k[j]          j a slot that row t sees
+//     lse[t]  = log sum_j exp(x[t, j])
+//     o[t]    = sum_j exp(x[t, j] - lse[t]) v[j]
+// A row that sees nothing has o = 0 and lse = -inf.  With a window, row t sees of those slots
+// the ones from lengths + t - window + 1 on and the first `sinks`.
+//
+// One pass over the slots with the running maximum and sum of each row's softmax.
+// The rows that share a cache head (block tokens x query heads of the group) are
+// the columns of both products:
+//     S^T [slots x rows] = K Q^T          O^T [channels x rows] += V^T P^T
+// and a lane holds scores of sixteen consecutive slots of one row, which are two operands
+// of the second product: P stays in its lane.  Codes become the queries' type by
+// the conversion instruction, exactly; a block's key scale joins the factor of its
+// scores, its value scale is applied by the conversion.  Both products are 16-bit ones: the
+// 8-bit matrix instructions add products at 2^-12 of the largest of a group (measured),
+// which a float32 lse would show.  Weights enter as two bf16 parts (2^-17 of each, whatever its
+// size).  Scores, maxima, sums and outputs are fp32.
+#include <algorithm>
+
+#include "kv8.h"
+
+namespace dels {
+
+namespace {
+
+constexpr int kWaves = kLineWaves, kThreads = 64 * kWaves;
+// What a row's weights are relative to lies this many binary orders above its largest score
+// when it moves, and moves when a score passes it: until then the outputs need no rescaling
+// and no weight is above 1.
+constexpr float kLag = 8.f;
+constexpr int kMinPages = 2 * kWaves;  // fewest pages of a part
+// Most parts of one tile group: their states are joined by one workgroup.
+constexpr int kMostParts = 32;
+
+// Shapes of a wave's work on MT rows: MT x MT tiles of the matrix instructions.
+template <int D, int MT_> struct Shape8 {
+    static constexpr int MT = MT_;
+    static constexpr int NG = 64 / MT;              // lane groups: lane = MT * group + row
+    static constexpr int KS = D / NG / 8;           // steps of the first product: 8 channels a lane
+    static constexpr int KL = KS / 2;               // loads of a key tile: 16 channels a lane
+    static constexpr int NT = 64 / MT;              // key tiles of a page
+    static constexpr int ACC = MT == 16 ? 4 : 16;   // accumulator registers of a tile
+    static constexpr int RUNS = MT / 16;            // runs of 16 consecutive slots that a lane has scores of
+    static constexpr int CT = D / MT;               // channel tiles of the output
+    using Acc = typename std::conditional<MT == 16, f32x4, f32x16>::type;
+    // first slot of a lane group's run within the page, and its block
+    __device__ static int run_slot(int run, int g) { return MT == 16 ? 16 * g : 32 * run + 16 * g; }
+    // first of the four channels of registers 4 j .. 4 j + 3 of channel tile `t`
+    __device__ static int channel_of(int t, int j, int g) { return MT * t + (MT == 16 ? 4 * g : 8 * j + 4 * g); }
+};
+
+// Eight codes, times a power of two.
+template <typename T>
+__device__ __forceinline__ typename Frag<T>::type widen8(uint32_t lo, uint32_t hi, float scale) {
+    if constexpr (std::is_same<T, bf16_t>::value) {
+        const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false);
+        const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);
+        const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false);
+        const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
+        return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+    } else {
+        const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, scale, false);
+        const f16x2 b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, scale, true);
+        const f16x2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, scale, false);
+        const f16x2 d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, scale, true);
+        return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+    }
+}
+
+// The lowest k of 16 bits.
+__device__ __forceinline__ uint32_t lowest(int k) { return (1u << min(max(k, 0), 16)) - 1u; }
+
+template <int D, int MT> struct KeyRegs {
+    using S = Shape8<D, MT>;
+    u32x4 code[S::NT][S::KL];
+    uint32_t exponents[S::RUNS], bad[S::RUNS];
+    __device__ __forceinline__ void load(const uint8_t* page, int col, int g) {
+        const int lane = MT == 16 ? 32 * D * (col >> 3) + 512 * g + 16 * (col & 7) : 512 * g + 16 * col;
+#pragma unroll
+        for (int t = 0; t < S::NT; ++t)
+#pragma unroll
+            for (int i = 0; i < S::KL; ++i)
+                code[t][i] = *reinterpret_cast<const u32x4*>(page + lane + 512 * S::NG * i + (MT == 16 ? 128 : 32 * D) * t);
+#pragma unroll
+        for (int r = 0; r < S::RUNS; ++r) {
+            const auto w = *reinterpret_cast<const u32x2*>(page + Kv8<D>::kHead + 8 * (MT == 16 ? g / 2 : r));
+            exponents[r] = w[0];
+            bad[r] = w[1];
+        }
+    }
+};
+
+template <int D, int MT> struct ValueRegs {
+    using S = Shape8<D, MT>;
+    u32x4 code[S::RUNS][S::CT];
+    __device__ __forceinline__ void load(const uint8_t* page, int col, int g) {
+        const int lane = Kv8<D>::kValue + 16 * D * g + 16 * col;
+#pragma unroll
+        for (int r = 0; r < S::RUNS; ++r)
+#pragma unroll
+            for (int t = 0; t < S::CT; ++t)
+                code[r][t] = *reinterpret_cast<const u32x4*>(page + lane + 32 * D * r + 16 * MT * t);
+    }
+};
+
+// Which slots a row sees.
+struct Sight {
+    int n, filled;             // context; slots that hold anything
+    int lim, lo;               // the row sees slots below lim,
+    uint64_t bits;             // and those of the block whose bits are set, from lo on
+    int sinks;                 // or below this
+    __device__ uint32_t of_run(int j0) const {             // of slots j0 .. j0 + 15
+        const int d = j0 - n;
+        uint32_t by_bit = d >= 64 || d <= -16 ? 0u : (uint32_t)(d >= 0 ? bits >> d : bits << -d) & 0xffffu;
+        by_bit &= lowest(filled - j0);
+        return (lowest(lim - j0) | by_bit) & (~lowest(lo - j0) | lowest(sinks - j0));
+    }
+};
+
+// The rows' state of a wave, and one page's part in it.
+template <typename T, int D, int MT> struct Rows8 {
+    using S = Shape8<D, MT>;
+    using F = typename Frag<T>::type;
+    typename S::Acc o[S::CT];
+    float top, total;          // what weights are relative to (binary logarithm) and this lane's part of their sum
+
+    // scores of a page; q: this lane's operands of the queries in LDS, 64 apart
+    __device__ __forceinline__ void scores(const F* q, const KeyRegs<D, MT>& keys, typename S::Acc (&acc)[S::NT]) {
+#pragma unroll
+        for (int t = 0; t < S::NT; ++t)
+#pragma unroll
+            for (int i = 0; i < S::ACC; ++i) acc[t][i] = 0.f;
+        F next_q = q[0];
+#pragma unroll
+        for (int k = 0; k < S::KS; ++k) {
+            const F qk = next_q;
+            if (k + 1 < S::KS) next_q = q[64 * (k + 1)];       // read a step ahead
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int t = 0; t < S::NT; ++t)
+                acc[t] = mma(widen8<T>(keys.code[t][k / 2][2 * (k % 2)], keys.code[t][k / 2][2 * (k % 2) + 1], 1.f), qk, acc[t]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+
+    // exponents, bad: of the blocks of the lane's runs; unit: binary logarithms per raw product
+    __device__ __forceinline__ void weigh(const typename S::Acc (&acc)[S::NT], const uint32_t (&exponents)[S::RUNS],
+                                          const uint32_t (&bad)[S::RUNS], ValueRegs<D, MT>& values, bool masked, bool last,
+                                          int first_slot, const Sight& sight, int g, float unit) {
+        float x[S::RUNS][16], factor[S::RUNS], vscale[S::RUNS];
+        uint32_t any_bad = 0u;
+#pragma unroll
+        for (int r = 0; r < S::RUNS; ++r) {
+            const int ke = min(max((int)(exponents[r] & 255u), kKv8Low), kKv8High);
+            const int ve = min(max((int)(exponents[r] >> 8 & 255u), kKv8Low), kKv8High);
+            factor[r] = fmaxf(unit * kv8_pow2(ke), 1e-37f);
+            vscale[r] = kv8_pow2(ve);
+            any_bad |= bad[r];
+#pragma unroll
+            for (int v = 0; v < 16; ++v) x[r][v] = MT == 16 ? acc[v / 4 % S::NT][v % 4] : acc[r % S::NT][v % S::ACC];
+        }
+        if (masked) {
+            asm volatile("");                              // a branch, not selections on every page
+#pragma unroll
+            for (int r = 0; r < S::RUNS; ++r) {
+                const uint32_t sees = sight.of_run(first_slot + S::run_slot(r, g));
+#pragma unroll
+                for (int v = 0; v < 16; ++v)
+                    if (!(sees >> v & 1u)) x[r][v] = -__builtin_inff();
+            }
+        }
+        if (__any(any_bad != 0u)) {
+            asm volatile("");
+#pragma unroll
+            for (int r = 0; r < S::RUNS; ++r) {
+                const int j = S::run_slot(r, g);
+                const uint32_t none = bad[r] >> (j & 31) & sight.of_run(first_slot + j) & 0xffffu;
+#pragma unroll
+                for (int v = 0; v < 16; ++v)
+                    if (none >> v & 1u) x[r][v] = __builtin_nanf("");
+            }
+        }
+        if (last) {
+            asm volatile("");
+            // behind the last slot anything may lie, and a weight of 0 does not make it 0
+#pragma unroll
+            for (int r = 0; r < S::RUNS; ++r) {
+                const uint32_t keep = lowest(sight.filled - first_slot - S::run_slot(r, g));
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const uint32_t four = keep >> (4 * w) & 15u;
+                    // bit i to byte i
+                    const uint32_t bytes = ((four * 0x00204081u) & 0x01010101u) * 255u;
+#pragma unroll
+                    for (int t = 0; t < S::CT; ++t) values.code[r][t][w] &= bytes;
+                }
+            }
+        }
+        float best = -__builtin_inff();
+#pragma unroll
+        for (int r = 0; r < S::RUNS; ++r) {
+            float m = x[r][0];
+#pragma unroll
+            for (int v = 1; v < 16; ++v) m = fmaxf(m, x[r][v]);
+            best = fmaxf(best, m * factor[r]);
+        }
+        best = max_over_groups<MT>(best);
+        if (__any(best > top)) {
+            const float now = fmaxf(top, best + kLag), f = fade(top, now);
+            top = now;
+            total *= f;
+#pragma unroll
+            for (int t = 0; t < S::CT; ++t)
+#pragma unroll
+                for (int i = 0; i < S::ACC; ++i) o[t][i] *= f;
+        }
+        const float ref = top == -__builtin_inff() ? 0.f : top;
+        // The weights of eight slots are made while those before multiply the values: between two
+        // matrix instructions stand vector ones, in this order (the fences keep it), so that
+        // neither waits for the other.
+        u32x4 hi[2], lo[2];
+        float even = 0.f;
+        constexpr int kSteps = 2 * S::RUNS;
+        auto make = [&](int u, int i) {
+            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[u / 2][8 * (u % 2) + i], factor[u / 2], -ref));
+            total += e;
+            if (i % 2 == 0) {
+                even = e;
+            } else {
+                const uint32_t h = pack_bf16(even, e);
+                hi[u & 1][i / 2] = h;
+                lo[u & 1][i / 2] = pack_bf16(even - __uint_as_float(h << 16), e - __uint_as_float(h & 0xffff0000u));
+            }
+        };
+#pragma unroll
+        for (int i = 0; i < 8; ++i) make(0, i);
+#pragma unroll
+        for (int u = 0; u < kSteps; ++u) {
+            const bool more = u + 1 < kSteps;
+            constexpr int kFirst = S::CT >= 8 ? 0 : 4 / S::CT;     // weights before a tile's first product,
+            constexpr int kBoth = 8 / S::CT;                       // and before its second
+#pragma unroll
+            for (int t = 0; t < S::CT; ++t) {
+                const u32x4& w = values.code[u / 2][t];
+                const bf16x8 vf = widen8<bf16_t>(w[2 * (u % 2)], w[2 * (u % 2) + 1], vscale[u / 2]);
+#pragma unroll
+                for (int i = t * kBoth; more && i < t * kBoth + kFirst; ++i) make(u + 1, i);
+                __builtin_amdgcn_sched_barrier(0);
+                o[t] = mma(vf, __builtin_bit_cast(bf16x8, hi[u & 1]), o[t]);
+#pragma unroll
+                for (int i = t * kBoth + kFirst; more && i < (t + 1) * kBoth; ++i) make(u + 1, i);
+                __builtin_amdgcn_sched_barrier(0);
+                o[t] = mma(vf, __builtin_bit_cast(bf16x8, lo[u & 1]), o[t]);
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+};
+
+// Four channels of a row's output.
+template <typename T>
+__device__ __forceinline__ void store4(const Kv8AttentionArgs& a, int b, const Row& row, int ch, const float* o, float inv) {
+    if (!row.in_block) return;
+    uint16_t* p = static_cast<uint16_t*>(a.out) + (int64_t)b * a.out_batch + (int64_t)row.t * a.out_token +
+                  (int64_t)row.hq * a.out_head + ch;
+    uint32_t w[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const float x = row.valid ? o[2 * i] * inv : 0.f, y = row.valid ? o[2 * i + 1] * inv : 0.f;
+        w[i] = (uint32_t)round_to<T>(x) | ((uint32_t)round_to<T>(y) << 16);
+    }
+    *reinterpret_cast<u32x2*>(p) = u32x2{w[0], w[1]};
+}
+
+// `ref`: binary logarithm of the unit that `total` counts in.  A sum of 0 is a row that saw
+// nothing (the largest score's weight is at least 2^-kLag, or nearly).
+__device__ __forceinline__ void store_lse8(const Kv8AttentionArgs& a, int b, const Row& row, float ref, float total) {
+    if (!row.in_block) return;
+    const float x = row.valid && total != 0.f ? (ref + __builtin_amdgcn_logf(total)) * 0.693147180559945309f
+                                             : -__builtin_inff();
+    a.lse[((int64_t)b * a.block.T + row.t) * a.q_heads + row.hq] = x;
+}
+
+// Floats of a piece's state in the workspace: outputs as the lanes hold them, then references and sums.
+template <int D, int MT> constexpr int kStateFloats = MT * D + 2 * MT;
+
+// The pages that the rows of a tile group see: [0, sinks) and [from, end) of the sequence's row.
+struct Seen {
+    int sinks, from, end;
+    __device__ int count() const { return sinks + end - from; }
+    __device__ int page(int i) const { return i < sinks ? i : i - sinks + from; }
+};
+
+// The sequences of a call, for the line of their pages: as many as any of their tile groups sees.
+struct Kv8Seqs {
+    const Kv8AttentionArgs& a;
+    int batch, tokens;         // most tokens that the rows of a tile group lie in
+    __device__ Kv8Seqs(const Kv8AttentionArgs& a_, int rows, int group)
+        : a(a_), batch(a_.cache.batch), tokens(divide(rows - 1, group) + 2) {}
+    __device__ int length(int b) const { return paged_length(a.block.lengths, b, a.cache.slots()); }
+    __device__ int count(int b) const { return paged_count(a.block.counts, b, a.block.T); }
+    __device__ int pages(int n, int count) const {
+        const int all = seq_pages(seq_end(a.block, n, count, a.cache.slots()));
+        if (!a.window) return all;
+        const int64_t more = a.block.mode == DELS_KV4_CAUSAL ? min(tokens, count) : a.block.mode == DELS_KV4_NONE ? 0 : count;
+        const int64_t span = (a.window + more + kCachePage - 2) / kCachePage + 1 + (a.sinks + kCachePage - 1) / kCachePage;
+        return (int)min((int64_t)all, span);
+    }
+    // of rows first .. last of the block (tokens)
+    __device__ Seen seen(int n, int count, int first, int last) const {
+        int end = seq_end(a.block, n, count, a.cache.slots());
+        if (a.block.mode == DELS_KV4_CAUSAL) end = (int)min((int64_t)end, (int64_t)n + last + 1);
+        Seen s{0, 0, (end + kCachePage - 1) / kCachePage};
+        if (a.window) {
+            const int64_t start = max((int64_t)n + first - a.window + 1, (int64_t)0);
+            s.from = (int)min(start / kCachePage, (int64_t)s.end);
+            s.sinks = (int)min((a.sinks + kCachePage - 1) / kCachePage, (int64_t)s.from);
+        }
+        return s;
+    }
+};
+
+template <typename T, int D, int MT, int WAYS>
+__global__ __launch_bounds__(kThreads, 2) void kv8_attention_kernel(Kv8AttentionArgs a, Line line, float* states,
+                                                                    unsigned int* counters) {
+    using S = Shape8<D, MT>;
+    using F = typename Frag<T>::type;
+    constexpr int kRegs = S::CT * S::ACC;                   // output registers
+    constexpr int kRound = 32;                              // registers joined at a time
+    __shared__ float s_o[kWaves][kRound][64];
+    __shared__ float s_m[kWaves][MT], s_l[kWaves][MT];
+    constexpr int kTiles = kWaves / WAYS;
+    __shared__ F s_q[kTiles][S::KS][64];
+    __shared__ bool s_last;
+
+    const PagedCache& c = a.cache;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane % MT, g = lane / MT, tile = wave / WAYS, way = wave % WAYS;
+    const int slots = c.slots(), group = a.q_heads / c.heads;
+    // pieces that follow each other on one XCD: they share pages where a head has several row tiles
+    const int piece = (int)gridDim.x % 8 ? (int)blockIdx.x
+                                         : (int)(blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8);
+    const Kv8Seqs seqs(a, kTiles * MT, group);
+    Scan<Kv8Seqs> scan(seqs, c.heads * line.tiles);
+    const Cuts cuts(scan, line, kMostParts);
+    Scan<Kv8Seqs>::Place at{};
+    const int2 mine = cuts.piece(scan, piece, at);
+    int u = mine.x;
+    const int u_end = mine.y;
+    if (u >= u_end) return;
+    // scores in units of the maximum: |scale| and the query's sign
+    const float mag = fabsf(a.scale);
+    const float unit = (mag == 0.f ? 1.f : mag) * kLog2e;
+    const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u, zero = mag == 0.f ? 0u : ~0u;
+
+    while (u < u_end) {
+        if (u >= at.start + at.pages * scan.per) at = scan.place(u);
+        const int b = at.b;
+        const int rel = u - at.start, ht = divide(rel, at.pages), first = rel - ht * at.pages;
+        const int h = divide(ht, line.tiles), rt0 = (ht - h * line.tiles) * kTiles, rt = rt0 + tile;
+        const int last = min(at.pages, first + (u_end - u));
+        const int n = at.n, count = at.count, last_t = a.block.T - 1;
+        // tokens of the tile group, and of this wave's tile
+        const Seen seen = seqs.seen(n, count, divide(rt0 * MT, group), min(divide((rt0 + kTiles) * MT - 1, group), last_t));
+        const int t_first = divide(rt * MT, group), t_last = min(divide(rt * MT + MT - 1, group), last_t);
+        const int stop = rt * MT >= a.block.T * group ? 0 : min(last, seen.count());   // 0: past the block's rows
+        Sight sight;
+        sight.n = n;
+        sight.filled = seq_end(a.block, n, count, slots);     // slots past it may hold anything
+        sight.sinks = a.window ? (int)min(a.sinks, (int64_t)slots) : slots;
+        // slots from `clear` on are seen by no more rows than these bounds say: pages between need no mask
+        const int clear_to = min(sight.filled, a.block.mode == DELS_KV4_CAUSAL ? n + t_first + 1
+                                               : a.block.mode == DELS_KV4_FULL ? n + count : n);
+        const int64_t clear_from = a.window ? (int64_t)n + t_last - a.window + 1 : 0;
+
+        // the wave's pages
+        const int32_t* ids = c.table + (int64_t)b * c.ld_table;
+        const uint8_t* heads = c.data + (int64_t)h * Kv8<D>::kBytes;
+        const int64_t page_stride = (int64_t)c.heads * Kv8<D>::kBytes;
+        int p = first + way;
+        // the numbers of the wave's next 64 pages, one a lane: a load per page would be
+        // waited for with the first read of LDS
+        int ids64, base;
+        auto fetch_ids = [&](int from) {
+            base = from;
+            const int i = from + lane * WAYS;
+            ids64 = i < stop ? ids[seen.page(i)] : -1;
+        };
+        auto id_at = [&](int i) {
+            if (i - base >= 64 * WAYS) fetch_ids(i);
+            return __builtin_amdgcn_readlane(ids64, (i - base) / WAYS);
+        };
+        fetch_ids(p);
+
+        // the queries of all tiles, in operand order: step k of lane group g has channels
+        // 16 (NG (k / 2) + g) + 8 (k % 2) .. + 7
+        constexpr int kPerWave = (kTiles * S::KS + kWaves - 1) / kWaves;
+        u32x4 qw[kPerWave];
+#pragma unroll
+        for (int i = 0; i < kPerWave; ++i) {
+            const int e = wave + i * kWaves, k = e % S::KS;
+            const Row of = row_of((rt0 + e / S::KS) * MT + col, group, h, a.block.T, count);
+            qw[i] = u32x4{0u, 0u, 0u, 0u};
+            if (of.valid && e < kTiles * S::KS)
+                qw[i] = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q.p) + (int64_t)b * a.q.batch +
+                                                        (int64_t)of.t * a.q.token + (int64_t)of.hq * a.q.head +
+                                                        16 * (S::NG * (k / 2) + g) + 8 * (k % 2));
+        }
+        const Row row = row_of(rt * MT + col, group, h, a.block.T, count);
+        Rows8<T, D, MT> rows;
+        sight.bits = 0;
+        sight.lim = sight.lo = 0;
+        if (row.valid) {
+            sight.lim = a.block.mode == DELS_KV4_CAUSAL ? n + row.t + 1 : a.block.mode == DELS_KV4_FULL ? n + count : n;
+            if (a.window) sight.lo = (int)max((int64_t)n + row.t - a.window + 1, (int64_t)0);
+            if (a.block.mode == DELS_KV4_MASK)
+                sight.bits = (uint64_t)a.block.mask[(int64_t)b * a.block.ld_mask + row.t] &
+                             (count >= 64 ? ~0ull : (1ull << count) - 1);
+        }
+        sight.lim = min(sight.lim, sight.filled);
+        rows.top = -__builtin_inff();
+        rows.total = 0.f;
+#pragma unroll
+        for (int t = 0; t < S::CT; ++t)
+#pragma unroll
+            for (int i = 0; i < S::ACC; ++i) rows.o[t][i] = 0.f;
+
+        // Pages p, p + WAYS, ... below `stop`; one that the table does not name is passed over.
+        // Keys of the next page are loaded into their registers once the scores are made, values
+        // once the products are: each is on its way during the other's work.  The loads are
+        // unconditional (of page 0 where there is none to load) and in this order, so that each
+        // wait covers only what it needs.
+        auto named = [&](int id) { return id >= 0 && id < c.num_pages; };
+        auto address = [&](int id) { return heads + (named(id) ? id : 0) * page_stride; };
+        KeyRegs<D, MT> keys;
+        ValueRegs<D, MT> values;
+        int id = id_at(p);
+        if (p < stop) {
+            keys.load(address(id), col, g);
+            values.load(address(id), col, g);
+        }
+#pragma unroll
+        for (int i = 0; i < kPerWave; ++i) {
+            const int e = wave + i * kWaves;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) qw[i][x] = (qw[i][x] ^ flip) & zero;
+            if (e < kTiles * S::KS) s_q[e / S::KS][e % S::KS][lane] = __builtin_bit_cast(F, qw[i]);
+        }
+        lds_barrier();                                        // the loads stay in flight
+        for (; p < stop; p += WAYS) {
+            const int next = id_at(p + WAYS);
+            typename S::Acc acc[S::NT];
+            rows.scores(&s_q[tile][0][lane], keys, acc);
+            uint32_t exponents[S::RUNS], bad[S::RUNS];
+#pragma unroll
+            for (int r = 0; r < S::RUNS; ++r) exponents[r] = keys.exponents[r], bad[r] = keys.bad[r];
+            keys.load(address(next), col, g);
+            asm volatile("" ::: "memory");
+            if (named(id)) {
+                const int slot = seen.page(p) * kCachePage;
+                const bool masked = slot + kCachePage > clear_to || (slot < clear_from && slot + kCachePage > sight.sinks);
+                rows.weigh(acc, exponents, bad, values, masked, slot + kCachePage > sight.filled, slot, sight, g, unit);
+            }
+            values.load(address(next), col, g);
+            asm volatile("" ::: "memory");
+            id = next;
+        }
+
+        // ---- join the waves
+        const float ref = rows.top;
+        const float total = sum_over_groups<MT>(rows.total);
+        if (g == 0) {
+            s_m[wave][col] = ref;
+            s_l[wave][col] = total;
+        }
+        __syncthreads();
+        const bool whole = first == 0 && last == at.pages;
+        // a piece has at most one state of rows that it begins and one of rows that it goes on with
+        auto state_of = [&](int w, bool begins) {
+            return states + ((int64_t)(2 * w + (begins ? 1 : 0)) * kTiles + tile) * kStateFloats<D, MT>;
+        };
+        float* state = state_of(piece, first == 0);
+        float m = -__builtin_inff(), l = 0.f;
+#pragma unroll
+        for (int w = tile * WAYS; w < (tile + 1) * WAYS; ++w) m = fmaxf(m, s_m[w][col]);
+#pragma unroll
+        for (int w = tile * WAYS; w < (tile + 1) * WAYS; ++w) l += s_l[w][col] * fade(s_m[w][col], m);
+        const float f = fade(ref, m), inv = l != 0.f ? 1.f / l : 0.f;
+#pragma unroll
+        for (int r0 = 0; r0 < kRegs; r0 += kRound) {
+#pragma unroll
+            for (int j = 0; j < kRound && r0 + j < kRegs; ++j)
+                s_o[wave][j][lane] = rows.o[(r0 + j) / S::ACC][(r0 + j) % S::ACC] * f;
+            __syncthreads();
+            for (int jq = way; 4 * jq < kRound && r0 + 4 * jq < kRegs; jq += WAYS) {
+                float sum[4];
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                    sum[v] = 0.f;
+#pragma unroll
+                    for (int w = 0; w < WAYS; ++w) sum[v] += s_o[tile * WAYS + w][4 * jq + v][lane];
+                }
+                const int q = r0 / 4 + jq;                    // registers 4 q .. 4 q + 3
+                if (whole) {
+                    store4<T>(a, b, row, S::channel_of(q / (S::ACC / 4), q % (S::ACC / 4), g), sum, inv);
+                } else {
+                    auto* to = reinterpret_cast<unsigned long long*>(state + (q * 64 + lane) * 4);
+#pragma unroll
+                    for (int v = 0; v < 4; v += 2)
+                        atomic_store_u64(to + v / 2, (unsigned long long)__float_as_uint(sum[v + 1]) << 32 |
+                                                         __float_as_uint(sum[v]));
+                }
+            }
+            __syncthreads();
+        }
+        if (way == 0 && g == 0) {
+            if (whole) {
+                store_lse8(a, b, row, m, l);
+            } else {
+                auto* to = reinterpret_cast<unsigned int*>(state + MT * D + col);
+                atomic_store_u32(to, __float_as_uint(m));
+                atomic_store_u32(to + MT, __float_as_uint(l));
+            }
+        }
+        if (!whole) {
+            // The states are written and read with device-coherent stores and loads, and every
+            // store is waited for before the arrival is counted: no cache fences.
+            const int lo = at.start + ht * at.pages;
+            const int2 held = cuts.holders(scan, b, ht, lo, lo + at.pages);
+            __builtin_amdgcn_s_waitcnt(0);
+            asm volatile("" ::: "memory");
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                unsigned int* counter = counters + held.x * kCounterWords;
+                const unsigned prev = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                s_last = prev == (unsigned)(held.y - held.x) - 1u;
+                if (s_last) __hip_atomic_exchange(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+            __syncthreads();
+            if (s_last) {
+                auto load = [&](const float* p) {
+                    return __uint_as_float(__hip_atomic_load(reinterpret_cast<const unsigned int*>(p), __ATOMIC_RELAXED,
+                                                             __HIP_MEMORY_SCOPE_AGENT));
+                };
+                constexpr int kMine = (kRegs / 4 + WAYS - 1) / WAYS;
+                float sum[kMine][4];
+#pragma unroll
+                for (int i = 0; i < kMine; ++i)
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) sum[i][v] = 0.f;
+                m = -__builtin_inff(), l = 0.f;
+                constexpr int kFlight = WAYS;                 // states in flight: their loads go to memory
+                for (int w0 = held.x; w0 < held.y; w0 += kFlight) {
+                    float tops[kFlight], sums[kFlight];
+                    unsigned long long two[kFlight][kMine][2];
+#pragma unroll
+                    for (int e = 0; e < kFlight; ++e) {
+                        const int w = min(w0 + e, held.y - 1);
+                        const float* st = state_of(w, w == held.x);
+                        tops[e] = load(st + MT * D + col);
+                        sums[e] = load(st + MT * D + MT + col);
+#pragma unroll
+                        for (int i = 0; i < kMine; ++i) {
+                            const int q = min(way + i * WAYS, kRegs / 4 - 1);
+                            auto* from = reinterpret_cast<unsigned long long*>(const_cast<float*>(st + (q * 64 + lane) * 4));
+#pragma unroll
+                            for (int v = 0; v < 2; ++v) two[e][i][v] = atomic_load_u64(from + v);
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < kFlight; ++e) {
+                        if (w0 + e >= held.y) break;
+                        const float now = fmaxf(m, tops[e]), old = fade(m, now), f = fade(tops[e], now);
+                        m = now;
+                        l = l * old + sums[e] * f;
+#pragma unroll
+                        for (int i = 0; i < kMine; ++i)
+#pragma unroll
+                            for (int v = 0; v < 4; ++v)
+                                sum[i][v] = sum[i][v] * old +
+                                            __uint_as_float((uint32_t)(two[e][i][v / 2] >> (32 * (v & 1)))) * f;
+                    }
+                }
+                const float inv = l != 0.f ? 1.f / l : 0.f;
+#pragma unroll
+                for (int i = 0; i < kMine; ++i) {
+                    const int q = way + i * WAYS;
+                    if (q < kRegs / 4)
+                        store4<T>(a, b, row, S::channel_of(q / (S::ACC / 4), q % (S::ACC / 4), g), sum[i], inv);
+                }
+                if (way == 0 && g == 0) store_lse8(a, b, row, m, l);
+            }
+        }
+        u += last - first;
+    }
+}
+
+struct Plan { int rows, ways; Line line; };
+
+Plan plan(int64_t batch, int64_t T, int64_t q_heads, int64_t heads, int64_t max_pages) {
+    Plan p{};
+    const int64_t rows = T * (q_heads / heads);
+    p.rows = rows <= 16 ? 16 : 32;
+    const int64_t tiles = (rows + p.rows - 1) / p.rows, cus = device_cu_count();
+    const int64_t fours = (tiles + 3) / 4;
+    p.ways = p.rows == 32 && batch * heads * fours >= cus && 8 * tiles >= 7 * 4 * fours ? 2 : 8;
+    const int per = kWaves / p.ways;
+    p.line.tiles = (int)((tiles + per - 1) / per);
+    p.line.least = kMinPages;
+    const int64_t units = batch * heads * p.line.tiles * std::max<int64_t>(max_pages, 1);
+    p.line.pieces = (int)std::min<int64_t>({cus, kMaxCounters / kCounterWords,
+                                            std::max(batch * heads * p.line.tiles, (units + kMinPages - 1) / kMinPages)});
+    return p;
+}
+
+}  // namespace
+
+size_t kv8_attention_data_bytes(int64_t batch, int64_t T, int64_t q_heads, int64_t heads, int64_t head_dim,
+                                int64_t max_pages) {
+    const Plan p = plan(batch, T, q_heads, heads, max_pages);
+    // four tiles a piece where this or a shorter block has them, so that a workspace for the
+    // longest block serves every shorter one
+    const int64_t tiles = (T * (q_heads / heads) + p.rows - 1) / p.rows;
+    const bool four = p.ways == 2 || (p.rows == 32 && batch * heads * (tiles / 4) >= device_cu_count());
+    return align256((size_t)p.line.pieces * 2 * (four ? 4 : 1) * sizeof(float) * (p.rows * head_dim + 2 * p.rows));
+}
+
+hipError_t launch_kv8_attention(const Kv8AttentionArgs& a, void* ws, size_t data_off, hipStream_t s) {
+    const PagedCache& c = a.cache;
+    const Plan p = plan(c.batch, a.block.T, a.q_heads, c.heads, c.max_pages);
+    auto* states = reinterpret_cast<float*>(static_cast<char*>(ws) + data_off);
+    auto* counters = reinterpret_cast<unsigned int*>(static_cast<char*>(ws) + kCountersOff);
+    auto by_size = [&](auto tag, auto size) {
+        using T = decltype(tag);
+        constexpr int D = decltype(size)::value;
+        auto go = [&](auto rows, auto ways) {
+            hipLaunchKernelGGL((kv8_attention_kernel<T, D, decltype(rows)::value, decltype(ways)::value>),
+                               dim3(p.line.pieces), dim3(kThreads), 0, s, a, p.line, states, counters);
+        };
+        using std::integral_constant;
+        if (p.rows == 16) go(integral_constant<int, 16>{}, integral_constant<int, 8>{});
+        else if (p.ways == 8) go(integral_constant<int, 32>{}, integral_constant<int, 8>{});
+        else go(integral_constant<int, 32>{}, integral_constant<int, 2>{});
+    };
+    auto by_type = [&](auto tag) {
+        if (c.head_dim == 64) by_size(tag, std::integral_constant<int, 64>{});
+        else by_size(tag, std::integral_constant<int, 128>{});
+    };
+    if (a.dtype == DELS_DTYPE_BF16) by_type(bf16_t{});
+    else by_type(f16_t{});
+    return hipGetLastError();
+}
+
+}  // namespace dels

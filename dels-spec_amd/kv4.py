@@ -53,8 +53,8 @@ def _row_stride(t: torch.Tensor, columns: int, name: str) -> int:
     return stride
 
 
-class KV4Cache:
-    """Pages of a 4-bit key/value cache and the table that hands them out.
+class PagedCache:
+    """Pages of a key/value cache and the table that hands them out; a class a format.
 
     ``data`` uint8 ``[num_pages, kv_heads, page_bytes(head_dim)]``, contiguous;
     ``block_table`` int32 ``[batch, max_pages]``, unit column stride: slot ``j`` of
@@ -64,12 +64,19 @@ class KV4Cache:
     tensors; a table can be rewritten in place.
     """
 
+    bits: int              # of a key or value
+
+    @staticmethod
+    def page_bytes(head_dim: int) -> int:
+        """Bytes of one key/value head's page of 64 slots."""
+        raise NotImplementedError
+
     def __init__(self, data: torch.Tensor, block_table: torch.Tensor, head_dim: int):
         _require_cuda(data, "data")
         _require_cuda(block_table, "block_table")
-        if data.dtype != torch.uint8 or data.dim() != 3 or data.shape[2] != page_bytes(head_dim):
-            raise ValueError(f"data must be uint8 [num_pages, kv_heads, {page_bytes(head_dim)}], got {data.dtype} "
-                             f"{tuple(data.shape)}")
+        if data.dtype != torch.uint8 or data.dim() != 3 or data.shape[2] != self.page_bytes(head_dim):
+            raise ValueError(f"data must be uint8 [num_pages, kv_heads, {self.page_bytes(head_dim)}], got "
+                             f"{data.dtype} {tuple(data.shape)}")
         if data.shape[1] < 1:
             raise ValueError("data must have one key/value head at least")
         if not data.is_contiguous():
@@ -97,21 +104,34 @@ class KV4Cache:
         self._ref = ctypes.byref(self._params)
 
     @classmethod
-    def allocate(cls, batch: int, max_len: int, kv_heads: int, head_dim: int, device) -> "KV4Cache":
+    def allocate(cls, batch: int, max_len: int, kv_heads: int, head_dim: int, device) -> "PagedCache":
         """An empty cache in which every sequence owns the pages of ``max_len`` slots."""
         pages = -(-max_len // PAGE)
-        data = torch.zeros(batch * pages, kv_heads, page_bytes(head_dim), dtype=torch.uint8, device=device)
+        data = torch.zeros(batch * pages, kv_heads, cls.page_bytes(head_dim), dtype=torch.uint8, device=device)
         table = torch.arange(batch * pages, dtype=torch.int32, device=device).view(batch, pages)
         return cls(data, table, head_dim)
 
 
-def _elsewhere(t, cache: KV4Cache, name: str) -> None:
+class KV4Cache(PagedCache):
+    """Pages of a 4-bit key/value cache and the table that hands them out (``PagedCache`` says how)."""
+
+    bits = 4
+    page_bytes = staticmethod(page_bytes)
+
+
+def _require_cache(cache: PagedCache, bits: int) -> None:
+    """Refuse a cache of the other format: its pages have another size."""
+    if cache.bits != bits:
+        raise TypeError(f"cache holds {cache.bits} bits a value, the call is for {bits}")
+
+
+def _elsewhere(t, cache: PagedCache, name: str) -> None:
     """Raise for a tensor that is not on the cache's GPU."""
     _require_cuda(t, name)
     raise ValueError(f"{name} is on {t.device}, the cache on {cache.device}")
 
 
-def _require_ints(t: Optional[torch.Tensor], cache: KV4Cache, name: str) -> Optional[int]:
+def _require_ints(t: Optional[torch.Tensor], cache: PagedCache, name: str) -> Optional[int]:
     """Pointer of an int32 [batch] device array (None where there is none)."""
     if t is None:
         return None
@@ -124,7 +144,7 @@ def _require_ints(t: Optional[torch.Tensor], cache: KV4Cache, name: str) -> Opti
     return t.data_ptr()
 
 
-def _require_rows(t: torch.Tensor, cache: KV4Cache, heads: Optional[int], name: str, dtypes) -> tuple[int, int, int, int]:
+def _require_rows(t: torch.Tensor, cache: PagedCache, heads: Optional[int], name: str, dtypes) -> tuple[int, int, int, int]:
     """(pointer, strides) of a [batch, T, heads, head_dim] tensor with unit channel stride."""
     if not isinstance(t, torch.Tensor) or t.get_device() != cache._index:
         _elsewhere(t, cache, name)
@@ -146,7 +166,7 @@ def _require_rows(t: torch.Tensor, cache: KV4Cache, heads: Optional[int], name: 
 _capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
 
 
-def _own_workspace(given: Optional[torch.Tensor], cache: KV4Cache, need: int, *, counters: bool) -> torch.Tensor:
+def _own_workspace(given: Optional[torch.Tensor], cache: PagedCache, need: int, *, counters: bool) -> torch.Tensor:
     """The caller's workspace, or else a captured call's own.
 
     The stream's shared one may be replaced by a larger one between a graph's replays, its
@@ -176,6 +196,7 @@ def kv4_append(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, lengths: torch
     keep rows 16-byte aligned.  ``lengths`` is not changed; rows past the table's
     slots are dropped.
     """
+    _require_cache(cache, 4)
     kp = _require_rows(k, cache, cache.kv_heads, "k", _DTYPES)
     vp = _require_rows(v, cache, cache.kv_heads, "v", _DTYPES)
     if v.dtype != k.dtype or v.shape != k.shape:
@@ -193,6 +214,7 @@ def kv4_read(cache: KV4Cache, starts: torch.Tensor, T: int, *, counts: Optional[
     Returns ``(k, v)``, each ``[batch, T, kv_heads, head_dim]`` of ``dtype``; zeros from
     ``counts[b]`` on (None: none) and past the table's slots.
     """
+    _require_cache(cache, 4)
     if dtype not in _DTYPES:
         raise TypeError(f"dtype {dtype} not supported")
     sp, cp = _require_ints(starts, cache, "starts"), _require_ints(counts, cache, "counts")
@@ -207,7 +229,7 @@ def kv4_read(cache: KV4Cache, starts: torch.Tensor, T: int, *, counts: Optional[
 Block = Union[str, torch.Tensor]
 
 
-def _block_args(block: Block, cache: KV4Cache, T: int) -> tuple[int, Optional[int], int]:
+def _block_args(block: Block, cache: PagedCache, T: int) -> tuple[int, Optional[int], int]:
     """(mode, mask pointer, mask row stride)."""
     if isinstance(block, torch.Tensor):
         if block.get_device() != cache._index:
@@ -240,6 +262,7 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, lengths: torch.Tensor, *, bl
     logarithm of each softmax's sum; rows that see nothing give 0 and -inf, rows that see
     a score of NaN or +inf NaN in both.
     """
+    _require_cache(cache, 4)
     qp = _require_rows(q, cache, None, "q", _Q_DTYPES)
     batch, T, q_heads, D = q.shape
     if q_heads % cache.kv_heads:
@@ -274,7 +297,7 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, lengths: torch.Tensor, *, bl
     return out, lse
 
 
-def _require_lse(lse: torch.Tensor, cache: KV4Cache, T: int, q_heads: int) -> None:
+def _require_lse(lse: torch.Tensor, cache: PagedCache, T: int, q_heads: int) -> None:
     if not isinstance(lse, torch.Tensor) or lse.get_device() != cache._index:
         _elsewhere(lse, cache, "lse")
     if lse.dtype != torch.float32 or lse.shape != (cache.batch, T, q_heads) or not lse.is_contiguous():
@@ -302,6 +325,7 @@ def kv4_weights(q: torch.Tensor, cache: KV4Cache, lengths: torch.Tensor, lse: to
     valid rows) summed over the query heads of each cache head; the block's own slots
     start from 0, and slots past the block are 0.  ``out`` may be ``weights``.
     """
+    _require_cache(cache, 4)
     qp = _require_rows(q, cache, None, "q", _Q_DTYPES)
     batch, T, q_heads, D = q.shape
     if q_heads % cache.kv_heads:
@@ -340,6 +364,7 @@ def kv4_evict(cache: KV4Cache, lengths: torch.Tensor, weights: torch.Tensor, kee
     which whatever else is kept per slot follows.  Slots of a table entry that names no
     page hold nothing, so none of them stays or moves, and as places they take nothing.
     """
+    _require_cache(cache, 4)
     lp = _require_ints(lengths, cache, "lengths")
     _require_weights(weights, cache, "weights")
     if keep < 1 or recent < 0:

@@ -657,6 +657,84 @@ size_t dels_kv4_evict_ws_bytes(int64_t batch, int64_t kv_heads, int64_t keep);
 int dels_kv4_evict(const dels_kv4_cache* c, const int32_t* lengths, const float* weights, int64_t keep, int64_t recent,
                    int32_t* out_lengths, float* out_weights, int32_t* source, void* ws, size_t ws_bytes, void* stream);
 
+/* ---- key/value cache held in 8 bits -------------------------------------------
+ *
+ * The same for whom four bits are too few, and with the position rotation on the way into
+ * the cache.  Pages of 64 slots of one key/value head, two blocks u of 32 slots; D = 64 or
+ * 128 channels.  A page of 128 D + 128 bytes holds
+ *   keys    e4m3, channel 16 c + i of slot s of block u at byte 32 D u + 512 c + 16 pos(s) + i,
+ *           pos(s) = 8 (s % 16 / 4) + 4 (s / 16) + s % 4;
+ *   values  e4m3, channel c of slot 16 h + i of block u at byte 64 D + 32 D u + 16 D h + 16 c + i;
+ *   for each block, from byte 128 D on, 8 bytes: the exponents e of its keys and of its values
+ *           (2^(e - 127)), two of 0, and a little-endian word with the bits of the slots whose row
+ *           was not finite;
+ *   112 bytes of nothing.
+ * Numbers are rounded to nearest, ties to even.  An exponent is the smallest of 63 .. 191 whose
+ * 448-fold holds the largest magnitude of the rows that a call writes into the block, or that
+ * of the rows which the block keeps (those before lengths[b]), if there are any and it is larger;
+ * if it is smaller, they are rounded once more.  A row of which a key or value is NaN, infinite
+ * or over 448 * 2^64 in magnitude is not held: it reads as NaN, its scores are NaN, and
+ * it takes no part in the exponents.  A call that writes a block's first row writes the
+ * whole block's values (0 behind its rows).
+ *
+ * The table, its entries, lengths and counts are as for the 4-bit cache; so is the struct.
+ * No two sequences may write into one block.
+ */
+typedef dels_kv4_cache dels_kv8_cache;
+
+/* Angles of positions 0 .. positions - 1: fp32 rows of channels / 2 cosines and sines, row
+ * stride ld, 16-byte aligned rows; channels a multiple of 16, at most D.  Pair i is
+ * channels i and i + channels / 2, or 2 i and 2 i + 1 where interleaved is not 0. */
+typedef struct dels_rotary {
+    const float* cos;
+    const float* sin;
+    int64_t ld;
+    int64_t positions;
+    int64_t channels;
+    int interleaved;
+} dels_rotary;
+
+/* Bytes of a page of one head (0 for a head size that is not supported). */
+size_t dels_kv8_page_bytes(int64_t head_dim);
+
+/*
+ * Rows t < counts[b] (NULL: T) of k and v [batch, T, kv_heads, D] into slots lengths[b] + t;
+ * rows past the table's slots are dropped.  Strides in elements, unit channel stride,
+ * 16-byte aligned rows.  dtype DELS_DTYPE_*.
+ *   rotary (NULL: none) rotates the keys, and q [batch, T, q_heads, D] (NULL: none) of the same
+ *     dtype into q_out (rows from counts[b] on 0; q_out may be q with its strides): (a, b) becomes
+ *     (a c - b s, b c + a s), each product, sum and difference rounded to fp32, q then to dtype.
+ *   positions [batch, ld_positions >= T, or 0 for one row that all sequences read] (NULL:
+ *     lengths[b] + t); a position that the table does not have makes the row NaN.
+ */
+int dels_kv8_append(const dels_kv8_cache* c, const void* k, int64_t k_batch, int64_t k_token, int64_t k_head,
+                    const void* v, int64_t v_batch, int64_t v_token, int64_t v_head, int dtype,
+                    const int32_t* lengths, const int32_t* counts, int64_t T, const dels_rotary* rotary,
+                    const int32_t* positions, int64_t ld_positions, const void* q, int64_t q_batch, int64_t q_token,
+                    int64_t q_head, int64_t q_heads, void* q_out, int64_t out_batch, int64_t out_token,
+                    int64_t out_head, void* stream);
+
+/*
+ * The values that slots starts[b] + t, t < counts[b] (NULL: T), stand for, into
+ * contiguous k and v [batch, T, kv_heads, D] of `dtype`; 0 from counts[b] on and past the
+ * table's slots, NaN for rows that were not finite.
+ */
+int dels_kv8_read(const dels_kv8_cache* c, const int32_t* starts, const int32_t* counts, int64_t T, void* k, void* v,
+                  int dtype, void* stream);
+
+/*
+ * Attention of a block's rows over the cache, as dels_kv4_attention, q bf16 or fp16.  With a
+ * window (0: none), row t sees of the slots that it would see otherwise those from
+ * lengths[b] + t - window + 1 on and those below `sinks`; pages that no row sees are not read.
+ */
+size_t dels_kv8_attention_ws_bytes(int64_t batch, int64_t T, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                                   int64_t max_pages);
+int dels_kv8_attention(const dels_kv8_cache* c, const void* q, int64_t q_batch, int64_t q_token, int64_t q_head,
+                       int dtype, int64_t q_heads, int64_t T, const int32_t* lengths, const int32_t* counts,
+                       int block, const int64_t* mask, int64_t ld_mask, float scale, int64_t window, int64_t sinks,
+                       void* out, int64_t out_batch, int64_t out_token, int64_t out_head, float* lse, void* ws,
+                       size_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -11,3 +11,4 @@ from . import sampling  # noqa: F401
 from . import domino  # noqa: F401
 from . import bounds  # noqa: F401
 from . import kv4  # noqa: F401
+from . import kv8  # noqa: F401
