@@ -15,8 +15,9 @@
 // the conversion instruction, exactly; a block's key scale joins the factor of its
 // scores, its value scale is applied by the conversion.  Both products are 16-bit ones: the
 // 8-bit matrix instructions add products at 2^-12 of the largest of a group (measured),
-// which a float32 lse would show.  Weights enter as two bf16 parts (2^-17 of each, whatever its
-// size).  Scores, maxima, sums and outputs are fp32.
+// which a float32 lse would show.  Weights enter as f16 numbers (2^-11 of each, an eighth of half a
+// step of a bf16 output), for f16 outputs in two parts.  Scores, maxima, sums and outputs are
+// fp32.
 #include <algorithm>
 
 #include "kv8.h"
@@ -30,23 +31,33 @@ constexpr int kWaves = kLineWaves, kThreads = 64 * kWaves;
 // when it moves, and moves when a score passes it: until then the outputs need no rescaling
 // and no weight is above 1.
 constexpr float kLag = 8.f;
+// Weights enter the second product as f16 numbers of up to 2^kLift (below 2^-14 their steps
+// are 2^-24, so a weight 2^-31 of the largest still counts), values as f16 numbers of up to 448 * 2^7: a
+// block's scale is relative to the largest of the blocks so far, with kHead binary orders to spare
+// when it moves.  Once the scales of a wave's blocks lie more than kSpan orders apart, neither
+// small values nor small weights of large ones are safe there, and further products are of bf16
+// numbers, whose range knows no such bounds, with weights in two parts.
+constexpr float kLift = 15.f;
+constexpr int kHead = 2, kSpan = 12;
 constexpr int kMinPages = 2 * kWaves;  // fewest pages of a part
 // Most parts of one tile group: their states are joined by one workgroup.
 constexpr int kMostParts = 32;
 
-// Shapes of a wave's work on MT rows: MT x MT tiles of the matrix instructions.
+// Shapes of a wave's work on MT rows: MT x MT tiles of the matrix instructions.  A step is
+// 32 * 32 / MT slots, so that a lane has scores of 16 consecutive slots: a page's two blocks at
+// once for 16 rows, one after the other for 32.
 template <int D, int MT_> struct Shape8 {
     static constexpr int MT = MT_;
     static constexpr int NG = 64 / MT;              // lane groups: lane = MT * group + row
-    static constexpr int KS = D / NG / 8;           // steps of the first product: 8 channels a lane
+    static constexpr int KS = D / NG / 8;           // steps of the first product's contraction: 8 channels a lane
     static constexpr int KL = KS / 2;               // loads of a key tile: 16 channels a lane
-    static constexpr int NT = 64 / MT;              // key tiles of a page
+    static constexpr int STEPS = MT / 16;           // steps of a page
+    static constexpr int NT = 64 / MT / STEPS;      // key tiles of a step
     static constexpr int ACC = MT == 16 ? 4 : 16;   // accumulator registers of a tile
-    static constexpr int RUNS = MT / 16;            // runs of 16 consecutive slots that a lane has scores of
     static constexpr int CT = D / MT;               // channel tiles of the output
     using Acc = typename std::conditional<MT == 16, f32x4, f32x16>::type;
-    // first slot of a lane group's run within the page, and its block
-    __device__ static int run_slot(int run, int g) { return MT == 16 ? 16 * g : 32 * run + 16 * g; }
+    // first slot of a lane group's run in a step, within the page
+    __device__ static int run_slot(int step, int g) { return MT == 16 ? 16 * g : 32 * step + 16 * g; }
     // first of the four channels of registers 4 j .. 4 j + 3 of channel tile `t`
     __device__ static int channel_of(int t, int j, int g) { return MT * t + (MT == 16 ? 4 * g : 8 * j + 4 * g); }
 };
@@ -69,39 +80,40 @@ __device__ __forceinline__ typename Frag<T>::type widen8(uint32_t lo, uint32_t h
     }
 }
 
+// Two numbers rounded to a 16-bit type, the first in the low half, and a half widened again.
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    if constexpr (std::is_same<T, bf16_t>::value) return pack_bf16(a, b);
+    else return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), f16x2));
+}
+
 // The lowest k of 16 bits.
 __device__ __forceinline__ uint32_t lowest(int k) { return (1u << min(max(k, 0), 16)) - 1u; }
 
 template <int D, int MT> struct KeyRegs {
     using S = Shape8<D, MT>;
-    u32x4 code[S::NT][S::KL];
-    uint32_t exponents[S::RUNS], bad[S::RUNS];
-    __device__ __forceinline__ void load(const uint8_t* page, int col, int g) {
+    u32x4 code[S::STEPS][S::NT][S::KL];
+    u32x2 head[S::STEPS];
+    __device__ __forceinline__ void load(const uint8_t* page, int col, int g, int step) {
         const int lane = MT == 16 ? 32 * D * (col >> 3) + 512 * g + 16 * (col & 7) : 512 * g + 16 * col;
 #pragma unroll
         for (int t = 0; t < S::NT; ++t)
 #pragma unroll
             for (int i = 0; i < S::KL; ++i)
-                code[t][i] = *reinterpret_cast<const u32x4*>(page + lane + 512 * S::NG * i + (MT == 16 ? 128 : 32 * D) * t);
-#pragma unroll
-        for (int r = 0; r < S::RUNS; ++r) {
-            const auto w = *reinterpret_cast<const u32x2*>(page + Kv8<D>::kHead + 8 * (MT == 16 ? g / 2 : r));
-            exponents[r] = w[0];
-            bad[r] = w[1];
-        }
+                code[step][t][i] =
+                    *reinterpret_cast<const u32x4*>(page + lane + 512 * S::NG * i + (MT == 16 ? 128 * t : 32 * D * step));
+        head[step] = *reinterpret_cast<const u32x2*>(page + Kv8<D>::kHead + 8 * (MT == 16 ? g / 2 : step));
     }
 };
 
 template <int D, int MT> struct ValueRegs {
     using S = Shape8<D, MT>;
-    u32x4 code[S::RUNS][S::CT];
-    __device__ __forceinline__ void load(const uint8_t* page, int col, int g) {
+    u32x4 code[S::STEPS][S::CT];
+    __device__ __forceinline__ void load(const uint8_t* page, int col, int g, int step) {
         const int lane = Kv8<D>::kValue + 16 * D * g + 16 * col;
 #pragma unroll
-        for (int r = 0; r < S::RUNS; ++r)
-#pragma unroll
-            for (int t = 0; t < S::CT; ++t)
-                code[r][t] = *reinterpret_cast<const u32x4*>(page + lane + 32 * D * r + 16 * MT * t);
+        for (int t = 0; t < S::CT; ++t)
+            code[step][t] = *reinterpret_cast<const u32x4*>(page + lane + 32 * D * step + 16 * MT * t);
     }
 };
 
@@ -119,15 +131,34 @@ struct Sight {
     }
 };
 
-// The rows' state of a wave, and one page's part in it.
+// The rows' state of a wave, and one step's part in it.
 template <typename T, int D, int MT> struct Rows8 {
     using S = Shape8<D, MT>;
     using F = typename Frag<T>::type;
-    typename S::Acc o[S::CT];
+    typename S::Acc o[S::CT];  // in units of 2^(vref - 134) times that of the weights
     float top, total;          // what weights are relative to (binary logarithm) and this lane's part of their sum
+    int vref, vlow;            // exponent of values that the outputs are relative to; least of the blocks so far
 
-    // scores of a page; q: this lane's operands of the queries in LDS, 64 apart
-    __device__ __forceinline__ void scores(const F* q, const KeyRegs<D, MT>& keys, typename S::Acc (&acc)[S::NT]) {
+    __device__ __forceinline__ void clear() {
+        top = -__builtin_inff();
+        total = 0.f;
+        vref = 0;
+        vlow = 255;
+#pragma unroll
+        for (int t = 0; t < S::CT; ++t)
+#pragma unroll
+            for (int i = 0; i < S::ACC; ++i) o[t][i] = 0.f;
+    }
+
+    __device__ __forceinline__ void rescale(float f) {
+#pragma unroll
+        for (int t = 0; t < S::CT; ++t)
+#pragma unroll
+            for (int i = 0; i < S::ACC; ++i) o[t][i] *= f;
+    }
+
+    // scores of a step; q: this lane's operands of the queries in LDS, 64 apart
+    __device__ __forceinline__ void scores(const F* q, const u32x4 (&code)[S::NT][S::KL], typename S::Acc (&acc)[S::NT]) {
 #pragma unroll
         for (int t = 0; t < S::NT; ++t)
 #pragma unroll
@@ -140,122 +171,119 @@ template <typename T, int D, int MT> struct Rows8 {
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int t = 0; t < S::NT; ++t)
-                acc[t] = mma(widen8<T>(keys.code[t][k / 2][2 * (k % 2)], keys.code[t][k / 2][2 * (k % 2) + 1], 1.f), qk, acc[t]);
+                acc[t] = mma(widen8<T>(code[t][k / 2][2 * (k % 2)], code[t][k / 2][2 * (k % 2) + 1], 1.f), qk, acc[t]);
         }
         __builtin_amdgcn_sched_barrier(0);
     }
 
-    // exponents, bad: of the blocks of the lane's runs; unit: binary logarithms per raw product
-    __device__ __forceinline__ void weigh(const typename S::Acc (&acc)[S::NT], const uint32_t (&exponents)[S::RUNS],
-                                          const uint32_t (&bad)[S::RUNS], ValueRegs<D, MT>& values, bool masked, bool last,
-                                          int first_slot, const Sight& sight, int g, float unit) {
-        float x[S::RUNS][16], factor[S::RUNS], vscale[S::RUNS];
-        uint32_t any_bad = 0u;
-#pragma unroll
-        for (int r = 0; r < S::RUNS; ++r) {
-            const int ke = min(max((int)(exponents[r] & 255u), kKv8Low), kKv8High);
-            const int ve = min(max((int)(exponents[r] >> 8 & 255u), kKv8Low), kKv8High);
-            factor[r] = fmaxf(unit * kv8_pow2(ke), 1e-37f);
-            vscale[r] = kv8_pow2(ve);
-            any_bad |= bad[r];
-#pragma unroll
-            for (int v = 0; v < 16; ++v) x[r][v] = MT == 16 ? acc[v / 4 % S::NT][v % 4] : acc[r % S::NT][v % S::ACC];
-        }
-        if (masked) {
-            asm volatile("");                              // a branch, not selections on every page
-#pragma unroll
-            for (int r = 0; r < S::RUNS; ++r) {
-                const uint32_t sees = sight.of_run(first_slot + S::run_slot(r, g));
-#pragma unroll
-                for (int v = 0; v < 16; ++v)
-                    if (!(sees >> v & 1u)) x[r][v] = -__builtin_inff();
-            }
-        }
-        if (__any(any_bad != 0u)) {
-            asm volatile("");
-#pragma unroll
-            for (int r = 0; r < S::RUNS; ++r) {
-                const int j = S::run_slot(r, g);
-                const uint32_t none = bad[r] >> (j & 31) & sight.of_run(first_slot + j) & 0xffffu;
-#pragma unroll
-                for (int v = 0; v < 16; ++v)
-                    if (none >> v & 1u) x[r][v] = __builtin_nanf("");
-            }
-        }
-        if (last) {
-            asm volatile("");
-            // behind the last slot anything may lie, and a weight of 0 does not make it 0
-#pragma unroll
-            for (int r = 0; r < S::RUNS; ++r) {
-                const uint32_t keep = lowest(sight.filled - first_slot - S::run_slot(r, g));
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const uint32_t four = keep >> (4 * w) & 15u;
-                    // bit i to byte i
-                    const uint32_t bytes = ((four * 0x00204081u) & 0x01010101u) * 255u;
-#pragma unroll
-                    for (int t = 0; t < S::CT; ++t) values.code[r][t][w] &= bytes;
-                }
-            }
-        }
-        float best = -__builtin_inff();
-#pragma unroll
-        for (int r = 0; r < S::RUNS; ++r) {
-            float m = x[r][0];
-#pragma unroll
-            for (int v = 1; v < 16; ++v) m = fmaxf(m, x[r][v]);
-            best = fmaxf(best, m * factor[r]);
-        }
-        best = max_over_groups<MT>(best);
-        if (__any(best > top)) {
-            const float now = fmaxf(top, best + kLag), f = fade(top, now);
-            top = now;
-            total *= f;
-#pragma unroll
-            for (int t = 0; t < S::CT; ++t)
-#pragma unroll
-                for (int i = 0; i < S::ACC; ++i) o[t][i] *= f;
-        }
-        const float ref = top == -__builtin_inff() ? 0.f : top;
+    // Adds weights times values; x: scores, their binary logarithms are x * factor - ref.
+    // P: type and number of parts of a weight.
+    template <typename P, int PARTS>
+    __device__ __forceinline__ void multiply(const float (&x)[16], float factor, float ref, const u32x4 (&code)[S::CT],
+                                             float vscale) {
+        using V = typename Frag<P>::type;
         // The weights of eight slots are made while those before multiply the values: between two
         // matrix instructions stand vector ones, in this order (the fences keep it), so that
         // neither waits for the other.
-        u32x4 hi[2], lo[2];
+        u32x4 part[PARTS][2];
         float even = 0.f;
-        constexpr int kSteps = 2 * S::RUNS;
         auto make = [&](int u, int i) {
-            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[u / 2][8 * (u % 2) + i], factor[u / 2], -ref));
+            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * u + i], factor, -ref));
             total += e;
             if (i % 2 == 0) {
                 even = e;
             } else {
-                const uint32_t h = pack_bf16(even, e);
-                hi[u & 1][i / 2] = h;
-                lo[u & 1][i / 2] = pack_bf16(even - __uint_as_float(h << 16), e - __uint_as_float(h & 0xffff0000u));
+                const uint32_t h = pack2<P>(even, e);
+                part[0][u][i / 2] = h;
+                if constexpr (PARTS == 2)
+                    part[1][u][i / 2] = pack2<P>(even - widen_raw<P>(h & 0xffffu), e - widen_raw<P>(h >> 16));
             }
         };
 #pragma unroll
         for (int i = 0; i < 8; ++i) make(0, i);
+        constexpr int kEach = 8 / S::CT;                       // weights for the next half by channel tile
 #pragma unroll
-        for (int u = 0; u < kSteps; ++u) {
-            const bool more = u + 1 < kSteps;
-            constexpr int kFirst = S::CT >= 8 ? 0 : 4 / S::CT;     // weights before a tile's first product,
-            constexpr int kBoth = 8 / S::CT;                       // and before its second
+        for (int u = 0; u < 2; ++u) {
 #pragma unroll
             for (int t = 0; t < S::CT; ++t) {
-                const u32x4& w = values.code[u / 2][t];
-                const bf16x8 vf = widen8<bf16_t>(w[2 * (u % 2)], w[2 * (u % 2) + 1], vscale[u / 2]);
+                const V vf = widen8<P>(code[t][2 * u], code[t][2 * u + 1], vscale);
 #pragma unroll
-                for (int i = t * kBoth; more && i < t * kBoth + kFirst; ++i) make(u + 1, i);
+                for (int i = t * kEach; u == 0 && i < (t + 1) * kEach; ++i) make(1, i);
                 __builtin_amdgcn_sched_barrier(0);
-                o[t] = mma(vf, __builtin_bit_cast(bf16x8, hi[u & 1]), o[t]);
 #pragma unroll
-                for (int i = t * kBoth + kFirst; more && i < (t + 1) * kBoth; ++i) make(u + 1, i);
-                __builtin_amdgcn_sched_barrier(0);
-                o[t] = mma(vf, __builtin_bit_cast(bf16x8, lo[u & 1]), o[t]);
+                for (int p = 0; p < PARTS; ++p) o[t] = mma(vf, __builtin_bit_cast(V, part[p][u]), o[t]);
             }
         }
         __builtin_amdgcn_sched_barrier(0);
+    }
+
+    // head: of the block of the lane's run; unit: binary logarithms per raw product; none: the
+    // page is no page
+    __device__ __forceinline__ void weigh(const typename S::Acc (&acc)[S::NT], u32x2 head, u32x4 (&code)[S::CT],
+                                          bool masked, bool last, bool none, int first_slot, const Sight& sight,
+                                          float unit) {
+        const int ke = min(max((int)(head[0] & 255u), kKv8Low), kKv8High);
+        int ve = min(max((int)(head[0] >> 8 & 255u), kKv8Low), kKv8High);
+        const float factor = fmaxf(unit * kv8_pow2(ke), 1e-37f);
+        float x[16];
+#pragma unroll
+        for (int v = 0; v < 16; ++v) x[v] = acc[MT == 16 ? v / 4 % S::NT : 0][v % S::ACC];
+        if (masked) {
+            asm volatile("");                              // a branch, not selections on every page
+            const uint32_t sees = none ? 0u : sight.of_run(first_slot);
+#pragma unroll
+            for (int v = 0; v < 16; ++v)
+                if (!(sees >> v & 1u)) x[v] = -__builtin_inff();
+        }
+        if (__any(head[1] != 0u)) {
+            asm volatile("");
+            const uint32_t lost = none ? 0u : head[1] >> (first_slot & 16) & sight.of_run(first_slot);
+#pragma unroll
+            for (int v = 0; v < 16; ++v)
+                if (lost >> v & 1u) x[v] = __builtin_nanf("");
+        }
+        if (last) {
+            asm volatile("");
+            // behind the last slot anything may lie, and a weight of 0 does not make it 0
+            const uint32_t keep = none ? 0u : lowest(sight.filled - first_slot);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                // bit i to byte i
+                const uint32_t bytes = (((keep >> (4 * w) & 15u) * 0x00204081u) & 0x01010101u) * 255u;
+#pragma unroll
+                for (int t = 0; t < S::CT; ++t) code[t][w] &= bytes;
+            }
+            // a block that holds nothing yet has no exponent either
+            const int first = uniform(ve);
+            if (none || (first_slot & ~31) >= sight.filled) ve = none || MT == 32 ? vref : first;
+        }
+        float best = x[0];
+#pragma unroll
+        for (int v = 1; v < 16; ++v) best = fmaxf(best, x[v]);
+        best = max_over_groups<MT>(best * factor);
+        if (__any(best > top)) {
+            const float now = fmaxf(top, best + kLag), f = fade(top, now);
+            top = now;
+            total *= f;
+            rescale(f);
+        }
+        // exponents of the step's blocks, the same for the whole wave
+        const int v0 = uniform(ve), v1 = MT == 16 ? __builtin_amdgcn_readlane(ve, 32) : v0;
+        const int vmax = max(v0, v1);
+        if (vmax) vlow = min(vlow, min(v0, v1));           // 0: no block has been held yet
+        if (vmax > vref) {
+            const int now = min(vmax + kHead, kKv8High);
+            rescale(vref ? kv8_pow2(max(127 + vref - now, 0)) : 1.f);
+            vref = now;
+        }
+        const float ref = (top == -__builtin_inff() ? 0.f : top) - kLift;
+        const float vscale = kv8_pow2(134 + ve - vref);
+        if (vlow >= vref - kSpan) {
+            multiply<f16_t, std::is_same<T, f16_t>::value ? 2 : 1>(x, factor, ref, code, vscale);
+        } else {
+            asm volatile("");
+            multiply<bf16_t, 2>(x, factor, ref, code, vscale);
+        }
     }
 };
 
@@ -278,7 +306,7 @@ __device__ __forceinline__ void store4(const Kv8AttentionArgs& a, int b, const R
 // nothing (the largest score's weight is at least 2^-kLag, or nearly).
 __device__ __forceinline__ void store_lse8(const Kv8AttentionArgs& a, int b, const Row& row, float ref, float total) {
     if (!row.in_block) return;
-    const float x = row.valid && total != 0.f ? (ref + __builtin_amdgcn_logf(total)) * 0.693147180559945309f
+    const float x = row.valid && total != 0.f ? (ref - kLift + __builtin_amdgcn_logf(total)) * 0.693147180559945309f
                                              : -__builtin_inff();
     a.lse[((int64_t)b * a.block.T + row.t) * a.q_heads + row.hq] = x;
 }
@@ -420,26 +448,24 @@ __global__ __launch_bounds__(kThreads, 2) void kv8_attention_kernel(Kv8Attention
                              (count >= 64 ? ~0ull : (1ull << count) - 1);
         }
         sight.lim = min(sight.lim, sight.filled);
-        rows.top = -__builtin_inff();
-        rows.total = 0.f;
-#pragma unroll
-        for (int t = 0; t < S::CT; ++t)
-#pragma unroll
-            for (int i = 0; i < S::ACC; ++i) rows.o[t][i] = 0.f;
+        rows.clear();
 
         // Pages p, p + WAYS, ... below `stop`; one that the table does not name is passed over.
-        // Keys of the next page are loaded into their registers once the scores are made, values
-        // once the products are: each is on its way during the other's work.  The loads are
-        // unconditional (of page 0 where there is none to load) and in this order, so that each
-        // wait covers only what it needs.
+        // Keys and values of the next page are loaded into their registers once a step's scores or
+        // products are made, a page's work ahead of their use.  The loads are unconditional (of
+        // page 0 where there is none to load) and in the order of their use, so that each wait
+        // covers only what it needs.
         auto named = [&](int id) { return id >= 0 && id < c.num_pages; };
         auto address = [&](int id) { return heads + (named(id) ? id : 0) * page_stride; };
         KeyRegs<D, MT> keys;
         ValueRegs<D, MT> values;
         int id = id_at(p);
         if (p < stop) {
-            keys.load(address(id), col, g);
-            values.load(address(id), col, g);
+#pragma unroll
+            for (int step = 0; step < S::STEPS; ++step) {
+                keys.load(address(id), col, g, step);
+                values.load(address(id), col, g, step);
+            }
         }
 #pragma unroll
         for (int i = 0; i < kPerWave; ++i) {
@@ -451,20 +477,23 @@ __global__ __launch_bounds__(kThreads, 2) void kv8_attention_kernel(Kv8Attention
         lds_barrier();                                        // the loads stay in flight
         for (; p < stop; p += WAYS) {
             const int next = id_at(p + WAYS);
-            typename S::Acc acc[S::NT];
-            rows.scores(&s_q[tile][0][lane], keys, acc);
-            uint32_t exponents[S::RUNS], bad[S::RUNS];
+            const uint8_t* next_page = address(next);
+            const bool none = !named(id);
+            const int slot = seen.page(p) * kCachePage;
+            const bool masked = none || slot + kCachePage > clear_to ||
+                                (slot < clear_from && slot + kCachePage > sight.sinks);
+            const bool end = none || slot + kCachePage > sight.filled;
 #pragma unroll
-            for (int r = 0; r < S::RUNS; ++r) exponents[r] = keys.exponents[r], bad[r] = keys.bad[r];
-            keys.load(address(next), col, g);
-            asm volatile("" ::: "memory");
-            if (named(id)) {
-                const int slot = seen.page(p) * kCachePage;
-                const bool masked = slot + kCachePage > clear_to || (slot < clear_from && slot + kCachePage > sight.sinks);
-                rows.weigh(acc, exponents, bad, values, masked, slot + kCachePage > sight.filled, slot, sight, g, unit);
+            for (int step = 0; step < S::STEPS; ++step) {
+                typename S::Acc acc[S::NT];
+                rows.scores(&s_q[tile][0][lane], keys.code[step], acc);
+                const u32x2 head = keys.head[step];
+                keys.load(next_page, col, g, step);
+                asm volatile("" ::: "memory");
+                rows.weigh(acc, head, values.code[step], masked, end, none, slot + S::run_slot(step, g), sight, unit);
+                values.load(next_page, col, g, step);
+                asm volatile("" ::: "memory");
             }
-            values.load(address(next), col, g);
-            asm volatile("" ::: "memory");
             id = next;
         }
 
@@ -487,7 +516,8 @@ __global__ __launch_bounds__(kThreads, 2) void kv8_attention_kernel(Kv8Attention
         for (int w = tile * WAYS; w < (tile + 1) * WAYS; ++w) m = fmaxf(m, s_m[w][col]);
 #pragma unroll
         for (int w = tile * WAYS; w < (tile + 1) * WAYS; ++w) l += s_l[w][col] * fade(s_m[w][col], m);
-        const float f = fade(ref, m), inv = l != 0.f ? 1.f / l : 0.f;
+        const float inv = l != 0.f ? 1.f / l : 0.f;
+        const float f = fade(ref, m) * kv8_pow2(max(rows.vref - 7, 0));
 #pragma unroll
         for (int r0 = 0; r0 < kRegs; r0 += kRound) {
 #pragma unroll

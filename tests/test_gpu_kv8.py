@@ -3,15 +3,14 @@
 Bounds.  What append writes and read gives back is exact: rotation and rounding are defined to the
 bit.  Attention: the products of queries with codes are exact (at most 11 and 4 significant
 bits) and summed in fp32, 128 terms of 2^-24 each, the factor and the scaling a few more: a score is
-off by less than 2^-16 of its sum of magnitudes.  A weight meets the values as two bf16
-parts (2^-17); what else an output may be off by is oracle.kv4.output_range's.
+off by less than 2^-16 of its sum of magnitudes.  What outputs may be off by is derived at
+oracle.kv8.output_range.
 """
 
 import numpy as np
 import pytest
 import torch
 
-from oracle import kv4 as O4
 from oracle import kv8 as O
 
 pytestmark = pytest.mark.gpu
@@ -323,7 +322,7 @@ def attention_inputs(pkg, dev, B, T, HQ, H, D, pages, dtype, block, lengths, cou
     return cache, q, masks
 
 
-def check_attention(cache, q, dtype, block, lengths, counts, masks, scale, out, lse, window=None, sinks=0):
+def check_attention(cache, q, dtype, block, lengths, counts, masks, scale, out, lse, window=None, sinks=0, steep=False):
     K, V = contents(cache)
     B, T = q.shape[:2]
     count = [min(T if counts is None else counts[b], T) for b in range(B)]
@@ -341,7 +340,9 @@ def check_attention(cache, q, dtype, block, lengths, counts, masks, scale, out, 
     err = mass * 2.0 ** -16
     with np.errstate(invalid="ignore"):
         assert np.all(np.abs(lse - rl)[f] <= (err + 2.0 ** -20 * (1 + np.abs(rl)))[f])
-        lo, hi = O4.output_range(ro, weight, err, dtype)
+        # steep: no weight that matters is so small that it has fewer bits
+        most = 0.0 if steep else V.shape[2] * np.nanmax(np.abs(V), initial=0.0)
+        lo, hi = O.output_range(ro, weight, err, dtype, most)
     ok = (out >= lo) & (out <= hi)
     assert ok[f].all(), (np.argwhere(~ok & f[..., None])[:4], out[~ok & f[..., None]][:4], ro[~ok & f[..., None]][:4])
 
@@ -428,6 +429,27 @@ def test_values_up_to_what_the_cache_holds(pkg, dev, T, n, dtype, step):
         assert np.array_equal(out.cpu().numpy(), np.sign(ref) * np.inf)
     else:
         check_attention(cache, q, dtype, "causal", [n], None, None, scale, out, lse)
+
+
+@pytest.mark.parametrize("T,dtype", [(1, "bf16"), (3, "f16"), (20, "bf16"), (40, "f16")])
+@pytest.mark.parametrize("up", [True, False])
+def test_blocks_of_very_different_scales(pkg, dev, T, dtype, up):
+    """Values from 2^-60 to 2^60, block by block, where the large ones weigh nothing: the small ones count in full."""
+    say("scales", T, dtype, up)
+    HQ, H, D, n = 4, 2, 64, 500
+    g = torch.Generator().manual_seed(T)
+    cache = pkg.KV8Cache.allocate(1, n + T, H, D, dev)
+    order = torch.arange(n + T) // 32 * 7 - 55                     # binary orders of a block's values
+    size = order.float() if up else -order.float() - 1
+    v = torch.randn(1, n + T, H, D, generator=g) * torch.exp2(size)[None, :, None, None]
+    k = torch.zeros(1, n + T, H, D)
+    k[0, :, :, 0] = -size[:, None] * 1.5                           # the larger, the less it is looked at
+    pkg.kv8_append(cache, k.to(dev), v.to(dev), ints([0], dev))
+    q = torch.zeros(1, T, HQ, D, dtype=DT[dtype])
+    q[..., 0] = torch.linspace(0.3, 3.0, HQ)
+    out, lse = pkg.kv8_attention(q.to(dev), cache, ints([n], dev), block="full", scale=1.0)
+    torch.cuda.synchronize()
+    check_attention(cache, q, dtype, "full", [n], None, None, 1.0, out, lse, steep=True)
 
 
 @pytest.mark.parametrize("T,block,window", [(1, "causal", None), (9, "causal", None), (9, "mask", None),
@@ -524,13 +546,14 @@ def test_attention_of_many_row_tiles(pkg, dev, B, H, T, G, D, dtype, block, ragg
                                  sinks=sinks, block=block if masks is None else masks.to(dev))
     torch.cuda.synchronize()
     c = [T] * B if counts is None else counts
+    most = cache.slots * np.nanmax(np.abs(contents(cache)[1]))
     for b, (ro, rl, weight, mass) in enumerate(attention_64(cache, q, lengths, c, block, masks, window, sinks)):
         err = mass * 2.0 ** -16
         got = lse[b].double().view(T, H, G)
         f = rl > -INF
         assert torch.equal(f, got > -INF)
         assert torch.all((got - rl)[f].abs() <= (err + 2.0 ** -20 * (1 + rl.abs()))[f]), b
-        lo, hi = O4.output_range(ro.cpu().numpy(), weight.cpu().numpy(), err.cpu().numpy(), dtype)
+        lo, hi = O.output_range(ro.cpu().numpy(), weight.cpu().numpy(), err.cpu().numpy(), dtype, most)
         o = out[b].double().view(T, H, G, D).cpu().numpy()
         assert np.all((o >= lo) & (o <= hi)), b
 
@@ -555,11 +578,12 @@ def test_attention_of_any_cut(pkg, dev, B, T, HQ, H, pages, lengths, window):
     again = pkg.kv8_attention(q.to(dev), cache, ints(lengths, dev), window=window, sinks=5 if window else 0)
     torch.cuda.synchronize()
     assert torch.equal(out, again[0]) and torch.equal(lse, again[1])
+    most = cache.slots * np.nanmax(np.abs(contents(cache)[1]))
     for b, (ro, rl, weight, mass) in enumerate(attention_64(cache, q, lengths, [T] * B, "causal", None, window,
                                                             5 if window else 0)):
         err = mass * 2.0 ** -16
         got = lse[b].double().view(rl.shape)
         assert torch.all((got - rl).abs() <= err + 2.0 ** -20 * (1 + rl.abs())), b
-        lo, hi = O4.output_range(ro.cpu().numpy(), weight.cpu().numpy(), err.cpu().numpy(), "bf16")
+        lo, hi = O.output_range(ro.cpu().numpy(), weight.cpu().numpy(), err.cpu().numpy(), "bf16", most)
         o = out[b].double().view(ro.shape).cpu().numpy()
         assert np.all((o >= lo) & (o <= hi)), b

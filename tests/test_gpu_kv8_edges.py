@@ -81,7 +81,7 @@ def test_lengths_counts_and_pages_out_of_range(pkg, dev):
                 x, err = k @ row, (k.abs() @ row.abs()).max().item() * 2.0 ** -16
                 p, rl = torch.softmax(x, 0), torch.logsumexp(x, 0).item()
                 assert abs(lse[b, t, hq].item() - rl) <= err + 2.0 ** -20 * (1 + abs(rl))
-                off = (p @ v.abs()) * (2.0 ** -16 + 2 * err + 2.0 ** -19)
+                off = (p @ v.abs()) * (2.0 ** -11 + 2.0 ** -16 + 2 * err + 2.0 ** -19)    # an f16 weight
                 want = p @ v                               # and half a step of bf16
                 assert torch.all((out[b, t, hq].double().cpu() - want).abs() <= off + (want.abs() + off) * 2.0 ** -8)
     # slots past the table's, entries of no page: nothing is written anywhere
