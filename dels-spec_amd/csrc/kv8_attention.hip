@@ -87,13 +87,18 @@ template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b
     else return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), f16x2));
 }
 
+// a where bit v of `bits` is set, else b.
+__device__ __forceinline__ float choose(uint32_t bits, int v, float a, float b) {
+    const uint32_t all = (uint32_t)((int32_t)(bits << (31 - v)) >> 31);
+    return __uint_as_float((__float_as_uint(a) & all) | (__float_as_uint(b) & ~all));
+}
+
 // The lowest k of 16 bits.
 __device__ __forceinline__ uint32_t lowest(int k) { return (1u << min(max(k, 0), 16)) - 1u; }
 
 template <int D, int MT> struct KeyRegs {
     using S = Shape8<D, MT>;
     u32x4 code[S::STEPS][S::NT][S::KL];
-    u32x2 head[S::STEPS];
     __device__ __forceinline__ void load(const uint8_t* page, int col, int g, int step) {
         const int lane = MT == 16 ? 32 * D * (col >> 3) + 512 * g + 16 * (col & 7) : 512 * g + 16 * col;
 #pragma unroll
@@ -102,7 +107,6 @@ template <int D, int MT> struct KeyRegs {
             for (int i = 0; i < S::KL; ++i)
                 code[step][t][i] =
                     *reinterpret_cast<const u32x4*>(page + lane + 512 * S::NG * i + (MT == 16 ? 128 * t : 32 * D * step));
-        head[step] = *reinterpret_cast<const u32x2*>(page + Kv8<D>::kHead + 8 * (MT == 16 ? g / 2 : step));
     }
 };
 
@@ -128,6 +132,25 @@ struct Sight {
         uint32_t by_bit = d >= 64 || d <= -16 ? 0u : (uint32_t)(d >= 0 ? bits >> d : bits << -d) & 0xffffu;
         by_bit &= lowest(filled - j0);
         return (lowest(lim - j0) | by_bit) & (~lowest(lo - j0) | lowest(sinks - j0));
+    }
+};
+
+// A page as a wave meets it: what its two blocks say of themselves, and what of it is seen.
+struct Page {
+    int key[2], value[2];      // exponents; of a block that holds nothing the value's is 0
+    uint32_t bad[2];
+    int slot;                  // first of its slots
+    bool none, masked, last;   // is no page; some row does not see all of it; slots behind the last hold nothing
+    __device__ __forceinline__ Page(u32x4 head, int slot_, bool none_, bool masked_, int filled) : slot(slot_), none(none_) {
+        last = none || slot + kCachePage > filled;
+        masked = none || masked_;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int e = uniform((int)head[2 * u]);
+            key[u] = min(max(e & 255, kKv8Low), kKv8High);
+            value[u] = none || slot + 32 * u >= filled ? 0 : min(max(e >> 8 & 255, kKv8Low), kKv8High);
+            bad[u] = none ? 0u : (uint32_t)uniform((int)head[2 * u + 1]);
+        }
     }
 };
 
@@ -157,17 +180,18 @@ template <typename T, int D, int MT> struct Rows8 {
             for (int i = 0; i < S::ACC; ++i) o[t][i] *= f;
     }
 
-    // scores of a step; q: this lane's operands of the queries in LDS, 64 apart
-    __device__ __forceinline__ void scores(const F* q, const u32x4 (&code)[S::NT][S::KL], typename S::Acc (&acc)[S::NT]) {
+    // scores of a step; q(k): this lane's operand of the queries for step k of the contraction
+    template <typename Q>
+    __device__ __forceinline__ void scores(Q&& q, const u32x4 (&code)[S::NT][S::KL], typename S::Acc (&acc)[S::NT]) {
 #pragma unroll
         for (int t = 0; t < S::NT; ++t)
 #pragma unroll
             for (int i = 0; i < S::ACC; ++i) acc[t][i] = 0.f;
-        F next_q = q[0];
+        F next_q = q(0);
 #pragma unroll
         for (int k = 0; k < S::KS; ++k) {
             const F qk = next_q;
-            if (k + 1 < S::KS) next_q = q[64 * (k + 1)];       // read a step ahead
+            if (k + 1 < S::KS) next_q = q(k + 1);              // read a step ahead
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int t = 0; t < S::NT; ++t)
@@ -217,35 +241,45 @@ template <typename T, int D, int MT> struct Rows8 {
         __builtin_amdgcn_sched_barrier(0);
     }
 
-    // head: of the block of the lane's run; unit: binary logarithms per raw product; none: the
-    // page is no page
-    __device__ __forceinline__ void weigh(const typename S::Acc (&acc)[S::NT], u32x2 head, u32x4 (&code)[S::CT],
-                                          bool masked, bool last, bool none, int first_slot, const Sight& sight,
-                                          float unit) {
-        const int ke = min(max((int)(head[0] & 255u), kKv8Low), kKv8High);
-        int ve = min(max((int)(head[0] >> 8 & 255u), kKv8Low), kKv8High);
+    // Takes a page's scales in; whether its products can be of f16 numbers.
+    __device__ __forceinline__ bool admit(const Page& page) {
+        const int high = max(page.value[0], page.value[1]);
+        if (high) vlow = min(vlow, page.value[1] ? min(page.value[0], page.value[1]) : page.value[0]);
+        if (high > vref) {
+            const int now = min(high + kHead, kKv8High);
+            rescale(vref ? kv8_pow2(max(127 + vref - now, 0)) : 1.f);
+            vref = now;
+        }
+        return vlow >= vref - kSpan;
+    }
+
+    // WIDE: the scales lie far apart; unit: binary logarithms per raw product
+    template <bool WIDE>
+    __device__ __forceinline__ void weigh(const typename S::Acc (&acc)[S::NT], const Page& page, int step, int g,
+                                          u32x4 (&code)[S::CT], const Sight& sight, float unit) {
+        const int slot = page.slot + S::run_slot(step, g);
+        const bool second = MT == 16 ? g >= 2 : step == 1;     // of the page's blocks
+        const int ke = second ? page.key[1] : page.key[0], ve = second ? page.value[1] : page.value[0];
         const float factor = fmaxf(unit * kv8_pow2(ke), 1e-37f);
         float x[16];
 #pragma unroll
         for (int v = 0; v < 16; ++v) x[v] = acc[MT == 16 ? v / 4 % S::NT : 0][v % S::ACC];
-        if (masked) {
+        if (page.masked) {
             asm volatile("");                              // a branch, not selections on every page
-            const uint32_t sees = none ? 0u : sight.of_run(first_slot);
+            const uint32_t sees = page.none ? 0u : sight.of_run(slot);
 #pragma unroll
-            for (int v = 0; v < 16; ++v)
-                if (!(sees >> v & 1u)) x[v] = -__builtin_inff();
+            for (int v = 0; v < 16; ++v) x[v] = choose(sees, v, x[v], -__builtin_inff());
         }
-        if (__any(head[1] != 0u)) {
+        if (page.bad[0] | page.bad[1]) {
             asm volatile("");
-            const uint32_t lost = none ? 0u : head[1] >> (first_slot & 16) & sight.of_run(first_slot);
+            const uint32_t lost = (second ? page.bad[1] : page.bad[0]) >> (slot & 16) & sight.of_run(slot);
 #pragma unroll
-            for (int v = 0; v < 16; ++v)
-                if (lost >> v & 1u) x[v] = __builtin_nanf("");
+            for (int v = 0; v < 16; ++v) x[v] = choose(~lost, v, x[v], __builtin_nanf(""));
         }
-        if (last) {
+        if (page.last) {
             asm volatile("");
             // behind the last slot anything may lie, and a weight of 0 does not make it 0
-            const uint32_t keep = none ? 0u : lowest(sight.filled - first_slot);
+            const uint32_t keep = page.none ? 0u : lowest(sight.filled - slot);
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
                 // bit i to byte i
@@ -253,9 +287,6 @@ template <typename T, int D, int MT> struct Rows8 {
 #pragma unroll
                 for (int t = 0; t < S::CT; ++t) code[t][w] &= bytes;
             }
-            // a block that holds nothing yet has no exponent either
-            const int first = uniform(ve);
-            if (none || (first_slot & ~31) >= sight.filled) ve = none || MT == 32 ? vref : first;
         }
         float best = x[0];
 #pragma unroll
@@ -267,23 +298,10 @@ template <typename T, int D, int MT> struct Rows8 {
             total *= f;
             rescale(f);
         }
-        // exponents of the step's blocks, the same for the whole wave
-        const int v0 = uniform(ve), v1 = MT == 16 ? __builtin_amdgcn_readlane(ve, 32) : v0;
-        const int vmax = max(v0, v1);
-        if (vmax) vlow = min(vlow, min(v0, v1));           // 0: no block has been held yet
-        if (vmax > vref) {
-            const int now = min(vmax + kHead, kKv8High);
-            rescale(vref ? kv8_pow2(max(127 + vref - now, 0)) : 1.f);
-            vref = now;
-        }
         const float ref = (top == -__builtin_inff() ? 0.f : top) - kLift;
-        const float vscale = kv8_pow2(134 + ve - vref);
-        if (vlow >= vref - kSpan) {
-            multiply<f16_t, std::is_same<T, f16_t>::value ? 2 : 1>(x, factor, ref, code, vscale);
-        } else {
-            asm volatile("");
-            multiply<bf16_t, 2>(x, factor, ref, code, vscale);
-        }
+        const float vscale = kv8_pow2(ve ? 134 + ve - vref : 127);
+        if constexpr (WIDE) multiply<bf16_t, 2>(x, factor, ref, code, vscale);
+        else multiply<f16_t, std::is_same<T, f16_t>::value ? 2 : 1>(x, factor, ref, code, vscale);
     }
 };
 
@@ -350,18 +368,38 @@ struct Kv8Seqs {
     }
 };
 
-template <typename T, int D, int MT, int WAYS>
+// LDS of a workgroup.  Where TILES row tiles go over the same pages, each way keeps a ring of
+// them there: the page as it lies in memory but for its head, of which every wave has its own.
+template <typename T, int D, int MT, int TILES> struct Lds {
+    using S = Shape8<D, MT>;
+    static constexpr int kWays = kWaves / TILES;
+    static constexpr int kRing = TILES == 1 ? 0 : kWays * D > 256 ? 2 : 3;
+    static constexpr int kRound = 32;                       // output registers joined at a time
+    union {
+        uint8_t page[kWays][kRing ? kRing : 1][TILES == 1 ? 16 : Kv8<D>::kHead];
+        float o[kWaves][kRound][64];
+    };
+    uint32_t head[kWaves][kRing ? kRing : 1][64];
+    typename Frag<T>::type q[TILES][S::KS][64];             // the tiles' queries, in operand order
+    float m[kWaves][MT], l[kWaves][MT];
+    bool last;
+};
+
+// TILES of 8 waves share a way: row tiles over the same pages.  8 / TILES ways take every
+// (8 / TILES)-th page each.
+template <typename T, int D, int MT, int TILES>
 __global__ __launch_bounds__(kThreads, 2) void kv8_attention_kernel(Kv8AttentionArgs a, Line line, float* states,
                                                                     unsigned int* counters) {
     using S = Shape8<D, MT>;
     using F = typename Frag<T>::type;
+    using L = Lds<T, D, MT, TILES>;
+    constexpr int WAYS = L::kWays, kTiles = TILES, kRound = L::kRound;
     constexpr int kRegs = S::CT * S::ACC;                   // output registers
-    constexpr int kRound = 32;                              // registers joined at a time
-    __shared__ float s_o[kWaves][kRound][64];
-    __shared__ float s_m[kWaves][MT], s_l[kWaves][MT];
-    constexpr int kTiles = kWaves / WAYS;
-    __shared__ F s_q[kTiles][S::KS][64];
-    __shared__ bool s_last;
+    __shared__ __attribute__((aligned(128))) L lds;
+    auto& s_o = lds.o;
+    auto& s_m = lds.m;
+    auto& s_l = lds.l;
+    auto& s_last = lds.last;
 
     const PagedCache& c = a.cache;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -393,7 +431,8 @@ __global__ __launch_bounds__(kThreads, 2) void kv8_attention_kernel(Kv8Attention
         // tokens of the tile group, and of this wave's tile
         const Seen seen = seqs.seen(n, count, divide(rt0 * MT, group), min(divide((rt0 + kTiles) * MT - 1, group), last_t));
         const int t_first = divide(rt * MT, group), t_last = min(divide(rt * MT + MT - 1, group), last_t);
-        const int stop = rt * MT >= a.block.T * group ? 0 : min(last, seen.count());   // 0: past the block's rows
+        const int stop = min(last, seen.count());
+        const bool past = rt * MT >= count * group;           // the tile has no valid row
         Sight sight;
         sight.n = n;
         sight.filled = seq_end(a.block, n, count, slots);     // slots past it may hold anything
@@ -422,19 +461,22 @@ __global__ __launch_bounds__(kThreads, 2) void kv8_attention_kernel(Kv8Attention
         };
         fetch_ids(p);
 
-        // the queries of all tiles, in operand order: step k of lane group g has channels
-        // 16 (NG (k / 2) + g) + 8 (k % 2) .. + 7
-        constexpr int kPerWave = (kTiles * S::KS + kWaves - 1) / kWaves;
-        u32x4 qw[kPerWave];
+        // the queries in operand order: step k of lane group g has channels
+        // 16 (NG (k / 2) + g) + 8 (k % 2) .. + 7.  The waves of a tile share them out.
+        constexpr int kQ = (S::KS + WAYS - 1) / WAYS;
+        auto q_step = [&](int i) { return way + i * WAYS; };
+        u32x4 qw[kQ];
+        {
+            const Row of = row_of(rt * MT + col, group, h, a.block.T, count);
+            const uint16_t* from = static_cast<const uint16_t*>(a.q.p) + (int64_t)b * a.q.batch +
+                                   (int64_t)of.t * a.q.token + (int64_t)of.hq * a.q.head;
 #pragma unroll
-        for (int i = 0; i < kPerWave; ++i) {
-            const int e = wave + i * kWaves, k = e % S::KS;
-            const Row of = row_of((rt0 + e / S::KS) * MT + col, group, h, a.block.T, count);
-            qw[i] = u32x4{0u, 0u, 0u, 0u};
-            if (of.valid && e < kTiles * S::KS)
-                qw[i] = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q.p) + (int64_t)b * a.q.batch +
-                                                        (int64_t)of.t * a.q.token + (int64_t)of.hq * a.q.head +
-                                                        16 * (S::NG * (k / 2) + g) + 8 * (k % 2));
+            for (int i = 0; i < kQ; ++i) {
+                const int k = q_step(i);
+                qw[i] = u32x4{0u, 0u, 0u, 0u};
+                if (of.valid && k < S::KS)
+                    qw[i] = *reinterpret_cast<const u32x4*>(from + 16 * (S::NG * (k / 2) + g) + 8 * (k % 2));
+            }
         }
         const Row row = row_of(rt * MT + col, group, h, a.block.T, count);
         Rows8<T, D, MT> rows;
@@ -450,51 +492,143 @@ __global__ __launch_bounds__(kThreads, 2) void kv8_attention_kernel(Kv8Attention
         sight.lim = min(sight.lim, sight.filled);
         rows.clear();
 
-        // Pages p, p + WAYS, ... below `stop`; one that the table does not name is passed over.
-        // Keys and values of the next page are loaded into their registers once a step's scores or
-        // products are made, a page's work ahead of their use.  The loads are unconditional (of
-        // page 0 where there is none to load) and in the order of their use, so that each wait
-        // covers only what it needs.
+        // Pages p, p + WAYS, ... below `stop`; one that the table does not name is seen by no row.
         auto named = [&](int id) { return id >= 0 && id < c.num_pages; };
         auto address = [&](int id) { return heads + (named(id) ? id : 0) * page_stride; };
-        KeyRegs<D, MT> keys;
-        ValueRegs<D, MT> values;
-        int id = id_at(p);
-        if (p < stop) {
+        auto put_queries = [&] {
 #pragma unroll
-            for (int step = 0; step < S::STEPS; ++step) {
-                keys.load(address(id), col, g, step);
-                values.load(address(id), col, g, step);
+            for (int i = 0; i < kQ; ++i) {
+#pragma unroll
+                for (int x = 0; x < 4; ++x) qw[i][x] = (qw[i][x] ^ flip) & zero;
+                if (q_step(i) < S::KS) lds.q[tile][q_step(i)][lane] = __builtin_bit_cast(F, qw[i]);
             }
-        }
+        };
+        auto query = [&](int k) { return lds.q[tile][k][lane]; };
+        auto page_at = [&](int i, int id, u32x4 head) {
+            const int slot = seen.page(i) * kCachePage;
+            return Page(head, slot, !named(id),
+                        slot + kCachePage > clear_to || (slot < clear_from && slot + kCachePage > sight.sinks), sight.filled);
+        };
+        using Narrow = std::false_type;
+        using Wide = std::true_type;
+        if constexpr (TILES == 1) {
+            // Keys and values of the next page are loaded into their registers once a step's scores
+            // or products are made, a page's work ahead of their use.  The loads are unconditional
+            // (of page 0 where there is none to load) and in the order of their use, so that each
+            // wait covers only what it needs.
+            KeyRegs<D, MT> keys;
+            ValueRegs<D, MT> values;
+            u32x4 head;
+            int id = id_at(p);
+            auto load_head = [&](const uint8_t* page) { head = *reinterpret_cast<const u32x4*>(page + Kv8<D>::kHead); };
+            if (p < stop) {
+                load_head(address(id));
 #pragma unroll
-        for (int i = 0; i < kPerWave; ++i) {
-            const int e = wave + i * kWaves;
-#pragma unroll
-            for (int x = 0; x < 4; ++x) qw[i][x] = (qw[i][x] ^ flip) & zero;
-            if (e < kTiles * S::KS) s_q[e / S::KS][e % S::KS][lane] = __builtin_bit_cast(F, qw[i]);
-        }
-        lds_barrier();                                        // the loads stay in flight
-        for (; p < stop; p += WAYS) {
-            const int next = id_at(p + WAYS);
-            const uint8_t* next_page = address(next);
-            const bool none = !named(id);
-            const int slot = seen.page(p) * kCachePage;
-            const bool masked = none || slot + kCachePage > clear_to ||
-                                (slot < clear_from && slot + kCachePage > sight.sinks);
-            const bool end = none || slot + kCachePage > sight.filled;
-#pragma unroll
-            for (int step = 0; step < S::STEPS; ++step) {
-                typename S::Acc acc[S::NT];
-                rows.scores(&s_q[tile][0][lane], keys.code[step], acc);
-                const u32x2 head = keys.head[step];
-                keys.load(next_page, col, g, step);
-                asm volatile("" ::: "memory");
-                rows.weigh(acc, head, values.code[step], masked, end, none, slot + S::run_slot(step, g), sight, unit);
-                values.load(next_page, col, g, step);
-                asm volatile("" ::: "memory");
+                for (int step = 0; step < S::STEPS; ++step) {
+                    keys.load(address(id), col, g, step);
+                    values.load(address(id), col, g, step);
+                }
             }
-            id = next;
+            put_queries();
+            lds_barrier();                                    // the loads stay in flight
+            auto work = [&](auto wide, const Page& page) {
+                const int next = id_at(p + WAYS);
+                const uint8_t* next_page = address(next);
+                load_head(next_page);
+#pragma unroll
+                for (int step = 0; step < S::STEPS; ++step) {
+                    typename S::Acc acc[S::NT];
+                    rows.scores(query, keys.code[step], acc);
+                    keys.load(next_page, col, g, step);
+                    asm volatile("" ::: "memory");
+                    rows.template weigh<decltype(wide)::value>(acc, page, step, g, values.code[step], sight, unit);
+                    values.load(next_page, col, g, step);
+                    asm volatile("" ::: "memory");
+                }
+                id = next;
+                p += WAYS;
+            };
+            while (p < stop) {
+                const Page page = page_at(p, id, head);
+                if (!rows.admit(page)) break;                 // and from there on
+                work(Narrow{}, page);
+            }
+            while (p < stop) {
+                const Page page = page_at(p, id, head);
+                rows.admit(page);
+                work(Wide{}, page);
+            }
+        } else {
+            // The waves of a way copy a page into its ring, a share of 1 KiB pieces and the head each,
+            // kRing - 1 pages ahead.  One barrier a page: past it, all shares of the page have
+            // arrived and nobody reads the buffer that the next copy goes to.
+            constexpr int kShare = Kv8<D>::kHead / 1024 / TILES, kPer = kShare + 1;
+            const int pages = max(0, (stop - first + WAYS - 1) / WAYS);      // of the first way, which has most
+            auto copy = [&](int i) {
+                const int id = id_at(first + way + i * WAYS);
+                const uint8_t* from = address(id);
+                const int slot = i % L::kRing;
+#pragma unroll
+                for (int e = 0; e < kShare; ++e) {
+                    const int at = 1024 * (tile * kShare + e);
+                    dma16(from + at, 16 * lane, &lds.page[way][slot][at]);
+                }
+                dma4(from + Kv8<D>::kHead, 4 * (lane & 31), lds.head[wave][slot]);
+                return id;
+            };
+            put_queries();
+            int ids_ahead[L::kRing];                          // of pages i, i + 1, ..
+#pragma unroll
+            for (int i = 0; i < L::kRing - 1; ++i) ids_ahead[i + 1] = i < pages ? copy(i) : -1;
+            auto arrive = [&](int i) {
+                // what may still be on its way: the pages behind this one
+                if (i + L::kRing - 2 < pages) asm volatile("s_waitcnt vmcnt(%0)" : : "n"((L::kRing - 2) * kPer) : "memory");
+                else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                lds_barrier();
+                p = first + way + i * WAYS;
+#pragma unroll
+                for (int e = 0; e < L::kRing - 1; ++e) ids_ahead[e] = ids_ahead[e + 1];
+                if (i + L::kRing - 1 < pages) ids_ahead[L::kRing - 1] = copy(i + L::kRing - 1);
+                return !past && p < stop;
+            };
+            auto take = [&](int i) {
+                return page_at(p, ids_ahead[0], *reinterpret_cast<const u32x4*>(lds.head[wave][i % L::kRing]));
+            };
+            auto work = [&](auto wide, int i, const Page& page) {
+                const uint8_t* at = lds.page[way][i % L::kRing] + 16 * lane;
+#pragma nounroll
+                for (int step = 0; step < S::STEPS; ++step) {
+                    u32x4 keys[S::NT][S::KL], values[S::CT];
+#pragma unroll
+                    for (int e = 0; e < S::KL; ++e)
+                        keys[0][e] = *reinterpret_cast<const u32x4*>(at + 32 * D * step + 1024 * e);
+#pragma unroll
+                    for (int t = 0; t < S::CT; ++t)
+                        values[t] = *reinterpret_cast<const u32x4*>(at + Kv8<D>::kValue + 32 * D * step +
+                                                                    (16 * D - 512) * g + 512 * t);
+                    typename S::Acc acc[S::NT];
+                    rows.scores(query, keys, acc);
+                    rows.template weigh<decltype(wide)::value>(acc, page, step, g, values, sight, unit);
+                }
+            };
+            int i = 0;
+            bool here = false;                                // page i has been met, but not worked on
+            for (; i < pages; ++i) {
+                if (!arrive(i)) continue;
+                const Page page = take(i);
+                here = !rows.admit(page);
+                if (here) break;                              // and from there on
+                work(Narrow{}, i, page);
+            }
+            for (; i < pages; ++i) {
+                const bool mine = here || arrive(i);
+                here = false;
+                if (!mine) continue;
+                const Page page = take(i);
+                rows.admit(page);
+                work(Wide{}, i, page);
+            }
+            __syncthreads();                                  // the ring's place is the join's
         }
 
         // ---- join the waves
@@ -627,17 +761,23 @@ __global__ __launch_bounds__(kThreads, 2) void kv8_attention_kernel(Kv8Attention
     }
 }
 
-struct Plan { int rows, ways; Line line; };
+struct Plan { int rows, tiles; Line line; };
 
 Plan plan(int64_t batch, int64_t T, int64_t q_heads, int64_t heads, int64_t max_pages) {
     Plan p{};
-    const int64_t rows = T * (q_heads / heads);
+    const int64_t rows = T * (q_heads / heads), cus = device_cu_count();
     p.rows = rows <= 16 ? 16 : 32;
-    const int64_t tiles = (rows + p.rows - 1) / p.rows, cus = device_cu_count();
-    const int64_t fours = (tiles + 3) / 4;
-    p.ways = p.rows == 32 && batch * heads * fours >= cus && 8 * tiles >= 7 * 4 * fours ? 2 : 8;
-    const int per = kWaves / p.ways;
-    p.line.tiles = (int)((tiles + per - 1) / per);
+    const int64_t tiles = (rows + p.rows - 1) / p.rows;
+    // the widest workgroup that leaves the fewest waves without a tile
+    p.tiles = 1;
+    if (tiles > 1) {
+        int64_t best = INT64_MAX;
+        for (int wide : {8, 4, 2}) {
+            const int64_t waves = (tiles + wide - 1) / wide * wide;
+            if (waves < best) best = waves, p.tiles = wide;
+        }
+    }
+    p.line.tiles = (int)((tiles + p.tiles - 1) / p.tiles);
     p.line.least = kMinPages;
     const int64_t units = batch * heads * p.line.tiles * std::max<int64_t>(max_pages, 1);
     p.line.pieces = (int)std::min<int64_t>({cus, kMaxCounters / kCounterWords,
@@ -649,12 +789,13 @@ Plan plan(int64_t batch, int64_t T, int64_t q_heads, int64_t heads, int64_t max_
 
 size_t kv8_attention_data_bytes(int64_t batch, int64_t T, int64_t q_heads, int64_t heads, int64_t head_dim,
                                 int64_t max_pages) {
-    const Plan p = plan(batch, T, q_heads, heads, max_pages);
-    // four tiles a piece where this or a shorter block has them, so that a workspace for the
-    // longest block serves every shorter one
-    const int64_t tiles = (T * (q_heads / heads) + p.rows - 1) / p.rows;
-    const bool four = p.ways == 2 || (p.rows == 32 && batch * heads * (tiles / 4) >= device_cu_count());
-    return align256((size_t)p.line.pieces * 2 * (four ? 4 : 1) * sizeof(float) * (p.rows * head_dim + 2 * p.rows));
+    // what any shorter block takes too, so that a workspace for the longest serves every one: up to
+    // 8 tiles of 32 rows a piece, and no fewer pieces
+    const int64_t rows = T * (q_heads / heads);
+    const int64_t tiles = rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 ? 4 : 8;
+    const int64_t pieces = std::min<int64_t>(device_cu_count(), kMaxCounters / kCounterWords);
+    (void)batch, (void)max_pages;
+    return align256((size_t)pieces * 2 * tiles * sizeof(float) * (32 * head_dim + 2 * 32));
 }
 
 hipError_t launch_kv8_attention(const Kv8AttentionArgs& a, void* ws, size_t data_off, hipStream_t s) {
@@ -665,14 +806,18 @@ hipError_t launch_kv8_attention(const Kv8AttentionArgs& a, void* ws, size_t data
     auto by_size = [&](auto tag, auto size) {
         using T = decltype(tag);
         constexpr int D = decltype(size)::value;
-        auto go = [&](auto rows, auto ways) {
-            hipLaunchKernelGGL((kv8_attention_kernel<T, D, decltype(rows)::value, decltype(ways)::value>),
+        auto go = [&](auto rows, auto tiles) {
+            hipLaunchKernelGGL((kv8_attention_kernel<T, D, decltype(rows)::value, decltype(tiles)::value>),
                                dim3(p.line.pieces), dim3(kThreads), 0, s, a, p.line, states, counters);
         };
         using std::integral_constant;
-        if (p.rows == 16) go(integral_constant<int, 16>{}, integral_constant<int, 8>{});
-        else if (p.ways == 8) go(integral_constant<int, 32>{}, integral_constant<int, 8>{});
-        else go(integral_constant<int, 32>{}, integral_constant<int, 2>{});
+        using I16 = integral_constant<int, 16>;
+        using I32 = integral_constant<int, 32>;
+        if (p.rows == 16) go(I16{}, integral_constant<int, 1>{});
+        else if (p.tiles == 1) go(I32{}, integral_constant<int, 1>{});
+        else if (p.tiles == 2) go(I32{}, integral_constant<int, 2>{});
+        else if (p.tiles == 4) go(I32{}, integral_constant<int, 4>{});
+        else go(I32{}, integral_constant<int, 8>{});
     };
     auto by_type = [&](auto tag) {
         if (c.head_dim == 64) by_size(tag, std::integral_constant<int, 64>{});
