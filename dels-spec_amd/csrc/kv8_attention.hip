@@ -135,23 +135,15 @@ struct Sight {
     }
 };
 
-// A page as a wave meets it: what its two blocks say of themselves, and what of it is seen.
+// What a page's two blocks say of themselves, the same for the whole wave.
 struct Page {
-    int key[2], value[2];      // exponents; of a block that holds nothing the value's is 0
-    uint32_t bad[2];
-    int slot;                  // first of its slots
-    bool none, masked, last;   // is no page; some row does not see all of it; slots behind the last hold nothing
-    __device__ __forceinline__ Page(u32x4 head, int slot_, bool none_, bool masked_, int filled) : slot(slot_), none(none_) {
-        last = none || slot + kCachePage > filled;
-        masked = none || masked_;
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int e = uniform((int)head[2 * u]);
-            key[u] = min(max(e & 255, kKv8Low), kKv8High);
-            value[u] = none || slot + 32 * u >= filled ? 0 : min(max(e >> 8 & 255, kKv8Low), kKv8High);
-            bad[u] = none ? 0u : (uint32_t)uniform((int)head[2 * u + 1]);
-        }
-    }
+    uint32_t exponents[2], bad[2];
+    __device__ Page() = default;
+    __device__ __forceinline__ explicit Page(u32x4 head)
+        : exponents{(uint32_t)uniform((int)head[0]), (uint32_t)uniform((int)head[2])},
+          bad{(uint32_t)uniform((int)head[1]), (uint32_t)uniform((int)head[3])} {}
+    __device__ int key(int u) const { return min(max((int)(exponents[u] & 255u), kKv8Low), kKv8High); }
+    __device__ int value(int u) const { return min(max((int)(exponents[u] >> 8 & 255u), kKv8Low), kKv8High); }
 };
 
 // The rows' state of a wave, and one step's part in it.
@@ -180,60 +172,55 @@ template <typename T, int D, int MT> struct Rows8 {
             for (int i = 0; i < S::ACC; ++i) o[t][i] *= f;
     }
 
-    // scores of a step; q(k): this lane's operand of the queries for step k of the contraction
-    template <typename Q>
-    __device__ __forceinline__ void scores(Q&& q, const u32x4 (&code)[S::NT][S::KL], typename S::Acc (&acc)[S::NT]) {
-#pragma unroll
-        for (int t = 0; t < S::NT; ++t)
-#pragma unroll
-            for (int i = 0; i < S::ACC; ++i) acc[t][i] = 0.f;
-        F next_q = q(0);
-#pragma unroll
-        for (int k = 0; k < S::KS; ++k) {
-            const F qk = next_q;
-            if (k + 1 < S::KS) next_q = q(k + 1);              // read a step ahead
-            __builtin_amdgcn_sched_barrier(0);
+    // Step k of the contraction of a step's scores; q: this lane's operand of the queries.
+    static __device__ __forceinline__ void score(int k, const F& q, const u32x4 (&code)[S::NT][S::KL],
+                                                 typename S::Acc (&acc)[S::NT]) {
+        if (k == 0)
 #pragma unroll
             for (int t = 0; t < S::NT; ++t)
-                acc[t] = mma(widen8<T>(code[t][k / 2][2 * (k % 2)], code[t][k / 2][2 * (k % 2) + 1], 1.f), qk, acc[t]);
-        }
-        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int i = 0; i < S::ACC; ++i) acc[t][i] = 0.f;
+#pragma unroll
+        for (int t = 0; t < S::NT; ++t)
+            acc[t] = mma(widen8<T>(code[t][k / 2][2 * (k % 2)], code[t][k / 2][2 * (k % 2) + 1], 1.f), q, acc[t]);
     }
 
     // Adds weights times values; x: scores, their binary logarithms are x * factor - ref.
-    // P: type and number of parts of a weight.
-    template <typename P, int PARTS>
+    // P: type and number of parts of a weight; next(k): step k of the next step's scores.
+    template <typename P, int PARTS, typename Next>
     __device__ __forceinline__ void multiply(const float (&x)[16], float factor, float ref, const u32x4 (&code)[S::CT],
-                                             float vscale) {
+                                             float vscale, Next&& next) {
         using V = typename Frag<P>::type;
-        // The weights of eight slots are made while those before multiply the values: between two
-        // matrix instructions stand vector ones, in this order (the fences keep it), so that
-        // neither waits for the other.
+        // The weights are made while the next scores are: between two matrix instructions stand as
+        // many cycles of vector ones, in this order (the fences keep it), so that neither waits for
+        // the other.
         u32x4 part[PARTS][2];
         float even = 0.f;
-        auto make = [&](int u, int i) {
-            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * u + i], factor, -ref));
-            total += e;
-            if (i % 2 == 0) {
-                even = e;
-            } else {
-                const uint32_t h = pack2<P>(even, e);
-                part[0][u][i / 2] = h;
-                if constexpr (PARTS == 2)
-                    part[1][u][i / 2] = pack2<P>(even - widen_raw<P>(h & 0xffffu), e - widen_raw<P>(h >> 16));
-            }
-        };
+        constexpr int kEach = 16 / S::KS;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) make(0, i);
-        constexpr int kEach = 8 / S::CT;                       // weights for the next half by channel tile
+        for (int k = 0; k < S::KS; ++k) {
+            __builtin_amdgcn_sched_barrier(0);
+            next(k);
+#pragma unroll
+            for (int i = k * kEach; i < (k + 1) * kEach; ++i) {
+                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], factor, -ref));
+                total += e;
+                if (i % 2 == 0) {
+                    even = e;
+                } else {
+                    const uint32_t h = pack2<P>(even, e);
+                    part[0][i / 8][i / 2 % 4] = h;
+                    if constexpr (PARTS == 2)
+                        part[1][i / 8][i / 2 % 4] = pack2<P>(even - widen_raw<P>(h & 0xffffu), e - widen_raw<P>(h >> 16));
+                }
+            }
+        }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
 #pragma unroll
             for (int t = 0; t < S::CT; ++t) {
-                const V vf = widen8<P>(code[t][2 * u], code[t][2 * u + 1], vscale);
-#pragma unroll
-                for (int i = t * kEach; u == 0 && i < (t + 1) * kEach; ++i) make(1, i);
                 __builtin_amdgcn_sched_barrier(0);
+                const V vf = widen8<P>(code[t][2 * u], code[t][2 * u + 1], vscale);
 #pragma unroll
                 for (int p = 0; p < PARTS; ++p) o[t] = mma(vf, __builtin_bit_cast(V, part[p][u]), o[t]);
             }
@@ -241,67 +228,74 @@ template <typename T, int D, int MT> struct Rows8 {
         __builtin_amdgcn_sched_barrier(0);
     }
 
-    // Takes a page's scales in; whether its products can be of f16 numbers.
-    __device__ __forceinline__ bool admit(const Page& page) {
-        const int high = max(page.value[0], page.value[1]);
-        if (high) vlow = min(vlow, page.value[1] ? min(page.value[0], page.value[1]) : page.value[0]);
-        if (high > vref) {
-            const int now = min(high + kHead, kKv8High);
+    // Takes a page's scales in (of its first `blocks` blocks; the others hold nothing yet); whether
+    // its products can be of f16 numbers.
+    __device__ __forceinline__ bool admit(const Page& page, int blocks) {
+        if (!blocks) return vlow >= vref - kSpan;
+        const int v0 = page.value(0), v1 = blocks > 1 ? page.value(1) : v0;
+        vlow = min(vlow, min(v0, v1));
+        if (__builtin_expect(max(v0, v1) > vref, 0)) {
+            asm volatile("");
+            const int now = min(max(v0, v1) + kHead, kKv8High);
             rescale(vref ? kv8_pow2(max(127 + vref - now, 0)) : 1.f);
             vref = now;
         }
         return vlow >= vref - kSpan;
     }
 
-    // WIDE: the scales lie far apart; unit: binary logarithms per raw product
-    template <bool WIDE>
-    __device__ __forceinline__ void weigh(const typename S::Acc (&acc)[S::NT], const Page& page, int step, int g,
-                                          u32x4 (&code)[S::CT], const Sight& sight, float unit) {
-        const int slot = page.slot + S::run_slot(step, g);
+    // WIDE: the scales lie far apart.  MASKED: some row does not see all of the page, some slot holds
+    // nothing or nothing finite, or the page is none.  unit: binary logarithms per raw product.
+    // next: as multiply's.
+    template <bool WIDE, bool MASKED, typename Next>
+    __device__ __forceinline__ void weigh(const typename S::Acc (&acc)[S::NT], const Page& page, bool none, int slot,
+                                          int step, int g, u32x4 (&code)[S::CT], const Sight& sight, float unit,
+                                          Next&& next) {
         const bool second = MT == 16 ? g >= 2 : step == 1;     // of the page's blocks
-        const int ke = second ? page.key[1] : page.key[0], ve = second ? page.value[1] : page.value[0];
-        const float factor = fmaxf(unit * kv8_pow2(ke), 1e-37f);
+        const float factor = fmaxf(unit * kv8_pow2(second ? page.key(1) : page.key(0)), 1e-37f);
+        int ve = second ? page.value(1) : page.value(0);
         float x[16];
 #pragma unroll
         for (int v = 0; v < 16; ++v) x[v] = acc[MT == 16 ? v / 4 % S::NT : 0][v % S::ACC];
-        if (page.masked) {
-            asm volatile("");                              // a branch, not selections on every page
-            const uint32_t sees = page.none ? 0u : sight.of_run(slot);
+        if constexpr (MASKED) {
+            slot += S::run_slot(step, g);
+            const uint32_t sees = none ? 0u : sight.of_run(slot);
 #pragma unroll
             for (int v = 0; v < 16; ++v) x[v] = choose(sees, v, x[v], -__builtin_inff());
-        }
-        if (page.bad[0] | page.bad[1]) {
-            asm volatile("");
-            const uint32_t lost = (second ? page.bad[1] : page.bad[0]) >> (slot & 16) & sight.of_run(slot);
+            const uint32_t lost = (second ? page.bad[1] : page.bad[0]) >> (slot & 16) & sees;
+            if (__any(lost != 0u)) {
+                asm volatile("");
 #pragma unroll
-            for (int v = 0; v < 16; ++v) x[v] = choose(~lost, v, x[v], __builtin_nanf(""));
-        }
-        if (page.last) {
-            asm volatile("");
-            // behind the last slot anything may lie, and a weight of 0 does not make it 0
-            const uint32_t keep = page.none ? 0u : lowest(sight.filled - slot);
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                // bit i to byte i
-                const uint32_t bytes = (((keep >> (4 * w) & 15u) * 0x00204081u) & 0x01010101u) * 255u;
-#pragma unroll
-                for (int t = 0; t < S::CT; ++t) code[t][w] &= bytes;
+                for (int v = 0; v < 16; ++v) x[v] = choose(~lost, v, x[v], __builtin_nanf(""));
             }
+            // behind the last slot anything may lie, and a weight of 0 does not make it 0
+            const uint32_t keep = none ? 0u : lowest(sight.filled - slot);
+            if (__any(keep != 0xffffu)) {
+                asm volatile("");
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    // bit i to byte i
+                    const uint32_t bytes = (((keep >> (4 * w) & 15u) * 0x00204081u) & 0x01010101u) * 255u;
+#pragma unroll
+                    for (int t = 0; t < S::CT; ++t) code[t][w] &= bytes;
+                }
+            }
+            if (!keep) ve = vref;                          // nor need its scale be one
         }
         float best = x[0];
 #pragma unroll
         for (int v = 1; v < 16; ++v) best = fmaxf(best, x[v]);
         best = max_over_groups<MT>(best * factor);
-        if (__any(best > top)) {
+        if (__builtin_expect(__any(best > top), 0)) {
+            asm volatile("");
             const float now = fmaxf(top, best + kLag), f = fade(top, now);
             top = now;
             total *= f;
             rescale(f);
         }
         const float ref = (top == -__builtin_inff() ? 0.f : top) - kLift;
-        const float vscale = kv8_pow2(ve ? 134 + ve - vref : 127);
-        if constexpr (WIDE) multiply<bf16_t, 2>(x, factor, ref, code, vscale);
-        else multiply<f16_t, std::is_same<T, f16_t>::value ? 2 : 1>(x, factor, ref, code, vscale);
+        const float vscale = kv8_pow2(134 + ve - vref);
+        if constexpr (WIDE) multiply<bf16_t, 2>(x, factor, ref, code, vscale, next);
+        else multiply<f16_t, std::is_same<T, f16_t>::value ? 2 : 1>(x, factor, ref, code, vscale, next);
     }
 };
 
@@ -370,13 +364,13 @@ struct Kv8Seqs {
 
 // LDS of a workgroup.  Where TILES row tiles go over the same pages, each way keeps a ring of
 // them there: the page as it lies in memory but for its head, of which every wave has its own.
-template <typename T, int D, int MT, int TILES> struct Lds {
+template <typename T, int D, int MT, int TILES, bool RING> struct Lds {
     using S = Shape8<D, MT>;
     static constexpr int kWays = kWaves / TILES;
-    static constexpr int kRing = TILES == 1 ? 0 : kWays * D > 256 ? 2 : 3;
+    static constexpr int kRing = !RING ? 0 : 4;
     static constexpr int kRound = 32;                       // output registers joined at a time
     union {
-        uint8_t page[kWays][kRing ? kRing : 1][TILES == 1 ? 16 : Kv8<D>::kHead];
+        uint8_t page[kWays][kRing ? kRing : 1][RING ? Kv8<D>::kHead : 16];
         float o[kWaves][kRound][64];
     };
     uint32_t head[kWaves][kRing ? kRing : 1][64];
@@ -387,12 +381,12 @@ template <typename T, int D, int MT, int TILES> struct Lds {
 
 // TILES of 8 waves share a way: row tiles over the same pages.  8 / TILES ways take every
 // (8 / TILES)-th page each.
-template <typename T, int D, int MT, int TILES>
+template <typename T, int D, int MT, int TILES, bool RING>
 __global__ __launch_bounds__(kThreads, 2) void kv8_attention_kernel(Kv8AttentionArgs a, Line line, float* states,
                                                                     unsigned int* counters) {
     using S = Shape8<D, MT>;
     using F = typename Frag<T>::type;
-    using L = Lds<T, D, MT, TILES>;
+    using L = Lds<T, D, MT, TILES, RING>;
     constexpr int WAYS = L::kWays, kTiles = TILES, kRound = L::kRound;
     constexpr int kRegs = S::CT * S::ACC;                   // output registers
     __shared__ __attribute__((aligned(128))) L lds;
@@ -430,17 +424,24 @@ __global__ __launch_bounds__(kThreads, 2) void kv8_attention_kernel(Kv8Attention
         const int n = at.n, count = at.count, last_t = a.block.T - 1;
         // tokens of the tile group, and of this wave's tile
         const Seen seen = seqs.seen(n, count, divide(rt0 * MT, group), min(divide((rt0 + kTiles) * MT - 1, group), last_t));
-        const int t_first = divide(rt * MT, group), t_last = min(divide(rt * MT + MT - 1, group), last_t);
-        const int stop = min(last, seen.count());
         const bool past = rt * MT >= count * group;           // the tile has no valid row
+        const int stop = !RING && past ? 0 : min(last, seen.count());
         Sight sight;
         sight.n = n;
         sight.filled = seq_end(a.block, n, count, slots);     // slots past it may hold anything
         sight.sinks = a.window ? (int)min(a.sinks, (int64_t)slots) : slots;
-        // slots from `clear` on are seen by no more rows than these bounds say: pages between need no mask
-        const int clear_to = min(sight.filled, a.block.mode == DELS_KV4_CAUSAL ? n + t_first + 1
-                                               : a.block.mode == DELS_KV4_FULL ? n + count : n);
-        const int64_t clear_from = a.window ? (int64_t)n + t_last - a.window + 1 : 0;
+        // entries of the list of pages that every row of the tile sees whole: there nothing is masked
+        int plain, plain_end;
+        {
+            const int to = min(sight.filled, a.block.mode == DELS_KV4_CAUSAL ? n + divide(rt * MT, group) + 1
+                                             : a.block.mode == DELS_KV4_FULL ? n + count : n);
+            plain = seen.sinks;
+            if (a.window) {
+                const int64_t from = max((int64_t)n + min(divide(rt * MT + MT - 1, group), last_t) - a.window + 1, (int64_t)0);
+                plain += max(0, (int)min((from + kCachePage - 1) / kCachePage, (int64_t)seen.end) - seen.from);
+            }
+            plain_end = seen.sinks + to / kCachePage - seen.from;
+        }
 
         // the wave's pages
         const int32_t* ids = c.table + (int64_t)b * c.ld_table;
@@ -504,24 +505,29 @@ __global__ __launch_bounds__(kThreads, 2) void kv8_attention_kernel(Kv8Attention
             }
         };
         auto query = [&](int k) { return lds.q[tile][k][lane]; };
-        auto page_at = [&](int i, int id, u32x4 head) {
-            const int slot = seen.page(i) * kCachePage;
-            return Page(head, slot, !named(id),
-                        slot + kCachePage > clear_to || (slot < clear_from && slot + kCachePage > sight.sinks), sight.filled);
+        using False = std::false_type;
+        using True = std::true_type;
+        // blocks of page i that hold anything, and whether it needs masks
+        auto blocks_of = [&](int slot, int id) {
+            return named(id) ? min(2, (sight.filled - slot + kKv8Block - 1) / kKv8Block) : 0;
         };
-        using Narrow = std::false_type;
-        using Wide = std::true_type;
-        if constexpr (TILES == 1) {
-            // Keys and values of the next page are loaded into their registers once a step's scores
-            // or products are made, a page's work ahead of their use.  The loads are unconditional
-            // (of page 0 where there is none to load) and in the order of their use, so that each
-            // wait covers only what it needs.
+        auto is_plain = [&](int i, int id, const Page& page) {
+            return i >= plain && i < plain_end && named(id) && !(page.bad[0] | page.bad[1]);
+        };
+        if constexpr (!RING) {
+            // A step's scores are made during the step before.  Keys of a page are loaded into their
+            // registers once the scores of the page before are made, values once the products are: a
+            // page's work ahead of their use.  The loads are unconditional (of page 0 where there is
+            // none to load) and in the order of their use, so that each wait covers only what it
+            // needs.
             KeyRegs<D, MT> keys;
             ValueRegs<D, MT> values;
             u32x4 head;
-            int id = id_at(p);
+            typename S::Acc acc[S::NT];
             auto load_head = [&](const uint8_t* page) { head = *reinterpret_cast<const u32x4*>(page + Kv8<D>::kHead); };
+            int id = id_at(p), next_id = -1;                  // of pages p and p + WAYS
             if (p < stop) {
+                next_id = id_at(p + WAYS);
                 load_head(address(id));
 #pragma unroll
                 for (int step = 0; step < S::STEPS; ++step) {
@@ -531,39 +537,69 @@ __global__ __launch_bounds__(kThreads, 2) void kv8_attention_kernel(Kv8Attention
             }
             put_queries();
             lds_barrier();                                    // the loads stay in flight
-            auto work = [&](auto wide, const Page& page) {
-                const int next = id_at(p + WAYS);
-                const uint8_t* next_page = address(next);
-                load_head(next_page);
+            if (p < stop) {
+#pragma unroll
+                for (int k = 0; k < S::KS; ++k) Rows8<T, D, MT>::score(k, query(k), keys.code[0], acc);
+                keys.load(address(next_id), col, g, 0);
+                asm volatile("" ::: "memory");
+            }
+            auto work = [&](auto wide, auto masked, const Page& page, int slot) {
+                const int after = id_at(p + 2 * WAYS);
+                const bool none = !named(id);
+                load_head(address(next_id));
 #pragma unroll
                 for (int step = 0; step < S::STEPS; ++step) {
-                    typename S::Acc acc[S::NT];
-                    rows.scores(query, keys.code[step], acc);
-                    keys.load(next_page, col, g, step);
+                    constexpr int kLast = S::STEPS - 1;
+                    typename S::Acc next[S::NT];
+                    auto& code = keys.code[step == kLast ? 0 : step + 1];
+                    rows.template weigh<decltype(wide)::value, decltype(masked)::value>(
+                        acc, page, none, slot, step, g, values.code[step], sight, unit,
+                        [&](int k) { Rows8<T, D, MT>::score(k, query(k), code, next); });
+                    keys.load(address(step == kLast ? after : next_id), col, g, step == kLast ? 0 : step + 1);
+                    values.load(address(next_id), col, g, step);
                     asm volatile("" ::: "memory");
-                    rows.template weigh<decltype(wide)::value>(acc, page, step, g, values.code[step], sight, unit);
-                    values.load(next_page, col, g, step);
-                    asm volatile("" ::: "memory");
+#pragma unroll
+                    for (int t = 0; t < S::NT; ++t) acc[t] = next[t];
                 }
-                id = next;
+                id = next_id;
+                next_id = after;
                 p += WAYS;
             };
-            while (p < stop) {
-                const Page page = page_at(p, id, head);
-                if (!rows.admit(page)) break;                 // and from there on
-                work(Narrow{}, page);
+            // one loop for each kind of page: what they change stays in its registers
+            Page page;
+            int slot = 0;
+            bool whole_page = false, narrow = true;
+            auto meet = [&] {
+                if (p >= stop) return;
+                page = Page(head);
+                slot = seen.page(p) * kCachePage;
+                whole_page = is_plain(p, id, page);
+                narrow = rows.admit(page, blocks_of(slot, id));
+            };
+            meet();
+            while (p < stop && narrow) {
+                while (p < stop && narrow && !whole_page) {
+                    work(False{}, True{}, page, slot);
+                    meet();
+                }
+                while (p < stop && narrow && whole_page) {
+                    work(False{}, False{}, page, slot);
+                    meet();
+                }
             }
             while (p < stop) {
-                const Page page = page_at(p, id, head);
-                rows.admit(page);
-                work(Wide{}, page);
+                work(True{}, True{}, page, slot);
+                meet();
             }
         } else {
             // The waves of a way copy a page into its ring, a share of 1 KiB pieces and the head each,
-            // kRing - 1 pages ahead.  One barrier a page: past it, all shares of the page have
-            // arrived and nobody reads the buffer that the next copy goes to.
-            constexpr int kShare = Kv8<D>::kHead / 1024 / TILES, kPer = kShare + 1;
+            // kRing - 2 pages ahead of the one that arrives.  One barrier a page, at the start of the
+            // work on the page before, which reads this one's keys ahead: past it, all shares of the
+            // page have arrived and nobody reads the buffer that the next copy goes to, that of
+            // two pages before.
+            constexpr int kShare = Kv8<D>::kHead / 1024 / TILES, kPer = kShare + 1, kAhead = L::kRing - 2;
             const int pages = max(0, (stop - first + WAYS - 1) / WAYS);      // of the first way, which has most
+            int ids_ahead[kAhead + 2];                        // of the page that is worked on, the next, ..
             auto copy = [&](int i) {
                 const int id = id_at(first + way + i * WAYS);
                 const uint8_t* from = address(id);
@@ -577,107 +613,158 @@ __global__ __launch_bounds__(kThreads, 2) void kv8_attention_kernel(Kv8Attention
                 return id;
             };
             put_queries();
-            int ids_ahead[L::kRing];                          // of pages i, i + 1, ..
 #pragma unroll
-            for (int i = 0; i < L::kRing - 1; ++i) ids_ahead[i + 1] = i < pages ? copy(i) : -1;
+            for (int i = 0; i < kAhead; ++i) ids_ahead[i + 1] = i < pages ? copy(i) : -1;
+            // waits for page i, past what may still be on its way: the pages behind it
             auto arrive = [&](int i) {
-                // what may still be on its way: the pages behind this one
-                if (i + L::kRing - 2 < pages) asm volatile("s_waitcnt vmcnt(%0)" : : "n"((L::kRing - 2) * kPer) : "memory");
+                if (i + kAhead <= pages) asm volatile("s_waitcnt vmcnt(%0)" : : "n"((kAhead - 1) * kPer) : "memory");
                 else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
                 lds_barrier();
-                p = first + way + i * WAYS;
-#pragma unroll
-                for (int e = 0; e < L::kRing - 1; ++e) ids_ahead[e] = ids_ahead[e + 1];
-                if (i + L::kRing - 1 < pages) ids_ahead[L::kRing - 1] = copy(i + L::kRing - 1);
-                return !past && p < stop;
+                ids_ahead[kAhead + 1] = i + kAhead < pages ? copy(i + kAhead) : -1;
             };
-            auto take = [&](int i) {
-                return page_at(p, ids_ahead[0], *reinterpret_cast<const u32x4*>(lds.head[wave][i % L::kRing]));
+            F qr[S::KS];                                      // the tile's queries
+            // keys of the next two steps: those of the next one in keys[0] while the page's first step
+            // is worked on, in keys[1] during its second
+            u32x4 keys[2][1][S::KL];
+            typename S::Acc acc[1];
+            auto load_keys = [&](int i, int step) {
+                const uint8_t* at = lds.page[way][i % L::kRing] + 16 * lane + 32 * D * step;
+#pragma unroll
+                for (int e = 0; e < S::KL; ++e) keys[1 - step][0][e] = *reinterpret_cast<const u32x4*>(at + 1024 * e);
             };
-            auto work = [&](auto wide, int i, const Page& page) {
-                const uint8_t* at = lds.page[way][i % L::kRing] + 16 * lane;
-#pragma nounroll
-                for (int step = 0; step < S::STEPS; ++step) {
-                    u32x4 keys[S::NT][S::KL], values[S::CT];
-#pragma unroll
-                    for (int e = 0; e < S::KL; ++e)
-                        keys[0][e] = *reinterpret_cast<const u32x4*>(at + 32 * D * step + 1024 * e);
-#pragma unroll
-                    for (int t = 0; t < S::CT; ++t)
-                        values[t] = *reinterpret_cast<const u32x4*>(at + Kv8<D>::kValue + 32 * D * step +
-                                                                    (16 * D - 512) * g + 512 * t);
-                    typename S::Acc acc[S::NT];
-                    rows.scores(query, keys, acc);
-                    rows.template weigh<decltype(wide)::value>(acc, page, step, g, values, sight, unit);
-                }
+            auto score = [&](int k, const u32x4(&code)[1][S::KL], typename S::Acc(&to)[1]) {
+                Rows8<T, D, MT>::score(k, qr[k], code, to);
             };
             int i = 0;
-            bool here = false;                                // page i has been met, but not worked on
-            for (; i < pages; ++i) {
-                if (!arrive(i)) continue;
-                const Page page = take(i);
-                here = !rows.admit(page);
-                if (here) break;                              // and from there on
-                work(Narrow{}, i, page);
+            Page page;
+            int slot = 0;
+            bool mine = false, whole_page = false, narrow = true;
+            auto meet = [&] {                                 // page i, which has arrived
+                if (i >= pages) return;
+#pragma unroll
+                for (int e = 0; e <= kAhead; ++e) ids_ahead[e] = ids_ahead[e + 1];
+                p = first + way + i * WAYS;
+                mine = !past && p < stop;
+                whole_page = false;
+                if (!mine) return;
+                page = Page(*reinterpret_cast<const u32x4*>(lds.head[wave][i % L::kRing]));
+                slot = seen.page(p) * kCachePage;
+                whole_page = is_plain(p, ids_ahead[0], page);
+                narrow = rows.admit(page, blocks_of(slot, ids_ahead[0]));
+            };
+            // page i, and the first scores of the one behind it
+            auto work = [&](auto wide, auto masked) {
+                const bool none = !named(ids_ahead[0]);
+                const uint8_t* at = lds.page[way][i % L::kRing] + Kv8<D>::kValue + (16 * D - 512) * g + 16 * lane;
+#pragma unroll
+                for (int step = 0; step < S::STEPS; ++step) {
+                    if (step == 0 && i + 1 < pages) arrive(i + 1);
+                    load_keys(i + 1, step);                   // for the step after next
+                    u32x4 values[S::CT];
+#pragma unroll
+                    for (int t = 0; t < S::CT; ++t)
+                        values[t] = *reinterpret_cast<const u32x4*>(at + 32 * D * step + 512 * t);
+                    typename S::Acc next[1];
+                    rows.template weigh<decltype(wide)::value, decltype(masked)::value>(
+                        acc, page, none, slot, step, g, values, sight, unit, [&](int k) { score(k, keys[step], next); });
+                    acc[0] = next[0];
+                }
+                ++i;
+            };
+            auto pass = [&] {                                 // a page that this wave has no part in
+                if (i + 1 < pages) arrive(i + 1);
+                ++i;
+            };
+            if (pages) {
+                arrive(0);
+#pragma unroll
+                for (int k = 0; k < S::KS; ++k) qr[k] = query(k);
+                load_keys(0, 0);
+#pragma unroll
+                for (int k = 0; k < S::KS; ++k) score(k, keys[S::STEPS - 1], acc);
+                load_keys(0, 1);
             }
-            for (; i < pages; ++i) {
-                const bool mine = here || arrive(i);
-                here = false;
-                if (!mine) continue;
-                const Page page = take(i);
-                rows.admit(page);
-                work(Wide{}, i, page);
+            // one loop for each kind of page: what they change stays in its registers
+            meet();
+            while (i < pages && narrow) {
+                while (i < pages && narrow && !whole_page) {
+                    if (mine) work(False{}, True{});
+                    else pass();
+                    meet();
+                }
+                while (i < pages && narrow && whole_page) {
+                    work(False{}, False{});
+                    meet();
+                }
+            }
+            while (i < pages) {
+                if (mine) work(True{}, True{});
+                else pass();
+                meet();
             }
             __syncthreads();                                  // the ring's place is the join's
         }
 
         // ---- join the waves
-        const float ref = rows.top;
         const float total = sum_over_groups<MT>(rows.total);
-        if (g == 0) {
-            s_m[wave][col] = ref;
-            s_l[wave][col] = total;
-        }
-        __syncthreads();
         const bool whole = first == 0 && last == at.pages;
         // a piece has at most one state of rows that it begins and one of rows that it goes on with
         auto state_of = [&](int w, bool begins) {
             return states + ((int64_t)(2 * w + (begins ? 1 : 0)) * kTiles + tile) * kStateFloats<D, MT>;
         };
         float* state = state_of(piece, first == 0);
-        float m = -__builtin_inff(), l = 0.f;
+        float m = rows.top, l = total;
+        // registers 4 q .. 4 q + 3 of the joined outputs
+        auto put = [&](int q, const float* sum) {
+            if (whole) {
+                store4<T>(a, b, row, S::channel_of(q / (S::ACC / 4), q % (S::ACC / 4), g), sum, l != 0.f ? 1.f / l : 0.f);
+            } else {
+                auto* to = reinterpret_cast<unsigned long long*>(state + (q * 64 + lane) * 4);
 #pragma unroll
-        for (int w = tile * WAYS; w < (tile + 1) * WAYS; ++w) m = fmaxf(m, s_m[w][col]);
+                for (int v = 0; v < 4; v += 2)
+                    atomic_store_u64(to + v / 2, (unsigned long long)__float_as_uint(sum[v + 1]) << 32 |
+                                                     __float_as_uint(sum[v]));
+            }
+        };
+        const float shift = kv8_pow2(max(rows.vref - 7, 0));
+        if constexpr (WAYS == 1) {
 #pragma unroll
-        for (int w = tile * WAYS; w < (tile + 1) * WAYS; ++w) l += s_l[w][col] * fade(s_m[w][col], m);
-        const float inv = l != 0.f ? 1.f / l : 0.f;
-        const float f = fade(ref, m) * kv8_pow2(max(rows.vref - 7, 0));
+            for (int q = 0; q < kRegs / 4; ++q) {
+                float o[4];
 #pragma unroll
-        for (int r0 = 0; r0 < kRegs; r0 += kRound) {
-#pragma unroll
-            for (int j = 0; j < kRound && r0 + j < kRegs; ++j)
-                s_o[wave][j][lane] = rows.o[(r0 + j) / S::ACC][(r0 + j) % S::ACC] * f;
-            __syncthreads();
-            for (int jq = way; 4 * jq < kRound && r0 + 4 * jq < kRegs; jq += WAYS) {
-                float sum[4];
-#pragma unroll
-                for (int v = 0; v < 4; ++v) {
-                    sum[v] = 0.f;
-#pragma unroll
-                    for (int w = 0; w < WAYS; ++w) sum[v] += s_o[tile * WAYS + w][4 * jq + v][lane];
-                }
-                const int q = r0 / 4 + jq;                    // registers 4 q .. 4 q + 3
-                if (whole) {
-                    store4<T>(a, b, row, S::channel_of(q / (S::ACC / 4), q % (S::ACC / 4), g), sum, inv);
-                } else {
-                    auto* to = reinterpret_cast<unsigned long long*>(state + (q * 64 + lane) * 4);
-#pragma unroll
-                    for (int v = 0; v < 4; v += 2)
-                        atomic_store_u64(to + v / 2, (unsigned long long)__float_as_uint(sum[v + 1]) << 32 |
-                                                         __float_as_uint(sum[v]));
-                }
+                for (int v = 0; v < 4; ++v) o[v] = rows.o[(4 * q + v) / S::ACC][(4 * q + v) % S::ACC] * shift;
+                put(q, o);
+            }
+        } else {
+            if (g == 0) {
+                s_m[wave][col] = rows.top;
+                s_l[wave][col] = total;
             }
             __syncthreads();
+            m = -__builtin_inff(), l = 0.f;
+#pragma unroll
+            for (int w = tile * WAYS; w < (tile + 1) * WAYS; ++w) m = fmaxf(m, s_m[w][col]);
+#pragma unroll
+            for (int w = tile * WAYS; w < (tile + 1) * WAYS; ++w) l += s_l[w][col] * fade(s_m[w][col], m);
+            const float f = fade(rows.top, m) * shift;
+#pragma unroll
+            for (int r0 = 0; r0 < kRegs; r0 += kRound) {
+#pragma unroll
+                for (int j = 0; j < kRound && r0 + j < kRegs; ++j)
+                    s_o[wave][j][lane] = rows.o[(r0 + j) / S::ACC][(r0 + j) % S::ACC] * f;
+                __syncthreads();
+                for (int jq = way; 4 * jq < kRound && r0 + 4 * jq < kRegs; jq += WAYS) {
+                    float sum[4];
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) {
+                        sum[v] = 0.f;
+#pragma unroll
+                        for (int w = 0; w < WAYS; ++w) sum[v] += s_o[tile * WAYS + w][4 * jq + v][lane];
+                    }
+                    put(r0 / 4 + jq, sum);
+                }
+                __syncthreads();
+            }
         }
         if (way == 0 && g == 0) {
             if (whole) {
@@ -768,14 +855,18 @@ Plan plan(int64_t batch, int64_t T, int64_t q_heads, int64_t heads, int64_t max_
     const int64_t rows = T * (q_heads / heads), cus = device_cu_count();
     p.rows = rows <= 16 ? 16 : 32;
     const int64_t tiles = (rows + p.rows - 1) / p.rows;
-    // the widest workgroup that leaves the fewest waves without a tile
+    // Tiles of a workgroup: the more, the fewer times a page is loaded and waves' states are joined,
+    // as long as there is a workgroup for each CU; of those numbers the one that leaves the fewest
+    // waves without a tile, and never half of them.  One otherwise: its pages are split over
+    // eight waves, and over workgroups.  8 heads of 128, 4 rows a token: 32 sequences of 1000 slots, 8
+    // tiles 108 us one by one, 56 in eights, 2 tiles 35 and 29 in twos; 2 of 16000, 8 tiles 50 us
+    // one by one, 98 in eights.
     p.tiles = 1;
-    if (tiles > 1) {
-        int64_t best = INT64_MAX;
-        for (int wide : {8, 4, 2}) {
-            const int64_t waves = (tiles + wide - 1) / wide * wide;
-            if (waves < best) best = waves, p.tiles = wide;
-        }
+    int64_t fewest = 2 * tiles;
+    for (int64_t wide : {8, 4, 2}) {
+        const int64_t groups = (tiles + wide - 1) / wide;
+        if (p.rows == 32 && batch * heads * groups >= cus && groups * wide < fewest)
+            fewest = groups * wide, p.tiles = (int)wide;
     }
     p.line.tiles = (int)((tiles + p.tiles - 1) / p.tiles);
     p.line.least = kMinPages;
@@ -789,13 +880,16 @@ Plan plan(int64_t batch, int64_t T, int64_t q_heads, int64_t heads, int64_t max_
 
 size_t kv8_attention_data_bytes(int64_t batch, int64_t T, int64_t q_heads, int64_t heads, int64_t head_dim,
                                 int64_t max_pages) {
-    // what any shorter block takes too, so that a workspace for the longest serves every one: up to
-    // 8 tiles of 32 rows a piece, and no fewer pieces
-    const int64_t rows = T * (q_heads / heads);
-    const int64_t tiles = rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 ? 4 : 8;
-    const int64_t pieces = std::min<int64_t>(device_cu_count(), kMaxCounters / kCounterWords);
-    (void)batch, (void)max_pages;
-    return align256((size_t)pieces * 2 * tiles * sizeof(float) * (32 * head_dim + 2 * 32));
+    // what any shorter block takes too, so that a workspace for the longest serves every one: pieces
+    // as if each tile were a group of its own, and as many tiles a piece as there are groups for
+    const int64_t rows = T * (q_heads / heads), tile_rows = rows <= 16 ? 16 : 32, cus = device_cu_count();
+    const int64_t tiles = (rows + tile_rows - 1) / tile_rows, groups = batch * heads * tiles;
+    const int64_t units = groups * std::max<int64_t>(max_pages, 1);
+    const int64_t pieces = std::min<int64_t>({cus, kMaxCounters / kCounterWords,
+                                              std::max(groups, (units + kMinPages - 1) / kMinPages)});
+    int64_t wide = 1;
+    while (tile_rows == 32 && wide < 8 && wide < tiles && batch * heads * ((tiles + 2 * wide - 1) / (2 * wide)) >= cus) wide *= 2;
+    return align256((size_t)pieces * 2 * wide * sizeof(float) * (tile_rows * head_dim + 2 * tile_rows));
 }
 
 hipError_t launch_kv8_attention(const Kv8AttentionArgs& a, void* ws, size_t data_off, hipStream_t s) {
@@ -806,18 +900,19 @@ hipError_t launch_kv8_attention(const Kv8AttentionArgs& a, void* ws, size_t data
     auto by_size = [&](auto tag, auto size) {
         using T = decltype(tag);
         constexpr int D = decltype(size)::value;
-        auto go = [&](auto rows, auto tiles) {
-            hipLaunchKernelGGL((kv8_attention_kernel<T, D, decltype(rows)::value, decltype(tiles)::value>),
+        auto go = [&](auto rows, auto tiles, auto ring) {
+            hipLaunchKernelGGL((kv8_attention_kernel<T, D, decltype(rows)::value, decltype(tiles)::value, decltype(ring)::value>),
                                dim3(p.line.pieces), dim3(kThreads), 0, s, a, p.line, states, counters);
         };
         using std::integral_constant;
         using I16 = integral_constant<int, 16>;
         using I32 = integral_constant<int, 32>;
-        if (p.rows == 16) go(I16{}, integral_constant<int, 1>{});
-        else if (p.tiles == 1) go(I32{}, integral_constant<int, 1>{});
-        else if (p.tiles == 2) go(I32{}, integral_constant<int, 2>{});
-        else if (p.tiles == 4) go(I32{}, integral_constant<int, 4>{});
-        else go(I32{}, integral_constant<int, 8>{});
+        using No = std::false_type;
+        if (p.rows == 16) go(I16{}, integral_constant<int, 1>{}, No{});
+        else if (p.tiles == 1) go(I32{}, integral_constant<int, 1>{}, No{});
+        else if (p.tiles == 2) go(I32{}, integral_constant<int, 2>{}, No{});
+        else if (p.tiles == 4) go(I32{}, integral_constant<int, 4>{}, No{});
+        else go(I32{}, integral_constant<int, 8>{}, std::true_type{});
     };
     auto by_type = [&](auto tag) {
         if (c.head_dim == 64) by_size(tag, std::integral_constant<int, 64>{});

@@ -18,7 +18,6 @@ alike: row ``t`` of a block lies in slot ``lengths[b] + t``.
 from __future__ import annotations
 
 import ctypes
-from contextlib import nullcontext
 from typing import Optional
 
 import torch
@@ -78,17 +77,33 @@ class RotaryTable:
         self._ref = ctypes.byref(self._params)
 
 
-def _on(cache: PagedCache):
-    """The cache's GPU made the current one where it is not."""
-    if cache._index < 0 or torch.cuda.current_device() == cache._index:
-        return nullcontext()
-    return torch.cuda.device(cache._index)
+# the current GPU, without the wrapper's check that there is one
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
-def _position_args(positions: Optional[torch.Tensor], cache: PagedCache, T: int) -> tuple[Optional[int], int]:
+def _elsewhere_current(cache: PagedCache) -> bool:
+    """Whether the current GPU is not the cache's: then it is made so for the call."""
+    return cache._index >= 0 and _current_device() != cache._index
+
+
+def _require_pair(k: torch.Tensor, v: torch.Tensor, cache: PagedCache) -> tuple:
+    """(pointer, strides) of keys and values that are alike."""
+    kp = _require_rows(k, cache, cache.kv_heads, "k", _DTYPES)
+    if not isinstance(v, torch.Tensor) or v.get_device() != cache._index:
+        _elsewhere(v, cache, "v")
+    if v.dtype != k.dtype or v.shape != k.shape:
+        _require_rows(v, cache, cache.kv_heads, "v", _DTYPES)
+        raise ValueError("k and v must have one shape and dtype")
+    if v.stride() == k.stride():
+        return kp, (v.data_ptr(), *kp[1:])
+    return kp, _require_rows(v, cache, cache.kv_heads, "v", _DTYPES)
+
+
+_NO_ROWS = (None, 0, 0, 0)
+
+
+def _position_args(positions: torch.Tensor, cache: PagedCache, T: int) -> tuple[int, int]:
     """(pointer, row stride) of int32 [batch, T] positions."""
-    if positions is None:
-        return None, 0
     if not isinstance(positions, torch.Tensor) or positions.get_device() != cache._index:
         _elsewhere(positions, cache, "positions")
     if positions.dtype != torch.int32 or positions.shape != (cache.batch, T):
@@ -120,39 +135,43 @@ def kv8_append(cache: KV8Cache, k: torch.Tensor, v: torch.Tensor, lengths: torch
     table's slots are dropped.
     """
     _require_cache(cache, 8)
-    kp = _require_rows(k, cache, cache.kv_heads, "k", _DTYPES)
-    vp = _require_rows(v, cache, cache.kv_heads, "v", _DTYPES)
-    if v.dtype != k.dtype or v.shape != k.shape:
-        raise ValueError("k and v must have one shape and dtype")
+    if _elsewhere_current(cache):
+        with torch.cuda.device(cache._index):
+            return kv8_append(cache, k, v, lengths, counts=counts, rotary=rotary, positions=positions, q=q,
+                              q_out=q_out)
+    kp, vp = _require_pair(k, v, cache)
     T = k.shape[1]
     lp, cp = _require_ints(lengths, cache, "lengths"), _require_ints(counts, cache, "counts")
     if rotary is None and (positions is not None or q is not None):
         raise ValueError("positions and q are for a rotary table")
     if q is None and q_out is not None:
         raise ValueError("q_out is for q")
-    ref, qp, op, heads = None, (None, 0, 0, 0), (None, 0, 0, 0), 0
+    ref, qp, op, heads, pp, ldp = None, _NO_ROWS, _NO_ROWS, 0, None, 0
     if rotary is not None:
         if rotary._index != cache._index:
             raise ValueError(f"the rotary table is on {rotary.cos.device}, the cache on {cache.device}")
         if rotary.channels > cache.head_dim:
             raise ValueError(f"{rotary.channels} rotated channels, heads of {cache.head_dim}")
         ref = rotary._ref
-    pp, ldp = _position_args(positions, cache, T)
+        if positions is not None:
+            pp, ldp = _position_args(positions, cache, T)
     if q is not None:
         qp = _require_rows(q, cache, None, "q", (k.dtype,))
-        heads = q.shape[2]
-        if q.shape[1] != T or heads < 1 or heads % cache.kv_heads:
+        shape = q.shape
+        heads = shape[2]
+        if shape[1] != T or heads < 1 or heads % cache.kv_heads:
             raise ValueError(f"q must be [{cache.batch}, {T}, a multiple of {cache.kv_heads}, {cache.head_dim}], got "
-                             f"{tuple(q.shape)}")
+                             f"{tuple(shape)}")
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=cache.device)
-        elif q_out.shape != q.shape:
-            raise ValueError(f"q_out must be {tuple(q.shape)}, got {tuple(q_out.shape)}")
-        op = _require_rows(q_out, cache, heads, "q_out", (q.dtype,))
-    lib = _lib.load()
-    with _on(cache):
-        _lib.check(lib.dels_kv8_append(cache._ref, *kp, *vp, _DTYPES[k.dtype], lp, cp, T, ref, pp, ldp, *qp, heads,
-                                       *op, _stream_ptr(cache.device)), "dels_kv8_append")
+            q_out = torch.empty(shape, dtype=q.dtype, device=cache.device)
+            D = cache.head_dim
+            op = (q_out.data_ptr(), T * heads * D, heads * D, D)
+        elif q_out.shape != shape:
+            raise ValueError(f"q_out must be {tuple(shape)}, got {tuple(q_out.shape)}")
+        else:
+            op = _require_rows(q_out, cache, heads, "q_out", (q.dtype,))
+    _lib.check(_lib.load().dels_kv8_append(cache._ref, *kp, *vp, _DTYPES[k.dtype], lp, cp, T, ref, pp, ldp, *qp,
+                                           heads, *op, _stream_ptr(cache.device)), "dels_kv8_append")
     return q_out
 
 
@@ -164,15 +183,16 @@ def kv8_read(cache: KV8Cache, starts: torch.Tensor, T: int, *, counts: Optional[
     ``counts[b]`` on (None: none) and past the table's slots, NaN for rows that were not finite.
     """
     _require_cache(cache, 8)
+    if _elsewhere_current(cache):
+        with torch.cuda.device(cache._index):
+            return kv8_read(cache, starts, T, counts=counts, dtype=dtype)
     if dtype not in _DTYPES:
         raise TypeError(f"dtype {dtype} not supported")
     sp, cp = _require_ints(starts, cache, "starts"), _require_ints(counts, cache, "counts")
     k = torch.empty(cache.batch, T, cache.kv_heads, cache.head_dim, dtype=dtype, device=cache.device)
     v = torch.empty_like(k)
-    lib = _lib.load()
-    with _on(cache):
-        _lib.check(lib.dels_kv8_read(cache._ref, sp, cp, T, k.data_ptr(), v.data_ptr(), _DTYPES[dtype],
-                                     _stream_ptr(cache.device)), "dels_kv8_read")
+    _lib.check(_lib.load().dels_kv8_read(cache._ref, sp, cp, T, k.data_ptr(), v.data_ptr(), _DTYPES[dtype],
+                                         _stream_ptr(cache.device)), "dels_kv8_read")
     return k, v
 
 
@@ -196,6 +216,10 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, lengths: torch.Tensor, *, bl
     that see a score of NaN or +inf NaN in both.
     """
     _require_cache(cache, 8)
+    if _elsewhere_current(cache):
+        with torch.cuda.device(cache._index):
+            return kv8_attention(q, cache, lengths, block=block, counts=counts, scale=scale, window=window,
+                                 sinks=sinks, out=out, lse=lse, workspace=workspace)
     qp = _require_rows(q, cache, None, "q", _Q_DTYPES)
     batch, T, q_heads, D = q.shape
     if q_heads % cache.kv_heads:
@@ -220,17 +244,16 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, lengths: torch.Tensor, *, bl
     else:
         _require_lse(lse, cache, T, q_heads)
     lib = _lib.load()
-    with _on(cache):
-        need = cache._ws_bytes.get((T, q_heads))
-        if need is None:
-            need = lib.dels_kv8_attention_ws_bytes(batch, T, q_heads, cache.kv_heads, D, cache.max_pages)
-            cache._ws_bytes[T, q_heads] = need
-        stream = _stream_ptr(cache.device)
-        if workspace is None and not _capturing():
-            ws = _WORKSPACES.get(cache.device, need, stream)
-        else:
-            ws = _own_workspace(workspace, cache, need, counters=True)
-        _lib.check(lib.dels_kv8_attention(cache._ref, *qp, _DTYPES[q.dtype], q_heads, T, lp, cp, mode, mask, ld_mask,
-                                          cache._scale if scale is None else scale, window, sinks, *op,
-                                          lse.data_ptr(), ws.data_ptr(), ws.numel(), stream), "dels_kv8_attention")
+    need = cache._ws_bytes.get((T, q_heads))
+    if need is None:
+        need = lib.dels_kv8_attention_ws_bytes(batch, T, q_heads, cache.kv_heads, D, cache.max_pages)
+        cache._ws_bytes[T, q_heads] = need
+    stream = _stream_ptr(cache.device)
+    if workspace is None and not _capturing():
+        ws = _WORKSPACES.get(cache.device, need, stream)
+    else:
+        ws = _own_workspace(workspace, cache, need, counters=True)
+    _lib.check(lib.dels_kv8_attention(cache._ref, *qp, _DTYPES[q.dtype], q_heads, T, lp, cp, mode, mask, ld_mask,
+                                      cache._scale if scale is None else scale, window, sinks, *op, lse.data_ptr(),
+                                      ws.data_ptr(), ws.numel(), stream), "dels_kv8_attention")
     return out, lse
