@@ -96,6 +96,13 @@ __device__ __forceinline__ float choose(uint32_t bits, int v, float a, float b) 
 // The lowest k of 16 bits.
 __device__ __forceinline__ uint32_t lowest(int k) { return (1u << min(max(k, 0), 16)) - 1u; }
 
+// 16 bytes of a page.  Where 16 rows are all there are, each page is read once.
+template <int MT> __device__ __forceinline__ u32x4 page_words(const uint8_t* p) {
+    const auto* w = reinterpret_cast<const u32x4*>(p);
+    if constexpr (MT == 16) return __builtin_nontemporal_load(w);
+    else return *w;
+}
+
 template <int D, int MT> struct KeyRegs {
     using S = Shape8<D, MT>;
     u32x4 code[S::STEPS][S::NT][S::KL];
@@ -106,7 +113,7 @@ template <int D, int MT> struct KeyRegs {
 #pragma unroll
             for (int i = 0; i < S::KL; ++i)
                 code[step][t][i] =
-                    *reinterpret_cast<const u32x4*>(page + lane + 512 * S::NG * i + (MT == 16 ? 128 * t : 32 * D * step));
+                    page_words<MT>(page + lane + 512 * S::NG * i + (MT == 16 ? 128 * t : 32 * D * step));
     }
 };
 
@@ -117,7 +124,7 @@ template <int D, int MT> struct ValueRegs {
         const int lane = Kv8<D>::kValue + 16 * D * g + 16 * col;
 #pragma unroll
         for (int t = 0; t < S::CT; ++t)
-            code[step][t] = *reinterpret_cast<const u32x4*>(page + lane + 32 * D * step + 16 * MT * t);
+            code[step][t] = page_words<MT>(page + lane + 32 * D * step + 16 * MT * t);
     }
 };
 
