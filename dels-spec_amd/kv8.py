@@ -28,6 +28,7 @@ from .kv4 import (_Q_DTYPES, HEAD_DIMS, Block, PagedCache, _block_args, _capturi
 from .ops import _DTYPES, _WORKSPACES, _require_cuda, _stream_ptr
 
 BLOCK = 32             # slots that share a scale
+_FAR = 1 << 40         # past every slot
 
 
 def page_bytes(head_dim: int) -> int:
@@ -128,8 +129,8 @@ def kv8_append(cache: KV8Cache, k: torch.Tensor, v: torch.Tensor, lengths: torch
     its rows from ``counts[b]`` on 0.
 
     A block of 32 slots has one exponent for its keys and one for its values: the smallest
-    that holds its new rows, or that of the rows before them in the block if it is larger; if it
-    is smaller, those rows are rounded again.  A row of which something is NaN, infinite or over
+    that holds its new rows, or that of the rows before them in the block if it is larger (rows that
+    were rejected leave it as they made it); if it is smaller, those rows are rounded again.  A row of which something is NaN, infinite or over
     448 * 2^64, or whose position the table does not have, reads as NaN and gives scores of
     NaN, and takes no part in the exponents.  ``lengths`` is not changed; rows past the
     table's slots are dropped.
@@ -230,6 +231,8 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, lengths: torch.Tensor, *, bl
         window = 0
     elif window < 1 or sinks < 0:
         raise ValueError(f"window must be at least 1 and sinks at least 0, got {window} and {sinks}")
+    else:
+        window, sinks = min(window, _FAR), min(sinks, _FAR)
     lp, cp = _require_ints(lengths, cache, "lengths"), _require_ints(counts, cache, "counts")
     mode, mask, ld_mask = _block_args(block, cache, T)
     if out is None:

@@ -215,3 +215,7 @@ def test_attention_arguments(on_cpu, monkeypatch):
     assert got[-1][-3:-1] == (mine.data_ptr(), mine.numel()) and got[-1][14:16] == (0, 0)
     with pytest.raises(ValueError, match="workspace must be"):
         pkg.kv8_attention(q, cache, n, workspace=torch.zeros(1 << 18))
+    # numbers past 64 bits arrive as numbers past every slot
+    for big in (2**62, 2**63, 2**64 + 5):
+        pkg.kv8_attention(q, cache, n, window=big, sinks=big, workspace=mine)
+        assert min(got[-1][14:16]) > 1 << 31 and max(got[-1][14:16]) < 1 << 63
