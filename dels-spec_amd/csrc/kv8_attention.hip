@@ -375,10 +375,10 @@ template <typename T, int D, int MT, int TILES, bool RING> struct Lds {
     using S = Shape8<D, MT>;
     static constexpr int kWays = kWaves / TILES;
     static constexpr int kRing = !RING ? 0 : 4;
-    static constexpr int kRound = 32;                       // output registers joined at a time
+    static constexpr int kRound = TILES <= 2 ? 16 : 8;      // output registers joined at a time, in fours
     union {
         uint8_t page[kWays][kRing ? kRing : 1][RING ? Kv8<D>::kHead : 16];
-        float o[kWaves][kRound][64];
+        f32x4 o[kWaves][kRound][64];
     };
     uint32_t head[kWaves][kRing ? kRing : 1][64];
     typename Frag<T>::type q[TILES][S::KS][64];             // the tiles' queries, in operand order
@@ -755,20 +755,24 @@ __global__ __launch_bounds__(kThreads, 2) void kv8_attention_kernel(Kv8Attention
             for (int w = tile * WAYS; w < (tile + 1) * WAYS; ++w) l += s_l[w][col] * fade(s_m[w][col], m);
             const float f = fade(rows.top, m) * shift;
 #pragma unroll
-            for (int r0 = 0; r0 < kRegs; r0 += kRound) {
+            for (int r0 = 0; r0 < kRegs / 4; r0 += kRound) {
 #pragma unroll
-                for (int j = 0; j < kRound && r0 + j < kRegs; ++j)
-                    s_o[wave][j][lane] = rows.o[(r0 + j) / S::ACC][(r0 + j) % S::ACC] * f;
+                for (int j = 0; j < kRound && r0 + j < kRegs / 4; ++j) {
+                    f32x4 x;
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) x[v] = rows.o[4 * (r0 + j) / S::ACC][(4 * (r0 + j) + v) % S::ACC] * f;
+                    s_o[wave][j][lane] = x;
+                }
                 __syncthreads();
-                for (int jq = way; 4 * jq < kRound && r0 + 4 * jq < kRegs; jq += WAYS) {
-                    float sum[4];
+                for (int j = way; j < kRound && r0 + j < kRegs / 4; j += WAYS) {
+                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int v = 0; v < 4; ++v) {
-                        sum[v] = 0.f;
+                    for (int w = 0; w < WAYS; ++w) {
+                        const f32x4 x = s_o[tile * WAYS + w][j][lane];
 #pragma unroll
-                        for (int w = 0; w < WAYS; ++w) sum[v] += s_o[tile * WAYS + w][4 * jq + v][lane];
+                        for (int v = 0; v < 4; ++v) sum[v] += x[v];
                     }
-                    put(r0 / 4 + jq, sum);
+                    put(r0 + j, sum);
                 }
                 __syncthreads();
             }
@@ -809,38 +813,45 @@ __global__ __launch_bounds__(kThreads, 2) void kv8_attention_kernel(Kv8Attention
 #pragma unroll
                     for (int v = 0; v < 4; ++v) sum[i][v] = 0.f;
                 m = -__builtin_inff(), l = 0.f;
-                constexpr int kFlight = WAYS;                 // states in flight: their loads go to memory
-                for (int w0 = held.x; w0 < held.y; w0 += kFlight) {
-                    float tops[kFlight], sums[kFlight];
-                    unsigned long long two[kFlight][kMine][2];
+                // several states in flight: their loads go to memory
+                auto add = [&](auto flight) {
+                    constexpr int kFlight = decltype(flight)::value;
+                    for (int w0 = held.x; w0 < held.y; w0 += kFlight) {
+                        float tops[kFlight], sums[kFlight];
+                        unsigned long long two[kFlight][kMine][2];
 #pragma unroll
-                    for (int e = 0; e < kFlight; ++e) {
-                        const int w = min(w0 + e, held.y - 1);
-                        const float* st = state_of(w, w == held.x);
-                        tops[e] = load(st + MT * D + col);
-                        sums[e] = load(st + MT * D + MT + col);
+                        for (int e = 0; e < kFlight; ++e) {
+                            const int w = min(w0 + e, held.y - 1);
+                            const float* st = state_of(w, w == held.x);
+                            tops[e] = load(st + MT * D + col);
+                            sums[e] = load(st + MT * D + MT + col);
 #pragma unroll
-                        for (int i = 0; i < kMine; ++i) {
-                            const int q = min(way + i * WAYS, kRegs / 4 - 1);
-                            auto* from = reinterpret_cast<unsigned long long*>(const_cast<float*>(st + (q * 64 + lane) * 4));
+                            for (int i = 0; i < kMine; ++i) {
+                                const int q = min(way + i * WAYS, kRegs / 4 - 1);
+                                auto* from = reinterpret_cast<unsigned long long*>(const_cast<float*>(st + (q * 64 + lane) * 4));
 #pragma unroll
-                            for (int v = 0; v < 2; ++v) two[e][i][v] = atomic_load_u64(from + v);
+                                for (int v = 0; v < 2; ++v) two[e][i][v] = atomic_load_u64(from + v);
+                            }
+                        }
+#pragma unroll
+                        for (int e = 0; e < kFlight; ++e) {
+                            if (w0 + e >= held.y) break;
+                            const float now = fmaxf(m, tops[e]), old = fade(m, now), f = fade(tops[e], now);
+                            m = now;
+                            l = l * old + sums[e] * f;
+#pragma unroll
+                            for (int i = 0; i < kMine; ++i)
+#pragma unroll
+                                for (int v = 0; v < 4; ++v)
+                                    sum[i][v] = sum[i][v] * old +
+                                                __uint_as_float((uint32_t)(two[e][i][v / 2] >> (32 * (v & 1)))) * f;
                         }
                     }
-#pragma unroll
-                    for (int e = 0; e < kFlight; ++e) {
-                        if (w0 + e >= held.y) break;
-                        const float now = fmaxf(m, tops[e]), old = fade(m, now), f = fade(tops[e], now);
-                        m = now;
-                        l = l * old + sums[e] * f;
-#pragma unroll
-                        for (int i = 0; i < kMine; ++i)
-#pragma unroll
-                            for (int v = 0; v < 4; ++v)
-                                sum[i][v] = sum[i][v] * old +
-                                            __uint_as_float((uint32_t)(two[e][i][v / 2] >> (32 * (v & 1)))) * f;
-                    }
-                }
+                };
+                const int many = held.y - held.x;
+                if (WAYS > 4 && many > 4) add(std::integral_constant<int, WAYS>{});
+                else if (WAYS > 2 && many > 2) add(std::integral_constant<int, std::min(WAYS, 4)>{});
+                else add(std::integral_constant<int, std::min(WAYS, 2)>{});
                 const float inv = l != 0.f ? 1.f / l : 0.f;
 #pragma unroll
                 for (int i = 0; i < kMine; ++i) {
