@@ -11,7 +11,8 @@ int check_rotary(const dels_rotary* p, const PagedCache& c, int64_t T, const int
     if (!p) return positions ? fail(DELS_ERR_INVALID_ARGUMENT, "positions without a rotary table") : DELS_OK;
     if (p->channels < 16 || p->channels % 16 || p->channels > c.head_dim)
         return fail(DELS_ERR_INVALID_ARGUMENT, "%lld rotated channels of %d", (long long)p->channels, c.head_dim);
-    if (p->positions < 0 || p->positions >= (int64_t(1) << 40) || p->ld < p->channels / 2 || p->ld >= (int64_t(1) << 24))
+    if (p->positions < 0 || p->positions >= (int64_t(1) << 40) || p->ld < p->channels / 2 ||
+        p->ld >= (int64_t(1) << 24))
         return fail(DELS_ERR_INVALID_ARGUMENT, "bad rotary extents positions=%lld ld=%lld", (long long)p->positions,
                     (long long)p->ld);
     if (p->positions == 0) return fail(DELS_ERR_INVALID_ARGUMENT, "a rotary table of no positions");
@@ -55,7 +56,8 @@ int dels_kv8_append(const dels_kv8_cache* p, const void* k, int64_t k_batch, int
     if (q) {
         if (!rotary) return fail(DELS_ERR_INVALID_ARGUMENT, "q without a rotary table");
         if (q_heads <= 0 || !extent_ok(q_heads) || q_heads % c.heads || !grid_ok({q_heads / c.heads, 32, 8}))
-            return fail(DELS_ERR_INVALID_ARGUMENT, "%lld query heads over %d key/value heads", (long long)q_heads, c.heads);
+            return fail(DELS_ERR_INVALID_ARGUMENT, "%lld query heads over %d key/value heads", (long long)q_heads,
+                        c.heads);
         if ((rc = check_rows(q, q_batch, q_token, q_head, dtype, "q")) != DELS_OK) return rc;
         if ((rc = check_rows(q_out, out_batch, out_token, out_head, dtype, "q_out")) != DELS_OK) return rc;
     }

@@ -66,8 +66,9 @@ inline bool attention_ok(int64_t batch, int64_t T, int64_t q_heads, int64_t kv_h
 }
 
 // The arguments that attention and its weights share.
-inline int check_block(const PagedCache& c, const void* q, int64_t qb, int64_t qt, int64_t qh, int dtype, int64_t q_heads,
-                int64_t T, const int32_t* lengths, int block, const int64_t* mask, int64_t ld_mask, float scale) {
+inline int check_block(const PagedCache& c, const void* q, int64_t qb, int64_t qt, int64_t qh, int dtype,
+                       int64_t q_heads, int64_t T, const int32_t* lengths, int block, const int64_t* mask,
+                       int64_t ld_mask, float scale) {
     int rc = check_type(dtype, false);
     if (rc != DELS_OK) return rc;
     if (!extent_ok(T)) return fail(DELS_ERR_INVALID_ARGUMENT, "bad block length %lld", (long long)T);

@@ -18,6 +18,17 @@
 // which a float32 lse would show.  Weights enter as f16 numbers (2^-11 of each, an eighth of half a
 // step of a bf16 output), for f16 outputs in two parts.  Scores, maxima, sums and outputs are
 // fp32.
+//
+// What bounds it, at 32 query and 8 cache heads of 128 in bf16 (kernel times):
+//   32 sequences of up to 16300 slots, 1 token     154 us  memory: 935 MB at 6.1 TB/s
+//   131k slots, 16 tokens                            62 us  memory and issue: 270 MB at 4.4 TB/s, matrix cores 22 %
+//   4093 tokens through a window of 1024            113 us  issue: a step of 32 x 32 has 16 matrix
+//                                                           instructions (512 cycles) and 140 vector ones, 64 of
+//                                                           them conversions; 0.65 PFLOP/s, those masked counted
+//   8 sequences of up to 4000 slots, 16 tokens       20 us  latency: 2 us to know its pages, 13 for two or three
+//                                                           pages a wave, 5 joining waves and parts
+// Pages go straight from memory to registers, the next one's loads in flight behind a page's work; where
+// eight row tiles share them, through LDS.
 #include <algorithm>
 
 #include "kv8.h"
@@ -96,7 +107,8 @@ __device__ __forceinline__ float choose(uint32_t bits, int v, float a, float b) 
 // The lowest k of 16 bits.
 __device__ __forceinline__ uint32_t lowest(int k) { return (1u << min(max(k, 0), 16)) - 1u; }
 
-// 16 bytes of a page.  Where 16 rows are all there are, each page is read once.
+// 16 bytes of a page.  Where 16 rows are all there are, each page is read once, and need not stay
+// in the caches: 32 sequences of 16300 slots 171 -> 152 us.
 template <int MT> __device__ __forceinline__ u32x4 page_words(const uint8_t* p) {
     const auto* w = reinterpret_cast<const u32x4*>(p);
     if constexpr (MT == 16) return __builtin_nontemporal_load(w);
@@ -218,7 +230,8 @@ template <typename T, int D, int MT> struct Rows8 {
                     const uint32_t h = pack2<P>(even, e);
                     part[0][i / 8][i / 2 % 4] = h;
                     if constexpr (PARTS == 2)
-                        part[1][i / 8][i / 2 % 4] = pack2<P>(even - widen_raw<P>(h & 0xffffu), e - widen_raw<P>(h >> 16));
+                        part[1][i / 8][i / 2 % 4] =
+                            pack2<P>(even - widen_raw<P>(h & 0xffffu), e - widen_raw<P>(h >> 16));
                 }
             }
         }
@@ -308,7 +321,8 @@ template <typename T, int D, int MT> struct Rows8 {
 
 // Four channels of a row's output.
 template <typename T>
-__device__ __forceinline__ void store4(const Kv8AttentionArgs& a, int b, const Row& row, int ch, const float* o, float inv) {
+__device__ __forceinline__ void store4(const Kv8AttentionArgs& a, int b, const Row& row, int ch, const float* o,
+                                       float inv) {
     if (!row.in_block) return;
     uint16_t* p = static_cast<uint16_t*>(a.out) + (int64_t)b * a.out_batch + (int64_t)row.t * a.out_token +
                   (int64_t)row.hq * a.out_head + ch;
@@ -351,9 +365,11 @@ struct Kv8Seqs {
     __device__ int pages(int n, int count) const {
         const int all = seq_pages(seq_end(a.block, n, count, a.cache.slots()));
         if (!a.window) return all;
-        const int64_t more = a.block.mode == DELS_KV4_CAUSAL ? min(tokens, count) : a.block.mode == DELS_KV4_NONE ? 0 : count;
-        const int64_t span = (a.window + more + kCachePage - 2) / kCachePage + 1 + (a.sinks + kCachePage - 1) / kCachePage;
-        return (int)min((int64_t)all, span);
+        const int64_t more = a.block.mode == DELS_KV4_CAUSAL ? min(tokens, count)
+                             : a.block.mode == DELS_KV4_NONE ? 0
+                                                             : count;
+        const int64_t span = (a.window + more + kCachePage - 2) / kCachePage + 1;
+        return (int)min((int64_t)all, span + (a.sinks + kCachePage - 1) / kCachePage);
     }
     // of rows first .. last of the block (tokens)
     __device__ Seen seen(int n, int count, int first, int last) const {
@@ -375,7 +391,8 @@ template <typename T, int D, int MT, int TILES, bool RING> struct Lds {
     using S = Shape8<D, MT>;
     static constexpr int kWays = kWaves / TILES;
     static constexpr int kRing = !RING ? 0 : 4;
-    static constexpr int kRound = TILES <= 2 ? 16 : 8;      // output registers joined at a time, in fours
+    // output registers joined at a time, in fours: all where LDS has room (131k slots 67 -> 63 us)
+    static constexpr int kRound = TILES <= 2 ? 16 : 8;
     union {
         uint8_t page[kWays][kRing ? kRing : 1][RING ? Kv8<D>::kHead : 16];
         f32x4 o[kWaves][kRound][64];
@@ -430,7 +447,8 @@ __global__ __launch_bounds__(kThreads, 2) void kv8_attention_kernel(Kv8Attention
         const int last = min(at.pages, first + (u_end - u));
         const int n = at.n, count = at.count, last_t = a.block.T - 1;
         // tokens of the tile group, and of this wave's tile
-        const Seen seen = seqs.seen(n, count, divide(rt0 * MT, group), min(divide((rt0 + kTiles) * MT - 1, group), last_t));
+        const Seen seen =
+            seqs.seen(n, count, divide(rt0 * MT, group), min(divide((rt0 + kTiles) * MT - 1, group), last_t));
         const bool past = rt * MT >= count * group;           // the tile has no valid row
         const int stop = !RING && past ? 0 : min(last, seen.count());
         Sight sight;
@@ -444,7 +462,8 @@ __global__ __launch_bounds__(kThreads, 2) void kv8_attention_kernel(Kv8Attention
                                              : a.block.mode == DELS_KV4_FULL ? n + count : n);
             plain = seen.sinks;
             if (a.window) {
-                const int64_t from = max((int64_t)n + min(divide(rt * MT + MT - 1, group), last_t) - a.window + 1, (int64_t)0);
+                const int last_row = min(divide(rt * MT + MT - 1, group), last_t);
+                const int64_t from = max((int64_t)n + last_row - a.window + 1, (int64_t)0);
                 plain += max(0, (int)min((from + kCachePage - 1) / kCachePage, (int64_t)seen.end) - seen.from);
             }
             plain_end = seen.sinks + to / kCachePage - seen.from;
@@ -673,7 +692,8 @@ __global__ __launch_bounds__(kThreads, 2) void kv8_attention_kernel(Kv8Attention
                         values[t] = *reinterpret_cast<const u32x4*>(at + 32 * D * step + 512 * t);
                     typename S::Acc next[1];
                     rows.template weigh<decltype(wide)::value, decltype(masked)::value>(
-                        acc, page, none, slot, step, g, values, sight, unit, [&](int k) { score(k, keys[step], next); });
+                        acc, page, none, slot, step, g, values, sight, unit,
+                        [&](int k) { score(k, keys[step], next); });
                     acc[0] = next[0];
                 }
                 ++i;
@@ -724,7 +744,8 @@ __global__ __launch_bounds__(kThreads, 2) void kv8_attention_kernel(Kv8Attention
         // registers 4 q .. 4 q + 3 of the joined outputs
         auto put = [&](int q, const float* sum) {
             if (whole) {
-                store4<T>(a, b, row, S::channel_of(q / (S::ACC / 4), q % (S::ACC / 4), g), sum, l != 0.f ? 1.f / l : 0.f);
+                const int ch = S::channel_of(q / (S::ACC / 4), q % (S::ACC / 4), g);
+                store4<T>(a, b, row, ch, sum, l != 0.f ? 1.f / l : 0.f);
             } else {
                 auto* to = reinterpret_cast<unsigned long long*>(state + (q * 64 + lane) * 4);
 #pragma unroll
@@ -813,7 +834,8 @@ __global__ __launch_bounds__(kThreads, 2) void kv8_attention_kernel(Kv8Attention
 #pragma unroll
                     for (int v = 0; v < 4; ++v) sum[i][v] = 0.f;
                 m = -__builtin_inff(), l = 0.f;
-                // several states in flight: their loads go to memory
+                // several states in flight: their loads go to memory (8 x 16 rows 22.0 -> 20.7 us where no
+                // more of them are loaded than there are, in powers of two)
                 auto add = [&](auto flight) {
                     constexpr int kFlight = decltype(flight)::value;
                     for (int w0 = held.x; w0 < held.y; w0 += kFlight) {
@@ -822,13 +844,13 @@ __global__ __launch_bounds__(kThreads, 2) void kv8_attention_kernel(Kv8Attention
 #pragma unroll
                         for (int e = 0; e < kFlight; ++e) {
                             const int w = min(w0 + e, held.y - 1);
-                            const float* st = state_of(w, w == held.x);
+                            float* st = state_of(w, w == held.x);
                             tops[e] = load(st + MT * D + col);
                             sums[e] = load(st + MT * D + MT + col);
 #pragma unroll
                             for (int i = 0; i < kMine; ++i) {
                                 const int q = min(way + i * WAYS, kRegs / 4 - 1);
-                                auto* from = reinterpret_cast<unsigned long long*>(const_cast<float*>(st + (q * 64 + lane) * 4));
+                                auto* from = reinterpret_cast<unsigned long long*>(st + (q * 64 + lane) * 4);
 #pragma unroll
                                 for (int v = 0; v < 2; ++v) two[e][i][v] = atomic_load_u64(from + v);
                             }
@@ -871,6 +893,9 @@ struct Plan { int rows, tiles; Line line; };
 Plan plan(int64_t batch, int64_t T, int64_t q_heads, int64_t heads, int64_t max_pages) {
     Plan p{};
     const int64_t rows = T * (q_heads / heads), cus = device_cu_count();
+    // Tiles of 16 rows where one takes all: 32 x 16 rows of 16300 slots 153 us, 175 as half a tile of 32;
+    // 8 x 16 rows of 4000 slots 17.8 and 21.1.  Two of them take twice as long as one of 32 does where
+    // memory bounds it (32 x 32 rows: 297 and 175 us), and 1.5 us less in short calls.
     p.rows = rows <= 16 ? 16 : 32;
     const int64_t tiles = (rows + p.rows - 1) / p.rows;
     // Tiles of a workgroup: the more, the fewer times a page is loaded and waves' states are joined,
@@ -878,7 +903,8 @@ Plan plan(int64_t batch, int64_t T, int64_t q_heads, int64_t heads, int64_t max_
     // waves without a tile, and never half of them.  One otherwise: its pages are split over
     // eight waves, and over workgroups.  8 heads of 128, 4 rows a token: 32 sequences of 1000 slots, 8
     // tiles 108 us one by one, 56 in eights, 2 tiles 35 and 29 in twos; 2 of 16000, 8 tiles 50 us
-    // one by one, 98 in eights.
+    // one by one, 98 in eights; 4093 tokens through a window of 1024: 174, 155, 135 and 115 us by
+    // ones, twos, fours and eights; 8 sequences of 4000 slots, 2 tiles: 21 by ones, 29 in twos.
     p.tiles = 1;
     int64_t fewest = 2 * tiles;
     for (int64_t wide : {8, 4, 2}) {
@@ -889,8 +915,8 @@ Plan plan(int64_t batch, int64_t T, int64_t q_heads, int64_t heads, int64_t max_
     p.line.tiles = (int)((tiles + p.tiles - 1) / p.tiles);
     p.line.least = kMinPages;
     const int64_t units = batch * heads * p.line.tiles * std::max<int64_t>(max_pages, 1);
-    p.line.pieces = (int)std::min<int64_t>({cus, kMaxCounters / kCounterWords,
-                                            std::max(batch * heads * p.line.tiles, (units + kMinPages - 1) / kMinPages)});
+    const int64_t most = std::max(batch * heads * p.line.tiles, (units + kMinPages - 1) / kMinPages);
+    p.line.pieces = (int)std::min<int64_t>({cus, kMaxCounters / kCounterWords, most});
     return p;
 }
 
@@ -906,7 +932,8 @@ size_t kv8_attention_data_bytes(int64_t batch, int64_t T, int64_t q_heads, int64
     const int64_t pieces = std::min<int64_t>({cus, kMaxCounters / kCounterWords,
                                               std::max(groups, (units + kMinPages - 1) / kMinPages)});
     int64_t wide = 1;
-    while (tile_rows == 32 && wide < 8 && wide < tiles && batch * heads * ((tiles + 2 * wide - 1) / (2 * wide)) >= cus) wide *= 2;
+    auto enough = [&](int64_t w) { return batch * heads * ((tiles + w - 1) / w) >= cus; };
+    while (tile_rows == 32 && wide < 8 && wide < tiles && enough(2 * wide)) wide *= 2;
     return align256((size_t)pieces * 2 * wide * sizeof(float) * (tile_rows * head_dim + 2 * tile_rows));
 }
 
@@ -919,8 +946,10 @@ hipError_t launch_kv8_attention(const Kv8AttentionArgs& a, void* ws, size_t data
         using T = decltype(tag);
         constexpr int D = decltype(size)::value;
         auto go = [&](auto rows, auto tiles, auto ring) {
-            hipLaunchKernelGGL((kv8_attention_kernel<T, D, decltype(rows)::value, decltype(tiles)::value, decltype(ring)::value>),
-                               dim3(p.line.pieces), dim3(kThreads), 0, s, a, p.line, states, counters);
+            constexpr int MT = decltype(rows)::value, TILES = decltype(tiles)::value;
+            constexpr bool RING = decltype(ring)::value;
+            hipLaunchKernelGGL((kv8_attention_kernel<T, D, MT, TILES, RING>), dim3(p.line.pieces), dim3(kThreads), 0, s,
+                               a, p.line, states, counters);
         };
         using std::integral_constant;
         using I16 = integral_constant<int, 16>;

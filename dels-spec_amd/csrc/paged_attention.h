@@ -211,7 +211,8 @@ struct Cuts {
     template <typename Seqs> __device__ Cuts(const Scan<Seqs>& s, const Line& line, int most) {
         // `least` keeps tiles of few pages whole; it gathers no more of them than an even share
         const int groups = s.seqs.batch * s.per;
-        share = max(min(line.least, divide(s.total + groups - 1, groups)), divide(s.total + line.pieces - 1, line.pieces));
+        share = max(min(line.least, divide(s.total + groups - 1, groups)),
+                    divide(s.total + line.pieces - 1, line.pieces));
         own_parts = false;
         parts = upto = 0;
         if (s.seqs.batch > 64) return;

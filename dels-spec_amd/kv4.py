@@ -144,7 +144,8 @@ def _require_ints(t: Optional[torch.Tensor], cache: PagedCache, name: str) -> Op
     return t.data_ptr()
 
 
-def _require_rows(t: torch.Tensor, cache: PagedCache, heads: Optional[int], name: str, dtypes) -> tuple[int, int, int, int]:
+def _require_rows(t: torch.Tensor, cache: PagedCache, heads: Optional[int], name: str,
+                  dtypes) -> tuple[int, int, int, int]:
     """(pointer, strides) of a [batch, T, heads, head_dim] tensor with unit channel stride."""
     if not isinstance(t, torch.Tensor) or t.get_device() != cache._index:
         _elsewhere(t, cache, name)

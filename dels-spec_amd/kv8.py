@@ -129,10 +129,11 @@ def kv8_append(cache: KV8Cache, k: torch.Tensor, v: torch.Tensor, lengths: torch
     its rows from ``counts[b]`` on 0.
 
     A block of 32 slots has one exponent for its keys and one for its values: the smallest
-    that holds its new rows, or that of the rows before them in the block if it is larger (rows that
-    were rejected leave it as they made it); if it is smaller, those rows are rounded again.  A row of which something is NaN, infinite or over
-    448 * 2^64, or whose position the table does not have, reads as NaN and gives scores of
-    NaN, and takes no part in the exponents.  ``lengths`` is not changed; rows past the
+    that holds its new rows, or that of the rows before them in the block if it is larger (rows
+    that were rejected leave it as they made it); if it is smaller, those rows are rounded again.
+    A row of which something is NaN, infinite or over 448 * 2^64, or whose position the table
+    does not have, reads as NaN and gives scores of NaN, and takes no part in the exponents.
+    ``lengths`` is not changed; rows past the
     table's slots are dropped.
     """
     _require_cache(cache, 8)
