@@ -21,7 +21,7 @@
 //
 // What bounds it, at 32 query and 8 cache heads of 128 in bf16 (kernel times):
 //   32 sequences of up to 16300 slots, 1 token     154 us  memory: 935 MB at 6.1 TB/s
-//   131k slots, 16 tokens                            62 us  memory and issue: 270 MB at 4.4 TB/s, matrix cores 22 %
+//   131k slots, 16 tokens                            62 us  memory and issue: 270 MB at 4.4 TB/s, matrix cores 23 %
 //   4093 tokens through a window of 1024            113 us  issue: a step of 32 x 32 has 16 matrix
 //                                                           instructions (512 cycles) and 140 vector ones, 64 of
 //                                                           them conversions; 0.65 PFLOP/s, those masked counted

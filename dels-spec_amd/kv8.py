@@ -133,8 +133,7 @@ def kv8_append(cache: KV8Cache, k: torch.Tensor, v: torch.Tensor, lengths: torch
     that were rejected leave it as they made it); if it is smaller, those rows are rounded again.
     A row of which something is NaN, infinite or over 448 * 2^64, or whose position the table
     does not have, reads as NaN and gives scores of NaN, and takes no part in the exponents.
-    ``lengths`` is not changed; rows past the
-    table's slots are dropped.
+    ``lengths`` is not changed; rows past the table's slots are dropped.
     """
     _require_cache(cache, 8)
     if _elsewhere_current(cache):
