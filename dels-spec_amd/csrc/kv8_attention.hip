@@ -107,15 +107,16 @@ __device__ __forceinline__ float choose(uint32_t bits, int v, float a, float b) 
 // The lowest k of 16 bits.
 __device__ __forceinline__ uint32_t lowest(int k) { return (1u << min(max(k, 0), 16)) - 1u; }
 
-// 16 bytes of a page.  Where 16 rows are all there are, each page is read once, and need not stay
-// in the caches: 32 sequences of 16300 slots 171 -> 152 us.
-template <int MT> __device__ __forceinline__ u32x4 page_words(const uint8_t* p) {
+// 16 bytes of a page.  ONCE: one row tile is all there is, so each page is read once, and need not
+// stay in the caches: 32 sequences of 16300 slots 171 -> 152 us for 16 rows, 175 -> 156 for 32.  Of two
+// tiles the second finds the page there: 64 rows 287 us, 302 without.
+template <bool ONCE> __device__ __forceinline__ u32x4 page_words(const uint8_t* p) {
     const auto* w = reinterpret_cast<const u32x4*>(p);
-    if constexpr (MT == 16) return __builtin_nontemporal_load(w);
+    if constexpr (ONCE) return __builtin_nontemporal_load(w);
     else return *w;
 }
 
-template <int D, int MT> struct KeyRegs {
+template <int D, int MT, bool ONCE> struct KeyRegs {
     using S = Shape8<D, MT>;
     u32x4 code[S::STEPS][S::NT][S::KL];
     __device__ __forceinline__ void load(const uint8_t* page, int col, int g, int step) {
@@ -125,18 +126,18 @@ template <int D, int MT> struct KeyRegs {
 #pragma unroll
             for (int i = 0; i < S::KL; ++i)
                 code[step][t][i] =
-                    page_words<MT>(page + lane + 512 * S::NG * i + (MT == 16 ? 128 * t : 32 * D * step));
+                    page_words<ONCE>(page + lane + 512 * S::NG * i + (MT == 16 ? 128 * t : 32 * D * step));
     }
 };
 
-template <int D, int MT> struct ValueRegs {
+template <int D, int MT, bool ONCE> struct ValueRegs {
     using S = Shape8<D, MT>;
     u32x4 code[S::STEPS][S::CT];
     __device__ __forceinline__ void load(const uint8_t* page, int col, int g, int step) {
         const int lane = Kv8<D>::kValue + 16 * D * g + 16 * col;
 #pragma unroll
         for (int t = 0; t < S::CT; ++t)
-            code[step][t] = page_words<MT>(page + lane + 32 * D * step + 16 * MT * t);
+            code[step][t] = page_words<ONCE>(page + lane + 32 * D * step + 16 * MT * t);
     }
 };
 
@@ -405,7 +406,7 @@ template <typename T, int D, int MT, int TILES, bool RING> struct Lds {
 
 // TILES of 8 waves share a way: row tiles over the same pages.  8 / TILES ways take every
 // (8 / TILES)-th page each.
-template <typename T, int D, int MT, int TILES, bool RING>
+template <typename T, int D, int MT, int TILES, bool RING, bool ONCE>
 __global__ __launch_bounds__(kThreads, 2) void kv8_attention_kernel(Kv8AttentionArgs a, Line line, float* states,
                                                                     unsigned int* counters) {
     using S = Shape8<D, MT>;
@@ -546,8 +547,8 @@ __global__ __launch_bounds__(kThreads, 2) void kv8_attention_kernel(Kv8Attention
             // page's work ahead of their use.  The loads are unconditional (of page 0 where there is
             // none to load) and in the order of their use, so that each wait covers only what it
             // needs.
-            KeyRegs<D, MT> keys;
-            ValueRegs<D, MT> values;
+            KeyRegs<D, MT, ONCE> keys;
+            ValueRegs<D, MT, ONCE> values;
             u32x4 head;
             typename S::Acc acc[S::NT];
             auto load_head = [&](const uint8_t* page) { head = *reinterpret_cast<const u32x4*>(page + Kv8<D>::kHead); };
@@ -569,7 +570,16 @@ __global__ __launch_bounds__(kThreads, 2) void kv8_attention_kernel(Kv8Attention
                 keys.load(address(next_id), col, g, 0);
                 asm volatile("" ::: "memory");
             }
+            // Tiles over the same pages go through them in step, so that the second finds a page in the
+            // caches: 64 rows over 32 sequences of 16300 slots 285 -> 224 us, of 2000 slots 38 -> 36; 128
+            // rows 379 -> 352 and 56 -> 57.  All waves wait as often, those without pages too.
+            int left = TILES == 1 ? 0 : max(0, (min(last, seen.count()) - first + WAYS - 1) / WAYS);
+            auto keep_step = [&] {
+                __builtin_amdgcn_s_barrier();
+                --left;
+            };
             auto work = [&](auto wide, auto masked, const Page& page, int slot) {
+                if constexpr (TILES > 1) keep_step();
                 const int after = id_at(p + 2 * WAYS);
                 const bool none = !named(id);
                 load_head(address(next_id));
@@ -617,6 +627,7 @@ __global__ __launch_bounds__(kThreads, 2) void kv8_attention_kernel(Kv8Attention
                 work(True{}, True{}, page, slot);
                 meet();
             }
+            while (left > 0) keep_step();
         } else {
             // The waves of a way copy a page into its ring, a share of 1 KiB pieces and the head each,
             // kRing - 2 pages ahead of the one that arrives.  One barrier a page, at the start of the
@@ -893,9 +904,9 @@ struct Plan { int rows, tiles; Line line; };
 Plan plan(int64_t batch, int64_t T, int64_t q_heads, int64_t heads, int64_t max_pages) {
     Plan p{};
     const int64_t rows = T * (q_heads / heads), cus = device_cu_count();
-    // Tiles of 16 rows where one takes all: 32 x 16 rows of 16300 slots 153 us, 175 as half a tile of 32;
+    // Tiles of 16 rows where one takes all: 32 x 16 rows of 16300 slots 153 us, 157 as half a tile of 32;
     // 8 x 16 rows of 4000 slots 17.8 and 21.1.  Two of them take twice as long as one of 32 does where
-    // memory bounds it (32 x 32 rows: 297 and 175 us), and 1.5 us less in short calls.
+    // memory bounds it (32 x 32 rows: 297 and 157 us), and 1.5 us less in short calls.
     p.rows = rows <= 16 ? 16 : 32;
     const int64_t tiles = (rows + p.rows - 1) / p.rows;
     // Tiles of a workgroup: the more, the fewer times a page is loaded and waves' states are joined,
@@ -945,21 +956,23 @@ hipError_t launch_kv8_attention(const Kv8AttentionArgs& a, void* ws, size_t data
     auto by_size = [&](auto tag, auto size) {
         using T = decltype(tag);
         constexpr int D = decltype(size)::value;
-        auto go = [&](auto rows, auto tiles, auto ring) {
+        auto go = [&](auto rows, auto tiles, auto ring, auto once) {
             constexpr int MT = decltype(rows)::value, TILES = decltype(tiles)::value;
-            constexpr bool RING = decltype(ring)::value;
-            hipLaunchKernelGGL((kv8_attention_kernel<T, D, MT, TILES, RING>), dim3(p.line.pieces), dim3(kThreads), 0, s,
-                               a, p.line, states, counters);
+            constexpr bool RING = decltype(ring)::value, ONCE = decltype(once)::value;
+            hipLaunchKernelGGL((kv8_attention_kernel<T, D, MT, TILES, RING, ONCE>), dim3(p.line.pieces), dim3(kThreads),
+                               0, s, a, p.line, states, counters);
         };
         using std::integral_constant;
         using I16 = integral_constant<int, 16>;
         using I32 = integral_constant<int, 32>;
+        using Yes = std::true_type;
         using No = std::false_type;
-        if (p.rows == 16) go(I16{}, integral_constant<int, 1>{}, No{});
-        else if (p.tiles == 1) go(I32{}, integral_constant<int, 1>{}, No{});
-        else if (p.tiles == 2) go(I32{}, integral_constant<int, 2>{}, No{});
-        else if (p.tiles == 4) go(I32{}, integral_constant<int, 4>{}, No{});
-        else go(I32{}, integral_constant<int, 8>{}, std::true_type{});
+        if (p.rows == 16) go(I16{}, integral_constant<int, 1>{}, No{}, Yes{});
+        else if (p.tiles == 1 && p.line.tiles == 1) go(I32{}, integral_constant<int, 1>{}, No{}, Yes{});
+        else if (p.tiles == 1) go(I32{}, integral_constant<int, 1>{}, No{}, No{});
+        else if (p.tiles == 2) go(I32{}, integral_constant<int, 2>{}, No{}, No{});
+        else if (p.tiles == 4) go(I32{}, integral_constant<int, 4>{}, No{}, No{});
+        else go(I32{}, integral_constant<int, 8>{}, Yes{}, No{});
     };
     auto by_type = [&](auto tag) {
         if (c.head_dim == 64) by_size(tag, std::integral_constant<int, 64>{});
