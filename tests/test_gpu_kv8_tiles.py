@@ -138,3 +138,31 @@ def test_queries_of_nan_stay_in_their_rows(pkg, dev):
         K[b, :, m + T:], V[b, :, m + T:] = 0, 0
     check(clean, K, V, np.ones((B, 64 * pages), bool), lengths, counts, "causal", None, None, 0, out, lse, "bf16",
           D ** -0.5)
+
+
+@pytest.mark.parametrize("T,D,window", [(8, 128, None), (16, 128, None), (32, 64, 100), (64, 128, None)])
+def test_tiles_replay_in_a_graph(pkg, dev, T, D, window):
+    """Captured once and replayed on new queries and lengths, twice each, with eager calls between: the same bits."""
+    say("tiles in a graph", T, D, window)
+    pages = 8
+    lengths = [(37 * b + 5) % (64 * pages - T) for b in range(B)]
+    cache, q, _ = attention_inputs(pkg, dev, B, T, H * G, H, D, pages, "bf16", "none", [64 * pages] * B, None, T)
+    n, qd = ints(lengths, dev), q.to(dev)
+    kw = dict(block="none", window=window, sinks=3 if window else 0)
+    pkg.kv8_attention(qd, cache, n, **kw)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = pkg.kv8_attention(qd, cache, n, **kw)
+    g = torch.Generator(device=dev).manual_seed(T)
+    for i in range(4):
+        qd.copy_(torch.randn(qd.shape, generator=g, device=dev))
+        n.copy_(torch.roll(n, 1))
+        eager = pkg.kv8_attention(qd, cache, n, **kw)
+        for _ in range(2):
+            for x in captured:
+                x.fill_(7)
+            graph.replay()
+            torch.cuda.synchronize()
+            for x, y in zip(captured, eager):
+                assert torch.equal(x, y), i
