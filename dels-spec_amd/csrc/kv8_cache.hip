@@ -106,7 +106,14 @@ __device__ __forceinline__ uint32_t exponent_of(float top) {
     return (uint32_t)min(max(e, kKv8Low), kKv8High);
 }
 
-// Four codes rounded under an exponent 2^-k times as large: by = 2^k.
+// What codes under the exponent `was` are multiplied by under a larger one.  Exponents lie up to 128
+// apart, and from 127 on the power of two is no normal float: 0, and far above that no code leaves
+// anything but its sign.
+__device__ __forceinline__ float shrink_factor(uint32_t was, uint32_t now) {
+    return kv8_pow2((uint32_t)max(127 + (int)was - (int)now, 0));
+}
+
+// Four codes rounded under a larger exponent.
 __device__ __forceinline__ uint32_t shrink(uint32_t w, float by) {
     const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
     return f32x4_to_e4m3(lo[0] * by, lo[1] * by, hi[0] * by, hi[1] * by);
@@ -246,7 +253,7 @@ __global__ __launch_bounds__(kCacheThreads) void kv8_append_kernel(AppendArgs a)
         *reinterpret_cast<u32x4*>(&s_v[row][16 * part]) = w;
     }
     if (kept && ke > old_ke) {                         // a thread: 16 channels of a kept slot
-        const float by = kv8_pow2(127u + old_ke - ke);
+        const float by = shrink_factor(old_ke, ke);
         const int place = tid % 32;
         const int s = 16 * (place / 4 % 2) + 4 * (place / 8) + place % 4;
         for (int piece = tid / 32; s < kept && piece < U; piece += kCacheThreads / 32) {
@@ -273,7 +280,7 @@ __global__ __launch_bounds__(kCacheThreads) void kv8_append_kernel(AppendArgs a)
     u32x4 w = {0u, 0u, 0u, 0u};
     if (kept) w = *p;
     if (moves) {
-        const float by = kv8_pow2(127u + old_ve - ve);
+        const float by = shrink_factor(old_ve, ve);
 #pragma unroll
         for (int i = 0; i < 4; ++i) w[i] = shrink(w[i], by);
     }
