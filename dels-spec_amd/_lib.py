@@ -115,8 +115,15 @@ class RotaryParams(ctypes.Structure):
                 ("interleaved", _int)]
 
 
+class Kv8OptionsParams(ctypes.Structure):
+    """Mirror of ``struct dels_kv8_options`` in include/dels.h."""
+
+    _fields_ = [("positions", _ptr), ("ld_positions", _i64)]
+
+
 _kv4 = ctypes.POINTER(Kv4CacheParams)
 _rotary = ctypes.POINTER(RotaryParams)
+_kv8_options = ctypes.POINTER(Kv8OptionsParams)
 
 # name -> (restype, argtypes); every symbol include/dels.h declares.
 SIGNATURES = {
@@ -198,6 +205,9 @@ SIGNATURES = {
     "dels_kv8_attention_ws_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64, _i64]),
     "dels_kv8_attention": (_int, [_kv4, _ptr, _i64, _i64, _i64, _int, _i64, _i64, _ptr, _ptr, _int, _ptr, _i64,
                                   ctypes.c_float, _i64, _i64, _ptr, _i64, _i64, _i64, _ptr, _ptr, _sz, _ptr]),
+    "dels_kv8_attention_ex": (_int, [_kv4, _ptr, _i64, _i64, _i64, _int, _i64, _i64, _ptr, _ptr, _int, _ptr, _i64,
+                                     ctypes.c_float, _i64, _i64, _kv8_options, _ptr, _i64, _i64, _i64, _ptr, _ptr,
+                                     _sz, _ptr]),
 }
 
 _lock = threading.Lock()

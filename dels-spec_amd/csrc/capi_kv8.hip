@@ -6,6 +6,13 @@ using namespace dels;
 
 namespace {
 
+// A row of positions for each sequence, or one for all.
+int check_positions(const int32_t* positions, int64_t ld, int64_t T) {
+    if (positions && ((ld < T && ld != 0) || ld >= (int64_t(1) << 40)))
+        return fail(DELS_ERR_INVALID_ARGUMENT, "positions row stride %lld out of range", (long long)ld);
+    return DELS_OK;
+}
+
 int check_rotary(const dels_rotary* p, const PagedCache& c, int64_t T, const int32_t* positions, int64_t ld_positions,
                  KvRotary& r) {
     if (!p) return positions ? fail(DELS_ERR_INVALID_ARGUMENT, "positions without a rotary table") : DELS_OK;
@@ -19,8 +26,8 @@ int check_rotary(const dels_rotary* p, const PagedCache& c, int64_t T, const int
     if (!p->cos || !p->sin) return fail(DELS_ERR_INVALID_ARGUMENT, "cos or sin is NULL");
     if (!aligned(p->cos, 16) || !aligned(p->sin, 16) || p->ld % 4)
         return fail(DELS_ERR_ALIGNMENT, "rotary rows must be 16-byte aligned");
-    if (positions && ((ld_positions < T && ld_positions != 0) || ld_positions >= (int64_t(1) << 40)))
-        return fail(DELS_ERR_INVALID_ARGUMENT, "positions row stride %lld out of range", (long long)ld_positions);
+    const int rc = check_positions(positions, ld_positions, T);
+    if (rc != DELS_OK) return rc;
     r = {p->cos, p->sin, p->ld, p->positions, (int)p->channels, p->interleaved != 0, positions, ld_positions};
     return DELS_OK;
 }
@@ -95,14 +102,28 @@ int dels_kv8_attention(const dels_kv8_cache* p, const void* q, int64_t q_batch, 
                        int block, const int64_t* mask, int64_t ld_mask, float scale, int64_t window, int64_t sinks,
                        void* out, int64_t out_batch, int64_t out_token, int64_t out_head, float* lse, void* ws,
                        size_t ws_bytes, void* stream) {
+    return dels_kv8_attention_ex(p, q, q_batch, q_token, q_head, dtype, q_heads, T, lengths, counts, block, mask,
+                                 ld_mask, scale, window, sinks, nullptr, out, out_batch, out_token, out_head, lse, ws,
+                                 ws_bytes, stream);
+}
+
+int dels_kv8_attention_ex(const dels_kv8_cache* p, const void* q, int64_t q_batch, int64_t q_token, int64_t q_head,
+                          int dtype, int64_t q_heads, int64_t T, const int32_t* lengths, const int32_t* counts,
+                          int block, const int64_t* mask, int64_t ld_mask, float scale, int64_t window, int64_t sinks,
+                          const dels_kv8_options* options, void* out, int64_t out_batch, int64_t out_token,
+                          int64_t out_head, float* lse, void* ws, size_t ws_bytes, void* stream) {
+    const dels_kv8_options given = options ? *options : dels_kv8_options{};
     Kv8AttentionArgs a{};
     int rc = cache_of(p, a.cache);
     if (rc != DELS_OK) return rc;
     if (window < 0 || sinks < 0 || (sinks && !window))
         return fail(DELS_ERR_INVALID_ARGUMENT, "bad window %lld with %lld sinks", (long long)window, (long long)sinks);
+    if (given.positions && (!window || block != DELS_KV4_MASK))
+        return fail(DELS_ERR_INVALID_ARGUMENT, "positions are for a window over a block mask");
     if (a.cache.batch == 0 || T == 0) return DELS_OK;
     rc = check_block(a.cache, q, q_batch, q_token, q_head, dtype, q_heads, T, lengths, block, mask, ld_mask, scale);
     if (rc != DELS_OK) return rc;
+    if ((rc = check_positions(given.positions, given.ld_positions, T)) != DELS_OK) return rc;
     if ((rc = check_rows(out, out_batch, out_token, out_head, dtype, "out")) != DELS_OK) return rc;
     if (!lse) return fail(DELS_ERR_INVALID_ARGUMENT, "lse is NULL");
     if (a.cache.num_pages == 0) a.cache.max_pages = 0;       // nothing to see
@@ -112,6 +133,7 @@ int dels_kv8_attention(const dels_kv8_cache* p, const void* q, int64_t q_batch, 
     // wider than everything is no window
     const int64_t all = (int64_t)a.cache.slots() + T;
     a.window = window > all ? 0 : window, a.sinks = std::min<int64_t>(sinks, all);
+    if (a.window) a.at = given.positions, a.ld_at = given.ld_positions;
     a.block = {lengths, counts, (int)T, block, mask, ld_mask};
     a.q = {q, q_batch, q_token, q_head};
     a.dtype = dtype, a.q_heads = (int)q_heads, a.scale = scale;

@@ -4,7 +4,8 @@
 //     lse[t]  = log sum_j exp(x[t, j])
 //     o[t]    = sum_j exp(x[t, j] - lse[t]) v[j]
 // A row that sees nothing has o = 0 and lse = -inf.  With a window, row t sees of those slots
-// the ones from lengths + t - window + 1 on and the first `sinks`.
+// the ones from lengths + t - window + 1 on and the first `sinks`; where a tree's rows have positions,
+// a row's own takes the place of lengths + t, and a slot of the block is where its row is.
 //
 // One pass over the slots with the running maximum and sum of each row's softmax.
 // The rows that share a cache head (block tokens x query heads of the group) are
@@ -144,16 +145,19 @@ template <int D, int MT, bool ONCE> struct ValueRegs {
 // Which slots a row sees.
 struct Sight {
     int n, filled;             // context; slots that hold anything
-    int lim, lo;               // the row sees slots below lim,
-    uint64_t bits;             // and those of the block whose bits are set, from lo on
-    int sinks;                 // or below this
+    int lim, lo;               // the row sees slots below lim, from lo on
+    int sinks;                 // or below this,
+    uint64_t bits;             // and those of the block whose bits are set
     __device__ uint32_t of_run(int j0) const {             // of slots j0 .. j0 + 15
         const int d = j0 - n;
         uint32_t by_bit = d >= 64 || d <= -16 ? 0u : (uint32_t)(d >= 0 ? bits >> d : bits << -d) & 0xffffu;
         by_bit &= lowest(filled - j0);
-        return (lowest(lim - j0) | by_bit) & (~lowest(lo - j0) | lowest(sinks - j0));
+        return (lowest(lim - j0) & (~lowest(lo - j0) | lowest(sinks - j0))) | by_bit;
     }
 };
+
+// The lowest k of 64 bits.
+__device__ __forceinline__ uint64_t lowest64(int64_t k) { return k <= 0 ? 0ull : k >= 64 ? ~0ull : (1ull << k) - 1; }
 
 // What a page's two blocks say of themselves, the same for the whole wave.
 struct Page {
@@ -378,6 +382,7 @@ struct Kv8Seqs {
         if (a.block.mode == DELS_KV4_CAUSAL) end = (int)min((int64_t)end, (int64_t)n + last + 1);
         Seen s{0, 0, (end + kCachePage - 1) / kCachePage};
         if (a.window) {
+            first = max(first - a.spread, 0);
             const int64_t start = max((int64_t)n + first - a.window + 1, (int64_t)0);
             s.from = (int)min(start / kCachePage, (int64_t)s.end);
             s.sinks = (int)min((a.sinks + kCachePage - 1) / kCachePage, (int64_t)s.from);
@@ -403,6 +408,28 @@ template <typename T, int D, int MT, int TILES, bool RING> struct Lds {
     float m[kWaves][MT], l[kWaves][MT];
     bool last;
 };
+
+// Rows of trees whose window goes by positions: where each begins to see, and which of the block's slots
+// that its bits name its window or the sinks hold.  A launch of its own (3 us), as a loop over a
+// tree's rows in the kernel below spills registers there (8 x 16 rows 20.8 -> 21.7 us, whatever their block).
+constexpr int kTreeRows = 64;           // a block mask has no more
+__global__ __launch_bounds__(kTreeRows) void kv8_tree_rows_kernel(Kv8AttentionArgs a, int64_t* bits, int32_t* lows) {
+    const int b = blockIdx.x, t = threadIdx.x, last = a.block.T - 1;
+    const int n = paged_length(a.block.lengths, b, a.cache.slots());
+    const int64_t p = (int64_t)a.at[(int64_t)b * a.ld_at + min(t, last)] - n;
+    const int depth = (int)min(max(p, (int64_t)0), (int64_t)last);
+    uint64_t held = 0;
+    for (int i = 0; i <= last; ++i) {
+        const int other = __shfl(depth, i, 64);
+        held |= (uint64_t)(other > depth - a.window || n + other < a.sinks) << i;
+    }
+    if (t > last) return;
+    bits[b * (int64_t)kTreeRows + t] = a.block.mask[(int64_t)b * a.block.ld_mask + t] & (int64_t)held;
+    lows[b * (int64_t)kTreeRows + t] = (int)max((int64_t)n + depth - a.window + 1, (int64_t)0);
+}
+size_t tree_rows_bytes(int64_t batch) {
+    return align256((size_t)batch * kTreeRows * (sizeof(int64_t) + sizeof(int32_t)));
+}
 
 // TILES of 8 waves share a way: row tiles over the same pages.  8 / TILES ways take every
 // (8 / TILES)-th page each.
@@ -463,7 +490,7 @@ __global__ __launch_bounds__(kThreads, 2) void kv8_attention_kernel(Kv8Attention
                                              : a.block.mode == DELS_KV4_FULL ? n + count : n);
             plain = seen.sinks;
             if (a.window) {
-                const int last_row = min(divide(rt * MT + MT - 1, group), last_t);
+                const int last_row = min(divide(rt * MT + MT - 1, group) + a.spread, last_t);
                 const int64_t from = max((int64_t)n + last_row - a.window + 1, (int64_t)0);
                 plain += max(0, (int)min((from + kCachePage - 1) / kCachePage, (int64_t)seen.end) - seen.from);
             }
@@ -513,9 +540,11 @@ __global__ __launch_bounds__(kThreads, 2) void kv8_attention_kernel(Kv8Attention
         if (row.valid) {
             sight.lim = a.block.mode == DELS_KV4_CAUSAL ? n + row.t + 1 : a.block.mode == DELS_KV4_FULL ? n + count : n;
             if (a.window) sight.lo = (int)max((int64_t)n + row.t - a.window + 1, (int64_t)0);
-            if (a.block.mode == DELS_KV4_MASK)
-                sight.bits = (uint64_t)a.block.mask[(int64_t)b * a.block.ld_mask + row.t] &
-                             (count >= 64 ? ~0ull : (1ull << count) - 1);
+            if (a.block.mode == DELS_KV4_MASK) {
+                sight.bits = (uint64_t)a.block.mask[(int64_t)b * a.block.ld_mask + row.t] & lowest64(count);
+                if (a.lows) sight.lo = a.lows[(int64_t)b * a.block.ld_mask + row.t];
+                else if (a.window) sight.bits &= ~lowest64(row.t - a.window + 1) | lowest64((int64_t)sight.sinks - n);
+            }
         }
         sight.lim = min(sight.lim, sight.filled);
         rows.clear();
@@ -945,13 +974,23 @@ size_t kv8_attention_data_bytes(int64_t batch, int64_t T, int64_t q_heads, int64
     int64_t wide = 1;
     auto enough = [&](int64_t w) { return batch * heads * ((tiles + w - 1) / w) >= cus; };
     while (tile_rows == 32 && wide < 8 && wide < tiles && enough(2 * wide)) wide *= 2;
-    return align256((size_t)pieces * 2 * wide * sizeof(float) * (tile_rows * head_dim + 2 * tile_rows));
+    return tree_rows_bytes(batch) +
+           align256((size_t)pieces * 2 * wide * sizeof(float) * (tile_rows * head_dim + 2 * tile_rows));
 }
 
-hipError_t launch_kv8_attention(const Kv8AttentionArgs& a, void* ws, size_t data_off, hipStream_t s) {
+hipError_t launch_kv8_attention(const Kv8AttentionArgs& given, void* ws, size_t data_off, hipStream_t s) {
+    Kv8AttentionArgs a = given;
     const PagedCache& c = a.cache;
     const Plan p = plan(c.batch, a.block.T, a.q_heads, c.heads, c.max_pages);
-    auto* states = reinterpret_cast<float*>(static_cast<char*>(ws) + data_off);
+    char* data = static_cast<char*>(ws) + data_off;
+    if (a.at) {
+        auto* bits = reinterpret_cast<int64_t*>(data);
+        auto* lows = reinterpret_cast<int32_t*>(bits + (int64_t)c.batch * kTreeRows);
+        hipLaunchKernelGGL(kv8_tree_rows_kernel, dim3(c.batch), dim3(kTreeRows), 0, s, a, bits, lows);
+        a.block.mask = bits, a.block.ld_mask = kTreeRows;
+        a.lows = lows, a.spread = a.block.T - 1;
+    }
+    auto* states = reinterpret_cast<float*>(data + tree_rows_bytes(c.batch));
     auto* counters = reinterpret_cast<unsigned int*>(static_cast<char*>(ws) + kCountersOff);
     auto by_size = [&](auto tag, auto size) {
         using T = decltype(tag);

@@ -200,8 +200,8 @@ def kv8_read(cache: KV8Cache, starts: torch.Tensor, T: int, *, counts: Optional[
 def kv8_attention(q: torch.Tensor, cache: KV8Cache, lengths: torch.Tensor, *, block: Block = "causal",
                   counts: Optional[torch.Tensor] = None, scale: Optional[float] = None,
                   window: Optional[int] = None, sinks: int = 0, out: Optional[torch.Tensor] = None,
-                  lse: Optional[torch.Tensor] = None,
-                  workspace: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
+                  lse: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None,
+                  positions: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
     """Attention of a block's rows over their sequences' context and the block itself.
 
     ``q`` ``[batch, T, q_heads, head_dim]`` bf16 or fp16, ``q_heads`` a multiple of the
@@ -211,6 +211,11 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, lengths: torch.Tensor, *, bl
     drafts; T at most 64; expanded where all sequences have one tree).  With a ``window``,
     row ``t`` sees of these only the slots from ``lengths[b] + t - window + 1`` on and the first
     ``sinks`` of the sequence; pages in between are not read, and the table need not name them.
+    That counts slots.  A tree's row lies in slot ``lengths[b] + t`` but at the position of its depth,
+    where decoding its branch alone would put it: give ``positions``, int32 ``[batch, T]`` as
+    ``kv8_append`` took them (between ``lengths[b]`` and ``lengths[b] + T - 1``, or the nearest of these),
+    and the row sees of the context the slots from ``positions[b, t] - window + 1`` on, and of
+    the block the rows that its bits name and whose positions are there (or below ``sinks``).
     ``counts`` int32 ``[batch]`` are the valid rows (None: T).  ``scale`` defaults to
     ``head_dim ** -0.5``.  Returns ``(out, lse)``: ``out`` like ``q``, ``lse`` fp32 ``[batch, T,
     q_heads]``, the logarithm of each softmax's sum; rows that see nothing give 0 and -inf, rows
@@ -220,7 +225,7 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, lengths: torch.Tensor, *, bl
     if _elsewhere_current(cache):
         with torch.cuda.device(cache._index):
             return kv8_attention(q, cache, lengths, block=block, counts=counts, scale=scale, window=window,
-                                 sinks=sinks, out=out, lse=lse, workspace=workspace)
+                                 sinks=sinks, out=out, lse=lse, workspace=workspace, positions=positions)
     qp = _require_rows(q, cache, None, "q", _Q_DTYPES)
     batch, T, q_heads, D = q.shape
     if q_heads % cache.kv_heads:
@@ -235,6 +240,11 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, lengths: torch.Tensor, *, bl
         window, sinks = min(window, _FAR), min(sinks, _FAR)
     lp, cp = _require_ints(lengths, cache, "lengths"), _require_ints(counts, cache, "counts")
     mode, mask, ld_mask = _block_args(block, cache, T)
+    options = ()
+    if positions is not None:
+        if not window or mode != _lib.KV4_BLOCK_MASK:
+            raise ValueError("positions are for a window over a block mask")
+        options = (ctypes.byref(_lib.Kv8OptionsParams(*_position_args(positions, cache, T))),)
     if out is None:
         out = torch.empty(batch, T, q_heads, D, dtype=q.dtype, device=cache.device)
         op = (out.data_ptr(), T * q_heads * D, q_heads * D, D)
@@ -256,7 +266,8 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, lengths: torch.Tensor, *, bl
         ws = _WORKSPACES.get(cache.device, need, stream)
     else:
         ws = _own_workspace(workspace, cache, need, counters=True)
-    _lib.check(lib.dels_kv8_attention(cache._ref, *qp, _DTYPES[q.dtype], q_heads, T, lp, cp, mode, mask, ld_mask,
-                                      cache._scale if scale is None else scale, window, sinks, *op, lse.data_ptr(),
-                                      ws.data_ptr(), ws.numel(), stream), "dels_kv8_attention")
+    call = lib.dels_kv8_attention_ex if options else lib.dels_kv8_attention
+    _lib.check(call(cache._ref, *qp, _DTYPES[q.dtype], q_heads, T, lp, cp, mode, mask, ld_mask,
+                    cache._scale if scale is None else scale, window, sinks, *options, *op, lse.data_ptr(),
+                    ws.data_ptr(), ws.numel(), stream), call.__name__)
     return out, lse

@@ -726,6 +726,8 @@ int dels_kv8_read(const dels_kv8_cache* c, const int32_t* starts, const int32_t*
  * Attention of a block's rows over the cache, as dels_kv4_attention, q bf16 or fp16.  With a
  * window (0: none), row t sees of the slots that it would see otherwise those from
  * lengths[b] + t - window + 1 on and those below `sinks`; pages that no row sees are not read.
+ * So the window goes by slots, which are positions but for the rows of a tree:
+ * dels_kv8_attention_ex takes theirs.
  */
 size_t dels_kv8_attention_ws_bytes(int64_t batch, int64_t T, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
                                    int64_t max_pages);
@@ -734,6 +736,24 @@ int dels_kv8_attention(const dels_kv8_cache* c, const void* q, int64_t q_batch, 
                        int block, const int64_t* mask, int64_t ld_mask, float scale, int64_t window, int64_t sinks,
                        void* out, int64_t out_batch, int64_t out_token, int64_t out_head, float* lse, void* ws,
                        size_t ws_bytes, void* stream);
+
+/* What dels_kv8_attention_ex takes beside dels_kv8_attention's arguments (NULL, or all zero: the same call).
+ *   positions [batch, ld_positions >= T, or 0 for one row that all sequences read], as dels_kv8_append took
+ *     them, for a window over DELS_KV4_MASK: row t sees of the context the slots from
+ *     positions[b][t] - window + 1 on and those below `sinks`, and of the block's slots whose bits it has
+ *     those whose rows have such a position.  One outside lengths[b] .. lengths[b] + T - 1
+ *     counts as the nearest of these.
+ */
+typedef struct dels_kv8_options {
+    const int32_t* positions;
+    int64_t ld_positions;
+} dels_kv8_options;
+
+int dels_kv8_attention_ex(const dels_kv8_cache* c, const void* q, int64_t q_batch, int64_t q_token, int64_t q_head,
+                          int dtype, int64_t q_heads, int64_t T, const int32_t* lengths, const int32_t* counts,
+                          int block, const int64_t* mask, int64_t ld_mask, float scale, int64_t window, int64_t sinks,
+                          const dels_kv8_options* options, void* out, int64_t out_batch, int64_t out_token,
+                          int64_t out_head, float* lse, void* ws, size_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -128,8 +128,8 @@ def append(state, k, v, n, count):
                 codes[h, lo:hi] = encode(rows * 2.0 ** (127 - e))
 
 
-def visible(n, count, T, slots, block, masks=None, window=None, sinks=0):
-    """Which slots the rows of a block see, [T, slots]."""
+def visible(n, count, T, slots, block, masks=None, window=None, sinks=0, positions=None):
+    """Which slots the rows of a block see, [T, slots]; the window goes by slots or by the rows' positions [T]."""
     j, t = np.arange(slots)[None], np.arange(T)[:, None]
     i = j - n
     if masks is not None:
@@ -137,12 +137,16 @@ def visible(n, count, T, slots, block, masks=None, window=None, sinks=0):
     else:
         own = {"causal": i <= t, "full": i >= 0, "none": np.zeros((T, slots), bool)}[block]
     see = (i < 0) | (own & (i < count))
-    if window is not None:
+    if window is not None and positions is not None:
+        depth = np.clip(np.asarray(positions, np.int64) - n, 0, T - 1)
+        place = np.where((i >= 0) & (i < T), depth[np.clip(i, 0, T - 1)], i)
+        see = see & ((place > depth[:, None] - window) | (n + place < sinks))
+    elif window is not None:
         see = see & ((i > t - window) | (j < sinks))
     return see & (t < count)
 
 
-def attention(q, K, V, lengths, counts, block, scale, masks=None, window=None, sinks=0):
+def attention(q, K, V, lengths, counts, block, scale, masks=None, window=None, sinks=0, positions=None):
     """q [B, T, HQ, D]; K, V [B, H, slots, D] (NaN: not finite).
 
     Returns out, lse, and for bounds: sum p |v| / sum p, and the largest sum of |q k| * |scale|
@@ -154,7 +158,8 @@ def attention(q, K, V, lengths, counts, block, scale, masks=None, window=None, s
     out, lse = np.zeros((B, T, HQ, D)), np.full((B, T, HQ), -np.inf)
     weight, mass = np.zeros((B, T, HQ, D)), np.zeros((B, T, HQ))
     for b in range(B):
-        see = visible(lengths[b], counts[b], T, slots, block, None if masks is None else masks[b], window, sinks)
+        see = visible(lengths[b], counts[b], T, slots, block, None if masks is None else masks[b], window, sinks,
+                      None if positions is None else positions[b])
         for h in range(H):
             none = np.isnan(K[b, h]).any(-1)
             k, v = np.nan_to_num(K[b, h]), np.nan_to_num(V[b, h])
