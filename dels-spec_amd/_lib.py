@@ -118,7 +118,7 @@ class RotaryParams(ctypes.Structure):
 class Kv8OptionsParams(ctypes.Structure):
     """Mirror of ``struct dels_kv8_options`` in include/dels.h."""
 
-    _fields_ = [("positions", _ptr), ("ld_positions", _i64)]
+    _fields_ = [("positions", _ptr), ("ld_positions", _i64), ("weight_parts", _int)]
 
 
 _kv4 = ctypes.POINTER(Kv4CacheParams)

@@ -120,6 +120,8 @@ int dels_kv8_attention_ex(const dels_kv8_cache* p, const void* q, int64_t q_batc
         return fail(DELS_ERR_INVALID_ARGUMENT, "bad window %lld with %lld sinks", (long long)window, (long long)sinks);
     if (given.positions && (!window || block != DELS_KV4_MASK))
         return fail(DELS_ERR_INVALID_ARGUMENT, "positions are for a window over a block mask");
+    if (given.weight_parts < 0 || given.weight_parts > 2)
+        return fail(DELS_ERR_INVALID_ARGUMENT, "weights in %d parts", given.weight_parts);
     if (a.cache.batch == 0 || T == 0) return DELS_OK;
     rc = check_block(a.cache, q, q_batch, q_token, q_head, dtype, q_heads, T, lengths, block, mask, ld_mask, scale);
     if (rc != DELS_OK) return rc;
@@ -136,7 +138,7 @@ int dels_kv8_attention_ex(const dels_kv8_cache* p, const void* q, int64_t q_batc
     if (a.window) a.at = given.positions, a.ld_at = given.ld_positions;
     a.block = {lengths, counts, (int)T, block, mask, ld_mask};
     a.q = {q, q_batch, q_token, q_head};
-    a.dtype = dtype, a.q_heads = (int)q_heads, a.scale = scale;
+    a.dtype = dtype, a.q_heads = (int)q_heads, a.scale = scale, a.split = given.weight_parts == 2;
     a.out = out, a.out_batch = out_batch, a.out_token = out_token, a.out_head = out_head, a.lse = lse;
     const hipError_t e = launch_kv8_attention(a, ws, kDataOff, static_cast<hipStream_t>(stream));
     return e == hipSuccess ? DELS_OK : hip_fail(e, "cache attention launch");

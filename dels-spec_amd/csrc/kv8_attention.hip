@@ -17,8 +17,12 @@
 // scores, its value scale is applied by the conversion.  Both products are 16-bit ones: the
 // 8-bit matrix instructions add products at 2^-12 of the largest of a group (measured),
 // which a float32 lse would show.  Weights enter as f16 numbers (2^-11 of each, an eighth of half a
-// step of a bf16 output), for f16 outputs in two parts.  Scores, maxima, sums and outputs are
-// fp32.
+// step of a bf16 output where values do not cancel), for f16 outputs in two parts, and for bf16 ones in two
+// bf16 parts (2^-17) where the caller asks for it.  By norm, bf16 outputs of 2 x 512 rows over 3500 slots are
+// 1.6713e-3 off the 64-bit ones, 1.6599e-3 with two parts or fp32 weights: the rounding of the output is
+// what there is.  Two parts take 24 matrix instructions a step for 16: 8 x 16 rows 21 -> 24 us, 131k slots
+// 60 -> 78, 2 x 512 rows 87 -> 124, 4093 rows through a window 114 -> 151, one row of 32 sequences
+// 152 -> 155.  Scores, maxima, sums and outputs are fp32.
 //
 // What bounds it, at 32 query and 8 cache heads of 128 in bf16 (kernel times):
 //   32 sequences of up to 16300 slots, 1 token     154 us  memory: 935 MB at 6.1 TB/s
@@ -467,6 +471,9 @@ __global__ __launch_bounds__(kThreads, 2) void kv8_attention_kernel(Kv8Attention
     const float unit = (mag == 0.f ? 1.f : mag) * kLog2e;
     const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u, zero = mag == 0.f ? 0u : ~0u;
 
+    // asked for by the caller; the loop that scales far apart need has weights in two parts
+    const bool split = std::is_same<T, bf16_t>::value && a.split;
+
     while (u < u_end) {
         if (u >= at.start + at.pages * scan.per) at = scan.place(u);
         const int b = at.b;
@@ -639,7 +646,7 @@ __global__ __launch_bounds__(kThreads, 2) void kv8_attention_kernel(Kv8Attention
                 page = Page(head);
                 slot = seen.page(p) * kCachePage;
                 whole_page = is_plain(p, id, page);
-                narrow = rows.admit(page, blocks_of(slot, id));
+                narrow = rows.admit(page, blocks_of(slot, id)) && !split;
             };
             meet();
             while (p < stop && narrow) {
@@ -716,7 +723,7 @@ __global__ __launch_bounds__(kThreads, 2) void kv8_attention_kernel(Kv8Attention
                 page = Page(*reinterpret_cast<const u32x4*>(lds.head[wave][i % L::kRing]));
                 slot = seen.page(p) * kCachePage;
                 whole_page = is_plain(p, ids_ahead[0], page);
-                narrow = rows.admit(page, blocks_of(slot, ids_ahead[0]));
+                narrow = rows.admit(page, blocks_of(slot, ids_ahead[0])) && !split;
             };
             // page i, and the first scores of the one behind it
             auto work = [&](auto wide, auto masked) {

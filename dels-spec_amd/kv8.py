@@ -201,7 +201,8 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, lengths: torch.Tensor, *, bl
                   counts: Optional[torch.Tensor] = None, scale: Optional[float] = None,
                   window: Optional[int] = None, sinks: int = 0, out: Optional[torch.Tensor] = None,
                   lse: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None,
-                  positions: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
+                  positions: Optional[torch.Tensor] = None,
+                  weight_parts: int = 1) -> tuple[torch.Tensor, torch.Tensor]:
     """Attention of a block's rows over their sequences' context and the block itself.
 
     ``q`` ``[batch, T, q_heads, head_dim]`` bf16 or fp16, ``q_heads`` a multiple of the
@@ -220,12 +221,18 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, lengths: torch.Tensor, *, bl
     ``head_dim ** -0.5``.  Returns ``(out, lse)``: ``out`` like ``q``, ``lse`` fp32 ``[batch, T,
     q_heads]``, the logarithm of each softmax's sum; rows that see nothing give 0 and -inf, rows
     that see a score of NaN or +inf NaN in both.
+
+    Scores, maxima, sums and outputs are fp32.  A slot's weight meets its value as one f16 number
+    for bf16 queries, as two for fp16 ones: before it is rounded, ``out`` may be off by 2^-11 (2^-17) of the
+    weighted sum of the values' magnitudes, which is more of it where values cancel.  ``weight_parts=2``
+    has two parts for bf16 queries, too; blocks of many rows take longer.
     """
     _require_cache(cache, 8)
     if _elsewhere_current(cache):
         with torch.cuda.device(cache._index):
             return kv8_attention(q, cache, lengths, block=block, counts=counts, scale=scale, window=window,
-                                 sinks=sinks, out=out, lse=lse, workspace=workspace, positions=positions)
+                                 sinks=sinks, out=out, lse=lse, workspace=workspace, positions=positions,
+                                 weight_parts=weight_parts)
     qp = _require_rows(q, cache, None, "q", _Q_DTYPES)
     batch, T, q_heads, D = q.shape
     if q_heads % cache.kv_heads:
@@ -241,10 +248,15 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, lengths: torch.Tensor, *, bl
     lp, cp = _require_ints(lengths, cache, "lengths"), _require_ints(counts, cache, "counts")
     mode, mask, ld_mask = _block_args(block, cache, T)
     options = ()
-    if positions is not None:
-        if not window or mode != _lib.KV4_BLOCK_MASK:
-            raise ValueError("positions are for a window over a block mask")
-        options = (ctypes.byref(_lib.Kv8OptionsParams(*_position_args(positions, cache, T))),)
+    if positions is not None or weight_parts != 1:
+        if weight_parts not in (1, 2):
+            raise ValueError(f"weight_parts must be 1 or 2, got {weight_parts}")
+        at = (None, 0)
+        if positions is not None:
+            if not window or mode != _lib.KV4_BLOCK_MASK:
+                raise ValueError("positions are for a window over a block mask")
+            at = _position_args(positions, cache, T)
+        options = (ctypes.byref(_lib.Kv8OptionsParams(*at, weight_parts)),)
     if out is None:
         out = torch.empty(batch, T, q_heads, D, dtype=q.dtype, device=cache.device)
         op = (out.data_ptr(), T * q_heads * D, q_heads * D, D)

@@ -728,6 +728,10 @@ int dels_kv8_read(const dels_kv8_cache* c, const int32_t* starts, const int32_t*
  * lengths[b] + t - window + 1 on and those below `sinks`; pages that no row sees are not read.
  * So the window goes by slots, which are positions but for the rows of a tree:
  * dels_kv8_attention_ex takes theirs.
+ * Scores, maxima, sums and outputs are fp32.  The weight of a slot meets its value as an f16 number for
+ * bf16 out, as two for fp16 out: before it is rounded to its type an output may be off by 2^-11
+ * (2^-17) of the weighted sum of the values' magnitudes, and where the values cancel that is more of what is
+ * left.  dels_kv8_attention_ex takes two parts for bf16 out, too.
  */
 size_t dels_kv8_attention_ws_bytes(int64_t batch, int64_t T, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
                                    int64_t max_pages);
@@ -743,10 +747,12 @@ int dels_kv8_attention(const dels_kv8_cache* c, const void* q, int64_t q_batch, 
  *     positions[b][t] - window + 1 on and those below `sinks`, and of the block's slots whose bits it has
  *     those whose rows have such a position.  One outside lengths[b] .. lengths[b] + T - 1
  *     counts as the nearest of these.
+ *   weight_parts 2 for weights in two parts (2^-17 of each), 1 or 0 for what the type of out has.
  */
 typedef struct dels_kv8_options {
     const int32_t* positions;
     int64_t ld_positions;
+    int weight_parts;
 } dels_kv8_options;
 
 int dels_kv8_attention_ex(const dels_kv8_cache* c, const void* q, int64_t q_batch, int64_t q_token, int64_t q_head,

@@ -180,17 +180,18 @@ def attention(q, K, V, lengths, counts, block, scale, masks=None, window=None, s
     return out, lse, weight, mass
 
 
-def output_range(out, weight, err, dtype, most):
+def output_range(out, weight, err, dtype, most, parts=1):
     """The numbers of a type that attention's outputs may be: (lowest, highest).
 
     err [B, T, HQ]: how far a row's scores may be off.  The weights then are off by that, by
     the 2^-20 of an argument of the exponential around the row's largest score, and by the f16
     number, or two of them for f16 outputs, that meets the values: 2^-11 or 2^-22 of each weight, and
     2^-32 of the row's largest where that is more (`most`: slots times the largest |value|).  A block
-    whose scale is far below the largest takes two bf16 parts, 2^-17.  Sums in fp32 over a few
+    whose scale is far below the largest takes two bf16 parts, 2^-17, as all do where a bf16 output is
+    asked for with weights in two `parts`.  Sums in fp32 over a few
     hundred slots add 2^-16.  What comes of it is rounded once, to its type: whatever lies
     between the roundings of both ends is right.
     """
-    part = 2.0 ** -11 if dtype == "bf16" else 2.0 ** -17
+    part = 2.0 ** -11 if dtype == "bf16" and parts == 1 else 2.0 ** -17
     off = weight * (part + 2.0 ** -16 + 2.0 * (err[..., None] + 2.0 ** -20)) + most * 2.0 ** -32 + 1e-30
     return kv4.round_to(out - off, dtype), kv4.round_to(out + off, dtype)
