@@ -132,7 +132,8 @@ def kv8_append(cache: KV8Cache, k: torch.Tensor, v: torch.Tensor, lengths: torch
     that holds its new rows, or that of the rows before them in the block if it is larger (rows
     that were rejected leave it as they made it); if it is smaller, those rows are rounded again.
     A row of which something is NaN, infinite or over 448 * 2^64, or whose position the table
-    does not have, reads as NaN and gives scores of NaN, and takes no part in the exponents.
+    does not have, reads as NaN and gives scores of NaN, and takes no part in the exponents; a query
+    at such a position has NaN in its rotated channels.
     ``lengths`` is not changed; rows past the table's slots are dropped.
     """
     _require_cache(cache, 8)

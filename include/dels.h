@@ -705,7 +705,8 @@ size_t dels_kv8_page_bytes(int64_t head_dim);
  *     dtype into q_out (rows from counts[b] on 0; q_out may be q with its strides): (a, b) becomes
  *     (a c - b s, b c + a s), each product, sum and difference rounded to fp32, q then to dtype.
  *   positions [batch, ld_positions >= T, or 0 for one row that all sequences read] (NULL:
- *     lengths[b] + t); a position that the table does not have makes the row NaN.
+ *     lengths[b] + t, lengths as they are clamped to the table's slots); at a position that the table does
+ *     not have a key is not held, and a query has NaN in its rotated channels.
  */
 int dels_kv8_append(const dels_kv8_cache* c, const void* k, int64_t k_batch, int64_t k_token, int64_t k_head,
                     const void* v, int64_t v_batch, int64_t v_token, int64_t v_head, int dtype,

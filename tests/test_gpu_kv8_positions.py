@@ -8,7 +8,8 @@ import pytest
 import torch
 
 from oracle import kv8 as O
-from test_gpu_kv8 import INF, attention_inputs, contents, ints, random_cache, say
+from test_gpu_kv8 import (INF, append_inputs, attention_inputs, check_append, contents, ints, random_cache, say,
+                          tables, unpacked)
 
 pytestmark = pytest.mark.gpu
 
@@ -211,3 +212,42 @@ def test_positions_in_a_graph(pkg, dev):
             torch.cuda.synchronize()
             for x, y in zip(captured, eager):
                 assert torch.equal(x, y), i
+
+
+@pytest.mark.parametrize("given", ["slots", "own", "one row"])
+def test_append_by_positions_writes_its_blocks_and_nothing_else(pkg, dev, given):
+    """Positions inside and outside the table: the oracle's blocks, and every other page as it was before the call."""
+    say("append by positions", given)
+    B, T, H, G, D = 3, 5, 2, 2, 64
+    k, v, q = append_inputs(B, T, H, G, D, "bf16", False, 8)
+    cos, sin = tables(50, 32, dev)
+    lengths = [0, 20, 47]
+    own = torch.tensor([[0, 1, 1, 2, 49], [3, 50, -1, 2 ** 31 - 1, -2 ** 31], [7, 7, 7, 7, 7]], dtype=torch.int32)
+    at = {"slots": None, "own": own.to(dev), "one row": own[1:2].to(dev).expand(B, T)}[given]
+    p = np.array(lengths)[:, None] + np.arange(T) if at is None else at.cpu().numpy().astype(np.int64)
+    cache = random_cache(pkg, dev, B, H, D, 2, seed=4)
+    before, spare = unpacked(cache), cache.data.cpu().numpy().copy()
+    turned = pkg.kv8_append(cache, k.to(dev), v.to(dev), ints(lengths, dev), positions=at, q=q.to(dev),
+                            rotary=pkg.RotaryTable(cos, sin))
+    torch.cuda.synchronize()
+    kt = np.stack([O.rotate(k.float().numpy()[:, :, h], cos.cpu().numpy(), sin.cpu().numpy(), p, False)
+                   for h in range(H)], 2)
+    values = v.float().numpy()
+    check_append(cache, before, spare, kt, values, lengths, None)
+    # the check itself notices a byte that changed in a page that no row of the table names
+    named = set(cache.block_table.cpu().flatten().tolist())
+    stray = spare.copy()
+    stray[next(i for i in range(len(spare)) if i not in named), 1, 77] ^= 1
+    with pytest.raises(AssertionError):
+        check_append(cache, before, stray, kt, values, lengths, None)
+    # a query at a position that the table does not have: its rotated channels are NaN, the others are kept,
+    # and all that it sees it scores NaN
+    lost = torch.tensor((p < 0) | (p >= 50))
+    assert lost.any() or given == "slots" and not lost[:2].any()
+    nan = turned.cpu().isnan()
+    assert torch.equal(nan[..., :32], lost[:, :, None, None].expand(B, T, H * G, 32)) and not nan[..., 32:].any()
+    assert torch.equal(turned.cpu()[..., 32:], q[..., 32:])
+    _, lse = pkg.kv8_attention(turned, cache, ints(lengths, dev), block="none")
+    torch.cuda.synchronize()
+    seen = torch.tensor(lengths)[:, None].expand(B, T) > 0
+    assert torch.equal(lse.cpu().isnan(), (lost & seen)[..., None].expand(B, T, H * G))
