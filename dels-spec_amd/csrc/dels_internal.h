@@ -396,9 +396,6 @@ struct Kv8AttentionArgs {
     int64_t window, sinks;               // window 0: rows see their whole context
     const int32_t* at; int64_t ld_at;    // [batch, T] positions of a tree's rows (null: their slots)
     bool split;                          // bf16 outputs: weights in two parts
-    // of the kernel's own: where rows with positions begin to see, laid out as the mask (which then has
-    // what their windows leave of it), and how many rows they may stand away from their slots
-    const int32_t* lows; int spread;
     void* out; int64_t out_batch, out_token, out_head;
     float* lse;                          // [batch, T, q_heads]
 };

@@ -146,6 +146,10 @@ template <int D, int MT, bool ONCE> struct ValueRegs {
     }
 };
 
+// A block mode of the kernel's own: a tree's rows have positions, and the mask has 64 words for each
+// sequence with what the rows' windows leave of their bits, then 64 with where they begin to see.
+constexpr int kTreeRows = 64, kTreeMode = DELS_KV4_MASK + 1;
+
 // Which slots a row sees.
 struct Sight {
     int n, filled;             // context; slots that hold anything
@@ -258,7 +262,7 @@ template <typename T, int D, int MT> struct Rows8 {
     }
 
     // Takes a page's scales in (of its first `blocks` blocks; the others hold nothing yet); whether
-    // its products can be of f16 numbers.
+    // its products can be of f16 numbers, with weights in one part for bf16 outputs.
     __device__ __forceinline__ bool admit(const Page& page, int blocks) {
         if (!blocks) return vlow >= vref - kSpan;
         const int v0 = page.value(0), v1 = blocks > 1 ? page.value(1) : v0;
@@ -386,7 +390,7 @@ struct Kv8Seqs {
         if (a.block.mode == DELS_KV4_CAUSAL) end = (int)min((int64_t)end, (int64_t)n + last + 1);
         Seen s{0, 0, (end + kCachePage - 1) / kCachePage};
         if (a.window) {
-            first = max(first - a.spread, 0);
+            if (a.block.mode == kTreeMode) first = 0;         // any row may be where the first one is
             const int64_t start = max((int64_t)n + first - a.window + 1, (int64_t)0);
             s.from = (int)min(start / kCachePage, (int64_t)s.end);
             s.sinks = (int)min((a.sinks + kCachePage - 1) / kCachePage, (int64_t)s.from);
@@ -413,11 +417,9 @@ template <typename T, int D, int MT, int TILES, bool RING> struct Lds {
     bool last;
 };
 
-// Rows of trees whose window goes by positions: where each begins to see, and which of the block's slots
-// that its bits name its window or the sinks hold.  A launch of its own (3 us), as a loop over a
-// tree's rows in the kernel below spills registers there (8 x 16 rows 20.8 -> 21.7 us, whatever their block).
-constexpr int kTreeRows = 64;           // a block mask has no more
-__global__ __launch_bounds__(kTreeRows) void kv8_tree_rows_kernel(Kv8AttentionArgs a, int64_t* bits, int32_t* lows) {
+// The words of kTreeMode.  A launch of its own (3 us), as a loop over a tree's rows in the kernel below
+// spills registers there (8 x 16 rows 20.8 -> 21.7 us, whatever their block).
+__global__ __launch_bounds__(kTreeRows) void kv8_tree_rows_kernel(Kv8AttentionArgs a, int64_t* words) {
     const int b = blockIdx.x, t = threadIdx.x, last = a.block.T - 1;
     const int n = paged_length(a.block.lengths, b, a.cache.slots());
     const int64_t p = (int64_t)a.at[(int64_t)b * a.ld_at + min(t, last)] - n;
@@ -428,12 +430,11 @@ __global__ __launch_bounds__(kTreeRows) void kv8_tree_rows_kernel(Kv8AttentionAr
         held |= (uint64_t)(other > depth - a.window || n + other < a.sinks) << i;
     }
     if (t > last) return;
-    bits[b * (int64_t)kTreeRows + t] = a.block.mask[(int64_t)b * a.block.ld_mask + t] & (int64_t)held;
-    lows[b * (int64_t)kTreeRows + t] = (int)max((int64_t)n + depth - a.window + 1, (int64_t)0);
+    words += 2 * (int64_t)kTreeRows * b + t;
+    words[0] = a.block.mask[(int64_t)b * a.block.ld_mask + t] & (int64_t)held;
+    words[kTreeRows] = max((int64_t)n + depth - a.window + 1, (int64_t)0);
 }
-size_t tree_rows_bytes(int64_t batch) {
-    return align256((size_t)batch * kTreeRows * (sizeof(int64_t) + sizeof(int32_t)));
-}
+size_t tree_rows_bytes(int64_t batch) { return align256((size_t)batch * 2 * kTreeRows * sizeof(int64_t)); }
 
 // TILES of 8 waves share a way: row tiles over the same pages.  8 / TILES ways take every
 // (8 / TILES)-th page each.
@@ -471,9 +472,6 @@ __global__ __launch_bounds__(kThreads, 2) void kv8_attention_kernel(Kv8Attention
     const float unit = (mag == 0.f ? 1.f : mag) * kLog2e;
     const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u, zero = mag == 0.f ? 0u : ~0u;
 
-    // asked for by the caller; the loop that scales far apart need has weights in two parts
-    const bool split = std::is_same<T, bf16_t>::value && a.split;
-
     while (u < u_end) {
         if (u >= at.start + at.pages * scan.per) at = scan.place(u);
         const int b = at.b;
@@ -497,7 +495,8 @@ __global__ __launch_bounds__(kThreads, 2) void kv8_attention_kernel(Kv8Attention
                                              : a.block.mode == DELS_KV4_FULL ? n + count : n);
             plain = seen.sinks;
             if (a.window) {
-                const int last_row = min(divide(rt * MT + MT - 1, group) + a.spread, last_t);
+                const int last_row =
+                    a.block.mode == kTreeMode ? last_t : min(divide(rt * MT + MT - 1, group), last_t);
                 const int64_t from = max((int64_t)n + last_row - a.window + 1, (int64_t)0);
                 plain += max(0, (int)min((from + kCachePage - 1) / kCachePage, (int64_t)seen.end) - seen.from);
             }
@@ -547,14 +546,17 @@ __global__ __launch_bounds__(kThreads, 2) void kv8_attention_kernel(Kv8Attention
         if (row.valid) {
             sight.lim = a.block.mode == DELS_KV4_CAUSAL ? n + row.t + 1 : a.block.mode == DELS_KV4_FULL ? n + count : n;
             if (a.window) sight.lo = (int)max((int64_t)n + row.t - a.window + 1, (int64_t)0);
-            if (a.block.mode == DELS_KV4_MASK) {
-                sight.bits = (uint64_t)a.block.mask[(int64_t)b * a.block.ld_mask + row.t] & lowest64(count);
-                if (a.lows) sight.lo = a.lows[(int64_t)b * a.block.ld_mask + row.t];
+            if (a.block.mode >= DELS_KV4_MASK) {
+                const int64_t* words = a.block.mask + (int64_t)b * a.block.ld_mask + row.t;
+                sight.bits = (uint64_t)words[0] & lowest64(count);
+                if (a.block.mode == kTreeMode) sight.lo = (int)words[kTreeRows];
                 else if (a.window) sight.bits &= ~lowest64(row.t - a.window + 1) | lowest64((int64_t)sight.sinks - n);
             }
         }
         sight.lim = min(sight.lim, sight.filled);
         rows.clear();
+        // two parts that the caller asks for are those of scales that lie far apart
+        if (std::is_same<T, bf16_t>::value && a.split) rows.vlow = -256;
 
         // Pages p, p + WAYS, ... below `stop`; one that the table does not name is seen by no row.
         auto named = [&](int id) { return id >= 0 && id < c.num_pages; };
@@ -646,7 +648,7 @@ __global__ __launch_bounds__(kThreads, 2) void kv8_attention_kernel(Kv8Attention
                 page = Page(head);
                 slot = seen.page(p) * kCachePage;
                 whole_page = is_plain(p, id, page);
-                narrow = rows.admit(page, blocks_of(slot, id)) && !split;
+                narrow = rows.admit(page, blocks_of(slot, id));
             };
             meet();
             while (p < stop && narrow) {
@@ -723,7 +725,7 @@ __global__ __launch_bounds__(kThreads, 2) void kv8_attention_kernel(Kv8Attention
                 page = Page(*reinterpret_cast<const u32x4*>(lds.head[wave][i % L::kRing]));
                 slot = seen.page(p) * kCachePage;
                 whole_page = is_plain(p, ids_ahead[0], page);
-                narrow = rows.admit(page, blocks_of(slot, ids_ahead[0])) && !split;
+                narrow = rows.admit(page, blocks_of(slot, ids_ahead[0]));
             };
             // page i, and the first scores of the one behind it
             auto work = [&](auto wide, auto masked) {
@@ -991,11 +993,9 @@ hipError_t launch_kv8_attention(const Kv8AttentionArgs& given, void* ws, size_t 
     const Plan p = plan(c.batch, a.block.T, a.q_heads, c.heads, c.max_pages);
     char* data = static_cast<char*>(ws) + data_off;
     if (a.at) {
-        auto* bits = reinterpret_cast<int64_t*>(data);
-        auto* lows = reinterpret_cast<int32_t*>(bits + (int64_t)c.batch * kTreeRows);
-        hipLaunchKernelGGL(kv8_tree_rows_kernel, dim3(c.batch), dim3(kTreeRows), 0, s, a, bits, lows);
-        a.block.mask = bits, a.block.ld_mask = kTreeRows;
-        a.lows = lows, a.spread = a.block.T - 1;
+        auto* words = reinterpret_cast<int64_t*>(data);
+        hipLaunchKernelGGL(kv8_tree_rows_kernel, dim3(c.batch), dim3(kTreeRows), 0, s, a, words);
+        a.block.mode = kTreeMode, a.block.mask = words, a.block.ld_mask = 2 * kTreeRows;
     }
     auto* states = reinterpret_cast<float*>(data + tree_rows_bytes(c.batch));
     auto* counters = reinterpret_cast<unsigned int*>(static_cast<char*>(ws) + kCountersOff);
