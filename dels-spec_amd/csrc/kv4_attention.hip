@@ -78,9 +78,6 @@ __device__ __forceinline__ void store_lse(const Kv4AttentionArgs& a, int b, cons
     a.lse[((int64_t)b * a.block.T + row.t) * a.q_heads + row.hq] = x;
 }
 
-// Floats of a piece's state in the workspace: outputs as the lanes hold them, then references and sums.
-template <int D, int MT> constexpr int kStateFloats = MT * D + 2 * MT;
-
 template <int D, int MT> struct ValueWords {
     using S = Shape<D, MT>;
     uint32_t code[2][S::PF][S::CT];
@@ -404,44 +401,19 @@ __global__ __launch_bounds__(kKv4Threads, 2) void kv4_attention_kernel(Kv4Attent
                 if (whole) {
                     store_out<T, S::VW>(a, b, row, S::channel_of(gi / S::ACC, gi % S::ACC, g), sum, inv);
                 } else {
-                    auto* to = reinterpret_cast<unsigned long long*>(state + (gi * 64 + lane) * S::VW);
-#pragma unroll
-                    for (int v = 0; v < S::VW; v += 2)
-                        atomic_store_u64(to + v / 2, (unsigned long long)__float_as_uint(sum[v + 1]) << 32 |
-                                                         __float_as_uint(sum[v]));
+                    store_state<S::VW>(state, gi, lane, sum);
                 }
             }
             __syncthreads();
         }
         if (way == 0 && g == 0) {
-            if (whole) {
-                store_lse(a, b, row, m, l);
-            } else {
-                auto* to = reinterpret_cast<unsigned int*>(state + MT * D + col);
-                atomic_store_u32(to, __float_as_uint(m));
-                atomic_store_u32(to + MT, __float_as_uint(l));
-            }
+            if (whole) store_lse(a, b, row, m, l);
+            else store_state_row<D, MT>(state, col, m, l);
         }
         if (!whole) {
-            // The states are written and read with device-coherent stores and loads, and every
-            // store is waited for before the arrival is counted: no cache fences.
             const int lo = at.start + ht * at.pages;
             const int2 held = cuts.holders(scan, b, ht, lo, lo + at.pages);
-            __builtin_amdgcn_s_waitcnt(0);
-            asm volatile("" ::: "memory");
-            __syncthreads();
-            if (threadIdx.x == 0) {
-                unsigned int* counter = counters + held.x * kCounterWords;
-                const unsigned prev = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                s_last = prev == (unsigned)(held.y - held.x) - 1u;
-                if (s_last) __hip_atomic_exchange(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            }
-            __syncthreads();
-            if (s_last) {
-                auto load = [&](const float* p) {
-                    return __uint_as_float(__hip_atomic_load(reinterpret_cast<const unsigned int*>(p), __ATOMIC_RELAXED,
-                                                             __HIP_MEMORY_SCOPE_AGENT));
-                };
+            if (last_to_arrive(counters, held, s_last)) {
                 constexpr int kMine = (kRegs / S::VW + WAYS - 1) / WAYS;
                 float sum[kMine][S::VW];
 #pragma unroll
@@ -449,39 +421,23 @@ __global__ __launch_bounds__(kKv4Threads, 2) void kv4_attention_kernel(Kv4Attent
 #pragma unroll
                     for (int v = 0; v < S::VW; ++v) sum[i][v] = 0.f;
                 m = -__builtin_inff(), l = 0.f;
-                // several states in flight: their loads go to memory (131k slots, 16 states: 91 us one
-                // at a time, 76 eight)
+                // several states in flight (131k slots, 16 states: 91 us one at a time, 76 eight)
                 constexpr int kFlight = WAYS;
                 for (int w0 = held.x; w0 < held.y; w0 += kFlight) {
-                    float tops[kFlight], sums[kFlight];
-                    unsigned long long two[kFlight][kMine][S::VW / 2];
-#pragma unroll
-                    for (int e = 0; e < kFlight; ++e) {
-                        const int w = min(w0 + e, held.y - 1);
-                        const float* st = state_of(w, w == held.x);
-                        tops[e] = load(st + MT * D + col);
-                        sums[e] = load(st + MT * D + MT + col);
-#pragma unroll
-                        for (int i = 0; i < kMine; ++i) {
-                            const int gi = min(way + i * WAYS, kRegs / S::VW - 1);
-                            auto* from = reinterpret_cast<unsigned long long*>(
-                                const_cast<float*>(st + (gi * 64 + lane) * S::VW));
-#pragma unroll
-                            for (int v = 0; v < S::VW / 2; ++v) two[e][i][v] = atomic_load_u64(from + v);
-                        }
-                    }
+                    const LoadedStates<kFlight, D, MT, WAYS, kRegs / S::VW, S::VW> loaded(
+                        w0, held, way, lane, col, [&](int w) { return state_of(w, w == held.x); });
 #pragma unroll
                     for (int e = 0; e < kFlight; ++e) {
                         if (w0 + e >= held.y) break;
-                        const float now = fmaxf(m, tops[e]), old = fade(m, now), f = fade(tops[e], now);
+                        const float top = loaded.reference[e], now = fmaxf(m, top), old = fade(m, now),
+                                    f = fade(top, now);
                         m = now;
-                        l = l * old + sums[e] * f;
+                        l = __builtin_fmaf(l, old, loaded.sum[e] * f);
 #pragma unroll
                         for (int i = 0; i < kMine; ++i)
 #pragma unroll
                             for (int v = 0; v < S::VW; ++v)
-                                sum[i][v] = sum[i][v] * old +
-                                            __uint_as_float((uint32_t)(two[e][i][v / 2] >> (32 * (v & 1)))) * f;
+                                sum[i][v] = __builtin_fmaf(sum[i][v], old, loaded.output(e, i, v) * f);
                     }
                 }
                 const float inv = l != 0.f ? kGrow / l : 0.f;

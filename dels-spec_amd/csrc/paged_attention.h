@@ -272,4 +272,78 @@ struct Cuts {
     }
 };
 
+// ---- states of parts, and who joins them ------------------------------------------
+//
+// A part of a tile group's pages leaves the state of its MT rows in the workspace: their outputs of D
+// channels as the lanes hold them, then each row's reference (a binary logarithm) and sum.  States are
+// written and read with device-coherent stores and loads, and every store is waited for before the
+// arrival is counted: no cache fences.  The last part to arrive joins all of them in their order, so that
+// results do not depend on who that is.
+
+// Floats of a state.
+template <int D, int MT> constexpr int kStateFloats = MT * D + 2 * MT;
+
+// N outputs of a lane, its i-th ones.
+template <int N> __device__ __forceinline__ void store_state(float* state, int i, int lane, const float* x) {
+    auto* to = reinterpret_cast<unsigned long long*>(state + (i * 64 + lane) * N);
+#pragma unroll
+    for (int v = 0; v < N; v += 2)
+        atomic_store_u64(to + v / 2, (unsigned long long)__float_as_uint(x[v + 1]) << 32 | __float_as_uint(x[v]));
+}
+template <int D, int MT>
+__device__ __forceinline__ void store_state_row(float* state, int row, float reference, float sum) {
+    auto* to = reinterpret_cast<unsigned int*>(state + MT * D + row);
+    atomic_store_u32(to, __float_as_uint(reference));
+    atomic_store_u32(to + MT, __float_as_uint(sum));
+}
+
+// Counts the arrival of this workgroup, which has one of the parts held.x .. held.y - 1 and has stored its
+// state; whether it is the last of them, which leaves the counter at 0.  `flag`: a word of LDS.
+__device__ __forceinline__ bool last_to_arrive(unsigned int* counters, int2 held, bool& flag) {
+    __builtin_amdgcn_s_waitcnt(0);
+    asm volatile("" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        unsigned int* counter = counters + held.x * kCounterWords;
+        const unsigned prev = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        flag = prev == (unsigned)(held.y - held.x) - 1u;
+        if (flag) __hip_atomic_exchange(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    return flag;
+}
+
+// FLIGHT states of parts w0 .. loaded at once, as their loads go to memory: a row's references and sums,
+// and of this lane's GROUPS outputs of N each the groups way, way + WAYS, ..
+template <int FLIGHT, int D, int MT, int WAYS, int GROUPS, int N> struct LoadedStates {
+    static constexpr int kMine = (GROUPS + WAYS - 1) / WAYS;
+    float reference[FLIGHT], sum[FLIGHT];
+    unsigned long long two[FLIGHT][kMine][N / 2];
+
+    // state_of(w): that of part w; parts past the last one are that again.
+    template <typename F>
+    __device__ __forceinline__ LoadedStates(int w0, int2 held, int way, int lane, int row, F&& state_of) {
+        auto load = [](const float* p) {
+            return __uint_as_float(__hip_atomic_load(reinterpret_cast<const unsigned int*>(p), __ATOMIC_RELAXED,
+                                                     __HIP_MEMORY_SCOPE_AGENT));
+        };
+#pragma unroll
+        for (int e = 0; e < FLIGHT; ++e) {
+            float* state = state_of(min(w0 + e, held.y - 1));
+            reference[e] = load(state + MT * D + row);
+            sum[e] = load(state + MT * D + MT + row);
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) {
+                auto* from = reinterpret_cast<unsigned long long*>(
+                    state + (min(way + i * WAYS, GROUPS - 1) * 64 + lane) * N);
+#pragma unroll
+                for (int v = 0; v < N / 2; ++v) two[e][i][v] = atomic_load_u64(from + v);
+            }
+        }
+    }
+    __device__ __forceinline__ float output(int e, int i, int v) const {
+        return __uint_as_float((uint32_t)(two[e][i][v / 2] >> (32 * (v & 1))));
+    }
+};
+
 }  // namespace dels
