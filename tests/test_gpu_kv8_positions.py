@@ -251,3 +251,38 @@ def test_append_by_positions_writes_its_blocks_and_nothing_else(pkg, dev, given)
     torch.cuda.synchronize()
     seen = torch.tensor(lengths)[:, None].expand(B, T) > 0
     assert torch.equal(lse.cpu().isnan(), (lost & seen)[..., None].expand(B, T, H * G))
+
+
+@pytest.mark.parametrize("pages,columns", [(0, 3), (3, 0)])
+def test_positions_over_caches_of_nothing(pkg, dev, pages, columns):
+    """No pages, or a table of no columns: every row sees nothing, whatever its position."""
+    say("positions and nothing", pages, columns)
+    cache = pkg.KV8Cache(torch.zeros(pages, 2, 8320, dtype=torch.uint8, device=dev),
+                         torch.zeros(2, columns, dtype=torch.int32, device=dev), 64)
+    q = torch.randn(2, 9, 4, 64, device=dev).to(torch.bfloat16)
+    masks, positions = trees(2, 9, 1, [100, 0])
+    for window in (1, 5, 9):
+        out, lse = pkg.kv8_attention(q, cache, ints([100, 0], dev), block=masks.to(dev), window=window, sinks=70,
+                                     positions=positions.to(dev), weight_parts=2)
+        torch.cuda.synchronize()
+        assert not out.any() and torch.all(lse == -INF)
+
+
+def test_positions_on_another_stream_with_a_workspace_of_the_callers(pkg, dev):
+    say("positions on a side stream")
+    B, T, HQ, H, D = 3, 14, 8, 2, 128
+    lengths = [1500, 20, 700]
+    cache, q, _ = attention_inputs(pkg, dev, B, T, HQ, H, D, 26, "bf16", "causal", lengths, None, 3)
+    masks, positions = (x.to(dev) for x in trees(B, T, 4, lengths))
+    n, qd = ints(lengths, dev), q.to(dev)
+    ws = pkg.ops.new_workspace(dev, 1 << 24)
+    want = pkg.kv8_attention(qd, cache, n, block=masks, window=90, sinks=3, positions=positions)
+    side = torch.cuda.Stream(dev)
+    side.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(side):
+        got = [pkg.kv8_attention(qd, cache, n, block=masks, window=90, sinks=3, positions=positions, workspace=ws)
+               for _ in range(3)]
+    side.synchronize()
+    check(cache, q, masks.cpu(), positions.cpu(), lengths, [T] * B, 90, 3, *want, "bf16")
+    for o, l in got:
+        assert torch.equal(o, want[0]) and torch.equal(l, want[1])

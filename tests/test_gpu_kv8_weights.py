@@ -9,7 +9,8 @@ import pytest
 import torch
 
 from oracle import kv8 as O
-from test_gpu_kv8 import ATTENTION, attention_64, attention_inputs, contents, ints, say
+from test_gpu_kv8 import ATTENTION, attention_64, attention_inputs, contents, ints, same, say
+from test_gpu_kv8_tiles import check
 
 pytestmark = pytest.mark.gpu
 
@@ -108,3 +109,37 @@ def test_fp16_outputs_have_two_parts_as_it_is(pkg, dev):
     assert one[1].isnan().any() and f.any()
     assert torch.all((one[1] - two[1])[f].abs() <= 2.0 ** -18 * (1 + two[1][f].abs()))
     assert np.array_equal(contents(cache)[0][0, 0, 100], np.full(64, np.nan), equal_nan=True)
+
+
+@pytest.mark.parametrize("block,window,sinks", [("causal", None, 0), ("mask", 100, 70), ("none", 130, 64)])
+@pytest.mark.parametrize("T,D", [(4, 128), (8, 64), (16, 128), (32, 64), (64, 128)])
+def test_two_parts_over_pages_of_all_kinds(pkg, dev, T, D, block, window, sinks):
+    """One, two, four and eight row tiles a workgroup, over pages that the table does not name, rows that are not
+    held and partial pages; in the queries' place, too."""
+    say("two parts, pages of all kinds", T, D, block, window, sinks)
+    B, H, G, pages = 32, 8, 4, 9
+    lengths = [(37 * b + 5) % (64 * pages - T) if b != 3 else 0 for b in range(B)]
+    counts = [T if b % 4 else (11 * b) % (T + 1) for b in range(B)]
+    cache, q, masks = attention_inputs(pkg, dev, B, T, H * G, H, D, pages, "bf16", block, lengths, counts, T + D)
+    ends = [n if block == "none" else n + c for n, c in zip(lengths, counts)]
+    for b in range(0, B, 3):                                       # a row of one head that is not held
+        slot = (29 * b) % max(1, ends[b])
+        at = 128 * D + 8 * (slot // 32 % 2) + 4 + slot % 32 // 8
+        cache.data[cache.block_table[b, slot // 64].item(), b % H, at] |= 1 << slot % 8
+    K, V = contents(cache)
+    named = np.ones((B, 64 * pages), bool)
+    for b in range(1, B, 2):
+        p = (5 * b) % pages
+        cache.block_table[b, p] = (-1, 10 ** 9, cache.data.shape[0])[b % 3]
+        named[b, 64 * p:64 * p + 64] = False
+    for b, n in enumerate(ends):                                   # what was spoiled is not there
+        K[b, :, n:], V[b, :, n:] = 0, 0
+    kw = dict(counts=ints(counts, dev), window=window, sinks=sinks, block=block if masks is None else masks.to(dev),
+              weight_parts=2)
+    n, qd = ints(lengths, dev), q.to(dev)
+    out, lse = pkg.kv8_attention(qd, cache, n, **kw)
+    torch.cuda.synchronize()
+    check(q, K, V, named, lengths, counts, block, masks, window, sinks, out, lse, "bf16", D ** -0.5)
+    there, again = pkg.kv8_attention(qd, cache, n, out=qd, **kw)
+    torch.cuda.synchronize()
+    assert there is qd and same(qd, out) and same(again, lse)
