@@ -24,13 +24,14 @@
 // 60 -> 78, 2 x 512 rows 87 -> 124, 4093 rows through a window 114 -> 151, one row of 32 sequences
 // 152 -> 155.  Scores, maxima, sums and outputs are fp32.
 //
-// What bounds it, at 32 query and 8 cache heads of 128 in bf16 (kernel times):
-//   32 sequences of up to 16300 slots, 1 token     154 us  memory: 935 MB at 6.1 TB/s
-//   131k slots, 16 tokens                            62 us  memory and issue: 270 MB at 4.4 TB/s, matrix cores 23 %
-//   4093 tokens through a window of 1024            113 us  issue: a step of 32 x 32 has 16 matrix
-//                                                           instructions (512 cycles) and 140 vector ones, 64 of
-//                                                           them conversions; 0.65 PFLOP/s, those masked counted
-//   8 sequences of up to 4000 slots, 16 tokens       20 us  latency: 2 us to know its pages, 13 for two or three
+// What bounds it, at 32 query and 8 cache heads of 128 in bf16 (kernel times, medians under the profiler; the
+// times above and beside the rules below are of calls without it):
+//   32 sequences of up to 16300 slots, 1 token     153 us  memory: 955 MB at 6.2 TB/s
+//   131k slots, 16 tokens                            61 us  memory and issue: 276 MB at 4.5 TB/s, matrix cores 23 %
+//   4093 tokens through a window of 1024            130 us  issue: a step of 32 x 32 has 16 matrix
+//                                                  (a call  instructions (512 cycles) and 140 vector ones, 64 of
+//                                                  113 us)  them conversions; 0.57 PFLOP/s, those masked counted
+//   8 sequences of up to 4000 slots, 16 tokens       21 us  latency: 2 us to know its pages, 13 for two or three
 //                                                           pages a wave, 5 joining waves and parts
 // Pages go straight from memory to registers, the next one's loads in flight behind a page's work; where
 // eight row tiles share them, through LDS.

@@ -8,9 +8,9 @@
 // stored as the threads have them, values go through LDS, from rows of channels to columns
 // of slots.  Queries are rotated by workgroups of their own behind those of the blocks.
 //
-// Memory bounds both at a prompt's size (4 x 2039 fp16 rows of 8 heads of 128, 32 query heads: append
-// 29.5 us, 5.5 TB/s by the 162 MB that it moves; read 10.3 us, 4.6 TB/s), latency at a block's (8 x 16 rows: 5.3
-// and 4.2 us, a launch of nothing 3.6).
+// Memory bounds both at a prompt's size (4 x 2039 fp16 rows of 8 heads of 128, 32 query heads, kernel times:
+// append 29.5 us, 5.8 TB/s by the 170 MB that it moves; read 10.1 us, 47 MB at 4.7 TB/s), latency at a block's
+// (8 x 16 rows: 5.3 and 4.2 us, a launch of nothing 3.6).
 #include <algorithm>
 
 #include "kv8.h"
