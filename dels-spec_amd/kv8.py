@@ -224,9 +224,9 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, lengths: torch.Tensor, *, bl
     that see a score of NaN or +inf NaN in both.
 
     Scores, maxima, sums and outputs are fp32.  A slot's weight meets its value as one f16 number
-    for bf16 queries, as two for fp16 ones: before it is rounded, ``out`` may be off by 2^-11 (2^-17) of the
-    weighted sum of the values' magnitudes, which is more of it where values cancel.  ``weight_parts=2``
-    has two parts for bf16 queries, too; blocks of many rows take longer.
+    for bf16 queries, as two for fp16 ones, which may put ``out``, before it is rounded, off by 2^-11 (2^-17) of
+    the weighted sum of the values' magnitudes: more of what is left where values cancel.
+    ``weight_parts=2`` has two parts for bf16 queries, too; blocks of many rows take longer.
     """
     _require_cache(cache, 8)
     if _elsewhere_current(cache):
